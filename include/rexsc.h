@@ -287,6 +287,118 @@ size_t rexsc_fixed_conv2d_workspace_bytes(const rexsc_fixed_desc *d);
 int rexsc_fixed_conv2d(const rexsc_fixed_desc *d, const float *x, const float *w, int32_t *out,
                        void *workspace, size_t workspace_bytes, rexsc_stream_t stream);
 
+/* ---- 8-bit linear layer ------------------------------------------------------------------------
+ * No counterpart in the reference.  y = x W^T + bias with both operands in 8 bits: rows of x (tokens) and rows of W
+ * (output channels) are held as int8 with one float32 scale each, the products are summed exactly in int32, and
+ * scales, bias and the rounding to the result's type are applied to the sum.
+ *
+ * Element types of the float tensors below. */
+enum { REXSC_F32 = 0, REXSC_F16 = 1, REXSC_BF16 = 2 };
+
+/* Rows in 8 bits: a = max |x[r][:]|, scale[r] = a / 127 (float32), q[r][k] = the integer nearest to 127 x[r][k] / a,
+ * ties to even, decided exactly (not on a rounded quotient).  A row of zeros gets scale 0; a row that holds a NaN or
+ * an infinity gets scale NaN and zeros, so that everything computed from it is NaN.  x: rows at distance x_stride
+ * elements, aligned to their element; q: rows at distance q_stride bytes, a multiple of 16, at least cols, q 16-byte
+ * aligned; the bytes from cols to q_stride are set to 0. */
+int rexsc_quantize_rows(const void *x, int dtype, size_t rows, size_t cols, size_t x_stride,
+                        int8_t *q, size_t q_stride, float *scale, rexsc_stream_t stream);
+
+typedef struct rexsc_int8_desc {
+    int32_t struct_size;     /* sizeof(rexsc_int8_desc) */
+    int32_t M, N, K;         /* tokens, output channels, reduction; 1 <= K <= 131071 (the int32 sum cannot overflow) */
+    int32_t dtype;           /* type of y (and of x, of the incoming gradient and of dx where a call has them) */
+    int32_t bias_dtype;      /* type of bias and of its gradient */
+    int32_t weight_dtype;    /* type of the weight's gradient */
+    int32_t reserved;        /* 0 */
+    int64_t x_stride;        /* distance of x's rows in elements (rexsc_int8_linear only) */
+    int64_t a_stride;        /* distance of the tokens' int8 rows in bytes: a multiple of 16, at least K */
+    int64_t b_stride;        /* distance of the channels' int8 rows in bytes: likewise */
+} rexsc_int8_desc;
+
+/* What a workspace is for. */
+enum { REXSC_INT8_PRODUCT = 0, REXSC_INT8_LINEAR = 1, REXSC_INT8_GRAD_INPUT = 2, REXSC_INT8_GRAD_WEIGHT = 3 };
+/* Bytes of workspace a call needs (0: none).  (size_t)-1 and rexsc_last_error() if the descriptor is invalid. */
+size_t rexsc_int8_workspace_bytes(const rexsc_int8_desc *d, int what);
+
+/* y[m][n] = (sum_k a[m][k] b[n][k]) * a_scale[m] * b_scale[n] + bias[n].  a, b: int8, 16-byte aligned, every value of
+ * -128..127 allowed; each row is readable up to the next multiple of 16 bytes, and what lies there does not matter.
+ * y: dense [M][N].  bias may be NULL. */
+int rexsc_int8_product(const rexsc_int8_desc *d, const int8_t *a, const float *a_scale, const int8_t *b,
+                       const float *b_scale, const void *bias, void *y, void *workspace, size_t workspace_bytes,
+                       rexsc_stream_t stream);
+/* The same from float tokens x, which are taken to 8 bits as rexsc_quantize_rows does (into the workspace, or, for
+ * few tokens, inside the product's kernel).  d->a_stride is not read. */
+int rexsc_int8_linear(const rexsc_int8_desc *d, const void *x, const int8_t *b, const float *b_scale, const void *bias,
+                      void *y, void *workspace, size_t workspace_bytes, rexsc_stream_t stream);
+
+/* Straight-through gradients (the quantisation passes the gradient on, as QuantizeGrad's backward does,
+ * utils_functional.py:117-123): dx[m][k] = sum_n g[m][n] b_scale[n] b[n][k] in d->dtype,
+ * dw[n][k] = sum_m g[m][n] a_scale[m] a[m][k] in d->weight_dtype, db[n] = sum_m g[m][n] in d->bias_dtype (NULL: not
+ * wanted; dw may be NULL too).  g: dense [M][N] of d->dtype, dx: dense [M][K], dw: dense [N][K]. */
+int rexsc_int8_grad_input(const rexsc_int8_desc *d, const void *g, const int8_t *b, const float *b_scale, void *dx,
+                          void *workspace, size_t workspace_bytes, rexsc_stream_t stream);
+int rexsc_int8_grad_weight(const rexsc_int8_desc *d, const void *g, const int8_t *a, const float *a_scale, void *dw,
+                           void *db, void *workspace, size_t workspace_bytes, rexsc_stream_t stream);
+
+/* ---- layer norm ----------------------------------------------------------------------------------
+ * No counterpart in the reference.  y = (x - mean) * rstd * weight + bias over each row of `cols` elements, with
+ * mean and rstd = 1 / sqrt(biased variance + eps) in float32, in two passes over the row (never as a difference of
+ * squares).  weight and bias: float32 or x's type (weight_dtype); either may be NULL. */
+typedef struct rexsc_norm_desc {
+    int32_t struct_size;     /* sizeof(rexsc_norm_desc) */
+    int32_t dtype;           /* type of x, y, grad_out and dx */
+    int32_t weight_dtype;    /* type of weight, bias, dw and db: REXSC_F32 or dtype */
+    float eps;
+    int64_t rows, cols;
+    int64_t x_stride;        /* distance of x's rows in elements; y, grad_out and dx are dense */
+} rexsc_norm_desc;
+/* mean, rstd: float32 [rows], or both NULL where no gradient will be asked for. */
+int rexsc_layer_norm_forward(const rexsc_norm_desc *d, const void *x, const void *weight, const void *bias, void *y,
+                             float *mean, float *rstd, rexsc_stream_t stream);
+size_t rexsc_layer_norm_backward_workspace_bytes(const rexsc_norm_desc *d);
+/* dx, dw, db: any of them may be NULL.  dw and db are summed per block and then over the blocks in a fixed order. */
+int rexsc_layer_norm_backward(const rexsc_norm_desc *d, const void *grad_out, const void *x, const void *weight,
+                              const float *mean, const float *rstd, void *dx, void *dw, void *db,
+                              void *workspace, size_t workspace_bytes, rexsc_stream_t stream);
+
+/* ---- AdamW step over many tensors ----------------------------------------------------------------
+ * No counterpart in the reference (its training loop calls torch.optim and clamps the weights in a pass of their own,
+ * utils_own.py:187-190).  For every tensor, with t its step number:
+ *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2,
+ *   p = clamp(p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps), lo, hi)
+ * in float32, p rounded to its type.  state_bits 32: m and v are float32.  state_bits 8: they are e4m3 values (one
+ * sign, four exponent, three mantissa bits; largest 448) with one float32 scale for every 256 consecutive elements,
+ *   m = value * scale with scale = max |m| / 448,   sqrt(v) = value * scale with scale = max sqrt(v) / 448,
+ * the update using m and v as computed, before they are rounded to 8 bits.  A positive v never becomes 0 there: its
+ * root is at least the smallest value, 2^-9, so that no element is divided by eps alone.  A block whose largest
+ * magnitude is below 2^-100 is stored as zeros; a block that takes in a NaN or an infinity is lost as a whole. */
+typedef struct rexsc_adamw_tensor {
+    void *param;             /* numel elements of the descriptor's dtype, dense */
+    const void *grad;        /* the same */
+    void *exp_avg;           /* m: float32, or e4m3 */
+    void *exp_avg_sq;        /* v: float32, or e4m3 of its root */
+    float *exp_avg_scale;    /* ceil(numel / 256) scales; NULL for 32-bit states */
+    float *exp_avg_sq_scale;
+    int64_t numel;
+} rexsc_adamw_tensor;
+typedef struct rexsc_adamw_desc {
+    int32_t struct_size;     /* sizeof(rexsc_adamw_desc) */
+    int32_t dtype;           /* of param and grad */
+    int32_t state_bits;      /* 32 or 8 */
+    int32_t use_clamp;
+    double lr, beta1, beta2, eps, weight_decay;
+    double clamp_lo, clamp_hi;
+    int64_t step;            /* t of this step, from 1 on; with step_dev: ignored */
+} rexsc_adamw_desc;
+/* tensors: HOST array, read before the call returns.  step_dev: NULL, or a device int64 that holds the number of
+ * steps taken; the call adds one to it on the stream and uses the result as t, which a captured call needs.
+ * grad_scale: NULL, or a device float32 that the gradients are divided by; found_inf: NULL, or a device float32:
+ * where it is not 0 nothing is written and step_dev stays.  grad_scale and found_inf need step_dev.
+ * coef: device workspace of REXSC_ADAMW_COEF_BYTES, needed with step_dev. */
+#define REXSC_ADAMW_COEF_BYTES 256
+int rexsc_adamw_step(const rexsc_adamw_desc *d, const rexsc_adamw_tensor *tensors, size_t n_tensors, int64_t *step_dev,
+                     const float *grad_scale, const float *found_inf, void *coef, rexsc_stream_t stream);
+
 /* ---- activation-calibration statistics -------------------------------------------------
  * One pass over (a_bit, a_act) producing, for each of n_win (<= 64) windows
  * win_lo[k] <= a_act < win_hi[k], the count, sum and sum of squares of err = a_bit - a_act

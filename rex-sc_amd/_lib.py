@@ -45,6 +45,31 @@ class FixedDesc(_Desc):
         "add_config", "precision_in", "precision_out")]
 
 
+class Int8Desc(_Desc):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "struct_size", "M", "N", "K", "dtype", "bias_dtype", "weight_dtype", "reserved")] + [
+        (n, ctypes.c_int64) for n in ("x_stride", "a_stride", "b_stride")]
+
+
+class NormDesc(_Desc):
+    _fields_ = [("struct_size", ctypes.c_int32), ("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("x_stride", ctypes.c_int64)]
+
+
+class AdamwDesc(_Desc):
+    _fields_ = [(n, ctypes.c_int32) for n in ("struct_size", "dtype", "state_bits", "use_clamp")] + [
+        (n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "clamp_lo", "clamp_hi")] + [
+        ("step", ctypes.c_int64)]
+
+
+# rexsc_adamw_tensor is seven 8-byte fields (param, grad, exp_avg, exp_avg_sq, their scales, numel): a table of them is
+# handed over as one array of integers
+ADAMW_TENSOR_FIELDS = 7
+ADAMW_COEF_BYTES = 256            # REXSC_ADAMW_COEF_BYTES
+F32, F16, BF16 = 0, 1, 2          # REXSC_F32, ...
+INT8_PRODUCT, INT8_LINEAR, INT8_GRAD_INPUT, INT8_GRAD_WEIGHT = 0, 1, 2, 3  # REXSC_INT8_*
+
+
 class ProfileRecord(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 64), ("calls", ctypes.c_int32), ("total_ms", ctypes.c_double),
                 ("total_work", ctypes.c_double)]
@@ -54,6 +79,7 @@ _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
 _int = ctypes.c_int
 _u64 = ctypes.c_uint64
+_i8d, _nd = ctypes.POINTER(Int8Desc), ctypes.POINTER(NormDesc)
 
 # name -> (restype, argtypes); every symbol include/rexsc.h declares
 SIGNATURES = {
@@ -91,6 +117,16 @@ SIGNATURES = {
                                    ctypes.POINTER(ctypes.c_uint32)]),
     "rexsc_fixed_conv2d_workspace_bytes": (_sz, [ctypes.POINTER(FixedDesc)]),
     "rexsc_fixed_conv2d": (_int, [ctypes.POINTER(FixedDesc), _vp, _vp, _vp, _vp, _sz, _vp]),
+    "rexsc_quantize_rows": (_int, [_vp, _int, _sz, _sz, _sz, _vp, _sz, _vp, _vp]),
+    "rexsc_int8_workspace_bytes": (_sz, [_i8d, _int]),
+    "rexsc_int8_product": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "rexsc_int8_linear": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "rexsc_int8_grad_input": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "rexsc_int8_grad_weight": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "rexsc_layer_norm_forward": (_int, [_nd, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "rexsc_layer_norm_backward_workspace_bytes": (_sz, [_nd]),
+    "rexsc_layer_norm_backward": (_int, [_nd, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "rexsc_adamw_step": (_int, [ctypes.POINTER(AdamwDesc), _vp, _sz, _vp, _vp, _vp, _vp, _vp]),
     "rexsc_profile_begin": (_int, []),
     "rexsc_profile_end": (_int, [ctypes.POINTER(ProfileRecord), _int]),
     "rexsc_valu_probe": (_int, [_int, _int, _vp, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),

@@ -669,3 +669,266 @@ def calib_stats(a_bit, a_act, win_lo, win_hi):
         rc = _lib.lib().rexsc_calib_stats(_ptr(ab), _ptr(aa), ab.numel(), lo, hi, n_win, _ptr(stats), _stream())
         _lib.check(rc, "rexsc_calib_stats")
     return stats
+
+
+# ---- 8-bit linear layer --------------------------------------------------------------------------
+
+_DTYPE_CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+ROW_PAD = 128  # int8 rows are laid out at a multiple of this many bytes: the product's step along the reduction
+MAX_K = 131071
+
+
+def _dtype_code(t, what):
+    code = _DTYPE_CODE.get(t.dtype if isinstance(t, torch.Tensor) else t)
+    if code is None:
+        raise RuntimeError("%s: expected float32, float16 or bfloat16 (got %s)" % (what, getattr(t, "dtype", t)))
+    return code
+
+
+def _same_device(what, first, *rest):
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise RuntimeError("%s: tensors on %s and on %s" % (what, first.device, t.device))
+
+
+def _rows_of(t):
+    """t [..., K] as a matrix whose rows lie at one distance and whose elements are neighbours (a view where t has such
+    a layout, else a copy)."""
+    t = t.detach()
+    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if m.stride(1) != 1 and m.shape[1] > 1 or (m.shape[0] > 1 and m.stride(0) < m.shape[1]):
+        m = m.contiguous()
+    return m
+
+
+def _row_stride(m):
+    return m.stride(0) if m.shape[0] > 1 else m.shape[1]
+
+
+def quantize_rows(x):
+    """Rows of x [..., K] in 8 bits -> (q int8 of x's shape, scale float32 of x.shape[:-1]).  q's rows lie at a multiple
+    of 128 bytes, padded with zeros."""
+    _require_cuda(x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError("quantize_rows: expected rows of at least one element (got shape %s)" % (tuple(x.shape),))
+    code = _dtype_code(x, "quantize_rows")
+    m = _rows_of(x)
+    R, K = m.shape
+    pad = -(-K // ROW_PAD) * ROW_PAD
+    with torch.cuda.device(x.device):
+        q = torch.empty((R, pad), dtype=torch.int8, device=x.device)
+        scale = torch.empty(R, dtype=torch.float32, device=x.device)
+        rc = _lib.lib().rexsc_quantize_rows(_ptr(m), code, R, K, _row_stride(m), _ptr(q), pad, _ptr(scale), _stream())
+        _lib.check(rc, "rexsc_quantize_rows")
+    q = q[:, :K]
+    if x.dim() != 2:
+        q, scale = q.view(x.shape) if x.dim() > 2 else q[0], scale.view(x.shape[:-1])
+    return q, scale
+
+
+def _operand8(t, what):
+    """int8 matrix as the product reads it: rows 16-byte aligned and readable to the next multiple of 16 bytes."""
+    if t.dtype != torch.int8 or t.dim() != 2 or not 1 <= t.shape[1] <= MAX_K:
+        raise RuntimeError("%s: expected an int8 matrix with 1 to %d columns (got %s %s)"
+                           % (what, MAX_K, t.dtype, tuple(t.shape)))
+    R, K = t.shape
+    fits = (K == 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0
+    if fits and R > 1:
+        fits = t.stride(0) % 16 == 0 and t.stride(0) >= K
+    if fits and K % 16:
+        last = t.storage_offset() + (R - 1) * t.stride(0) + -(-K // 16) * 16
+        fits = R == 0 or last <= t.untyped_storage().nbytes()
+    if fits:
+        return t, (t.stride(0) if R > 1 else -(-K // 16) * 16)
+    pad = -(-K // ROW_PAD) * ROW_PAD
+    out = torch.empty((R, pad), dtype=torch.int8, device=t.device)[:, :K]
+    out.copy_(t)  # what lies behind the K-th byte does not matter
+    return out, pad
+
+
+def _scale_vector(s, n, device, what):
+    if s.dtype != torch.float32 or s.numel() != n or s.device != device:
+        raise RuntimeError("%s: expected %d float32 scales on %s (got %d %s on %s)"
+                           % (what, n, device, s.numel(), s.dtype, s.device))
+    return s.detach().reshape(-1).contiguous()
+
+
+def _bias_vector(bias, n, what):
+    if bias is None:
+        return None, _lib.F32
+    if bias.numel() != n or bias.dim() != 1:
+        raise RuntimeError("%s: expected a bias of %d elements (got %s)" % (what, n, tuple(bias.shape)))
+    return bias.detach().contiguous(), _dtype_code(bias, what)
+
+
+def _int8_space(L, d, what, device):
+    nbytes = L.rexsc_int8_workspace_bytes(ctypes.byref(d), what)
+    if nbytes == ctypes.c_size_t(-1).value:
+        _lib.check(-1, "rexsc_int8_linear (planning)")
+    return (_workspace(nbytes, device), nbytes) if nbytes else (None, 0)
+
+
+def matmul_int8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
+    """(a [M, K] int8 times b [N, K] int8 transposed, summed in int32) * a_scale[:, None] * b_scale + bias -> [M, N]."""
+    _require_cuda(a, b)
+    _same_device("matmul_int8", a, b, bias)
+    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1]:
+        raise RuntimeError("matmul_int8: expected int8 matrices [M, K] and [N, K], got %s and %s"
+                           % (tuple(a.shape), tuple(b.shape)))
+    M, K = a.shape
+    N = b.shape[0]
+    a_scale = _scale_vector(a_scale, M, a.device, "matmul_int8")
+    b_scale = _scale_vector(b_scale, N, a.device, "matmul_int8")
+    bias, bias_code = _bias_vector(bias, N, "matmul_int8")
+    L = _lib.lib()
+    with torch.cuda.device(a.device):
+        a, sa = _operand8(a, "matmul_int8")
+        b, sb = _operand8(b, "matmul_int8")
+        d = _lib.Int8Desc(M, N, K, _dtype_code(out_dtype, "matmul_int8"), bias_code, _lib.F32, 0, 0, sa, sb)
+        y = torch.empty((M, N), dtype=out_dtype, device=a.device)
+        ws, nbytes = _int8_space(L, d, _lib.INT8_PRODUCT, a.device)
+        rc = L.rexsc_int8_product(ctypes.byref(d), _ptr(a), _ptr(a_scale), _ptr(b), _ptr(b_scale), _ptr(bias), _ptr(y),
+                                  _ptr(ws), nbytes, _stream())
+        _lib.check(rc, "rexsc_int8_product")
+    return y
+
+
+def int8_linear(x, wq, w_scale, bias=None):
+    """x [..., K] float times the 8-bit weights wq [N, K] -> [..., N] in x's type; x's rows are taken to 8 bits inside."""
+    _require_cuda(x, wq)
+    _same_device("linear_int8", x, wq, bias)
+    if wq.dim() != 2 or x.dim() < 1 or x.shape[-1] != wq.shape[1]:
+        raise RuntimeError("linear_int8: expected input [..., K] and weight [N, K], got %s and %s"
+                           % (tuple(x.shape), tuple(wq.shape)))
+    code = _dtype_code(x, "linear_int8")
+    m = _rows_of(x)
+    M, K = m.shape
+    N = wq.shape[0]
+    w_scale = _scale_vector(w_scale, N, x.device, "linear_int8")
+    bias, bias_code = _bias_vector(bias, N, "linear_int8")
+    L = _lib.lib()
+    with torch.cuda.device(x.device):
+        wq, sb = _operand8(wq, "linear_int8")
+        d = _lib.Int8Desc(M, N, K, code, bias_code, _lib.F32, 0, _row_stride(m), 0, sb)
+        y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+        ws, nbytes = _int8_space(L, d, _lib.INT8_LINEAR, x.device)
+        rc = L.rexsc_int8_linear(ctypes.byref(d), _ptr(m), _ptr(wq), _ptr(w_scale), _ptr(bias), _ptr(y), _ptr(ws), nbytes,
+                                 _stream())
+        _lib.check(rc, "rexsc_int8_linear")
+    return y
+
+
+def int8_grad_input(g, wq, w_scale):
+    """Straight-through gradient of the product with respect to its input: g [..., N] -> [..., K] in g's type."""
+    _require_cuda(g, wq)
+    _same_device("linear_int8", g, wq, w_scale)
+    code = _dtype_code(g, "linear_int8")
+    N, K = wq.shape
+    gm = g.detach().reshape(-1, N).contiguous()
+    L = _lib.lib()
+    with torch.cuda.device(g.device):
+        wq, sb = _operand8(wq, "linear_int8")
+        d = _lib.Int8Desc(gm.shape[0], N, K, code, _lib.F32, _lib.F32, 0, 0, 0, sb)
+        dx = torch.empty(g.shape[:-1] + (K,), dtype=g.dtype, device=g.device)
+        ws, nbytes = _int8_space(L, d, _lib.INT8_GRAD_INPUT, g.device)
+        rc = L.rexsc_int8_grad_input(ctypes.byref(d), _ptr(gm), _ptr(wq), _ptr(w_scale), _ptr(dx), _ptr(ws), nbytes,
+                                     _stream())
+        _lib.check(rc, "rexsc_int8_grad_input")
+    return dx
+
+
+def int8_grad_weight(g, xq, x_scale, weight_dtype=None, bias_dtype=None):
+    """Straight-through gradients with respect to weight and bias: (dw [N, K] of weight_dtype, db [N] of bias_dtype);
+    a type of None: not wanted."""
+    _require_cuda(g, xq)
+    _same_device("linear_int8", g, xq, x_scale)
+    code = _dtype_code(g, "linear_int8")
+    N = g.shape[-1]
+    M, K = xq.shape
+    gm = g.detach().reshape(M, N).contiguous()
+    L = _lib.lib()
+    with torch.cuda.device(g.device):
+        xq, sa = _operand8(xq, "linear_int8")
+        mk = lambda shape, dt: torch.empty(shape, dtype=dt, device=g.device) if dt is not None else None
+        dw, db = mk((N, K), weight_dtype), mk((N,), bias_dtype)
+        d = _lib.Int8Desc(M, N, K, code, _dtype_code(bias_dtype or torch.float32, "linear_int8"),
+                          _dtype_code(weight_dtype or torch.float32, "linear_int8"), 0, 0, sa, 0)
+        ws, nbytes = _int8_space(L, d, _lib.INT8_GRAD_WEIGHT, g.device)
+        rc = L.rexsc_int8_grad_weight(ctypes.byref(d), _ptr(gm), _ptr(xq), _ptr(x_scale), _ptr(dw), _ptr(db), _ptr(ws),
+                                      nbytes, _stream())
+        _lib.check(rc, "rexsc_int8_grad_weight")
+    return dw, db
+
+
+# ---- layer norm ----------------------------------------------------------------------------------
+
+def _norm_vectors(x, weight, bias):
+    """weight and bias as the kernels read them: one type for both, float32 or x's."""
+    dt = torch.float32
+    given = [t for t in (weight, bias) if t is not None]
+    for t in given:
+        if t.dim() != 1 or t.numel() != x.shape[-1]:
+            raise RuntimeError("layer_norm: expected weight and bias of %d elements (got %s)"
+                               % (x.shape[-1], tuple(t.shape)))
+        _dtype_code(t, "layer_norm")
+    if given and all(t.dtype == x.dtype for t in given):
+        dt = x.dtype
+    fit = lambda t: None if t is None else t.detach().to(dt).contiguous()
+    return fit(weight), fit(bias), dt
+
+
+def layer_norm_forward(x, weight, bias, eps, want_stats=True):
+    """(y, mean, rstd) of a layer norm over the last dimension; mean and rstd float32 per row (None unless wanted)."""
+    _require_cuda(x)
+    _same_device("layer_norm", x, weight, bias)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError("layer_norm: expected rows of at least one element (got shape %s)" % (tuple(x.shape),))
+    code = _dtype_code(x, "layer_norm")
+    w, b, wdt = _norm_vectors(x, weight, bias)
+    m = _rows_of(x)
+    R, D = m.shape
+    with torch.cuda.device(x.device):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean = torch.empty(R, dtype=torch.float32, device=x.device) if want_stats else None
+        rstd = torch.empty(R, dtype=torch.float32, device=x.device) if want_stats else None
+        d = _lib.NormDesc(code, _DTYPE_CODE[wdt], float(eps), R, D, _row_stride(m))
+        rc = _lib.lib().rexsc_layer_norm_forward(ctypes.byref(d), _ptr(m), _ptr(w), _ptr(b), _ptr(y), _ptr(mean),
+                                                 _ptr(rstd), _stream())
+        _lib.check(rc, "rexsc_layer_norm_forward")
+    return y, mean, rstd
+
+
+def layer_norm_backward(grad_output, x, weight, mean, rstd, eps, need_x=True, weight_dtype=None, bias_dtype=None):
+    """(dx in x's type, dw of weight_dtype, db of bias_dtype); a type of None: not wanted."""
+    _require_cuda(grad_output, x)
+    _same_device("layer_norm", x, grad_output, weight)
+    code = _dtype_code(x, "layer_norm")
+    w, _, _ = _norm_vectors(x, weight, None)
+    m = _rows_of(x)
+    R, D = m.shape
+    g = grad_output.detach().to(x.dtype).reshape(R, D).contiguous()
+    # the sums leave the kernel in float32 or in x's type; any other type is rounded once more
+    wanted = [t for t in (weight_dtype, bias_dtype) if t is not None]
+    sum_dt = x.dtype if wanted and all(t == x.dtype for t in wanted) else torch.float32
+    if w is not None and w.dtype != sum_dt:
+        w = w.to(sum_dt)
+    L = _lib.lib()
+    with torch.cuda.device(x.device):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        mk = lambda dt: torch.empty(D, dtype=sum_dt, device=x.device) if dt is not None else None
+        dw, db = mk(weight_dtype), mk(bias_dtype)
+        d = _lib.NormDesc(code, _DTYPE_CODE[sum_dt], float(eps), R, D, _row_stride(m))
+        ws = None
+        if wanted:
+            nbytes = L.rexsc_layer_norm_backward_workspace_bytes(ctypes.byref(d))
+            if nbytes == ctypes.c_size_t(-1).value:
+                _lib.check(-1, "rexsc_layer_norm_backward (planning)")
+            ws = _workspace(nbytes, x.device)
+        rc = L.rexsc_layer_norm_backward(ctypes.byref(d), _ptr(g), _ptr(m), _ptr(w), _ptr(mean), _ptr(rstd), _ptr(dx),
+                                         _ptr(dw), _ptr(db), _ptr(ws), ws.numel() if ws is not None else 0, _stream())
+        _lib.check(rc, "rexsc_layer_norm_backward")
+    if dw is not None and dw.dtype != weight_dtype:
+        dw = dw.to(weight_dtype)
+    if db is not None and db.dtype != bias_dtype:
+        db = db.to(bias_dtype)
+    return dx, dw, db

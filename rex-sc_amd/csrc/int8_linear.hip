@@ -1,0 +1,470 @@
+// 8-bit linear layer: rows to int8 with a scale each, the integer product with token and channel scales, and the
+// straight-through gradients.
+//
+//   q[r][k] = nearest(127 x[r][k] / a_r), s_r = a_r / 127, a_r = max_k |x[r][k]|
+//   y[m][n] = (sum_k qa[m][k] qb[n][k]) sa[m] sb[n] + bias[n]            sum exact in int32
+//   dx[m][k] = sum_n (g[m][n] sb[n]) qb[n][k]     dw[n][k] = sum_m (g[m][n] sa[m]) qa[m][k]     db[n] = sum_m g[m][n]
+//
+// The gradients run on the bfloat16 matrix instructions: an int8 value is exact in bfloat16, and the float32 factor
+// g * s is split into bfloat16 pieces whose sum it is (8 bits each: three pieces hold all 24 bits and serve float32
+// results, two hold 16 and serve 16-bit results, whose own rounding is far coarser), so nothing but the float32
+// accumulation is rounded.  Pieces and transposed operands are laid out in the workspace first, which makes both
+// gradients the same product of two row-major operands as the forward pass.
+#include "lowp.h"
+#include "profile.h"
+
+namespace rexsc {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int MAX_K = 131071; // 128 * 128 * K < 2^31
+
+// ---- rows to 8 bits ------------------------------------------------------------------------------
+constexpr int Q_THREADS = 256;
+constexpr float SMALL = 7.888609052210118e-31f; // 2^-100: below it 127 / a could overflow
+constexpr float LIFT = 1.2676506002282294e30f;  // 2^100
+
+// The integer nearest to 127 x / a, ties to even, exactly.  x * inv with inv = fl(127 / a) is off by less than 1e-4;
+// where that could decide, 127 x is compared with (the half-way point) * a in 64 bits, where both are exact.
+__device__ __forceinline__ int nearest127(float x, float a, float inv)
+{
+    const float t = x * inv, r = rintf(t), d = t - r;
+    int q = (int)r;
+    if (fabsf(fabsf(d) - 0.5f) < 1e-3f) {
+        const int o = d >= 0.f ? q + 1 : q - 1;
+        const double v = 127.0 * (double)x, half = 0.5 * (double)(q + o) * (double)a;
+        const int lo = q < o ? q : o, hi = q < o ? o : q;
+        q = v < half ? lo : v > half ? hi : (lo & 1) ? hi : lo;
+    }
+    return q;
+}
+
+struct RowScale { float a, inv, lift, scale; };
+__device__ __forceinline__ RowScale row_scale(unsigned top)
+{
+    RowScale r;
+    const float a = __uint_as_float(top);
+    if (top >= 0x7f800000u) { r.a = 1.f; r.inv = 0.f; r.lift = 0.f; r.scale = __uint_as_float(0x7fc00000u); return r; }
+    r.scale = a / 127.f;
+    r.lift = a < SMALL ? LIFT : 1.f; // exact: both powers of two
+    r.a = a * r.lift;
+    r.inv = a > 0.f ? 127.f / r.a : 0.f;
+    return r;
+}
+__device__ __forceinline__ int quant(float x, const RowScale &r)
+{   // a row with a NaN or an infinity: all zeros
+    return r.lift == 0.f || r.inv == 0.f ? 0 : nearest127(x * r.lift, r.a, r.inv);
+}
+
+template <typename T>
+__global__ __launch_bounds__(Q_THREADS) void quantize_rows_kernel(const T *x, size_t x_stride, int cols, int8_t *q,
+                                                                  size_t q_stride, float *scale)
+{
+    __shared__ unsigned lds[Q_THREADS / 64];
+    const T *src = x + (size_t)blockIdx.x * x_stride;
+    int8_t *dst = q + (size_t)blockIdx.x * q_stride;
+    unsigned top = 0;
+    for (int c = threadIdx.x; c < cols; c += Q_THREADS) top = max(top, mag_bits((float)src[c]));
+    top = wave_max(top);
+    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < Q_THREADS / 64; i++) top = max(top, lds[i]);
+    const RowScale rs = row_scale(top);
+    for (size_t c = threadIdx.x; c < q_stride; c += Q_THREADS) dst[c] = c < (size_t)cols ? (int8_t)quant((float)src[c], rs) : 0;
+    if (threadIdx.x == 0) scale[blockIdx.x] = rs.scale;
+}
+
+// ---- the product of two row-major operands --------------------------------------------------------
+// c[m][n] = sum_k a[m][k] b[n][k], rows as bytes: 16 bytes are one lane's share of a matrix instruction's operand in
+// either type (16 int8 or 8 bfloat16).
+struct TileArgs {
+    const char *a, *b;
+    size_t a_stride, b_stride;      // bytes
+    int M, N;
+    int kbytes;                     // length of a reduction row; the operands are readable to the next multiple of 16
+    int pieces;                     // a's row holds this many pieces, each multiplied by the same b row
+    size_t piece_stride;            // bytes
+    const float *a_scale, *b_scale; // NULL: 1 (the gradients)
+    const void *bias;
+    int bias_dtype;
+    void *y;
+    size_t y_stride;                // elements
+};
+
+struct OpI8 { typedef i32x4 acc; typedef int elem; };
+struct OpBF16 { typedef f32x4 acc; typedef float elem; };
+__device__ __forceinline__ i32x4 mma(OpI8, i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(OpBF16, i32x4 a, i32x4 b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Bytes of a 16-byte chunk at offset k that lie before `end`; the rest become 0.
+__device__ __forceinline__ i32x4 keep_before(i32x4 v, int k, int end)
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int n = end - k - 4 * i;
+        v[i] = n >= 4 ? v[i] : n <= 0 ? 0 : v[i] & (int)((1u << (8 * n)) - 1u);
+    }
+    return v;
+}
+
+constexpr int TILE = 64, KSTEP = 64, LDS_ROW = KSTEP + 16;
+
+template <typename Op, typename T>
+__global__ __launch_bounds__(256) void tile_kernel(TileArgs p)
+{
+    __shared__ __attribute__((aligned(16))) char la[TILE * LDS_ROW], lb[TILE * LDS_ROW];
+    const int tiles_n = (p.N + TILE - 1) / TILE;
+    const int m0 = (int)(blockIdx.x / tiles_n) * TILE, n0 = (int)(blockIdx.x % tiles_n) * TILE;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int wm = (wave / 2) * 32, wn = (wave % 2) * 32;
+    const int lr = threadIdx.x / 4, lc = (threadIdx.x % 4) * 16; // this thread's chunk of a tile
+    typename Op::acc acc[2][2] = {};
+    for (int piece = 0; piece < p.pieces; piece++)
+        for (int k = 0; k < p.kbytes; k += KSTEP) {
+            i32x4 va = {0, 0, 0, 0}, vb = {0, 0, 0, 0};
+            if (k + lc < p.kbytes) {
+                if (m0 + lr < p.M)
+                    va = keep_before(*(const i32x4 *)(p.a + (size_t)(m0 + lr) * p.a_stride + piece * p.piece_stride + k + lc),
+                                     k + lc, p.kbytes);
+                if (n0 + lr < p.N)
+                    vb = keep_before(*(const i32x4 *)(p.b + (size_t)(n0 + lr) * p.b_stride + k + lc), k + lc, p.kbytes);
+            }
+            __syncthreads();
+            *(i32x4 *)(la + lr * LDS_ROW + lc) = va;
+            *(i32x4 *)(lb + lr * LDS_ROW + lc) = vb;
+            __syncthreads();
+            i32x4 fa[2], fb[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                fa[i] = *(const i32x4 *)(la + (wm + i * 16 + lane % 16) * LDS_ROW + lane / 16 * 16);
+                fb[i] = *(const i32x4 *)(lb + (wn + i * 16 + lane % 16) * LDS_ROW + lane / 16 * 16);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) acc[i][j] = mma(Op{}, fb[j], fa[i], acc[i][j]);
+        }
+    // b is the first operand: a lane holds four neighbouring columns n of one row m
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int m = m0 + wm + i * 16 + lane % 16;
+        if (m >= p.M) continue;
+        const float sa = p.a_scale ? p.a_scale[m] : 1.f;
+        T *row = (T *)p.y + (size_t)m * p.y_stride;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int n = n0 + wn + j * 16 + lane / 16 * 4 + e;
+                if (n >= p.N) continue;
+                float v = (float)acc[i][j][e] * sa;
+                if (p.b_scale) v *= p.b_scale[n];
+                if (p.bias) v += load_any(p.bias, p.bias_dtype, n);
+                row[n] = (T)v;
+            }
+    }
+}
+
+// ---- operands of the gradients ---------------------------------------------------------------------
+// v = sum of `pieces` bfloat16 values.  Each but the last keeps the leading 8 bits (truncated, so that nothing
+// overflows), the last is rounded.  Of an infinity or NaN the first piece is all.
+__device__ __forceinline__ void split(float v, int pieces, bf16_t (&out)[3])
+{
+    const bool finite = mag_bits(v) < 0x7f800000u;
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        if (i >= pieces) break;
+        if (!finite) { out[i] = i == 0 ? (bf16_t)v : (bf16_t)0.f; continue; }
+        if (i + 1 == pieces) { out[i] = (bf16_t)v; break; }
+        const float head = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+        out[i] = (bf16_t)head;
+        v -= head;
+    }
+}
+
+// g [rows][cols] -> out [rows][pieces][ld], elements times scale[column], columns from cols to ld zero.
+template <typename T>
+__global__ __launch_bounds__(256) void split_rows_kernel(const T *g, const float *scale, int cols, int ld, int pieces, bf16_t *out)
+{
+    const size_t row = blockIdx.x;
+    for (int c = threadIdx.x; c < ld; c += 256) {
+        bf16_t q[3];
+        split(c < cols ? (float)g[row * cols + c] * scale[c] : 0.f, pieces, q);
+        for (int i = 0; i < pieces; i++) out[(row * pieces + i) * ld + c] = q[i];
+    }
+}
+
+// g [rows][cols] -> out [cols][pieces][ld], elements times scale[row], positions from rows to ld zero; and the sums of
+// g's columns over this block's 64 rows to part[row block][cols].  out NULL: only the sums.
+template <typename T>
+__global__ __launch_bounds__(256) void split_transposed_kernel(const T *g, const float *scale, int rows, int cols, int ld,
+                                                               int pieces, bf16_t *out, float *part)
+{
+    __shared__ float tile[64][65];
+    const int row_blocks = ld / 64;
+    const int r0 = (int)(blockIdx.x % row_blocks) * 64, c0 = (int)(blockIdx.x / row_blocks) * 64;
+    const int tx = threadIdx.x % 64, ty = threadIdx.x / 64;
+    for (int i = ty; i < 64; i += 4) {
+        const int r = r0 + i, c = c0 + tx;
+        tile[i][tx] = r < rows && c < cols ? (float)g[(size_t)r * cols + c] : 0.f;
+    }
+    __syncthreads();
+    if (part && ty == 0 && c0 + tx < cols) {
+        float s = 0.f;
+        for (int i = 0; i < 64; i++) s += tile[i][tx];
+        part[(size_t)(r0 / 64) * cols + c0 + tx] = s;
+    }
+    if (!out) return;
+    const float sc = r0 + tx < rows ? scale[r0 + tx] : 0.f;
+    for (int i = ty; i < 64; i += 4) {
+        if (c0 + i >= cols) break;
+        bf16_t q[3];
+        split(r0 + tx < rows ? tile[tx][i] * sc : 0.f, pieces, q);
+        for (int j = 0; j < pieces; j++) out[((size_t)(c0 + i) * pieces + j) * ld + r0 + tx] = q[j];
+    }
+}
+
+// q [rows][cols] int8 -> out [cols][ld] bfloat16, positions from rows to ld zero.
+__global__ __launch_bounds__(256) void transpose_i8_kernel(const int8_t *q, size_t stride, int rows, int cols, int ld, bf16_t *out)
+{
+    __shared__ int8_t tile[64][68];
+    const int row_blocks = ld / 64;
+    const int r0 = (int)(blockIdx.x % row_blocks) * 64, c0 = (int)(blockIdx.x / row_blocks) * 64;
+    const int tx = threadIdx.x % 64, ty = threadIdx.x / 64;
+    for (int i = ty; i < 64; i += 4) {
+        const int r = r0 + i, c = c0 + tx;
+        tile[i][tx] = r < rows && c < cols ? q[(size_t)r * stride + c] : (int8_t)0;
+    }
+    __syncthreads();
+    for (int i = ty; i < 64; i += 4) {
+        if (c0 + i >= cols) break;
+        out[(size_t)(c0 + i) * ld + r0 + tx] = (bf16_t)(float)tile[tx][i];
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+int check_int8(const rexsc_int8_desc *d)
+{
+    REXSC_CHECK_DESC(d, rexsc_int8_desc);
+    REXSC_CHECK_ARG(d->M >= 0 && d->N >= 0, "int8 linear: M %d, N %d", d->M, d->N);
+    REXSC_CHECK_ARG(d->K >= 1 && d->K <= MAX_K, "int8 linear: K must be 1..%d, so that the int32 sum cannot overflow (got %d)",
+                    MAX_K, d->K);
+    REXSC_CHECK_ARG(dtype_ok(d->dtype) && dtype_ok(d->bias_dtype) && dtype_ok(d->weight_dtype),
+                    "int8 linear: dtypes %d, %d, %d: each must be float32, float16 or bfloat16", d->dtype, d->bias_dtype,
+                    d->weight_dtype);
+    REXSC_CHECK_ARG(d->reserved == 0, "int8 linear: reserved field is %d, not 0", d->reserved);
+    return REXSC_OK;
+}
+
+int check_rows8(const char *what, const void *q, int64_t stride, int K)
+{
+    REXSC_CHECK_ARG(q != nullptr, "null pointer");
+    REXSC_CHECK_ARG((uintptr_t)q % 16 == 0 && stride % 16 == 0 && stride >= K,
+                    "int8 linear: the %s' int8 rows must be 16-byte aligned at a distance that is a multiple of 16 and at least "
+                    "K = %d (distance %lld)", what, K, (long long)stride);
+    return REXSC_OK;
+}
+
+inline int64_t pad64(int64_t n) { return (n + 63) / 64 * 64; }
+inline int pieces_of(int dtype) { return dtype == REXSC_F32 ? 3 : 2; }
+
+struct Space { size_t tokens, scales, pieces, transposed, part, total; };
+
+Space space(const rexsc_int8_desc *d, int what)
+{
+    Space s{};
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t o = at; at = align_up(at + bytes, 256); return o; };
+    const size_t M = d->M, N = d->N, K = d->K;
+    if (what == REXSC_INT8_LINEAR) {
+        s.tokens = take(M * align_up(K, 128));
+        s.scales = take(M * 4);
+    } else if (what == REXSC_INT8_GRAD_INPUT) {
+        const size_t ld = pad64(N);
+        s.pieces = take(M * ld * pieces_of(d->dtype) * 2);
+        s.transposed = take(K * ld * 2);
+    } else if (what == REXSC_INT8_GRAD_WEIGHT) {
+        const size_t ld = pad64(M);
+        s.pieces = take(N * ld * pieces_of(d->weight_dtype) * 2);
+        s.transposed = take(K * ld * 2);
+        s.part = take(ld / 64 * N * 4);
+    }
+    s.total = at;
+    return s;
+}
+
+int check_space(const Space &s, const void *workspace, size_t bytes)
+{
+    if (s.total && (!workspace || bytes < s.total)) {
+        set_error("int8 linear: workspace of %zu bytes needed, %zu given", s.total, workspace ? bytes : (size_t)0);
+        return REXSC_ERR_WORKSPACE;
+    }
+    REXSC_CHECK_ARG((uintptr_t)workspace % 16 == 0, "int8 linear: the workspace must be 16-byte aligned");
+    return REXSC_OK;
+}
+
+template <typename Op>
+int launch_tiles(const TileArgs &p, int out_dtype, const char *name, hipStream_t stream)
+{
+    const int64_t tiles = (int64_t)((p.M + TILE - 1) / TILE) * ((p.N + TILE - 1) / TILE);
+    REXSC_CHECK_ARG(tiles < (1ll << 31), "int8 linear: result of %d x %d is too large", p.M, p.N);
+    ProfScope prof(name, 2.0 * p.M * p.N * p.kbytes * p.pieces, stream);
+    REXSC_DTYPE_SWITCH(out_dtype, hipLaunchKernelGGL((tile_kernel<Op, T>), dim3((unsigned)tiles), dim3(256), 0, stream, p));
+    REXSC_CHECK_HIP(hipGetLastError());
+    return REXSC_OK;
+}
+
+int product(const rexsc_int8_desc *d, const int8_t *a, int64_t a_stride, const float *a_scale, const int8_t *b,
+            const float *b_scale, const void *bias, void *y, hipStream_t stream)
+{
+    const TileArgs p{(const char *)a, (const char *)b, (size_t)a_stride, (size_t)d->b_stride, d->M, d->N, d->K, 1, 0,
+                     a_scale, b_scale, bias, d->bias_dtype, y, (size_t)d->N};
+    return launch_tiles<OpI8>(p, d->dtype, "int8_product", stream);
+}
+
+int launch_quantize(const void *x, int dtype, size_t rows, size_t cols, size_t x_stride, int8_t *q, size_t q_stride,
+                    float *scale, hipStream_t stream)
+{
+    ProfScope prof("quantize_rows", (double)rows * cols * (dtype_size(dtype) + 1), stream);
+    REXSC_DTYPE_SWITCH(dtype, hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3((unsigned)rows), dim3(Q_THREADS), 0, stream,
+                                                 (const T *)x, x_stride, (int)cols, q, q_stride, scale));
+    REXSC_CHECK_HIP(hipGetLastError());
+    return REXSC_OK;
+}
+
+} // namespace
+} // namespace rexsc
+
+using namespace rexsc;
+
+extern "C" int rexsc_quantize_rows(const void *x, int dtype, size_t rows, size_t cols, size_t x_stride, int8_t *q,
+                                   size_t q_stride, float *scale, rexsc_stream_t stream)
+{
+    REXSC_CHECK_ARG(dtype_ok(dtype), "quantize_rows: dtype %d is not one of float32, float16, bfloat16", dtype);
+    REXSC_CHECK_ARG(cols >= 1 && cols < (1u << 30) && rows < (1ull << 31), "quantize_rows: %zu rows of %zu elements", rows, cols);
+    if (rows == 0) return REXSC_OK;
+    REXSC_CHECK_ARG(x && q && scale, "null pointer");
+    REXSC_CHECK_ARG((uintptr_t)x % dtype_size(dtype) == 0, "quantize_rows: x is not aligned to its element");
+    REXSC_CHECK_ARG((uintptr_t)q % 16 == 0 && q_stride % 16 == 0 && q_stride >= cols,
+                    "quantize_rows: the int8 rows must be 16-byte aligned at a distance that is a multiple of 16 and at least "
+                    "%zu (distance %zu)", cols, q_stride);
+    return launch_quantize(x, dtype, rows, cols, x_stride, q, q_stride, scale, (hipStream_t)stream);
+}
+
+extern "C" size_t rexsc_int8_workspace_bytes(const rexsc_int8_desc *d, int what)
+{
+    if (check_int8(d)) return (size_t)-1;
+    if (what < REXSC_INT8_PRODUCT || what > REXSC_INT8_GRAD_WEIGHT) {
+        set_error("int8 linear: no call has the number %d", what);
+        return (size_t)-1;
+    }
+    return space(d, what).total;
+}
+
+extern "C" int rexsc_int8_product(const rexsc_int8_desc *d, const int8_t *a, const float *a_scale, const int8_t *b,
+                                  const float *b_scale, const void *bias, void *y, void *workspace, size_t workspace_bytes,
+                                  rexsc_stream_t stream)
+{
+    if (int rc = check_int8(d)) return rc;
+    if (d->M == 0 || d->N == 0) return REXSC_OK;
+    if (int rc = check_rows8("tokens", a, d->a_stride, d->K)) return rc;
+    if (int rc = check_rows8("channels", b, d->b_stride, d->K)) return rc;
+    REXSC_CHECK_ARG(a_scale && b_scale && y, "null pointer");
+    if (int rc = check_space(space(d, REXSC_INT8_PRODUCT), workspace, workspace_bytes)) return rc;
+    return product(d, a, d->a_stride, a_scale, b, b_scale, bias, y, (hipStream_t)stream);
+}
+
+extern "C" int rexsc_int8_linear(const rexsc_int8_desc *d, const void *x, const int8_t *b, const float *b_scale,
+                                 const void *bias, void *y, void *workspace, size_t workspace_bytes, rexsc_stream_t stream_)
+{
+    hipStream_t stream = (hipStream_t)stream_;
+    if (int rc = check_int8(d)) return rc;
+    if (d->M == 0 || d->N == 0) return REXSC_OK;
+    if (int rc = check_rows8("channels", b, d->b_stride, d->K)) return rc;
+    REXSC_CHECK_ARG(x && b_scale && y, "null pointer");
+    REXSC_CHECK_ARG((uintptr_t)x % dtype_size(d->dtype) == 0 && (d->x_stride >= d->K || d->M == 1),
+                    "int8 linear: x is not aligned to its element, or its rows overlap (distance %lld)", (long long)d->x_stride);
+    const Space s = space(d, REXSC_INT8_LINEAR);
+    if (int rc = check_space(s, workspace, workspace_bytes)) return rc;
+    int8_t *q = (int8_t *)workspace + s.tokens;
+    float *scale = (float *)((char *)workspace + s.scales);
+    const size_t stride = align_up(d->K, 128);
+    if (int rc = launch_quantize(x, d->dtype, d->M, d->K, d->x_stride, q, stride, scale, stream)) return rc;
+    return product(d, q, (int64_t)stride, scale, b, b_scale, bias, y, stream);
+}
+
+extern "C" int rexsc_int8_grad_input(const rexsc_int8_desc *d, const void *g, const int8_t *b, const float *b_scale, void *dx,
+                                     void *workspace, size_t workspace_bytes, rexsc_stream_t stream_)
+{
+    hipStream_t stream = (hipStream_t)stream_;
+    if (int rc = check_int8(d)) return rc;
+    if (d->M == 0) return REXSC_OK;
+    REXSC_CHECK_ARG(d->N >= 1, "int8 linear: a gradient needs at least one output channel");
+    if (int rc = check_rows8("channels", b, d->b_stride, d->K)) return rc;
+    REXSC_CHECK_ARG(g && b_scale && dx, "null pointer");
+    const Space s = space(d, REXSC_INT8_GRAD_INPUT);
+    if (int rc = check_space(s, workspace, workspace_bytes)) return rc;
+    bf16_t *pieces = (bf16_t *)((char *)workspace + s.pieces), *bt = (bf16_t *)((char *)workspace + s.transposed);
+    const int P = pieces_of(d->dtype), ld = (int)pad64(d->N);
+    {
+        ProfScope prof("int8_grad_operands", (double)d->M * d->N * (dtype_size(d->dtype) + 2.0 * P), stream);
+        REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL(split_rows_kernel<T>, dim3((unsigned)d->M), dim3(256), 0, stream,
+                                                        (const T *)g, b_scale, d->N, ld, P, pieces));
+        REXSC_CHECK_HIP(hipGetLastError());
+    }
+    {
+        ProfScope prof("int8_grad_operands", 3.0 * d->N * d->K, stream);
+        hipLaunchKernelGGL(transpose_i8_kernel, dim3((unsigned)((ld / 64) * ((d->K + 63) / 64))), dim3(256), 0, stream, b,
+                           (size_t)d->b_stride, d->N, d->K, ld, bt);
+        REXSC_CHECK_HIP(hipGetLastError());
+    }
+    const TileArgs p{(const char *)pieces, (const char *)bt, (size_t)ld * P * 2, (size_t)ld * 2, d->M, d->K, ld * 2, P,
+                     (size_t)ld * 2, nullptr, nullptr, nullptr, REXSC_F32, dx, (size_t)d->K};
+    return launch_tiles<OpBF16>(p, d->dtype, "int8_grad_input", stream);
+}
+
+extern "C" int rexsc_int8_grad_weight(const rexsc_int8_desc *d, const void *g, const int8_t *a, const float *a_scale, void *dw,
+                                      void *db, void *workspace, size_t workspace_bytes, rexsc_stream_t stream_)
+{
+    hipStream_t stream = (hipStream_t)stream_;
+    if (int rc = check_int8(d)) return rc;
+    if (d->N == 0 || (!dw && !db)) return REXSC_OK;
+    const Space s = space(d, REXSC_INT8_GRAD_WEIGHT);
+    if (d->M > 0) {
+        if (dw)
+            if (int rc = check_rows8("tokens", a, d->a_stride, d->K)) return rc;
+        REXSC_CHECK_ARG(g && (a_scale || !dw), "null pointer");
+        if (int rc = check_space(s, workspace, workspace_bytes)) return rc;
+    }
+    bf16_t *pieces = (bf16_t *)((char *)workspace + s.pieces), *at = (bf16_t *)((char *)workspace + s.transposed);
+    float *part = (float *)((char *)workspace + s.part);
+    const int P = pieces_of(d->weight_dtype), ld = (int)pad64(d->M);
+    if (d->M > 0) {
+        ProfScope prof("int8_grad_operands", (double)d->M * d->N * (dtype_size(d->dtype) + (dw ? 2.0 * P : 0)), stream);
+        REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL(split_transposed_kernel<T>,
+                                                        dim3((unsigned)((ld / 64) * ((d->N + 63) / 64))), dim3(256), 0, stream,
+                                                        (const T *)g, a_scale, d->M, d->N, ld, P, dw ? pieces : nullptr,
+                                                        db ? part : nullptr));
+        REXSC_CHECK_HIP(hipGetLastError());
+    }
+    if (db)
+        if (int rc = launch_column_sums(part, (size_t)ld / 64, d->N, d->N, db, d->bias_dtype, stream)) return rc;
+    if (!dw) return REXSC_OK;
+    if (d->M > 0) {
+        ProfScope prof("int8_grad_operands", 3.0 * d->M * d->K, stream);
+        hipLaunchKernelGGL(transpose_i8_kernel, dim3((unsigned)((ld / 64) * ((d->K + 63) / 64))), dim3(256), 0, stream, a,
+                           (size_t)d->a_stride, d->M, d->K, ld, at);
+        REXSC_CHECK_HIP(hipGetLastError());
+    }
+    // without tokens the reduction is empty and the kernel writes zeros
+    const TileArgs p{(const char *)pieces, (const char *)at, (size_t)ld * P * 2, (size_t)ld * 2, d->N, d->K, ld * 2, P,
+                     (size_t)ld * 2, nullptr, nullptr, nullptr, REXSC_F32, dw, (size_t)d->K};
+    return launch_tiles<OpBF16>(p, d->weight_dtype, "int8_grad_weight", stream);
+}

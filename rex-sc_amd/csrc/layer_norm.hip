@@ -1,0 +1,503 @@
+// Layer norm, forward and backward, and the column sums of partial weight gradients.
+//
+//   y  = (x - mu) r w + b,     mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps)
+//   dx = r (gw - mean(gw) - h mean(gw h)),  gw = g w, h = (x - mu) r;   dw = sum_rows g h;   db = sum_rows g
+//
+// Bound by memory: forward reads x and writes y, backward reads x and g and writes dx, each once.  A row lives in the
+// registers of TPR threads (a wave, or a block of 256, 512 or 1024), at most 16 elements per thread, so the variance
+// is taken around the true mean without a second read.  Blocks are persistent over rows: w and b (forward), w and the
+// two gradient sums (backward) stay in registers from row to row, since re-reading float32 w and b from L2 for every
+// 16-bit row would move more bytes than the row itself.  The next row is loaded before the current one is reduced.
+// Rows longer than 16384 elements take the streaming kernels, which read the row again for each pass (from L2).
+#include "lowp.h"
+#include "profile.h"
+
+namespace rexsc {
+namespace {
+
+constexpr int MAX_EPT = 16;         // elements of a row per thread
+constexpr int STREAM_THREADS = 1024;
+
+struct NormParams {
+    const void *x, *w, *b, *g;
+    void *y, *dx;
+    float *mean, *rstd, *part;      // part: [blocks][2][cols]
+    size_t rows, x_stride;
+    int cols, w_dtype;
+    float eps;
+};
+
+// Sum over the TPR threads of a row, the result in all of them.  `slot` alternates between calls (0, 1), so that one
+// barrier per call is enough.
+template <int TPR, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float (*lds)[TPR / 64 + 1][N], int slot)
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = wave_sum(v[i]);
+    if constexpr (TPR > 64) {
+        const int wave = threadIdx.x / 64;
+        if (threadIdx.x % 64 == 0)
+#pragma unroll
+            for (int i = 0; i < N; i++) lds[slot][wave][i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float s = 0.f;
+#pragma unroll
+            for (int k = 0; k < TPR / 64; k++) s += lds[slot][k][i];
+            v[i] = s;
+        }
+    }
+}
+
+template <typename T, int V, int NV, int TPR>
+__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_forward_kernel(NormParams p)
+{
+    constexpr int RPB = TPR == 64 ? 4 : 1;
+    typedef typename VecOf<T, V>::type vec;
+    __shared__ float lds[2][TPR / 64 + 1][1];
+    const int tid = TPR == 64 ? threadIdx.x % 64 : threadIdx.x;
+    const int sub = TPR == 64 ? threadIdx.x / 64 : 0;
+    const float inv = 1.0f / (float)p.cols;
+    float w[NV][V], b[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const int c = (i * TPR + tid) * V + j;
+            w[i][j] = p.w && c < p.cols ? load_any(p.w, p.w_dtype, c) : 1.f;
+            b[i][j] = p.b && c < p.cols ? load_any(p.b, p.w_dtype, c) : 0.f;
+        }
+    const size_t step = (size_t)gridDim.x * RPB;
+    size_t row = (size_t)blockIdx.x * RPB + sub;
+    vec cur[NV];
+    auto fetch = [&](size_t r) {
+        const T *src = (const T *)p.x + r * p.x_stride;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * TPR + tid) * V;
+            cur[i] = c < p.cols ? *(const vec *)(src + c) : vec{};
+        }
+    };
+    if (row < p.rows) fetch(row);
+    for (; row < p.rows; row += step) {
+        float x[NV][V];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            if constexpr (V == 1) x[i][0] = (float)cur[i];
+            else
+#pragma unroll
+                for (int j = 0; j < V; j++) x[i][j] = (float)cur[i][j];
+        }
+        if (row + step < p.rows) fetch(row + step);
+        float s[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int j = 0; j < V; j++) s[0] += x[i][j];
+        row_sum<TPR, 1>(s, lds, 0);
+        const float mu = s[0] * inv;
+        float q[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                x[i][j] = (i * TPR + tid) * V < p.cols ? x[i][j] - mu : 0.f;
+                q[0] = fmaf(x[i][j], x[i][j], q[0]);
+            }
+        row_sum<TPR, 1>(q, lds, 1);
+        const float r = 1.0f / sqrtf(fmaf(q[0], inv, p.eps));
+        T *dst = (T *)p.y + row * (size_t)p.cols;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * TPR + tid) * V;
+            if (c < p.cols) {
+                float o[V];
+#pragma unroll
+                for (int j = 0; j < V; j++) o[j] = fmaf(x[i][j] * r, w[i][j], b[i][j]);
+                store_vec<V>(dst + c, o);
+            }
+        }
+        if (tid == 0 && p.mean) {
+            p.mean[row] = mu;
+            p.rstd[row] = r;
+        }
+    }
+}
+
+template <typename T, int V, int NV, int TPR>
+__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_backward_kernel(NormParams p)
+{
+    constexpr int RPB = TPR == 64 ? 4 : 1;
+    typedef typename VecOf<T, V>::type vec;
+    __shared__ float lds[2][TPR / 64 + 1][2];
+    const int tid = TPR == 64 ? threadIdx.x % 64 : threadIdx.x;
+    const int sub = TPR == 64 ? threadIdx.x / 64 : 0;
+    const float inv = 1.0f / (float)p.cols;
+    float w[NV][V], dw[NV][V], db[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const int c = (i * TPR + tid) * V + j;
+            w[i][j] = p.w && c < p.cols ? load_any(p.w, p.w_dtype, c) : 1.f;
+            dw[i][j] = db[i][j] = 0.f;
+        }
+    const size_t step = (size_t)gridDim.x * RPB;
+    size_t row = (size_t)blockIdx.x * RPB + sub;
+    vec cx[NV], cg[NV];
+    auto fetch = [&](size_t r) {
+        const T *sx = (const T *)p.x + r * p.x_stride, *sg = (const T *)p.g + r * (size_t)p.cols;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * TPR + tid) * V;
+            cx[i] = c < p.cols ? *(const vec *)(sx + c) : vec{};
+            cg[i] = c < p.cols ? *(const vec *)(sg + c) : vec{};
+        }
+    };
+    if (row < p.rows) fetch(row);
+    int slot = 0;
+    for (; row < p.rows; row += step) {
+        const float mu = p.mean[row], r = p.rstd[row];
+        float h[NV][V], gw[NV][V], s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                float xv, gv;
+                if constexpr (V == 1) { xv = (float)cx[i]; gv = (float)cg[i]; }
+                else { xv = (float)cx[i][j]; gv = (float)cg[i][j]; }
+                h[i][j] = (i * TPR + tid) * V < p.cols ? (xv - mu) * r : 0.f; // beyond the row: g is 0, h must be finite
+                dw[i][j] = fmaf(gv, h[i][j], dw[i][j]);
+                db[i][j] += gv;
+                gw[i][j] = gv * w[i][j];
+                s[0] += gw[i][j];
+                s[1] = fmaf(gw[i][j], h[i][j], s[1]);
+            }
+        if (row + step < p.rows) fetch(row + step);
+        if (p.dx) {
+            row_sum<TPR, 2>(s, lds, slot);
+            slot ^= 1;
+            const float m0 = s[0] * inv, m1 = s[1] * inv;
+            T *dst = (T *)p.dx + row * (size_t)p.cols;
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const int c = (i * TPR + tid) * V;
+                if (c < p.cols) {
+                    float o[V];
+#pragma unroll
+                    for (int j = 0; j < V; j++) o[j] = r * (gw[i][j] - m0 - h[i][j] * m1);
+                    store_vec<V>(dst + c, o);
+                }
+            }
+        }
+    }
+    if (!p.part) return;
+    float *out = p.part + (size_t)blockIdx.x * 2 * p.cols;
+    if constexpr (TPR == 64) {
+        // the block's four waves hold four sums of the same columns: joined in wave order
+        __shared__ float join[3][2][64 * NV * V];
+        if (sub > 0)
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    join[sub - 1][0][(i * V + j) * 64 + tid] = dw[i][j];
+                    join[sub - 1][1][(i * V + j) * 64 + tid] = db[i][j];
+                }
+        __syncthreads();
+        if (sub > 0) return;
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    dw[i][j] += join[k][0][(i * V + j) * 64 + tid];
+                    db[i][j] += join[k][1][(i * V + j) * 64 + tid];
+                }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * TPR + tid) * V;
+        if (c < p.cols)
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                out[c + j] = dw[i][j];
+                out[p.cols + c + j] = db[i][j];
+            }
+    }
+}
+
+// ---- rows of any length --------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(STREAM_THREADS) void norm_forward_stream_kernel(NormParams p)
+{
+    __shared__ float lds[2][STREAM_THREADS / 64 + 1][1];
+    const float inv = 1.0f / (float)p.cols;
+    for (size_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T *src = (const T *)p.x + row * p.x_stride;
+        float s[1] = {0.f};
+        for (int c = threadIdx.x; c < p.cols; c += STREAM_THREADS) s[0] += (float)src[c];
+        row_sum<STREAM_THREADS, 1>(s, lds, 0);
+        const float mu = s[0] * inv;
+        float q[1] = {0.f};
+        for (int c = threadIdx.x; c < p.cols; c += STREAM_THREADS) {
+            const float d = (float)src[c] - mu;
+            q[0] = fmaf(d, d, q[0]);
+        }
+        row_sum<STREAM_THREADS, 1>(q, lds, 1);
+        const float r = 1.0f / sqrtf(fmaf(q[0], inv, p.eps));
+        T *dst = (T *)p.y + row * (size_t)p.cols;
+        for (int c = threadIdx.x; c < p.cols; c += STREAM_THREADS) {
+            const float w = p.w ? load_any(p.w, p.w_dtype, c) : 1.f, b = p.b ? load_any(p.b, p.w_dtype, c) : 0.f;
+            dst[c] = (T)fmaf(((float)src[c] - mu) * r, w, b);
+        }
+        if (threadIdx.x == 0 && p.mean) {
+            p.mean[row] = mu;
+            p.rstd[row] = r;
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(STREAM_THREADS) void norm_dx_stream_kernel(NormParams p)
+{
+    __shared__ float lds[2][STREAM_THREADS / 64 + 1][2];
+    const float inv = 1.0f / (float)p.cols;
+    int slot = 0;
+    for (size_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T *sx = (const T *)p.x + row * p.x_stride, *sg = (const T *)p.g + row * (size_t)p.cols;
+        const float mu = p.mean[row], r = p.rstd[row];
+        float s[2] = {0.f, 0.f};
+        for (int c = threadIdx.x; c < p.cols; c += STREAM_THREADS) {
+            const float gw = (float)sg[c] * (p.w ? load_any(p.w, p.w_dtype, c) : 1.f);
+            s[0] += gw;
+            s[1] = fmaf(gw, ((float)sx[c] - mu) * r, s[1]);
+        }
+        row_sum<STREAM_THREADS, 2>(s, lds, slot);
+        slot ^= 1;
+        const float m0 = s[0] * inv, m1 = s[1] * inv;
+        T *dst = (T *)p.dx + row * (size_t)p.cols;
+        for (int c = threadIdx.x; c < p.cols; c += STREAM_THREADS) {
+            const float gw = (float)sg[c] * (p.w ? load_any(p.w, p.w_dtype, c) : 1.f);
+            dst[c] = (T)(r * (gw - m0 - ((float)sx[c] - mu) * r * m1));
+        }
+    }
+}
+
+// dw and db of 256 columns over a share of the rows: grid (column blocks, row shares).
+template <typename T>
+__global__ __launch_bounds__(256) void norm_dw_stream_kernel(NormParams p)
+{
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= p.cols) return;
+    float dw = 0.f, db = 0.f;
+    for (size_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
+        const float g = (float)((const T *)p.g)[row * (size_t)p.cols + c];
+        const float x = (float)((const T *)p.x)[row * p.x_stride + c];
+        dw = fmaf(g, (x - p.mean[row]) * p.rstd[row], dw);
+        db += g;
+    }
+    float *out = p.part + (size_t)blockIdx.y * 2 * p.cols;
+    out[c] = dw;
+    out[p.cols + c] = db;
+}
+
+// ---- column sums -----------------------------------------------------------------------------------
+// A block sums 32 columns, its eight row groups in turn over the rows and then joined in order.
+__global__ __launch_bounds__(256) void column_sums_kernel(const float *part, size_t rows, size_t cols, size_t ld, void *out,
+                                                          int out_dtype)
+{
+    __shared__ float lds[8][33];
+    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+    const size_t c = (size_t)blockIdx.x * 32 + tx;
+    float s = 0.f;
+    if (c < cols)
+        for (size_t r = ty; r < rows; r += 8) s += part[r * ld + c];
+    lds[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < cols) {
+#pragma unroll
+        for (int k = 1; k < 8; k++) s += lds[k][tx];
+        store_any(out, out_dtype, c, s);
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+struct NormPlan { int V, NV, TPR, grid; }; // TPR 0: streaming kernels
+
+int check_norm(const rexsc_norm_desc *d)
+{
+    REXSC_CHECK_DESC(d, rexsc_norm_desc);
+    REXSC_CHECK_ARG(dtype_ok(d->dtype), "layer norm: dtype %d is not one of float32, float16, bfloat16", d->dtype);
+    REXSC_CHECK_ARG(d->weight_dtype == REXSC_F32 || d->weight_dtype == d->dtype,
+                    "layer norm: weight and bias must be float32 or of x's type (codes %d, %d)", d->weight_dtype, d->dtype);
+    REXSC_CHECK_ARG(d->rows >= 0 && d->cols >= 1 && d->cols < (1 << 30), "layer norm: %lld rows of %lld elements",
+                    (long long)d->rows, (long long)d->cols);
+    REXSC_CHECK_ARG(d->x_stride >= d->cols || d->rows <= 1, "layer norm: rows of %lld elements at distance %lld",
+                    (long long)d->cols, (long long)d->x_stride);
+    REXSC_CHECK_ARG(d->eps >= 0.f, "layer norm: eps must not be negative (got %g)", (double)d->eps);
+    return REXSC_OK;
+}
+
+// Vectors of 16 bytes where every row starts on one, else single elements; the fewest threads that hold a row at 16
+// elements each.  `per_cu`: blocks' worth of 64-lane waves to put on each of the 256 CUs.
+NormPlan norm_plan(const rexsc_norm_desc *d, bool aligned, int waves_per_cu)
+{
+    NormPlan pl{};
+    const int VMAX = d->dtype == REXSC_F32 ? 4 : 8;
+    pl.V = aligned && d->cols % VMAX == 0 && (d->x_stride % VMAX == 0 || d->rows <= 1) ? VMAX : 1;
+    pl.TPR = d->cols <= 64 * MAX_EPT ? 64 : d->cols <= 256 * MAX_EPT ? 256 : d->cols <= 512 * MAX_EPT ? 512
+           : d->cols <= 1024 * MAX_EPT ? 1024 : 0;
+    const int64_t rpb = pl.TPR == 64 ? 4 : 1;
+    const int threads = pl.TPR == 0 ? STREAM_THREADS : pl.TPR == 64 ? 256 : pl.TPR;
+    const int64_t most = 256 * (int64_t)waves_per_cu * 64 / threads, want = (d->rows + rpb - 1) / rpb;
+    pl.grid = (int)(want < most ? want : most);
+    if (pl.TPR) {
+        const int64_t ept = (d->cols + pl.TPR - 1) / pl.TPR;
+        pl.NV = pl.V == 8 ? (ept <= 8 ? 1 : 2) : pl.V == 4 ? (ept <= 8 ? 2 : 4) : (ept <= 4 ? 4 : 16);
+    }
+    return pl;
+}
+
+template <typename T, int V, int NV>
+void launch_fwd_tpr(const NormPlan &pl, const NormParams &p, hipStream_t s)
+{
+    switch (pl.TPR) {
+    case 64: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 64>), dim3(pl.grid), dim3(256), 0, s, p); break;
+    case 256: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 256>), dim3(pl.grid), dim3(256), 0, s, p); break;
+    case 512: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 512>), dim3(pl.grid), dim3(512), 0, s, p); break;
+    default: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 1024>), dim3(pl.grid), dim3(1024), 0, s, p); break;
+    }
+}
+template <typename T, int V, int NV>
+void launch_bwd_tpr(const NormPlan &pl, const NormParams &p, hipStream_t s)
+{
+    switch (pl.TPR) {
+    case 64: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 64>), dim3(pl.grid), dim3(256), 0, s, p); break;
+    case 256: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 256>), dim3(pl.grid), dim3(256), 0, s, p); break;
+    case 512: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 512>), dim3(pl.grid), dim3(512), 0, s, p); break;
+    default: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 1024>), dim3(pl.grid), dim3(1024), 0, s, p); break;
+    }
+}
+#define NORM_NV(FN)                                                                         \
+    do {                                                                                    \
+        if constexpr (sizeof(T) == 4) {                                                     \
+            if (pl.V == 4 && pl.NV == 2) return FN<T, 4, 2>(pl, p, s);                      \
+            if (pl.V == 4) return FN<T, 4, 4>(pl, p, s);                                    \
+        } else {                                                                            \
+            if (pl.V == 8 && pl.NV == 1) return FN<T, 8, 1>(pl, p, s);                      \
+            if (pl.V == 8) return FN<T, 8, 2>(pl, p, s);                                    \
+        }                                                                                   \
+        if (pl.NV == 4) return FN<T, 1, 4>(pl, p, s);                                       \
+        return FN<T, 1, 16>(pl, p, s);                                                      \
+    } while (0)
+template <typename T> void launch_fwd(const NormPlan &pl, const NormParams &p, hipStream_t s) { NORM_NV(launch_fwd_tpr); }
+template <typename T> void launch_bwd(const NormPlan &pl, const NormParams &p, hipStream_t s) { NORM_NV(launch_bwd_tpr); }
+
+constexpr int FWD_WAVES = 16, BWD_WAVES = 8; // waves per CU of the persistent grids
+
+int bwd_blocks(const rexsc_norm_desc *d)
+{
+    if (d->cols <= 1024 * MAX_EPT) return norm_plan(d, false, BWD_WAVES).grid;
+    const int64_t shares = d->rows < 64 ? d->rows : 64;
+    return (int)shares;
+}
+
+bool aligned16(const void *a, const void *b, const void *c)
+{
+    return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15) == 0;
+}
+
+} // namespace
+
+int launch_column_sums(const float *part, size_t rows, size_t cols, size_t ld, void *out, int out_dtype, hipStream_t stream)
+{
+    ProfScope prof("column_sums", 4.0 * rows * cols, stream);
+    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, stream, part, rows, cols, ld,
+                       out, out_dtype);
+    REXSC_CHECK_HIP(hipGetLastError());
+    return REXSC_OK;
+}
+
+} // namespace rexsc
+
+using namespace rexsc;
+
+extern "C" int rexsc_layer_norm_forward(const rexsc_norm_desc *d, const void *x, const void *weight, const void *bias,
+                                        void *y, float *mean, float *rstd, rexsc_stream_t stream_)
+{
+    hipStream_t stream = (hipStream_t)stream_;
+    if (int rc = check_norm(d)) return rc;
+    if (d->rows == 0) return REXSC_OK;
+    REXSC_CHECK_ARG(x && y, "null pointer");
+    REXSC_CHECK_ARG((mean == nullptr) == (rstd == nullptr), "layer norm: mean and rstd are given together or not at all");
+    const size_t es = dtype_size(d->dtype);
+    REXSC_CHECK_ARG((((uintptr_t)x | (uintptr_t)y) % es) == 0, "layer norm: a tensor is not aligned to its element");
+    const NormPlan pl = norm_plan(d, aligned16(x, y, nullptr), FWD_WAVES);
+    const NormParams p{x, weight, bias, nullptr, y, nullptr, mean, rstd, nullptr, (size_t)d->rows, (size_t)d->x_stride,
+                       (int)d->cols, d->weight_dtype, d->eps};
+    ProfScope prof("layer_norm_forward", 2.0 * es * d->rows * d->cols, stream);
+    if (pl.TPR == 0)
+        REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL(norm_forward_stream_kernel<T>, dim3(pl.grid), dim3(STREAM_THREADS), 0,
+                                                        stream, p));
+    else
+        REXSC_DTYPE_SWITCH(d->dtype, launch_fwd<T>(pl, p, stream));
+    REXSC_CHECK_HIP(hipGetLastError());
+    return REXSC_OK;
+}
+
+extern "C" size_t rexsc_layer_norm_backward_workspace_bytes(const rexsc_norm_desc *d)
+{
+    if (check_norm(d)) return (size_t)-1;
+    return (size_t)bwd_blocks(d) * 2 * (size_t)d->cols * sizeof(float);
+}
+
+extern "C" int rexsc_layer_norm_backward(const rexsc_norm_desc *d, const void *grad_out, const void *x, const void *weight,
+                                         const float *mean, const float *rstd, void *dx, void *dw, void *db,
+                                         void *workspace, size_t workspace_bytes, rexsc_stream_t stream_)
+{
+    hipStream_t stream = (hipStream_t)stream_;
+    if (int rc = check_norm(d)) return rc;
+    const size_t es = dtype_size(d->dtype), cols = (size_t)d->cols;
+    const bool sums = dw || db;
+    if (!dx && !sums) return REXSC_OK;
+    if (d->rows == 0) { // sums over no rows
+        if (dw) if (int rc = launch_column_sums(nullptr, 0, cols, cols, dw, d->weight_dtype, stream)) return rc;
+        if (db) if (int rc = launch_column_sums(nullptr, 0, cols, cols, db, d->weight_dtype, stream)) return rc;
+        return REXSC_OK;
+    }
+    REXSC_CHECK_ARG(grad_out && x && mean && rstd, "null pointer");
+    REXSC_CHECK_ARG((((uintptr_t)x | (uintptr_t)grad_out | (uintptr_t)dx) % es) == 0,
+                    "layer norm: a tensor is not aligned to its element");
+    const size_t need = rexsc_layer_norm_backward_workspace_bytes(d);
+    if (sums && (!workspace || workspace_bytes < need)) {
+        set_error("layer norm: workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+        return REXSC_ERR_WORKSPACE;
+    }
+    const NormPlan pl = norm_plan(d, aligned16(x, grad_out, dx), BWD_WAVES);
+    const NormParams p{x, weight, nullptr, grad_out, nullptr, dx, const_cast<float *>(mean), const_cast<float *>(rstd),
+                       sums ? (float *)workspace : nullptr, (size_t)d->rows, (size_t)d->x_stride, (int)d->cols,
+                       d->weight_dtype, d->eps};
+    const int blocks = bwd_blocks(d);
+    {
+        ProfScope prof("layer_norm_backward", (dx ? 3.0 : 2.0) * es * d->rows * d->cols, stream);
+        if (pl.TPR == 0) {
+            if (dx)
+                REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL(norm_dx_stream_kernel<T>, dim3(pl.grid), dim3(STREAM_THREADS),
+                                                                0, stream, p));
+            if (sums)
+                REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL(norm_dw_stream_kernel<T>,
+                                                                dim3((unsigned)((cols + 255) / 256), blocks), dim3(256), 0,
+                                                                stream, p));
+        } else {
+            REXSC_DTYPE_SWITCH(d->dtype, launch_bwd<T>(pl, p, stream));
+        }
+        REXSC_CHECK_HIP(hipGetLastError());
+    }
+    const float *part = (const float *)workspace;
+    if (dw) if (int rc = launch_column_sums(part, blocks, cols, 2 * cols, dw, d->weight_dtype, stream)) return rc;
+    if (db) if (int rc = launch_column_sums(part + cols, blocks, cols, 2 * cols, db, d->weight_dtype, stream)) return rc;
+    return REXSC_OK;
+}

@@ -696,3 +696,103 @@ def linear_generic(activation, weight, **kwargs):
             result_pos_value.data = mean(pos)
             result_neg_value.data = mean(neg)
     return result_pos_value - result_neg_value
+
+
+# ---- 8-bit linear layer, layer norm --------------------------------------------------------------
+def quantize_rows(x):
+    """Rows of x [..., K] in 8 bits with a scale each: q = nearest(127 x / max|row|), ties to even and decided exactly,
+    scale = max|row| / 127 -> (q int8 of x's shape, scale float32 of x.shape[:-1]).  A row of zeros has scale 0; a row
+    with a NaN or an infinity has scale NaN and zeros, so that what is computed from it is NaN."""
+    return _ops.quantize_rows(x)
+
+
+def matmul_int8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
+    """a [M, K] int8 times b [N, K] int8 transposed, summed exactly in int32, times a_scale[m] * b_scale[n], plus bias
+    -> [M, N] of out_dtype (float32, float16 or bfloat16).  No gradient: linear_int8 is the differentiable form."""
+    return _ops.matmul_int8(a, a_scale, b, b_scale, bias, out_dtype)
+
+
+class Linear_Int8_Grad(torch.autograd.Function):
+    """The 8-bit product forward, straight-through backward (as QuantizeGrad, utils_functional.py:117-123): gradients are
+    those of the product of the dequantised operands, taken with respect to the unquantised ones."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, weight_scale):
+        if weight_scale is None:
+            wq, ws = _ops.quantize_rows(weight)
+        else:
+            wq, ws = weight, weight_scale
+        ctx.types = (weight.dtype if weight_scale is None else None, None if bias is None else bias.dtype)
+        ctx.shape = x.shape
+        if ctx.needs_input_grad[1]:  # the tokens are wanted in 8 bits again by the backward pass
+            xq, xs = _ops.quantize_rows(x.reshape(-1, x.shape[-1]))
+            y = _ops.matmul_int8(xq, xs, wq, ws, bias, x.dtype).view(x.shape[:-1] + (wq.shape[0],))
+            ctx.save_for_backward(wq, ws, xq, xs)
+        else:
+            y = _ops.int8_linear(x, wq, ws, bias)
+            ctx.save_for_backward(wq, ws, None, None)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output):
+        wq, ws, xq, xs = ctx.saved_tensors
+        w_dtype, b_dtype = ctx.types
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = _ops.int8_grad_input(grad_output, wq, ws) if need_x else None
+        dw = db = None
+        if need_w:
+            dw, db = _ops.int8_grad_weight(grad_output, xq, xs, w_dtype, b_dtype if need_b else None)
+        elif need_b:
+            db = grad_output.reshape(-1, grad_output.shape[-1]).sum(0, dtype=torch.float32).to(b_dtype)
+        return dx, dw, db, None
+
+
+def linear_int8(x, weight, bias=None, weight_scale=None):
+    """y = x W^T + bias with both operands in 8 bits: x [..., K] (float32, float16 or bfloat16) is taken to int8 with a
+    scale per row, W is either float [N, K], taken to int8 with a scale per output channel on every call (training), or
+    int8 [N, K] with weight_scale [N], as quantize_rows returns them (serving).  The sum over K <= 131071 is exact; y
+    has x's type.  Gradients pass straight through the quantisation.  Inside an autocast region x is cast to the
+    region's type first, as nn.functional.linear does."""
+    lowp = _autocast_dtype()
+    if lowp is not None and x.is_cuda and x.dtype != lowp:
+        x = x.to(lowp)
+    if (weight_scale is None) != (weight.dtype != torch.int8):
+        raise ValueError("linear_int8: an int8 weight comes with weight_scale, a float one without (got %s%s)"
+                         % (weight.dtype, "" if weight_scale is None else " and a weight_scale"))
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("linear_int8: expected input [..., K] and weight [N, K], got %s and %s"
+                         % (tuple(x.shape), tuple(weight.shape)))
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return Linear_Int8_Grad.apply(x, weight, bias, weight_scale)
+    if weight_scale is None:
+        weight, weight_scale = _ops.quantize_rows(weight)
+    return _ops.int8_linear(x, weight, weight_scale, bias)
+
+
+class Layer_Norm_Grad(torch.autograd.Function):
+    """Layer norm over the last dimension; x, mean and 1 / standard deviation are kept for the backward pass."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _ops.layer_norm_forward(x, weight, bias, eps)
+        ctx.eps = eps
+        ctx.types = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output):
+        x, weight, mean, rstd = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        return _ops.layer_norm_backward(grad_output, x, weight, mean, rstd, ctx.eps, need_x,
+                                        ctx.types[0] if need_w else None, ctx.types[1] if need_b else None) + (None,)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, var the biased variance.  x float32, float16
+    or bfloat16, the result of the same type (also inside an autocast region); arithmetic in float32."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return Layer_Norm_Grad.apply(x, weight, bias, eps)
+    return _ops.layer_norm_forward(x, weight, bias, eps, want_stats=False)[0]

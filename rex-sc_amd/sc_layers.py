@@ -128,3 +128,65 @@ class Linear_Or(nn.Linear):
         input = utils_f.QuantizeGrad.apply(input, self.run_args["prec"])
         weight = utils_f.QuantizeGrad.apply(self.weight, self.run_args["prec"])
         return utils_f.linear_generic_sc(input, weight, **{k: self.run_args[k] for k in keys})
+
+
+class Linear_Int8(nn.Linear):
+    """Linear layer computed in 8 bits: tokens and weights as int8 with a scale per token and per output channel, the sum
+    exact (sc_functional.linear_int8).  Arguments and parameters of nn.Linear; gradients pass straight through the
+    quantisation, so it trains like one.  freeze() turns it into its serving form: the float weight is replaced by the
+    buffers weight_q (int8, rows padded to a multiple of 128 bytes) and weight_scale, and only those are read after."""
+
+    def __init__(self, *kargs, **kwargs):
+        super(Linear_Int8, self).__init__(*kargs, **kwargs)
+        self.register_buffer("weight_q", None)
+        self.register_buffer("weight_scale", None)
+
+    @classmethod
+    def from_linear(cls, linear):
+        """The same parameters in 8-bit form."""
+        out = cls(linear.in_features, linear.out_features, bias=linear.bias is not None, device=linear.weight.device,
+                  dtype=linear.weight.dtype)
+        with torch.no_grad():
+            out.weight.copy_(linear.weight)
+            if linear.bias is not None:
+                out.bias.copy_(linear.bias)
+        return out
+
+    @property
+    def frozen(self):
+        return self.weight_q is not None
+
+    def freeze(self):
+        if not self.frozen:
+            q, scale = utils_f.quantize_rows(self.weight)
+            self.weight_q = q.as_strided((q.shape[0], q.stride(0)), q.stride())  # with the padding: one dense tensor
+            self.weight_scale = scale
+            self.weight = None
+        return self
+
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+        if prefix + "weight_q" in state_dict and not self.frozen:  # a frozen layer's state into one that is not
+            q, s = state_dict[prefix + "weight_q"], state_dict[prefix + "weight_scale"]
+            dev = self.weight.device
+            self.weight_q, self.weight_scale = torch.empty_like(q, device=dev), torch.empty_like(s, device=dev)
+            self.weight = None
+        return super(Linear_Int8, self)._load_from_state_dict(state_dict, prefix, *args, **kwargs)
+
+    def forward(self, input):
+        if self.frozen:
+            return utils_f.linear_int8(input, self.weight_q[:, :self.in_features], self.bias, self.weight_scale)
+        return utils_f.linear_int8(input, self.weight, self.bias)
+
+
+class LayerNorm(nn.LayerNorm):
+    """nn.LayerNorm on the HIP kernels (sc_functional.layer_norm): the same arguments and parameters.  The result has
+    the input's type, also inside an autocast region."""
+
+    def forward(self, input):
+        n = len(self.normalized_shape)
+        if tuple(input.shape[input.dim() - n:]) != tuple(self.normalized_shape):
+            raise RuntimeError("LayerNorm: expected input of shape [..., %s], got %s"
+                               % (", ".join(map(str, self.normalized_shape)), tuple(input.shape)))
+        flat = lambda t: None if t is None else t.reshape(-1)
+        x = input if n == 1 else input.flatten(input.dim() - n)
+        return utils_f.layer_norm(x, flat(self.weight), flat(self.bias), self.eps).view(input.shape)

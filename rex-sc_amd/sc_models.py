@@ -4,12 +4,15 @@ TinyConvSC   conv3x3 3->32->32, maxpool2, ->64->64, maxpool2, fc 4096->10 (float
 ResNet18SC   topology of the reference's resnet_sc.py (:48-99 BasicBlock, :158-260 ResNet):
              float 7x7 stem + BatchNorm(eps 1e-3) + Hardtanh(0,1) + AvgPool(3,2,1), BasicBlocks whose
              3x3 and 1x1 convs are SC layers, Hardtanh(0,1) activations, float fc; Kaiming init.
+
+classifier="int8" gives either network a head in 8 bits in place of the float fc: the features normalised per image
+(LayerNorm), then Linear_Int8.
 """
 import torch
 import torch.nn as nn
 
 import sc_functional as utils_f
-from sc_layers import Conv2d_Add_Partial
+from sc_layers import Conv2d_Add_Partial, LayerNorm, Linear_Int8
 
 
 def _sc3x3(cin, cout, stride, **sc):
@@ -20,8 +23,16 @@ def _sc1x1(cin, cout, stride, **sc):
     return Conv2d_Add_Partial(cin, cout, kernel_size=1, stride=stride, bias=False, **sc)
 
 
+def _classifier(kind, features, num_classes):
+    if kind == "float":
+        return nn.Linear(features, num_classes)
+    if kind == "int8":
+        return nn.Sequential(LayerNorm(features), Linear_Int8(features, num_classes))
+    raise ValueError("classifier must be 'float' or 'int8' (got %r)" % (kind,))
+
+
 class TinyConvSC(nn.Module):
-    def __init__(self, num_classes=10, **sc):
+    def __init__(self, num_classes=10, classifier="float", **sc):
         super().__init__()
         act = lambda: nn.Hardtanh(0, 1)
         self.features = nn.Sequential(
@@ -29,7 +40,7 @@ class TinyConvSC(nn.Module):
             _sc3x3(32, 32, 1, **sc), nn.BatchNorm2d(32), act(), nn.MaxPool2d(2),
             _sc3x3(32, 64, 1, **sc), nn.BatchNorm2d(64), act(),
             _sc3x3(64, 64, 1, **sc), nn.BatchNorm2d(64), act(), nn.MaxPool2d(2))
-        self.fc = nn.Linear(64 * 8 * 8, num_classes)
+        self.fc = _classifier(classifier, 64 * 8 * 8, num_classes)
         self.sync = 1
         for m in self.modules():
             if isinstance(m, nn.Conv2d):
@@ -62,7 +73,7 @@ class BasicBlock(nn.Module):
 
 
 class ResNet18SC(nn.Module):
-    def __init__(self, num_classes=1000, **sc):
+    def __init__(self, num_classes=1000, classifier="float", **sc):
         super().__init__()
         self.inplanes = 64
         strides = [1, 1, 2, 2] if num_classes < 1000 else [2, 2, 2, 2]
@@ -75,7 +86,7 @@ class ResNet18SC(nn.Module):
         self.layer3 = self._make_layer(256, 2, strides[2], sc)
         self.layer4 = self._make_layer(512, 2, strides[3], sc)
         self.avgpool = nn.AdaptiveAvgPool2d((1, 1))
-        self.fc = nn.Linear(512, num_classes)
+        self.fc = _classifier(classifier, 512, num_classes)
         self.sync = 1
         for m in self.modules():
             if isinstance(m, nn.Conv2d):

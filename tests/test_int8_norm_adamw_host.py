@@ -1,0 +1,177 @@
+"""What the 8-bit linear layer, layer norm and AdamW refuse, and their planning: host code, no GPU."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+FAKE = ctypes.c_void_p(1 << 20)  # an aligned address that is never read: every call below is refused before a launch
+ODD = ctypes.c_void_p((1 << 20) + 8)
+
+
+def _int8(M=4, N=4, K=32, dtype=0, bias=0, weight=0, reserved=0, xs=None, a=32, b=32):
+    import _lib
+    return _lib.Int8Desc(M, N, K, dtype, bias, weight, reserved, K if xs is None else xs, a, b)
+
+
+def _error(L):
+    return L.rexsc_last_error().decode()
+
+
+def test_descriptors_mirror_the_header():
+    import _lib
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "rexsc.h")).read(), flags=re.S)
+    kinds = {"int32_t": ctypes.c_int32, "int64_t": ctypes.c_int64, "float": ctypes.c_float, "double": ctypes.c_double}
+    for name, cls in (("rexsc_int8_desc", _lib.Int8Desc), ("rexsc_norm_desc", _lib.NormDesc), ("rexsc_adamw_desc", _lib.AdamwDesc)):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S).group(1)
+        fields = [(f.strip(), kinds[k]) for k, decl in re.findall(r"(int32_t|int64_t|float|double)([^;]*);", body) for f in decl.split(",")]
+        assert fields == list(cls._fields_), name
+    body = re.search(r"typedef struct rexsc_adamw_tensor \{(.*?)\} rexsc_adamw_tensor;", text, flags=re.S).group(1)
+    assert len(re.findall(r";", body)) == _lib.ADAMW_TENSOR_FIELDS
+    assert int(re.search(r"#define REXSC_ADAMW_COEF_BYTES (\d+)", text).group(1)) == _lib.ADAMW_COEF_BYTES
+
+
+def test_int8_workspace_and_refusals():
+    import _lib
+    L = _lib.lib()
+    none = ctypes.c_size_t(-1).value
+    ws = lambda d, what: L.rexsc_int8_workspace_bytes(ctypes.byref(d), what)
+    assert ws(_int8(M=1000, K=4096), _lib.INT8_LINEAR) >= 1000 * 4096 + 4000
+    assert ws(_int8(M=100, N=50, K=70), _lib.INT8_GRAD_INPUT) >= 100 * 64 * 3 * 2 + 70 * 64 * 2
+    assert ws(_int8(M=100, N=50, K=70, weight=2), _lib.INT8_GRAD_WEIGHT) >= 50 * 128 * 2 * 2 + 70 * 128 * 2
+    for d, text in ((_int8(K=0), "K must be"), (_int8(K=131072), "K must be"), (_int8(M=-1), "M -1"), (_int8(dtype=3), "dtypes"),
+                    (_int8(bias=-1), "dtypes"), (_int8(weight=9), "dtypes"), (_int8(reserved=1), "reserved")):
+        for what in range(4):
+            assert ws(d, what) == none and text in _error(L)
+    assert ws(_int8(), 4) == none and "number 4" in _error(L)
+    d = _int8()
+    d.struct_size -= 8
+    assert ws(d, 0) == none and "struct_size" in _error(L)
+
+
+def test_int8_calls_refuse():
+    import _lib
+    L = _lib.lib()
+    product = lambda d, a=FAKE, b=FAKE, sa=FAKE, y=FAKE: L.rexsc_int8_product(ctypes.byref(d), a, sa, b, FAKE, None, y, None, 0, None)
+    for d, kw, text in ((_int8(a=24), {}, "tokens"), (_int8(a=16), {}, "tokens"), (_int8(b=40), {}, "channels"),
+                        (_int8(), {"a": ODD}, "tokens"), (_int8(), {"b": ODD}, "channels"), (_int8(), {"a": None}, "null"),
+                        (_int8(), {"sa": None}, "null"), (_int8(), {"y": None}, "null")):
+        assert product(d, **kw) == -1 and text in _error(L), text
+    assert product(_int8(M=0), a=None, b=None) == 0 and product(_int8(N=0), a=None) == 0  # nothing to do
+    linear = lambda d, x=FAKE, ws=None, n=0: L.rexsc_int8_linear(ctypes.byref(d), x, FAKE, FAKE, None, FAKE, ws, n, None)
+    big = _int8(M=1000, K=32)
+    need = L.rexsc_int8_workspace_bytes(ctypes.byref(big), _lib.INT8_LINEAR)
+    assert linear(big) == -2 and "workspace" in _error(L)
+    assert linear(big, ws=FAKE, n=need - 1) == -2
+    assert linear(big, ws=ODD, n=need) == -1 and "16-byte" in _error(L)
+    assert linear(_int8(xs=31)) == -1 and "overlap" in _error(L)
+    assert linear(_int8(), x=ctypes.c_void_p(3)) == -1 and "aligned" in _error(L)
+    gi = lambda d, ws=None, n=0: L.rexsc_int8_grad_input(ctypes.byref(d), FAKE, FAKE, FAKE, FAKE, ws, n, None)
+    gw = lambda d, ws=None, n=0: L.rexsc_int8_grad_weight(ctypes.byref(d), FAKE, FAKE, FAKE, FAKE, FAKE, ws, n, None)
+    assert gi(_int8()) == -2 and gw(_int8()) == -2
+    assert gi(_int8(N=0)) == -1 and "output channel" in _error(L)
+    assert gi(_int8(M=0, N=1)) == 0 and gw(_int8(N=0)) == 0
+    q = lambda rows, cols, stride, out=FAKE, x=FAKE, dt=0: L.rexsc_quantize_rows(x, dt, rows, cols, cols, out, stride, FAKE, None)
+    assert q(0, 4, 16) == 0
+    for args, text in (((2, 0, 16), "elements"), ((2, 20, 16), "int8 rows"), ((2, 20, 24), "int8 rows"), ((2, 4, 16, ODD), "int8 rows"),
+                       ((2, 4, 16, None), "null"), ((2, 4, 16, FAKE, ctypes.c_void_p(2)), "aligned"),
+                       ((2, 4, 16, FAKE, FAKE, 5), "dtype")):
+        assert q(*args) == -1 and text in _error(L), text
+
+
+def test_layer_norm_refusals():
+    import _lib
+    L = _lib.lib()
+    D = lambda dt=0, wdt=0, eps=1e-5, rows=4, cols=8, xs=8: _lib.NormDesc(dt, wdt, eps, rows, cols, xs)
+    fwd = lambda d, x=FAKE, y=FAKE, m=FAKE, r=FAKE: L.rexsc_layer_norm_forward(ctypes.byref(d), x, FAKE, FAKE, y, m, r, None)
+    for d, kw, text in ((D(dt=3), {}, "dtype"), (D(dt=1, wdt=2), {}, "weight and bias"), (D(eps=-1.0), {}, "eps"),
+                        (D(eps=float("nan")), {}, "eps"), (D(rows=-1), {}, "rows"), (D(cols=0), {}, "rows"),
+                        (D(xs=7), {}, "distance"), (D(), {"x": None}, "null"), (D(), {"r": None}, "together"),
+                        (D(), {"x": ctypes.c_void_p(6)}, "aligned")):
+        assert fwd(d, **kw) == -1 and text in _error(L), text
+    assert fwd(D(rows=0), x=None, y=None) == 0
+    bytes_ = L.rexsc_layer_norm_backward_workspace_bytes
+    assert bytes_(ctypes.byref(D())) >= 2 * 8 * 4 and bytes_(ctypes.byref(D(cols=0))) == ctypes.c_size_t(-1).value
+    bwd = lambda d, g=FAKE, dx=FAKE, dw=FAKE, ws=None, n=0: L.rexsc_layer_norm_backward(
+        ctypes.byref(d), g, FAKE, FAKE, FAKE, FAKE, dx, dw, None, ws, n, None)
+    assert bwd(D()) == -2 and "workspace" in _error(L)
+    assert bwd(D(), g=None) == -1 and "null" in _error(L)
+    assert bwd(D(), dx=None, dw=None) == 0
+
+
+def test_adamw_refusals():
+    import _lib
+    L = _lib.lib()
+    T = lambda p=1 << 20, g=1 << 20, m=1 << 20, v=1 << 20, ms=0, vs=0, n=10: (p, g, m, v, ms, vs, n)
+    D = lambda dt=0, bits=32, clamp=0, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, wd=0.0, lo=0.0, hi=0.0, step=1: _lib.AdamwDesc(
+        dt, bits, clamp, lr, b1, b2, eps, wd, lo, hi, step)
+
+    def call(d, t, step=None, scale=None, inf=None, coef=None):
+        arr = (ctypes.c_int64 * 7)(*t)
+        return L.rexsc_adamw_step(ctypes.byref(d), ctypes.cast(arr, ctypes.c_void_p), 1, step, scale, inf, coef, None)
+
+    for d, t, kw, text in ((D(dt=4), T(), {}, "dtype"), (D(bits=16), T(), {}, "32 or 8"), (D(b1=1.0), T(), {}, "betas"),
+                           (D(b2=-0.1), T(), {}, "betas"), (D(lr=-1.0), T(), {}, "negative"), (D(eps=float("nan")), T(), {}, "negative"),
+                           (D(clamp=1, lo=1.0, hi=0.0), T(), {}, "clamp"), (D(step=0), T(), {}, "counts from 1"),
+                           (D(), T(), {"step": FAKE}, "workspace"), (D(), T(), {"scale": FAKE}, "need the step"),
+                           (D(), T(), {"inf": FAKE}, "need the step"), (D(), T(n=-1), {}, "elements"), (D(), T(g=0), {}, "null"),
+                           (D(), T(m=0), {}, "null"), (D(bits=8), T(), {}, "scales"), (D(), T(p=(1 << 20) + 2), {}, "aligned"),
+                           (D(), T(v=(1 << 20) + 1), {}, "aligned")):
+        assert call(d, t, **kw) == -1 and text in _error(L), text
+    assert call(D(), T(p=0, g=0, m=0, v=0, n=0)) == 0  # a tensor without elements
+
+
+def test_python_checks_need_no_gpu():
+    import _ops
+    import sc_functional as F
+    import sc_layers
+    import sc_optim
+    x, w = torch.randn(3, 8), torch.randn(4, 8)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        F.linear_int8(x, w)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        F.layer_norm(x)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        F.quantize_rows(x)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        sc_optim.adamw_step([x], [x], [x], [x], step=1, lr=1e-3)
+    with pytest.raises(ValueError, match="weight_scale"):
+        F.linear_int8(x, w.to(torch.int8))
+    with pytest.raises(ValueError, match="weight_scale"):
+        F.linear_int8(x, w, weight_scale=torch.ones(4))
+    with pytest.raises(ValueError, match="expected input"):
+        F.linear_int8(x, torch.randn(4, 9))
+    for t in (torch.zeros(2, 3), torch.zeros(2, 0, dtype=torch.int8), torch.zeros(6, dtype=torch.int8),
+              torch.zeros(1, 131072, dtype=torch.int8)):
+        with pytest.raises(RuntimeError, match="int8 matrix"):
+            _ops._operand8(t, "matmul_int8")
+    with pytest.raises(RuntimeError, match="scales"):
+        _ops._scale_vector(torch.ones(3), 4, torch.device("cpu"), "x")
+    with pytest.raises(RuntimeError, match="bias"):
+        _ops._bias_vector(torch.ones(3, 1), 3, "x")
+    for kw in ({"state_bits": 16}, {"lr": -1}, {"betas": (1.0, 0.9)}, {"clamp": (1, 0)}, {"eps": float("nan")}):
+        with pytest.raises(ValueError):
+            sc_optim.AdamW([torch.nn.Parameter(x)], **kw)
+    with pytest.raises(RuntimeError, match="lengths"):
+        sc_optim.adamw_step([x], [], [x], [x], step=1, lr=1e-3)
+    with pytest.raises(RuntimeError, match="both lists"):
+        sc_optim.adamw_step([x], [x], [x], [x], [x], step=1, lr=1e-3)
+    layer = sc_layers.Linear_Int8(8, 4)
+    assert not layer.frozen and set(layer.state_dict()) == {"weight", "bias"}
+
+
+def test_operand_layouts():
+    """Which int8 tensors are read in place: rows 16-byte aligned and readable to the next multiple of 16."""
+    import _ops
+    whole = torch.zeros(10, 64, dtype=torch.int8)
+    for t, kept in ((whole, True), (whole[:, :50], True), (whole[:, 16:40], True), (whole[2:, 5:30], False), (whole[::2], True),
+                    (whole.t(), False), (torch.zeros(4, 30, dtype=torch.int8), False), (whole[:1, :30], True),
+                    (torch.zeros(1, 30, dtype=torch.int8), False), (torch.zeros(46, dtype=torch.int8).as_strided((3, 14), (16, 1)), False)):
+        got, stride = _ops._operand8(t, "x")
+        assert (got.data_ptr() == t.data_ptr()) == kept and torch.equal(got, t) and stride % 16 == 0 and stride >= t.shape[1]
+    import sc_optim
+    d = sc_optim._dense
+    assert d(torch.zeros(3, 4)) and d(torch.zeros(3, 4).t()) and d(torch.zeros(2, 3, 4, 5).contiguous(memory_format=torch.channels_last))
+    assert not d(torch.zeros(3, 8)[:, :4]) and not d(torch.zeros(1, 4).expand(3, 4)) and d(torch.zeros(0, 4))
