@@ -10,15 +10,11 @@
 // results, two hold 16 and serve 16-bit results, whose own rounding is far coarser), so nothing but the float32
 // accumulation is rounded.  Pieces and transposed operands are laid out in the workspace first, which makes both
 // gradients the same product of two row-major operands as the forward pass.
-#include "lowp.h"
 #include "profile.h"
+#include "tile_product.h"
 
 namespace rexsc {
 namespace {
-
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int MAX_K = 131071; // 128 * 128 * K < 2^31
 
@@ -78,100 +74,6 @@ __global__ __launch_bounds__(Q_THREADS) void quantize_rows_kernel(const T *x, si
     if (threadIdx.x == 0) scale[blockIdx.x] = rs.scale;
 }
 
-// ---- the product of two row-major operands --------------------------------------------------------
-// c[m][n] = sum_k a[m][k] b[n][k], rows as bytes: 16 bytes are one lane's share of a matrix instruction's operand in
-// either type (16 int8 or 8 bfloat16).
-struct TileArgs {
-    const char *a, *b;
-    size_t a_stride, b_stride;      // bytes
-    int M, N;
-    int kbytes;                     // length of a reduction row; the operands are readable to the next multiple of 16
-    int pieces;                     // a's row holds this many pieces, each multiplied by the same b row
-    size_t piece_stride;            // bytes
-    const float *a_scale, *b_scale; // NULL: 1 (the gradients)
-    const void *bias;
-    int bias_dtype;
-    void *y;
-    size_t y_stride;                // elements
-};
-
-struct OpI8 { typedef i32x4 acc; typedef int elem; };
-struct OpBF16 { typedef f32x4 acc; typedef float elem; };
-__device__ __forceinline__ i32x4 mma(OpI8, i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x4 mma(OpBF16, i32x4 a, i32x4 b, f32x4 c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// Bytes of a 16-byte chunk at offset k that lie before `end`; the rest become 0.
-__device__ __forceinline__ i32x4 keep_before(i32x4 v, int k, int end)
-{
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int n = end - k - 4 * i;
-        v[i] = n >= 4 ? v[i] : n <= 0 ? 0 : v[i] & (int)((1u << (8 * n)) - 1u);
-    }
-    return v;
-}
-
-constexpr int TILE = 64, KSTEP = 64, LDS_ROW = KSTEP + 16;
-
-template <typename Op, typename T>
-__global__ __launch_bounds__(256) void tile_kernel(TileArgs p)
-{
-    __shared__ __attribute__((aligned(16))) char la[TILE * LDS_ROW], lb[TILE * LDS_ROW];
-    const int tiles_n = (p.N + TILE - 1) / TILE;
-    const int m0 = (int)(blockIdx.x / tiles_n) * TILE, n0 = (int)(blockIdx.x % tiles_n) * TILE;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int wm = (wave / 2) * 32, wn = (wave % 2) * 32;
-    const int lr = threadIdx.x / 4, lc = (threadIdx.x % 4) * 16; // this thread's chunk of a tile
-    typename Op::acc acc[2][2] = {};
-    for (int piece = 0; piece < p.pieces; piece++)
-        for (int k = 0; k < p.kbytes; k += KSTEP) {
-            i32x4 va = {0, 0, 0, 0}, vb = {0, 0, 0, 0};
-            if (k + lc < p.kbytes) {
-                if (m0 + lr < p.M)
-                    va = keep_before(*(const i32x4 *)(p.a + (size_t)(m0 + lr) * p.a_stride + piece * p.piece_stride + k + lc),
-                                     k + lc, p.kbytes);
-                if (n0 + lr < p.N)
-                    vb = keep_before(*(const i32x4 *)(p.b + (size_t)(n0 + lr) * p.b_stride + k + lc), k + lc, p.kbytes);
-            }
-            __syncthreads();
-            *(i32x4 *)(la + lr * LDS_ROW + lc) = va;
-            *(i32x4 *)(lb + lr * LDS_ROW + lc) = vb;
-            __syncthreads();
-            i32x4 fa[2], fb[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                fa[i] = *(const i32x4 *)(la + (wm + i * 16 + lane % 16) * LDS_ROW + lane / 16 * 16);
-                fb[i] = *(const i32x4 *)(lb + (wn + i * 16 + lane % 16) * LDS_ROW + lane / 16 * 16);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) acc[i][j] = mma(Op{}, fb[j], fa[i], acc[i][j]);
-        }
-    // b is the first operand: a lane holds four neighbouring columns n of one row m
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int m = m0 + wm + i * 16 + lane % 16;
-        if (m >= p.M) continue;
-        const float sa = p.a_scale ? p.a_scale[m] : 1.f;
-        T *row = (T *)p.y + (size_t)m * p.y_stride;
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int n = n0 + wn + j * 16 + lane / 16 * 4 + e;
-                if (n >= p.N) continue;
-                float v = (float)acc[i][j][e] * sa;
-                if (p.b_scale) v *= p.b_scale[n];
-                if (p.bias) v += load_any(p.bias, p.bias_dtype, n);
-                row[n] = (T)v;
-            }
-    }
-}
-
 // ---- operands of the gradients ---------------------------------------------------------------------
 // v = sum of `pieces` bfloat16 values.  Each but the last keeps the leading 8 bits (truncated, so that nothing
 // overflows), the last is rounded.  Of an infinity or NaN the first piece is all.
@@ -189,19 +91,19 @@ __device__ __forceinline__ void split(float v, int pieces, bf16_t (&out)[3])
     }
 }
 
-// g [rows][cols] -> out [rows][pieces][ld], elements times scale[column], columns from cols to ld zero.
+// g [rows][cols] -> out [pieces][rows][ld], elements times scale[column], columns from cols to ld zero.
 template <typename T>
 __global__ __launch_bounds__(256) void split_rows_kernel(const T *g, const float *scale, int cols, int ld, int pieces, bf16_t *out)
 {
-    const size_t row = blockIdx.x;
+    const size_t row = blockIdx.x, rows = gridDim.x;
     for (int c = threadIdx.x; c < ld; c += 256) {
         bf16_t q[3];
         split(c < cols ? (float)g[row * cols + c] * scale[c] : 0.f, pieces, q);
-        for (int i = 0; i < pieces; i++) out[(row * pieces + i) * ld + c] = q[i];
+        for (int i = 0; i < pieces; i++) out[(i * rows + row) * ld + c] = q[i];
     }
 }
 
-// g [rows][cols] -> out [cols][pieces][ld], elements times scale[row], positions from rows to ld zero; and the sums of
+// g [rows][cols] -> out [pieces][cols][ld], elements times scale[row], positions from rows to ld zero; and the sums of
 // g's columns over this block's 64 rows to part[row block][cols].  out NULL: only the sums.
 template <typename T>
 __global__ __launch_bounds__(256) void split_transposed_kernel(const T *g, const float *scale, int rows, int cols, int ld,
@@ -227,7 +129,7 @@ __global__ __launch_bounds__(256) void split_transposed_kernel(const T *g, const
         if (c0 + i >= cols) break;
         bf16_t q[3];
         split(r0 + tx < rows ? tile[tx][i] * sc : 0.f, pieces, q);
-        for (int j = 0; j < pieces; j++) out[((size_t)(c0 + i) * pieces + j) * ld + r0 + tx] = q[j];
+        for (int j = 0; j < pieces; j++) out[((size_t)j * cols + c0 + i) * ld + r0 + tx] = q[j];
     }
 }
 
@@ -310,23 +212,12 @@ int check_space(const Space &s, const void *workspace, size_t bytes)
     return REXSC_OK;
 }
 
-template <typename Op>
-int launch_tiles(const TileArgs &p, int out_dtype, const char *name, hipStream_t stream)
-{
-    const int64_t tiles = (int64_t)((p.M + TILE - 1) / TILE) * ((p.N + TILE - 1) / TILE);
-    REXSC_CHECK_ARG(tiles < (1ll << 31), "int8 linear: result of %d x %d is too large", p.M, p.N);
-    ProfScope prof(name, 2.0 * p.M * p.N * p.kbytes * p.pieces, stream);
-    REXSC_DTYPE_SWITCH(out_dtype, hipLaunchKernelGGL((tile_kernel<Op, T>), dim3((unsigned)tiles), dim3(256), 0, stream, p));
-    REXSC_CHECK_HIP(hipGetLastError());
-    return REXSC_OK;
-}
-
 int product(const rexsc_int8_desc *d, const int8_t *a, int64_t a_stride, const float *a_scale, const int8_t *b,
             const float *b_scale, const void *bias, void *y, hipStream_t stream)
 {
     const TileArgs p{(const char *)a, (const char *)b, (size_t)a_stride, (size_t)d->b_stride, d->M, d->N, d->K, 1, 0,
-                     a_scale, b_scale, bias, d->bias_dtype, y, (size_t)d->N};
-    return launch_tiles<OpI8>(p, d->dtype, "int8_product", stream);
+                     a_scale, b_scale, bias, d->bias_dtype, y};
+    return launch_tile_product(p, false, d->dtype, "int8_product", stream);
 }
 
 int launch_quantize(const void *x, int dtype, size_t rows, size_t cols, size_t x_stride, int8_t *q, size_t q_stride,
@@ -425,9 +316,9 @@ extern "C" int rexsc_int8_grad_input(const rexsc_int8_desc *d, const void *g, co
                            (size_t)d->b_stride, d->N, d->K, ld, bt);
         REXSC_CHECK_HIP(hipGetLastError());
     }
-    const TileArgs p{(const char *)pieces, (const char *)bt, (size_t)ld * P * 2, (size_t)ld * 2, d->M, d->K, ld * 2, P,
-                     (size_t)ld * 2, nullptr, nullptr, nullptr, REXSC_F32, dx, (size_t)d->K};
-    return launch_tiles<OpBF16>(p, d->dtype, "int8_grad_input", stream);
+    const TileArgs p{(const char *)pieces, (const char *)bt, (size_t)ld * 2, (size_t)ld * 2, d->M, d->K, ld * 2, P,
+                     (size_t)d->M * ld * 2, nullptr, nullptr, nullptr, REXSC_F32, dx};
+    return launch_tile_product(p, true, d->dtype, "int8_grad_input", stream);
 }
 
 extern "C" int rexsc_int8_grad_weight(const rexsc_int8_desc *d, const void *g, const int8_t *a, const float *a_scale, void *dw,
@@ -464,7 +355,7 @@ extern "C" int rexsc_int8_grad_weight(const rexsc_int8_desc *d, const void *g, c
         REXSC_CHECK_HIP(hipGetLastError());
     }
     // without tokens the reduction is empty and the kernel writes zeros
-    const TileArgs p{(const char *)pieces, (const char *)at, (size_t)ld * P * 2, (size_t)ld * 2, d->N, d->K, ld * 2, P,
-                     (size_t)ld * 2, nullptr, nullptr, nullptr, REXSC_F32, dw, (size_t)d->K};
-    return launch_tiles<OpBF16>(p, d->weight_dtype, "int8_grad_weight", stream);
+    const TileArgs p{(const char *)pieces, (const char *)at, (size_t)ld * 2, (size_t)ld * 2, d->N, d->K, ld * 2, P,
+                     (size_t)d->N * ld * 2, nullptr, nullptr, nullptr, REXSC_F32, dw};
+    return launch_tile_product(p, true, d->weight_dtype, "int8_grad_weight", stream);
 }

@@ -1,0 +1,261 @@
+// Product of two row-major operands: c[m][n] = sum_k a[m][k] b[n][k].
+#include <type_traits>
+
+#include "profile.h"
+#include "tile_product.h"
+
+namespace rexsc {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+
+struct OpI8 { typedef i32x4 acc; };
+struct OpBF16 { typedef f32x4 acc; };
+__device__ __forceinline__ i32x4 mma(OpI8, i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(OpBF16, i32x4 a, i32x4 b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Waits until this wave's loads into LDS have landed (before the barrier that shows them to the other waves).
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); } // vmcnt(0), the other counters at any value
+
+// Bytes of a 16-byte chunk at offset k that lie before `end`; the rest become 0.
+__device__ __forceinline__ i32x4 keep_before(i32x4 v, int k, int end)
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int n = end - k - 4 * i;
+        v[i] = n >= 4 ? v[i] : n <= 0 ? 0 : v[i] & (int)((1u << (8 * n)) - 1u);
+    }
+    return v;
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
+
+// 16 bytes per lane from base + lane offset + offset to LDS, at dst + 16 * lane.
+__device__ __forceinline__ void load_to_lds(const char *base, unsigned lane_offset, unsigned offset, char *dst)
+{
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0x7fffffff, 0x00027000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)dst, 16, lane_offset, offset, 0, 0);
+}
+
+constexpr int KSTEP = 128;          // bytes of the reduction per step
+constexpr int CHUNKS = KSTEP / 16;  // 16-byte chunks of a tile row
+
+// Where chunk c of tile row r lies in that row's 128 bytes of LDS.  A fragment read takes the same chunk of 16
+// consecutive rows: with the rows' pairs shifted against each other they fall on all 64 banks once.
+__device__ __forceinline__ int swizzle(int r, int c) { return c ^ ((r >> 1) & (CHUNKS - 1)); }
+
+// Tile of a block.  Workgroups go to the eight XCDs in turn, each with an L2 of its own: an XCD gets a contiguous run
+// of the tile order, and the order walks groups of GROUP_M tile rows column by column, so that the tiles an XCD has in
+// flight at once form a patch that shares operand rows.
+constexpr int XCDS = 8, GROUP_M = 4;
+__device__ __forceinline__ void tile_of(unsigned bid, int tiles_m, int tiles_n, int &tm, int &tn)
+{
+    const unsigned total = (unsigned)tiles_m * (unsigned)tiles_n, per = total / XCDS, extra = total % XCDS;
+    const unsigned x = bid % XCDS, i = bid / XCDS;
+    const unsigned t = x * per + (x < extra ? x : extra) + i;
+    const unsigned group = (unsigned)(GROUP_M * tiles_n), g = t / group, r = t % group;
+    const int left = tiles_m - (int)g * GROUP_M, rows = left < GROUP_M ? left : GROUP_M;
+    tm = (int)g * GROUP_M + (int)(r % rows);
+    tn = (int)(r / rows);
+}
+
+template <typename Op, typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
+{
+    constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+    constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES; // loads of 8 rows x 128 bytes per wave and step
+    static_assert(LA * WAVES * 8 == BM && LB * WAVES * 8 == BN, "tile rows must divide among the waves");
+    __shared__ __attribute__((aligned(1024))) char buf0[(BM + BN) * KSTEP];
+    __shared__ __attribute__((aligned(1024))) char buf1[(BM + BN) * KSTEP];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    int tm, tn;
+    tile_of(blockIdx.x, (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, tm, tn);
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int last_m = p.M - 1 - m0, last_n = p.N - 1 - n0; // rows behind the operand's last read that one again
+
+    // per load: where this lane's row begins, and its chunk, the same for all loads since their rows lie 16 apart (the
+    // LDS side of a load is fixed: 16 bytes per lane in lane order)
+    static_assert(WAVES % 2 == 0, "loads of one wave must be 16 rows apart");
+    unsigned offa[LA], offb[LB];
+#pragma unroll
+    for (int i = 0; i < LA; i++) {
+        const int r = (i * WAVES + wave) * 8 + lane / 8;
+        offa[i] = (unsigned)(r < last_m ? r : last_m) * (unsigned)p.a_stride;
+    }
+#pragma unroll
+    for (int i = 0; i < LB; i++) {
+        const int r = (i * WAVES + wave) * 8 + lane / 8;
+        offb[i] = (unsigned)(r < last_n ? r : last_n) * (unsigned)p.b_stride;
+    }
+    const unsigned chunk = (unsigned)swizzle(wave * 8 + lane / 8, lane % 8) * 16;
+    const char *base_a = p.a + (size_t)m0 * p.a_stride, *base_b = p.b + (size_t)n0 * p.b_stride;
+    const int steps = (p.kbytes + KSTEP - 1) / KSTEP, total = steps * p.pieces;
+    const unsigned last_chunk = (unsigned)(p.kbytes - 1) / 16 * 16; // of a row: lanes behind it read it instead
+
+    unsigned k = 0; // byte offset in the row of the step that is fetched next
+    auto fetch = [&](char *buf) __attribute__((always_inline)) {
+        const unsigned left = last_chunk - k, c = chunk < left ? chunk : left;
+#pragma unroll
+        for (int i = 0; i < LA; i++) load_to_lds(base_a, offa[i] + c, k, buf + (i * WAVES + wave) * 1024);
+#pragma unroll
+        for (int i = 0; i < LB; i++) load_to_lds(base_b, offb[i] + c, k, buf + BM * KSTEP + (i * WAVES + wave) * 1024);
+        k += KSTEP;
+        if (k >= (unsigned)p.kbytes) { k = 0; base_a += p.piece_stride; }
+    };
+
+    const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+    typename Op::acc acc[FM][FN] = {};
+    i32x4 fa[2][FM], fb[2][FN]; // fragments of the half step that is multiplied and of the next one
+    // Rows 16 apart lie at the same place of the swizzle, and the second half's chunks 64 bytes across it, so a
+    // fragment's address is one of two lane offsets plus a constant.
+    const int q = lane % 16 * KSTEP + swizzle(lane % 16, lane / 16) * 16;
+    const lds_char *const pa[2][2] = {{(const lds_char *)buf0 + wm * KSTEP + q, (const lds_char *)buf0 + wm * KSTEP + (q ^ 64)},
+                                      {(const lds_char *)buf1 + wm * KSTEP + q, (const lds_char *)buf1 + wm * KSTEP + (q ^ 64)}};
+    const lds_char *const pb[2][2] = {
+        {(const lds_char *)buf0 + (BM + wn) * KSTEP + q, (const lds_char *)buf0 + (BM + wn) * KSTEP + (q ^ 64)},
+        {(const lds_char *)buf1 + (BM + wn) * KSTEP + q, (const lds_char *)buf1 + (BM + wn) * KSTEP + (q ^ 64)}};
+    // Multiplies the fragments of `half` while (reads) the next half's are read from buffer `buf`: a row of a's
+    // fragment is replaced as soon as its products are issued, so the second set costs no more registers than b's.
+    // keep: bytes of this step that belong to the row, where it is the last (int8: what stands behind may be anything).
+    auto multiply = [&](int half, auto reads, int buf, auto masked, int keep) __attribute__((always_inline)) {
+        const int next = half ^ 1;
+#pragma unroll
+        for (int i = 0; i < FM; i++) {
+            if constexpr (masked) fa[half][i] = keep_before(fa[half][i], (half * 4 + lane / 16) * 16, keep);
+#pragma unroll
+            for (int j = 0; j < FN; j++) acc[i][j] = mma(Op{}, fb[half][j], fa[half][i], acc[i][j]);
+            if constexpr (reads) {
+                fa[next][i] = *(const lds_i32x4 *)(pa[buf][next] + i * 16 * KSTEP);
+#pragma unroll
+                for (int j = i * FN / FM; j < (i + 1) * FN / FM; j++) fb[next][j] = *(const lds_i32x4 *)(pb[buf][next] + j * 16 * KSTEP);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // One step from `cur`: its second half is read while the first is multiplied; then, with every wave's fragments of
+    // `cur` in registers and `nxt` filled, one barrier, behind which `cur` is filled anew and the first half of `nxt`
+    // is read while the second half is multiplied.
+    constexpr std::integral_constant<bool, false> no{};
+    constexpr std::integral_constant<bool, true> yes{};
+    auto step = [&](int cur, bool refill) __attribute__((always_inline)) {
+        multiply(0, yes, cur, no, 0);
+        loads_done();
+        __syncthreads();
+        if (refill) fetch(cur == 0 ? buf0 : buf1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(1, yes, cur ^ 1, no, 0);
+    };
+    auto last_step = [&](int cur) __attribute__((always_inline)) {
+        const int keep = p.kbytes - (steps - 1) * KSTEP;
+        multiply(0, yes, cur, yes, keep);
+        multiply(1, no, cur, yes, keep);
+    };
+    if (total > 0) {
+        fetch(buf0);
+        loads_done();
+        __syncthreads();
+        if (total > 1) fetch(buf1);
+#pragma unroll
+        for (int i = 0; i < FM; i++) fa[0][i] = *(const lds_i32x4 *)(pa[0][0] + i * 16 * KSTEP);
+#pragma unroll
+        for (int j = 0; j < FN; j++) fb[0][j] = *(const lds_i32x4 *)(pb[0][0] + j * 16 * KSTEP);
+        int s = 0;
+        for (; s + 2 < total; s += 2) {
+            step(0, true);
+            step(1, s + 3 < total);
+        }
+        if (s + 2 == total) {
+            step(0, false);
+            last_step(1);
+        } else {
+            last_step(0);
+        }
+    }
+
+    // Epilogue.  b was the first operand, so a lane holds four neighbouring columns n of one row m: written like that, a
+    // store would touch 16 rows with 8 bytes each.  The wave turns its part of the tile round in LDS (its own share, so
+    // one barrier in all) and stores 16 bytes per lane along the rows.  The rows' pitch is 16 bytes off a multiple of
+    // the banks, which spreads the 16 rows of a write over all of them.
+    constexpr int COLS = BN / WN, ROWS = BM / WM, VEC = 16 / sizeof(T), PITCH = COLS * sizeof(T) + 16;
+    constexpr int PART = sizeof(T) == 4 ? 32 : 64, CR = ROWS < PART ? ROWS : PART; // rows that are turned at a time
+    static_assert((WAVES + 1) / 2 * CR * PITCH <= (BM + BN) * KSTEP, "a buffer holds half of the waves' shares");
+    const int first_n = n0 + wn;
+    float sb[FN][4], bias[FN][4];
+#pragma unroll
+    for (int j = 0; j < FN; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int n = first_n + j * 16 + lane / 16 * 4 + e, c = n < p.N ? n : p.N - 1;
+            sb[j][e] = p.b_scale ? p.b_scale[c] : 1.f;
+            bias[j][e] = p.bias ? load_any(p.bias, p.bias_dtype, c) : 0.f;
+        }
+    __syncthreads();
+    lds_char *const mine = (lds_char *)(wave % 2 ? buf1 : buf0) + wave / 2 * (CR * PITCH);
+    const bool wide = ((size_t)p.N * sizeof(T) % 16 == 0) && ((uintptr_t)p.y % 16 == 0);
+#pragma unroll
+    for (int r0 = 0; r0 < ROWS; r0 += CR) {
+#pragma unroll
+        for (int i = 0; i < CR / 16; i++) {
+            const int m = m0 + wm + r0 + i * 16 + lane % 16;
+            const float sa = p.a_scale ? p.a_scale[m < p.M ? m : p.M - 1] : 1.f;
+#pragma unroll
+            for (int j = 0; j < FN; j++) {
+                typename VecOf<T, 4>::type v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = (T)((float)acc[r0 / 16 + i][j][e] * sa * sb[j][e] + bias[j][e]);
+                *(__attribute__((address_space(3))) typename VecOf<T, 4>::type *)(mine + (i * 16 + lane % 16) * PITCH +
+                                                                                  (j * 16 + lane / 16 * 4) * (int)sizeof(T)) = v;
+            }
+        }
+        const int rows = p.M - (m0 + wm + r0); // of this part, that exist
+        T *out = (T *)p.y + (size_t)(m0 + wm + r0) * p.N + first_n;
+        if (wide) {
+#pragma unroll
+            for (int t = 0; t < CR * COLS / VEC / 64; t++) {
+                const int at = t * 64 + lane, r = at / (COLS / VEC), c = at % (COLS / VEC) * VEC;
+                const i32x4 v = *(const lds_i32x4 *)(mine + r * PITCH + c * (int)sizeof(T));
+                if (r < rows && first_n + c < p.N) *(i32x4 *)(out + (size_t)r * p.N + c) = v;
+            }
+        } else {
+            for (int t = 0; t < CR * COLS / 64; t++) {
+                const int at = t * 64 + lane, r = at / COLS, c = at % COLS;
+                if (r < rows && first_n + c < p.N)
+                    out[(size_t)r * p.N + c] = *(const __attribute__((address_space(3))) T *)(mine + r * PITCH + c * (int)sizeof(T));
+            }
+        }
+    }
+}
+
+template <typename Op, typename T>
+void launch_size(const TileArgs &p, hipStream_t stream)
+{
+    auto tiles = [&](int bm, int bn) { return (unsigned)(((p.M + bm - 1) / bm) * (int64_t)((p.N + bn - 1) / bn)); };
+    if (tiles(256, 256) >= 192)
+        hipLaunchKernelGGL((tile_kernel<Op, T, 256, 256, 2, 2>), dim3(tiles(256, 256)), dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL((tile_kernel<Op, T, 64, 64, 2, 2>), dim3(tiles(64, 64)), dim3(256), 0, stream, p);
+}
+
+} // namespace
+
+int launch_tile_product(const TileArgs &p, bool bf16, int out_dtype, const char *name, hipStream_t stream)
+{
+    REXSC_CHECK_ARG(p.a_stride < MAX_ROW_BYTES && p.b_stride < MAX_ROW_BYTES,
+                    "int8 linear: operand rows of %zu and %zu bytes, at most %zu are supported", p.a_stride, p.b_stride,
+                    MAX_ROW_BYTES - 1);
+    const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64);
+    REXSC_CHECK_ARG(tiles < (1ll << 31), "int8 linear: result of %d x %d is too large", p.M, p.N);
+    ProfScope prof(name, 2.0 * p.M * p.N * (bf16 ? p.kbytes / 2 : p.kbytes) * p.pieces, stream);
+    if (bf16) REXSC_DTYPE_SWITCH(out_dtype, launch_size<OpBF16, T>(p, stream));
+    else REXSC_DTYPE_SWITCH(out_dtype, launch_size<OpI8, T>(p, stream));
+    REXSC_CHECK_HIP(hipGetLastError());
+    return REXSC_OK;
+}
+
+} // namespace rexsc
