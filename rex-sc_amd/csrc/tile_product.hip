@@ -71,8 +71,8 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
     constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
     constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES; // loads of 8 rows x 128 bytes per wave and step
     static_assert(LA * WAVES * 8 == BM && LB * WAVES * 8 == BN, "tile rows must divide among the waves");
-    __shared__ __attribute__((aligned(1024))) char buf0[(BM + BN) * KSTEP];
-    __shared__ __attribute__((aligned(1024))) char buf1[(BM + BN) * KSTEP];
+    constexpr int BUF = (BM + BN) * KSTEP;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * BUF];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     int tm, tn;
     tile_of(blockIdx.x, (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, tm, tn);
@@ -96,17 +96,27 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
     const unsigned chunk = (unsigned)swizzle(wave * 8 + lane / 8, lane % 8) * 16;
     const char *base_a = p.a + (size_t)m0 * p.a_stride, *base_b = p.b + (size_t)n0 * p.b_stride;
     const int steps = (p.kbytes + KSTEP - 1) / KSTEP, total = steps * p.pieces;
-    const unsigned last_chunk = (unsigned)(p.kbytes - 1) / 16 * 16; // of a row: lanes behind it read it instead
 
     unsigned k = 0; // byte offset in the row of the step that is fetched next
     auto fetch = [&](char *buf) __attribute__((always_inline)) {
-        const unsigned left = last_chunk - k, c = chunk < left ? chunk : left;
+        // a chunk behind the row's end is put outside of the descriptor's range and arrives as zeros
+        const unsigned c = k + chunk < (unsigned)p.kbytes ? chunk : 0x80000000u;
 #pragma unroll
-        for (int i = 0; i < LA; i++) load_to_lds(base_a, offa[i] + c, k, buf + (i * WAVES + wave) * 1024);
+        for (int i = 0; i < LA; i++) load_to_lds(base_a, c + offa[i], k, buf + (i * WAVES + wave) * 1024);
 #pragma unroll
-        for (int i = 0; i < LB; i++) load_to_lds(base_b, offb[i] + c, k, buf + BM * KSTEP + (i * WAVES + wave) * 1024);
+        for (int i = 0; i < LB; i++) load_to_lds(base_b, c + offb[i], k, buf + BM * KSTEP + (i * WAVES + wave) * 1024);
         k += KSTEP;
         if (k >= (unsigned)p.kbytes) { k = 0; base_a += p.piece_stride; }
+    };
+    // int8 rows whose last chunk is not full: what stands behind the row may be anything, and becomes 0 in a's tile
+    const int tail = p.kbytes % 16;
+    auto clear_tail = [&](lds_char *buf) __attribute__((always_inline)) {
+        const int c = p.kbytes % KSTEP / 16;
+        for (int r = threadIdx.x; r < BM; r += WAVES * 64) {
+            lds_i32x4 *at = (lds_i32x4 *)(buf + r * KSTEP + swizzle(r, c) * 16);
+            *at = keep_before(*at, 0, tail);
+        }
+        __syncthreads();
     };
 
     const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
@@ -115,66 +125,46 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
     // Rows 16 apart lie at the same place of the swizzle, and the second half's chunks 64 bytes across it, so a
     // fragment's address is one of two lane offsets plus a constant.
     const int q = lane % 16 * KSTEP + swizzle(lane % 16, lane / 16) * 16;
-    const lds_char *const pa[2][2] = {{(const lds_char *)buf0 + wm * KSTEP + q, (const lds_char *)buf0 + wm * KSTEP + (q ^ 64)},
-                                      {(const lds_char *)buf1 + wm * KSTEP + q, (const lds_char *)buf1 + wm * KSTEP + (q ^ 64)}};
-    const lds_char *const pb[2][2] = {
-        {(const lds_char *)buf0 + (BM + wn) * KSTEP + q, (const lds_char *)buf0 + (BM + wn) * KSTEP + (q ^ 64)},
-        {(const lds_char *)buf1 + (BM + wn) * KSTEP + q, (const lds_char *)buf1 + (BM + wn) * KSTEP + (q ^ 64)}};
-    // Multiplies the fragments of `half` while (reads) the next half's are read from buffer `buf`: a row of a's
-    // fragment is replaced as soon as its products are issued, so the second set costs no more registers than b's.
-    // keep: bytes of this step that belong to the row, where it is the last (int8: what stands behind may be anything).
-    auto multiply = [&](int half, auto reads, int buf, auto masked, int keep) __attribute__((always_inline)) {
-        const int next = half ^ 1;
+    lds_char *const base = (lds_char *)lds;
+    const int at_a[2] = {wm * KSTEP + q, wm * KSTEP + (q ^ 64)}, at_b[2] = {(BM + wn) * KSTEP + q, (BM + wn) * KSTEP + (q ^ 64)};
+    // Multiplies the fragments of `half` while the next half's are read from `buf`: a row of a's fragment is replaced as
+    // soon as its products are issued, so the second set costs no more registers than b's.
+    auto multiply = [&](auto half_, const lds_char *buf) __attribute__((always_inline)) {
+        constexpr int half = half_, next = half ^ 1;
+        const lds_char *const ra = buf + at_a[next], *const rb = buf + at_b[next];
 #pragma unroll
         for (int i = 0; i < FM; i++) {
-            if constexpr (masked) fa[half][i] = keep_before(fa[half][i], (half * 4 + lane / 16) * 16, keep);
 #pragma unroll
             for (int j = 0; j < FN; j++) acc[i][j] = mma(Op{}, fb[half][j], fa[half][i], acc[i][j]);
-            if constexpr (reads) {
-                fa[next][i] = *(const lds_i32x4 *)(pa[buf][next] + i * 16 * KSTEP);
+            fa[next][i] = *(const lds_i32x4 *)(ra + i * 16 * KSTEP);
 #pragma unroll
-                for (int j = i * FN / FM; j < (i + 1) * FN / FM; j++) fb[next][j] = *(const lds_i32x4 *)(pb[buf][next] + j * 16 * KSTEP);
-            }
+            for (int j = i * FN / FM; j < (i + 1) * FN / FM; j++) fb[next][j] = *(const lds_i32x4 *)(rb + j * 16 * KSTEP);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // One step from `cur`: its second half is read while the first is multiplied; then, with every wave's fragments of
-    // `cur` in registers and `nxt` filled, one barrier, behind which `cur` is filled anew and the first half of `nxt`
-    // is read while the second half is multiplied.
-    constexpr std::integral_constant<bool, false> no{};
-    constexpr std::integral_constant<bool, true> yes{};
-    auto step = [&](int cur, bool refill) __attribute__((always_inline)) {
-        multiply(0, yes, cur, no, 0);
-        loads_done();
-        __syncthreads();
-        if (refill) fetch(cur == 0 ? buf0 : buf1);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(1, yes, cur ^ 1, no, 0);
-    };
-    auto last_step = [&](int cur) __attribute__((always_inline)) {
-        const int keep = p.kbytes - (steps - 1) * KSTEP;
-        multiply(0, yes, cur, yes, keep);
-        multiply(1, no, cur, yes, keep);
-    };
+    // A step's second half is read while its first is multiplied; then, with every wave's fragments of this buffer in
+    // registers and the other buffer filled, one barrier, behind which this buffer is filled anew and the first half of
+    // the other is read while the second half is multiplied.  (Behind the last step that reads what is not used.)
     if (total > 0) {
-        fetch(buf0);
+        fetch(lds);
         loads_done();
         __syncthreads();
-        if (total > 1) fetch(buf1);
+        if (tail && total == 1) clear_tail(base);
+        if (total > 1) fetch(lds + BUF);
 #pragma unroll
-        for (int i = 0; i < FM; i++) fa[0][i] = *(const lds_i32x4 *)(pa[0][0] + i * 16 * KSTEP);
+        for (int i = 0; i < FM; i++) fa[0][i] = *(const lds_i32x4 *)(base + at_a[0] + i * 16 * KSTEP);
 #pragma unroll
-        for (int j = 0; j < FN; j++) fb[0][j] = *(const lds_i32x4 *)(pb[0][0] + j * 16 * KSTEP);
-        int s = 0;
-        for (; s + 2 < total; s += 2) {
-            step(0, true);
-            step(1, s + 3 < total);
-        }
-        if (s + 2 == total) {
-            step(0, false);
-            last_step(1);
-        } else {
-            last_step(0);
+        for (int j = 0; j < FN; j++) fb[0][j] = *(const lds_i32x4 *)(base + at_b[0] + j * 16 * KSTEP);
+        int cur = 0;
+        for (int s = 0; s < total; s++) {
+            multiply(std::integral_constant<int, 0>{}, base + cur);
+            loads_done();
+            __syncthreads();
+            if (tail && s + 2 == total) clear_tail(base + (cur ^ BUF));
+            if (s + 2 < total) fetch(lds + cur);
+            __builtin_amdgcn_sched_barrier(0);
+            cur ^= BUF;
+            multiply(std::integral_constant<int, 1>{}, base + cur);
         }
     }
 
@@ -184,7 +174,8 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
     // the banks, which spreads the 16 rows of a write over all of them.
     constexpr int COLS = BN / WN, ROWS = BM / WM, VEC = 16 / sizeof(T), PITCH = COLS * sizeof(T) + 16;
     constexpr int PART = sizeof(T) == 4 ? 32 : 64, CR = ROWS < PART ? ROWS : PART; // rows that are turned at a time
-    static_assert((WAVES + 1) / 2 * CR * PITCH <= (BM + BN) * KSTEP, "a buffer holds half of the waves' shares");
+    static_assert(WAVES * CR * PITCH <= 2 * BUF, "the waves' shares fit the buffers");
+    static_assert((BUF & (BUF - 1)) == 0, "buffers are switched by an exclusive or");
     const int first_n = n0 + wn;
     float sb[FN][4], bias[FN][4];
 #pragma unroll
@@ -196,7 +187,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
             bias[j][e] = p.bias ? load_any(p.bias, p.bias_dtype, c) : 0.f;
         }
     __syncthreads();
-    lds_char *const mine = (lds_char *)(wave % 2 ? buf1 : buf0) + wave / 2 * (CR * PITCH);
+    lds_char *const mine = base + wave * (CR * PITCH);
     const bool wide = ((size_t)p.N * sizeof(T) % 16 == 0) && ((uintptr_t)p.y % 16 == 0);
 #pragma unroll
     for (int r0 = 0; r0 < ROWS; r0 += CR) {
@@ -237,7 +228,7 @@ void launch_size(const TileArgs &p, hipStream_t stream)
 {
     auto tiles = [&](int bm, int bn) { return (unsigned)(((p.M + bm - 1) / bm) * (int64_t)((p.N + bn - 1) / bn)); };
     if (tiles(256, 256) >= 192)
-        hipLaunchKernelGGL((tile_kernel<Op, T, 256, 256, 2, 2>), dim3(tiles(256, 256)), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((tile_kernel<Op, T, 256, 256, 2, 4>), dim3(tiles(256, 256)), dim3(512), 0, stream, p);
     else
         hipLaunchKernelGGL((tile_kernel<Op, T, 64, 64, 2, 2>), dim3(tiles(64, 64)), dim3(256), 0, stream, p);
 }
