@@ -10,7 +10,11 @@
 // results, two hold 16 and serve 16-bit results, whose own rounding is far coarser), so nothing but the float32
 // accumulation is rounded.  Pieces and transposed operands are laid out in the workspace first, which makes both
 // gradients the same product of two row-major operands as the forward pass.
+#include <stdlib.h>
+
+#include "few_rows.h"
 #include "profile.h"
+#include "quant8.h"
 #include "tile_product.h"
 
 namespace rexsc {
@@ -19,59 +23,107 @@ namespace {
 constexpr int MAX_K = 131071; // 128 * 128 * K < 2^31
 
 // ---- rows to 8 bits ------------------------------------------------------------------------------
-constexpr int Q_THREADS = 256;
-constexpr float SMALL = 7.888609052210118e-31f; // 2^-100: below it 127 / a could overflow
-constexpr float LIFT = 1.2676506002282294e30f;  // 2^100
+// Bound by memory: x is read once.  A row lives in the registers of TPR threads (a wave, or a block of 256 or 1024), 16
+// elements a thread at most, all its loads in flight together; rows longer than 16384 are read twice.
+constexpr int Q_EPT = 16;
 
-// The integer nearest to 127 x / a, ties to even, exactly.  x * inv with inv = fl(127 / a) is off by less than 1e-4;
-// where that could decide, 127 x is compared with (the half-way point) * a in 64 bits, where both are exact.
-__device__ __forceinline__ int nearest127(float x, float a, float inv)
+struct QuantArgs {
+    const void *x;
+    int8_t *q;
+    float *scale;
+    size_t rows, x_stride, q_stride;
+    int cols;
+};
+
+// Largest magnitude of a row over its TPR threads.
+template <int TPR>
+__device__ __forceinline__ unsigned row_top(unsigned t, unsigned (&lds)[16])
 {
-    const float t = x * inv, r = rintf(t), d = t - r;
-    int q = (int)r;
-    if (fabsf(fabsf(d) - 0.5f) < 1e-3f) {
-        const int o = d >= 0.f ? q + 1 : q - 1;
-        const double v = 127.0 * (double)x, half = 0.5 * (double)(q + o) * (double)a;
-        const int lo = q < o ? q : o, hi = q < o ? o : q;
-        q = v < half ? lo : v > half ? hi : (lo & 1) ? hi : lo;
+    t = wave_max(t);
+    if constexpr (TPR > 64) {
+        if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = t;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TPR / 64; i++) t = max(t, lds[i]);
     }
-    return q;
+    return t;
 }
 
-struct RowScale { float a, inv, lift, scale; };
-__device__ __forceinline__ RowScale row_scale(unsigned top)
+template <typename T, int V, int TPR>
+__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void quantize_rows_kernel(QuantArgs p)
 {
-    RowScale r;
-    const float a = __uint_as_float(top);
-    if (top >= 0x7f800000u) { r.a = 1.f; r.inv = 0.f; r.lift = 0.f; r.scale = __uint_as_float(0x7fc00000u); return r; }
-    r.scale = a / 127.f;
-    r.lift = a < SMALL ? LIFT : 1.f; // exact: both powers of two
-    r.a = a * r.lift;
-    r.inv = a > 0.f ? 127.f / r.a : 0.f;
-    return r;
-}
-__device__ __forceinline__ int quant(float x, const RowScale &r)
-{   // a row with a NaN or an infinity: all zeros
-    return r.lift == 0.f || r.inv == 0.f ? 0 : nearest127(x * r.lift, r.a, r.inv);
+    constexpr int NV = Q_EPT / V;
+    typedef typename VecOf<T, V>::type vec;
+    __shared__ unsigned lds[16];
+    const int tid = TPR == 64 ? threadIdx.x % 64 : threadIdx.x;
+    const size_t row = TPR == 64 ? (size_t)blockIdx.x * 4 + threadIdx.x / 64 : blockIdx.x;
+    if (row >= p.rows) return; // TPR 64 only: a whole wave
+    const T *src = (const T *)p.x + row * p.x_stride;
+    vec v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * TPR + tid) * V;
+        v[i] = c < p.cols ? *(const vec *)(src + c) : vec{};
+    }
+    float x[NV][V];
+    unsigned t = 0;
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            if constexpr (V == 1) x[i][j] = (float)v[i];
+            else x[i][j] = (float)v[i][j];
+            t = max(t, mag_bits(x[i][j]));
+        }
+    const RowScale rs = row_scale(row_top<TPR>(t, lds));
+    int8_t *dst = p.q + row * p.q_stride;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * TPR + tid) * V;
+        if (c < p.cols) {
+            typename VecOf<int8_t, V>::type q;
+            if constexpr (V == 1) q = (int8_t)quant8(x[i][0], rs);
+            else
+#pragma unroll
+                for (int j = 0; j < V; j++) q[j] = (int8_t)quant8(x[i][j], rs);
+            *(typename VecOf<int8_t, V>::type *)(dst + c) = q;
+        }
+    }
+    for (size_t c = (size_t)p.cols + tid; c < p.q_stride; c += TPR) dst[c] = 0;
+    if (tid == 0) p.scale[row] = rs.scale;
 }
 
 template <typename T>
-__global__ __launch_bounds__(Q_THREADS) void quantize_rows_kernel(const T *x, size_t x_stride, int cols, int8_t *q,
-                                                                  size_t q_stride, float *scale)
+__global__ __launch_bounds__(1024) void quantize_long_rows_kernel(QuantArgs p)
 {
-    __shared__ unsigned lds[Q_THREADS / 64];
-    const T *src = x + (size_t)blockIdx.x * x_stride;
-    int8_t *dst = q + (size_t)blockIdx.x * q_stride;
-    unsigned top = 0;
-    for (int c = threadIdx.x; c < cols; c += Q_THREADS) top = max(top, mag_bits((float)src[c]));
-    top = wave_max(top);
-    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < Q_THREADS / 64; i++) top = max(top, lds[i]);
-    const RowScale rs = row_scale(top);
-    for (size_t c = threadIdx.x; c < q_stride; c += Q_THREADS) dst[c] = c < (size_t)cols ? (int8_t)quant((float)src[c], rs) : 0;
-    if (threadIdx.x == 0) scale[blockIdx.x] = rs.scale;
+    __shared__ unsigned lds[16];
+    const T *src = (const T *)p.x + blockIdx.x * p.x_stride;
+    unsigned t = 0;
+    for (int c = threadIdx.x; c < p.cols; c += 1024) t = max(t, mag_bits((float)src[c]));
+    const RowScale rs = row_scale(row_top<1024>(t, lds));
+    int8_t *dst = p.q + blockIdx.x * p.q_stride;
+    for (size_t c = threadIdx.x; c < p.q_stride; c += 1024) dst[c] = c < (size_t)p.cols ? (int8_t)quant8((float)src[c], rs) : (int8_t)0;
+    if (threadIdx.x == 0) p.scale[blockIdx.x] = rs.scale;
+}
+
+template <typename T, int V>
+void launch_quantize_v(const QuantArgs &p, hipStream_t s)
+{
+    const unsigned rows = (unsigned)p.rows;
+    if (p.cols <= 64 * Q_EPT) hipLaunchKernelGGL((quantize_rows_kernel<T, V, 64>), dim3((rows + 3) / 4), dim3(256), 0, s, p);
+    else if (p.cols <= 256 * Q_EPT) hipLaunchKernelGGL((quantize_rows_kernel<T, V, 256>), dim3(rows), dim3(256), 0, s, p);
+    else if (p.cols <= 1024 * Q_EPT) hipLaunchKernelGGL((quantize_rows_kernel<T, V, 1024>), dim3(rows), dim3(1024), 0, s, p);
+    else hipLaunchKernelGGL(quantize_long_rows_kernel<T>, dim3(rows), dim3(1024), 0, s, p);
+}
+
+// Vectors of 16 bytes where every row of x starts on one (and its int8 row, a multiple of 16 bytes, on V).
+template <typename T>
+void launch_quantize_t(const QuantArgs &p, hipStream_t s)
+{
+    constexpr int V = 16 / sizeof(T);
+    const bool aligned = (uintptr_t)p.x % 16 == 0 && p.cols % V == 0 && (p.x_stride % V == 0 || p.rows == 1);
+    if (aligned) launch_quantize_v<T, V>(p, s);
+    else launch_quantize_v<T, 1>(p, s);
 }
 
 // ---- operands of the gradients ---------------------------------------------------------------------
@@ -177,7 +229,7 @@ int check_rows8(const char *what, const void *q, int64_t stride, int K)
 inline int64_t pad64(int64_t n) { return (n + 63) / 64 * 64; }
 inline int pieces_of(int dtype) { return dtype == REXSC_F32 ? 3 : 2; }
 
-struct Space { size_t tokens, scales, pieces, transposed, part, total; };
+struct Space { size_t tokens, scales, pieces, transposed, part, product, total; };
 
 Space space(const rexsc_int8_desc *d, int what)
 {
@@ -185,15 +237,20 @@ Space space(const rexsc_int8_desc *d, int what)
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at = align_up(at + bytes, 256); return o; };
     const size_t M = d->M, N = d->N, K = d->K;
-    if (what == REXSC_INT8_LINEAR) {
+    if (what == REXSC_INT8_PRODUCT) {
+        s.product = take(tile_product_workspace(d->M, d->N, d->K, 1));
+    } else if (what == REXSC_INT8_LINEAR) {
+        s.product = take(tile_product_workspace(d->M, d->N, d->K, 1));
         s.tokens = take(M * align_up(K, 128));
         s.scales = take(M * 4);
     } else if (what == REXSC_INT8_GRAD_INPUT) {
         const size_t ld = pad64(N);
+        s.product = take(tile_product_workspace(d->M, d->K, (int)ld * 2, pieces_of(d->dtype)));
         s.pieces = take(M * ld * pieces_of(d->dtype) * 2);
         s.transposed = take(K * ld * 2);
     } else if (what == REXSC_INT8_GRAD_WEIGHT) {
         const size_t ld = pad64(M);
+        s.product = take(tile_product_workspace(d->N, d->K, (int)ld * 2, pieces_of(d->weight_dtype)));
         s.pieces = take(N * ld * pieces_of(d->weight_dtype) * 2);
         s.transposed = take(K * ld * 2);
         s.part = take(ld / 64 * N * 4);
@@ -213,19 +270,20 @@ int check_space(const Space &s, const void *workspace, size_t bytes)
 }
 
 int product(const rexsc_int8_desc *d, const int8_t *a, int64_t a_stride, const float *a_scale, const int8_t *b,
-            const float *b_scale, const void *bias, void *y, hipStream_t stream)
+            const float *b_scale, const void *bias, void *y, void *space, hipStream_t stream)
 {
     const TileArgs p{(const char *)a, (const char *)b, (size_t)a_stride, (size_t)d->b_stride, d->M, d->N, d->K, 1, 0,
                      a_scale, b_scale, bias, d->bias_dtype, y};
-    return launch_tile_product(p, false, d->dtype, "int8_product", stream);
+    if (d->M <= FEW_ROWS && !getenv("REXSC_TUNE_INT8_TILE")) return launch_few_rows(p, d->dtype, stream);
+    return launch_tile_product(p, false, d->dtype, space, "int8_product", stream);
 }
 
 int launch_quantize(const void *x, int dtype, size_t rows, size_t cols, size_t x_stride, int8_t *q, size_t q_stride,
                     float *scale, hipStream_t stream)
 {
     ProfScope prof("quantize_rows", (double)rows * cols * (dtype_size(dtype) + 1), stream);
-    REXSC_DTYPE_SWITCH(dtype, hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3((unsigned)rows), dim3(Q_THREADS), 0, stream,
-                                                 (const T *)x, x_stride, (int)cols, q, q_stride, scale));
+    const QuantArgs p{x, q, scale, rows, x_stride, q_stride, (int)cols};
+    REXSC_DTYPE_SWITCH(dtype, launch_quantize_t<T>(p, stream));
     REXSC_CHECK_HIP(hipGetLastError());
     return REXSC_OK;
 }
@@ -268,8 +326,9 @@ extern "C" int rexsc_int8_product(const rexsc_int8_desc *d, const int8_t *a, con
     if (int rc = check_rows8("tokens", a, d->a_stride, d->K)) return rc;
     if (int rc = check_rows8("channels", b, d->b_stride, d->K)) return rc;
     REXSC_CHECK_ARG(a_scale && b_scale && y, "null pointer");
-    if (int rc = check_space(space(d, REXSC_INT8_PRODUCT), workspace, workspace_bytes)) return rc;
-    return product(d, a, d->a_stride, a_scale, b, b_scale, bias, y, (hipStream_t)stream);
+    const Space s = space(d, REXSC_INT8_PRODUCT);
+    if (int rc = check_space(s, workspace, workspace_bytes)) return rc;
+    return product(d, a, d->a_stride, a_scale, b, b_scale, bias, y, (char *)workspace + s.product, (hipStream_t)stream);
 }
 
 extern "C" int rexsc_int8_linear(const rexsc_int8_desc *d, const void *x, const int8_t *b, const float *b_scale,
@@ -284,11 +343,16 @@ extern "C" int rexsc_int8_linear(const rexsc_int8_desc *d, const void *x, const 
                     "int8 linear: x is not aligned to its element, or its rows overlap (distance %lld)", (long long)d->x_stride);
     const Space s = space(d, REXSC_INT8_LINEAR);
     if (int rc = check_space(s, workspace, workspace_bytes)) return rc;
+    if (few_rows_fuses(d->M, d->K, x, (size_t)d->x_stride, d->dtype)) {
+        const TileArgs p{nullptr, (const char *)b, 0, (size_t)d->b_stride, d->M, d->N, d->K, 1, 0, nullptr, b_scale, bias,
+                         d->bias_dtype, y};
+        return launch_few_rows_fused(p, x, (size_t)d->x_stride, d->dtype, stream);
+    }
     int8_t *q = (int8_t *)workspace + s.tokens;
     float *scale = (float *)((char *)workspace + s.scales);
     const size_t stride = align_up(d->K, 128);
     if (int rc = launch_quantize(x, d->dtype, d->M, d->K, d->x_stride, q, stride, scale, stream)) return rc;
-    return product(d, q, (int64_t)stride, scale, b, b_scale, bias, y, stream);
+    return product(d, q, (int64_t)stride, scale, b, b_scale, bias, y, (char *)workspace + s.product, stream);
 }
 
 extern "C" int rexsc_int8_grad_input(const rexsc_int8_desc *d, const void *g, const int8_t *b, const float *b_scale, void *dx,
@@ -318,7 +382,7 @@ extern "C" int rexsc_int8_grad_input(const rexsc_int8_desc *d, const void *g, co
     }
     const TileArgs p{(const char *)pieces, (const char *)bt, (size_t)ld * 2, (size_t)ld * 2, d->M, d->K, ld * 2, P,
                      (size_t)d->M * ld * 2, nullptr, nullptr, nullptr, REXSC_F32, dx};
-    return launch_tile_product(p, true, d->dtype, "int8_grad_input", stream);
+    return launch_tile_product(p, true, d->dtype, (char *)workspace + s.product, "int8_grad_input", stream);
 }
 
 extern "C" int rexsc_int8_grad_weight(const rexsc_int8_desc *d, const void *g, const int8_t *a, const float *a_scale, void *dw,
@@ -357,5 +421,5 @@ extern "C" int rexsc_int8_grad_weight(const rexsc_int8_desc *d, const void *g, c
     // without tokens the reduction is empty and the kernel writes zeros
     const TileArgs p{(const char *)pieces, (const char *)at, (size_t)ld * 2, (size_t)ld * 2, d->N, d->K, ld * 2, P,
                      (size_t)d->N * ld * 2, nullptr, nullptr, nullptr, REXSC_F32, dw};
-    return launch_tile_product(p, true, d->weight_dtype, "int8_grad_weight", stream);
+    return launch_tile_product(p, true, d->weight_dtype, (char *)workspace + s.product, "int8_grad_weight", stream);
 }

@@ -20,7 +20,9 @@ struct TileArgs {
 
 constexpr size_t MAX_ROW_BYTES = 8u << 20; // 256 rows stay within 32-bit offsets
 
+// Bytes of workspace for partial results (0: the reduction is not split); 16-byte aligned.
+size_t tile_product_workspace(int M, int N, int kbytes, int pieces);
 // out_dtype: y's type; bf16: the operands are bfloat16 and kbytes is a multiple of 128, else int8.
-int launch_tile_product(const TileArgs &p, bool bf16, int out_dtype, const char *name, hipStream_t stream);
+int launch_tile_product(const TileArgs &p, bool bf16, int out_dtype, void *workspace, const char *name, hipStream_t stream);
 
 } // namespace rexsc

@@ -1,4 +1,6 @@
 // Product of two row-major operands: c[m][n] = sum_k a[m][k] b[n][k].
+#include <stdlib.h>
+
 #include <type_traits>
 
 #include "profile.h"
@@ -65,8 +67,10 @@ __device__ __forceinline__ void tile_of(unsigned bid, int tiles_m, int tiles_n, 
     tn = (int)(r / rows);
 }
 
-template <typename Op, typename T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
+// SPLIT: the grid holds `splits` times the tiles, and a block sums only its share of the steps, into a partial result
+// of the accumulator's type (T) that join_kernel finishes.
+template <typename Op, typename T, int BM, int BN, int WM, int WN, bool SPLIT>
+__global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int splits)
 {
     constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
     constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES; // loads of 8 rows x 128 bytes per wave and step
@@ -75,7 +79,8 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
     __shared__ __attribute__((aligned(1024))) char lds[2 * BUF];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     int tm, tn;
-    tile_of(blockIdx.x, (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, tm, tn);
+    const int share = SPLIT ? (int)(blockIdx.x % splits) : 0;
+    tile_of(SPLIT ? blockIdx.x / splits : blockIdx.x, (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const int last_m = p.M - 1 - m0, last_n = p.N - 1 - n0; // rows behind the operand's last read that one again
 
@@ -95,9 +100,12 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
     }
     const unsigned chunk = (unsigned)swizzle(wave * 8 + lane / 8, lane % 8) * 16;
     const char *base_a = p.a + (size_t)m0 * p.a_stride, *base_b = p.b + (size_t)n0 * p.b_stride;
-    const int steps = (p.kbytes + KSTEP - 1) / KSTEP, total = steps * p.pieces;
+    const int steps = (p.kbytes + KSTEP - 1) / KSTEP, every = steps * p.pieces;
+    const int begin = SPLIT ? (int)((int64_t)every * share / splits) : 0;
+    const int total = (SPLIT ? (int)((int64_t)every * (share + 1) / splits) : every) - begin;
+    if constexpr (SPLIT) base_a += (size_t)(begin / steps) * p.piece_stride;
 
-    unsigned k = 0; // byte offset in the row of the step that is fetched next
+    unsigned k = SPLIT ? (unsigned)(begin % steps) * KSTEP : 0; // byte offset in the row of the step that is fetched next
     auto fetch = [&](char *buf) __attribute__((always_inline)) {
         // a chunk behind the row's end is put outside of the descriptor's range and arrives as zeros
         const unsigned c = k + chunk < (unsigned)p.kbytes ? chunk : 0x80000000u;
@@ -109,7 +117,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
         if (k >= (unsigned)p.kbytes) { k = 0; base_a += p.piece_stride; }
     };
     // int8 rows whose last chunk is not full: what stands behind the row may be anything, and becomes 0 in a's tile
-    const int tail = p.kbytes % 16;
+    const int tail = begin + total == every ? p.kbytes % 16 : 0;
     auto clear_tail = [&](lds_char *buf) __attribute__((always_inline)) {
         const int c = p.kbytes % KSTEP / 16;
         for (int r = threadIdx.x; r < BM; r += WAVES * 64) {
@@ -183,29 +191,33 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const int n = first_n + j * 16 + lane / 16 * 4 + e, c = n < p.N ? n : p.N - 1;
-            sb[j][e] = p.b_scale ? p.b_scale[c] : 1.f;
-            bias[j][e] = p.bias ? load_any(p.bias, p.bias_dtype, c) : 0.f;
+            sb[j][e] = !SPLIT && p.b_scale ? p.b_scale[c] : 1.f;
+            bias[j][e] = !SPLIT && p.bias ? load_any(p.bias, p.bias_dtype, c) : 0.f;
         }
     __syncthreads();
     lds_char *const mine = base + wave * (CR * PITCH);
-    const bool wide = ((size_t)p.N * sizeof(T) % 16 == 0) && ((uintptr_t)p.y % 16 == 0);
+    T *const y = (T *)p.y + (SPLIT ? (size_t)share * p.M * p.N : 0);
+    const bool wide = ((size_t)p.N * sizeof(T) % 16 == 0) && ((uintptr_t)y % 16 == 0);
 #pragma unroll
     for (int r0 = 0; r0 < ROWS; r0 += CR) {
 #pragma unroll
         for (int i = 0; i < CR / 16; i++) {
             const int m = m0 + wm + r0 + i * 16 + lane % 16;
-            const float sa = p.a_scale ? p.a_scale[m < p.M ? m : p.M - 1] : 1.f;
+            const float sa = !SPLIT && p.a_scale ? p.a_scale[m < p.M ? m : p.M - 1] : 1.f;
 #pragma unroll
             for (int j = 0; j < FN; j++) {
                 typename VecOf<T, 4>::type v;
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = (T)((float)acc[r0 / 16 + i][j][e] * sa * sb[j][e] + bias[j][e]);
+                for (int e = 0; e < 4; e++) {
+                    if constexpr (SPLIT) v[e] = acc[r0 / 16 + i][j][e];
+                    else v[e] = (T)((float)acc[r0 / 16 + i][j][e] * sa * sb[j][e] + bias[j][e]);
+                }
                 *(__attribute__((address_space(3))) typename VecOf<T, 4>::type *)(mine + (i * 16 + lane % 16) * PITCH +
                                                                                   (j * 16 + lane / 16 * 4) * (int)sizeof(T)) = v;
             }
         }
         const int rows = p.M - (m0 + wm + r0); // of this part, that exist
-        T *out = (T *)p.y + (size_t)(m0 + wm + r0) * p.N + first_n;
+        T *out = y + (size_t)(m0 + wm + r0) * p.N + first_n;
         if (wide) {
 #pragma unroll
             for (int t = 0; t < CR * COLS / VEC / 64; t++) {
@@ -223,30 +235,121 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p)
     }
 }
 
-template <typename Op, typename T>
-void launch_size(const TileArgs &p, hipStream_t stream)
+// y = (sum of the partial results, in order) * scales + bias; ACC: int or float.  Four elements per thread.
+template <typename ACC, typename T>
+__global__ __launch_bounds__(256) void join_kernel(TileArgs p, const ACC *part, int splits)
 {
-    auto tiles = [&](int bm, int bn) { return (unsigned)(((p.M + bm - 1) / bm) * (int64_t)((p.N + bn - 1) / bn)); };
-    if (tiles(256, 256) >= 192)
-        hipLaunchKernelGGL((tile_kernel<Op, T, 256, 256, 2, 4>), dim3(tiles(256, 256)), dim3(512), 0, stream, p);
+    const size_t all = (size_t)p.M * p.N, at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= all) return;
+    ACC s[4] = {};
+    const int n = all - at < 4 ? (int)(all - at) : 4;
+    if (n == 4 && all % 4 == 0)
+        for (int z = 0; z < splits; z++) {
+            const typename VecOf<ACC, 4>::type v = *(const typename VecOf<ACC, 4>::type *)(part + z * all + at);
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] += v[e];
+        }
     else
-        hipLaunchKernelGGL((tile_kernel<Op, T, 64, 64, 2, 2>), dim3(tiles(64, 64)), dim3(256), 0, stream, p);
+        for (int z = 0; z < splits; z++)
+            for (int e = 0; e < n; e++) s[e] += part[z * all + at + e];
+    unsigned m = (unsigned)(at / p.N), c = (unsigned)(at - (size_t)m * p.N);
+    for (int e = 0; e < n; e++) {
+        float v = (float)s[e];
+        if (p.a_scale) v *= p.a_scale[m];
+        if (p.b_scale) v *= p.b_scale[c];
+        if (p.bias) v += load_any(p.bias, p.bias_dtype, c);
+        ((T *)p.y)[at + e] = (T)v;
+        if (++c == (unsigned)p.N) { c = 0; m++; }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+constexpr int CUS = 256, MAX_SPLITS = 16;
+
+struct TilePlan { int size, splits; };
+
+int tune(const char *name)
+{
+    const char *v = getenv(name);
+    return v ? atoi(v) : 0;
+}
+
+// Tile size by what a launch takes when its busiest CU gets n tiles, in units of one 256 x 256 tile (measured at
+// K = 4096 int8, 57 us each): one block of 256 x 256 per CU, n; two of 128 x 128 side by side 0.61, a single one 0.44;
+// 64 x 64, up to five side by side, 0.08 + 0.11 n.  E.g. 2048 x 4096: 38 us in 128s against 53 in 256s or 64s;
+// 4096 x 4096: 62 in 256s against 71 in 128s; 512 x 4096: 21 in 64s against 26 in 128s.
+// The reduction is split over blocks only where the result has tiles for less than half of the CUs and each share
+// keeps 16 steps: the partial results cost a second launch.  300 x 300 x 16384: 17 us in 8 shares against 64 in one;
+// with tiles for every CU, splitting lost in each case measured (256 x 4096 x 4096: 15 us against 20).
+TilePlan tile_plan(int M, int N, int kbytes, int pieces)
+{
+    const int steps = (kbytes + KSTEP - 1) / KSTEP * pieces;
+    auto tiles = [&](int b) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b); };
+    auto busiest = [&](int b) { return (tiles(b) + CUS - 1) / CUS; };
+    const int64_t n256 = busiest(256), n128 = busiest(128), n64 = busiest(64);
+    const double t256 = (double)n256, t128 = 0.61 * (double)(n128 / 2) + 0.44 * (double)(n128 % 2), t64 = 0.08 + 0.11 * (double)n64;
+    TilePlan pl{t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64, 1};
+    if (const int t = tune("REXSC_TUNE_INT8_TILE")) pl.size = t == 256 || t == 128 ? t : 64;
+    const int64_t n = tiles(pl.size);
+    if (n > 0 && 2 * n <= CUS) {
+        const int64_t fill = CUS / n, keep = steps / 16;
+        pl.splits = (int)(fill < keep ? fill : keep);
+    }
+    if (const int t = tune("REXSC_TUNE_INT8_SPLITS")) pl.splits = t;
+    pl.splits = pl.splits > steps ? steps : pl.splits > MAX_SPLITS ? MAX_SPLITS : pl.splits;
+    if (pl.splits < 1) pl.splits = 1;
+    return pl;
+}
+
+template <typename Op, typename T, int BM, int BN, int WM, int WN>
+int launch_one(const TileArgs &p, int splits, void *workspace, hipStream_t stream)
+{
+    typedef std::conditional_t<std::is_same_v<Op, OpI8>, int, float> ACC;
+    const unsigned tiles = (unsigned)(((p.M + BM - 1) / BM) * (int64_t)((p.N + BN - 1) / BN));
+    if (splits == 1) {
+        hipLaunchKernelGGL((tile_kernel<Op, T, BM, BN, WM, WN, false>), dim3(tiles), dim3(WM * WN * 64), 0, stream, p, 1);
+        REXSC_CHECK_HIP(hipGetLastError());
+        return REXSC_OK;
+    }
+    TileArgs q = p;
+    q.y = workspace;
+    hipLaunchKernelGGL((tile_kernel<Op, ACC, BM, BN, WM, WN, true>), dim3(tiles * splits), dim3(WM * WN * 64), 0, stream, q, splits);
+    REXSC_CHECK_HIP(hipGetLastError());
+    const size_t all = (size_t)p.M * p.N;
+    hipLaunchKernelGGL((join_kernel<ACC, T>), dim3((unsigned)((all + 1023) / 1024)), dim3(256), 0, stream, p, (const ACC *)workspace,
+                       splits);
+    REXSC_CHECK_HIP(hipGetLastError());
+    return REXSC_OK;
+}
+
+template <typename Op, typename T>
+int launch_size(const TileArgs &p, const TilePlan &pl, void *workspace, hipStream_t stream)
+{
+    if (pl.size == 256) return launch_one<Op, T, 256, 256, 2, 4>(p, pl.splits, workspace, stream);
+    if (pl.size == 128) return launch_one<Op, T, 128, 128, 2, 2>(p, pl.splits, workspace, stream);
+    return launch_one<Op, T, 64, 64, 2, 2>(p, pl.splits, workspace, stream);
 }
 
 } // namespace
 
-int launch_tile_product(const TileArgs &p, bool bf16, int out_dtype, const char *name, hipStream_t stream)
+size_t tile_product_workspace(int M, int N, int kbytes, int pieces)
+{
+    if (M == 0 || N == 0) return 0;
+    const TilePlan pl = tile_plan(M, N, kbytes, pieces);
+    return pl.splits > 1 ? (size_t)pl.splits * M * N * 4 : 0;
+}
+
+int launch_tile_product(const TileArgs &p, bool bf16, int out_dtype, void *workspace, const char *name, hipStream_t stream)
 {
     REXSC_CHECK_ARG(p.a_stride < MAX_ROW_BYTES && p.b_stride < MAX_ROW_BYTES,
                     "int8 linear: operand rows of %zu and %zu bytes, at most %zu are supported", p.a_stride, p.b_stride,
                     MAX_ROW_BYTES - 1);
+    const TilePlan pl = tile_plan(p.M, p.N, p.kbytes, p.pieces);
     const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64);
-    REXSC_CHECK_ARG(tiles < (1ll << 31), "int8 linear: result of %d x %d is too large", p.M, p.N);
+    REXSC_CHECK_ARG(tiles * pl.splits < (1ll << 31), "int8 linear: result of %d x %d is too large", p.M, p.N);
     ProfScope prof(name, 2.0 * p.M * p.N * (bf16 ? p.kbytes / 2 : p.kbytes) * p.pieces, stream);
-    if (bf16) REXSC_DTYPE_SWITCH(out_dtype, launch_size<OpBF16, T>(p, stream));
-    else REXSC_DTYPE_SWITCH(out_dtype, launch_size<OpI8, T>(p, stream));
-    REXSC_CHECK_HIP(hipGetLastError());
-    return REXSC_OK;
+    if (bf16) REXSC_DTYPE_SWITCH(out_dtype, return (launch_size<OpBF16, T>(p, pl, workspace, stream)));
+    else REXSC_DTYPE_SWITCH(out_dtype, return (launch_size<OpI8, T>(p, pl, workspace, stream)));
 }
 
 } // namespace rexsc
