@@ -673,7 +673,32 @@ def calib_stats(a_bit, a_act, win_lo, win_hi):
 
 # ---- 8-bit linear layer --------------------------------------------------------------------------
 
+# These calls are short enough on the GPU for the host's share to count: pointers go over as plain integers, the stream
+# as the raw handle, and the current device is switched only where it is another one.
 _DTYPE_CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+class _SameDevice:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_same = _SameDevice()
+
+
+def _on(index):
+    """Context in which device `index` is the current one."""
+    return _same if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 ROW_PAD = 128  # int8 rows are laid out at a multiple of this many bytes: the product's step along the reduction
 MAX_K = 131071
 

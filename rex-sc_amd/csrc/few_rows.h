@@ -4,7 +4,8 @@
 
 namespace rexsc {
 
-constexpr int FEW_ROWS = 64; // most tokens the kernel takes
+constexpr int FEW_ROWS = 48; // most tokens the kernel takes
+bool few_rows_takes(int M, int N); // whether it is the faster one
 
 // y = a b^T of int8 operands with their epilogue, as TileArgs says (one piece).
 int launch_few_rows(const TileArgs &p, int out_dtype, hipStream_t stream);

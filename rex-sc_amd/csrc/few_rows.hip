@@ -1,4 +1,4 @@
-// The 8-bit product for up to 64 tokens.
+// The 8-bit product for up to 48 tokens.
 //
 // The weights are read once, straight into the matrix instruction's first operand: a load takes 64 bytes of 16 weight
 // rows, two loads of a wave a cache line of each, and the eight waves of a block take neighbouring lines of the same
@@ -40,35 +40,30 @@ struct FewArgs {
     size_t x_stride;
 };
 
-// FM: fragments of 16 tokens; FN: fragments of 16 channels per block; U0: loads per wave of the first round; X: type of the tokens, or int8_t: already in 8 bits.
-template <int FM, int FN, int U0, typename T, typename X>
+// A block makes 16 channels.  FM: fragments of 16 tokens; U0: loads per wave of the first round; X: type of the tokens, or int8_t: already in 8 bits.
+template <int FM, int U0, typename T, typename X>
 __global__ __launch_bounds__(THREADS) void few_rows_kernel(FewArgs g)
 {
     constexpr bool FUSED = sizeof(X) > 1;
     const TileArgs &p = g.p;
     __shared__ __attribute__((aligned(16))) int8_t tokens[FUSED ? FUSED_ELEMS + FUSED_ROWS * 80 : 16];
-    __shared__ int sums[WAVES][FM * FN][256];
+    __shared__ int sums[WAVES][FM][256];
     __shared__ unsigned top[FUSED ? FUSED_ROWS : 1];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int n0 = blockIdx.x * (16 * FN), K = p.kbytes;
+    const int n0 = blockIdx.x * 16, K = p.kbytes;
     const int at = wave * 128 + lane / 16 * 16; // this lane's 16 bytes; a wave takes 128 neighbouring bytes of its rows
 
-    const char *w[FN];
-#pragma unroll
-    for (int j = 0; j < FN; j++) {
-        const int n = n0 + j * 16 + lane % 16;
-        w[j] = p.b + (size_t)(n < p.N ? n : p.N - 1) * p.b_stride;
-    }
+    const int row = n0 + lane % 16;
+    const char *const w = p.b + (size_t)(row < p.N ? row : p.N - 1) * p.b_stride;
     // offset of load u in the round that begins at k0; behind the row's end the row's first chunk is read instead (the
     // tokens are 0 there)
     auto place = [&](int k0, int u) __attribute__((always_inline)) { return k0 + u / 2 * (WAVES * 128) + u % 2 * 64 + at; };
-    i32x4 wq[LOADS][FN];
+    i32x4 wq[LOADS];
     auto load_w = [&](int k0, auto loads) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < loads; u++) {
-            const int k = place(k0, u), o = k < K ? k : 0;
-#pragma unroll
-            for (int j = 0; j < FN; j++) wq[u][j] = *(const i32x4 *)(w[j] + o);
+            const int k = place(k0, u);
+            wq[u] = *(const i32x4 *)(w + (k < K ? k : 0));
         }
     };
     load_w(0, std::integral_constant<int, U0>{});
@@ -122,7 +117,7 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(FewArgs g)
         const int m = i * 16 + lane % 16, r = m < p.M ? m : p.M - 1;
         a[i] = FUSED ? (const char *)tokens + r * pitch : p.a + (size_t)r * p.a_stride;
     }
-    i32x4 acc[FM][FN] = {};
+    i32x4 acc[FM] = {};
     auto multiply = [&](int k0, auto loads) __attribute__((always_inline)) {
         i32x4 xq[loads][FM];
 #pragma unroll
@@ -140,9 +135,7 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(FewArgs g)
 #pragma unroll
         for (int u = 0; u < loads; u++)
 #pragma unroll
-            for (int i = 0; i < FM; i++)
-#pragma unroll
-                for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wq[u][j], xq[u][i], acc[i][j], 0, 0, 0);
+            for (int i = 0; i < FM; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wq[u], xq[u][i], acc[i], 0, 0, 0);
     };
     multiply(0, std::integral_constant<int, U0>{});
     if constexpr (U0 == LOADS) {
@@ -159,13 +152,10 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(FewArgs g)
 
     // a lane holds channels 4 (lane / 16) + e of token lane % 16
 #pragma unroll
-    for (int i = 0; i < FM; i++)
-#pragma unroll
-        for (int j = 0; j < FN; j++)
-            *(i32x4 *)&sums[wave][i * FN + j][(lane % 16) * 16 + lane / 16 * 4] = acc[i][j];
+    for (int i = 0; i < FM; i++) *(i32x4 *)&sums[wave][i][lane % 16 * 16 + lane / 16 * 4] = acc[i];
     __syncthreads();
-    for (int o = threadIdx.x; o < FM * FN * 256; o += THREADS) {
-        const int f = o / 256, m = f / FN * 16 + o % 256 / 16, n = n0 + f % FN * 16 + o % 16;
+    for (int o = threadIdx.x; o < FM * 256; o += THREADS) {
+        const int f = o / 256, m = o / 16, n = n0 + o % 16;
         if (m >= p.M || n >= p.N) continue;
         int s = 0;
 #pragma unroll
@@ -179,29 +169,14 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(FewArgs g)
     }
 }
 
-// Channels per block: 16, so that a layer's few thousand give every CU a block; 32 where that leaves blocks for all of
-// them and more than 16 tokens would be read from L2 by each (half as often).
-template <int FM, int FN, typename T, typename X>
-void launch_u(const FewArgs &g, hipStream_t stream)
-{
-    const dim3 grid((unsigned)((g.p.N + 16 * FN - 1) / (16 * FN)));
-    // a round that is longer than the row would load its first chunk over and over
-    if (g.p.kbytes > 4 * UNIT) hipLaunchKernelGGL((few_rows_kernel<FM, FN, 8, T, X>), grid, dim3(THREADS), 0, stream, g);
-    else if (g.p.kbytes > 2 * UNIT) hipLaunchKernelGGL((few_rows_kernel<FM, FN, 4, T, X>), grid, dim3(THREADS), 0, stream, g);
-    else hipLaunchKernelGGL((few_rows_kernel<FM, FN, 2, T, X>), grid, dim3(THREADS), 0, stream, g);
-}
-
 template <int FM, typename T, typename X>
-int launch_fn(const FewArgs &g, hipStream_t stream)
+int launch_u(const FewArgs &g, hipStream_t stream)
 {
-    bool two = FM > 1 && g.p.N >= 32 * 256;
-    if (const char *v = getenv("FEW_FN")) two = FM > 1 && atoi(v) == 2;
-    if constexpr (FM > 1) {
-        if (two) launch_u<FM, 2, T, X>(g, stream);
-        else launch_u<FM, 1, T, X>(g, stream);
-    } else {
-        launch_u<FM, 1, T, X>(g, stream);
-    }
+    const dim3 grid((unsigned)((g.p.N + 15) / 16));
+    // a round that is longer than the row would load its first chunk over and over
+    if (g.p.kbytes > 4 * UNIT) hipLaunchKernelGGL((few_rows_kernel<FM, 8, T, X>), grid, dim3(THREADS), 0, stream, g);
+    else if (g.p.kbytes > 2 * UNIT) hipLaunchKernelGGL((few_rows_kernel<FM, 4, T, X>), grid, dim3(THREADS), 0, stream, g);
+    else hipLaunchKernelGGL((few_rows_kernel<FM, 2, T, X>), grid, dim3(THREADS), 0, stream, g);
     REXSC_CHECK_HIP(hipGetLastError());
     return REXSC_OK;
 }
@@ -209,11 +184,9 @@ int launch_fn(const FewArgs &g, hipStream_t stream)
 template <typename T>
 int launch_fm(const FewArgs &g, hipStream_t stream)
 {
-    const int M = g.p.M;
-    if (M <= 16) return launch_fn<1, T, int8_t>(g, stream);
-    if (M <= 32) return launch_fn<2, T, int8_t>(g, stream);
-    if (M <= 48) return launch_fn<3, T, int8_t>(g, stream);
-    return launch_fn<4, T, int8_t>(g, stream);
+    if (g.p.M <= 16) return launch_u<1, T, int8_t>(g, stream);
+    if (g.p.M <= 32) return launch_u<2, T, int8_t>(g, stream);
+    return launch_u<3, T, int8_t>(g, stream);
 }
 
 double work(const TileArgs &p) { return 2.0 * p.M * p.N * p.kbytes; }
@@ -227,6 +200,11 @@ int launch_few_rows(const TileArgs &p, int out_dtype, hipStream_t stream)
     REXSC_DTYPE_SWITCH(out_dtype, return launch_fm<T>(g, stream));
 }
 
+// Up to 8 tokens; up to 48 where the 64 x 64 tiles would leave half of the CUs without one.  Beyond, each block's reading
+// all tokens again costs more than the tiles' sharing them in LDS: 32 tokens x 4096 x 4096 9 us here and 12 in tiles,
+// but 37 x 11003 x 4099 27 us here and 15 in tiles, 16 x 16384 x 4096 19 and 17.5.
+bool few_rows_takes(int M, int N) { return M <= 8 || (M <= FEW_ROWS && N < 64 * 128); }
+
 bool few_rows_fuses(int M, int K, const void *x, size_t x_stride, int dtype)
 {
     const size_t es = dtype_size(dtype);
@@ -238,7 +216,7 @@ int launch_few_rows_fused(const TileArgs &p, const void *x, size_t x_stride, int
 {
     ProfScope prof("int8_linear_few", work(p), stream);
     const FewArgs g{p, x, x_stride};
-    REXSC_DTYPE_SWITCH(dtype, return (launch_fn<1, T, T>(g, stream)));
+    REXSC_DTYPE_SWITCH(dtype, return (launch_u<1, T, T>(g, stream)));
 }
 
 } // namespace rexsc

@@ -274,7 +274,7 @@ int product(const rexsc_int8_desc *d, const int8_t *a, int64_t a_stride, const f
 {
     const TileArgs p{(const char *)a, (const char *)b, (size_t)a_stride, (size_t)d->b_stride, d->M, d->N, d->K, 1, 0,
                      a_scale, b_scale, bias, d->bias_dtype, y};
-    if (d->M <= FEW_ROWS && !getenv("REXSC_TUNE_INT8_TILE")) return launch_few_rows(p, d->dtype, stream);
+    if (few_rows_takes(d->M, d->N) && !getenv("REXSC_TUNE_INT8_TILE")) return launch_few_rows(p, d->dtype, stream);
     return launch_tile_product(p, false, d->dtype, space, "int8_product", stream);
 }
 

@@ -21,8 +21,21 @@ __device__ __forceinline__ f32x4 mma(OpBF16, i32x4 a, i32x4 b, f32x4 c)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Waits until this wave's loads into LDS have landed (before the barrier that shows them to the other waves).
-__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); } // vmcnt(0), the other counters at any value
+// Waits until at most N of this wave's loads into LDS are still on their way (they land in order), and until its reads
+// of LDS are done: what a barrier needs that lets the other waves read the one and overwrite the other.  Nothing may be
+// moved across either by the compiler.
+template <int N>
+__device__ __forceinline__ void loads_left()
+{
+    static_assert(N < 64, "the counter has six bits");
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void reads_done()
+{
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 // Bytes of a 16-byte chunk at offset k that lie before `end`; the rest become 0.
 __device__ __forceinline__ i32x4 keep_before(i32x4 v, int k, int end)
@@ -69,14 +82,14 @@ __device__ __forceinline__ void tile_of(unsigned bid, int tiles_m, int tiles_n, 
 
 // SPLIT: the grid holds `splits` times the tiles, and a block sums only its share of the steps, into a partial result
 // of the accumulator's type (T) that join_kernel finishes.
-template <typename Op, typename T, int BM, int BN, int WM, int WN, bool SPLIT>
+template <typename Op, typename T, int BM, int BN, int WM, int WN, int STAGES, bool SPLIT>
 __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int splits)
 {
     constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
     constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES; // loads of 8 rows x 128 bytes per wave and step
     static_assert(LA * WAVES * 8 == BM && LB * WAVES * 8 == BN, "tile rows must divide among the waves");
     constexpr int BUF = (BM + BN) * KSTEP;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * BUF];
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * BUF];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     int tm, tn;
     const int share = SPLIT ? (int)(blockIdx.x % splits) : 0;
@@ -150,15 +163,19 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // A step's second half is read while its first is multiplied; then, with every wave's fragments of this buffer in
-    // registers and the other buffer filled, one barrier, behind which this buffer is filled anew and the first half of
-    // the other is read while the second half is multiplied.  (Behind the last step that reads what is not used.)
+    // STAGES buffers in a ring.  A step's second half is read while its first is multiplied; then, with every wave's
+    // fragments of this buffer in registers and the next buffer filled, one barrier, behind which this buffer is filled
+    // anew, STAGES steps ahead, and the first half of the next is read while the second half is multiplied.  (Behind
+    // the last step that reads what is not used.)
     if (total > 0) {
         fetch(lds);
-        loads_done();
-        __syncthreads();
+#pragma unroll
+        for (int i = 1; i < STAGES; i++)
+            if (i < total) fetch(lds + i * BUF);
+        if (total >= STAGES) loads_left<(STAGES - 1) * (LA + LB)>();
+        else loads_left<0>();
+        __builtin_amdgcn_s_barrier();
         if (tail && total == 1) clear_tail(base);
-        if (total > 1) fetch(lds + BUF);
 #pragma unroll
         for (int i = 0; i < FM; i++) fa[0][i] = *(const lds_i32x4 *)(base + at_a[0] + i * 16 * KSTEP);
 #pragma unroll
@@ -166,12 +183,16 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
         int cur = 0;
         for (int s = 0; s < total; s++) {
             multiply(std::integral_constant<int, 0>{}, base + cur);
-            loads_done();
-            __syncthreads();
-            if (tail && s + 2 == total) clear_tail(base + (cur ^ BUF));
-            if (s + 2 < total) fetch(lds + cur);
+            // the loads of steps s + 2 ... s + STAGES - 1 may still be on their way (towards the end there are fewer)
+            if (STAGES > 2 && s + STAGES - 1 < total) loads_left<(STAGES - 2) * (LA + LB)>();
+            else loads_left<0>();
+            reads_done();
+            __builtin_amdgcn_s_barrier();
+            const int next = cur + BUF < STAGES * BUF ? cur + BUF : 0;
+            if (tail && s + 2 == total) clear_tail(base + next);
+            if (s + STAGES < total) fetch(lds + cur);
             __builtin_amdgcn_sched_barrier(0);
-            cur ^= BUF;
+            cur = next;
             multiply(std::integral_constant<int, 1>{}, base + cur);
         }
     }
@@ -182,8 +203,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
     // the banks, which spreads the 16 rows of a write over all of them.
     constexpr int COLS = BN / WN, ROWS = BM / WM, VEC = 16 / sizeof(T), PITCH = COLS * sizeof(T) + 16;
     constexpr int PART = sizeof(T) == 4 ? 32 : 64, CR = ROWS < PART ? ROWS : PART; // rows that are turned at a time
-    static_assert(WAVES * CR * PITCH <= 2 * BUF, "the waves' shares fit the buffers");
-    static_assert((BUF & (BUF - 1)) == 0, "buffers are switched by an exclusive or");
+    static_assert(WAVES * CR * PITCH <= STAGES * BUF, "the waves' shares fit the buffers");
     const int first_n = n0 + wn;
     float sb[FN][4], bias[FN][4];
 #pragma unroll
@@ -276,11 +296,11 @@ int tune(const char *name)
 
 // Tile size by what a launch takes when its busiest CU gets n tiles, in units of one 256 x 256 tile (measured at
 // K = 4096 int8, 57 us each): one block of 256 x 256 per CU, n; two of 128 x 128 side by side 0.61, a single one 0.44;
-// 64 x 64, up to five side by side, 0.08 + 0.11 n.  E.g. 2048 x 4096: 38 us in 128s against 53 in 256s or 64s;
-// 4096 x 4096: 62 in 256s against 71 in 128s; 512 x 4096: 21 in 64s against 26 in 128s.
-// The reduction is split over blocks only where the result has tiles for less than half of the CUs and each share
-// keeps 16 steps: the partial results cost a second launch.  300 x 300 x 16384: 17 us in 8 shares against 64 in one;
-// with tiles for every CU, splitting lost in each case measured (256 x 4096 x 4096: 15 us against 20).
+// 64 x 64, up to five side by side, 0.08 + 0.11 n.  E.g. 2048 x 4096: 37 us in 128s against 52 in 256s and 58 in 64s;
+// 4096 x 4096: 59 in 256s against 69 in 128s; 512 x 4096: 19 in 64s against 26 in 128s.
+// The reduction is split over blocks only where the result has tiles for at most a quarter of the CUs and each share
+// keeps 8 steps: the partial results cost a second launch.  300 x 300 x 16384: 16 us in 8 shares against 37 in one;
+// with more tiles, splitting lost in each case measured (128 x 4096 x 4096: 14 us against 16 in two shares).
 TilePlan tile_plan(int M, int N, int kbytes, int pieces)
 {
     const int steps = (kbytes + KSTEP - 1) / KSTEP * pieces;
@@ -291,8 +311,8 @@ TilePlan tile_plan(int M, int N, int kbytes, int pieces)
     TilePlan pl{t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64, 1};
     if (const int t = tune("REXSC_TUNE_INT8_TILE")) pl.size = t == 256 || t == 128 ? t : 64;
     const int64_t n = tiles(pl.size);
-    if (n > 0 && 2 * n <= CUS) {
-        const int64_t fill = CUS / n, keep = steps / 16;
+    if (n > 0 && 4 * n <= CUS) {
+        const int64_t fill = CUS / n, keep = steps / 8;
         pl.splits = (int)(fill < keep ? fill : keep);
     }
     if (const int t = tune("REXSC_TUNE_INT8_SPLITS")) pl.splits = t;
@@ -301,19 +321,19 @@ TilePlan tile_plan(int M, int N, int kbytes, int pieces)
     return pl;
 }
 
-template <typename Op, typename T, int BM, int BN, int WM, int WN>
+template <typename Op, typename T, int BM, int BN, int WM, int WN, int STAGES>
 int launch_one(const TileArgs &p, int splits, void *workspace, hipStream_t stream)
 {
     typedef std::conditional_t<std::is_same_v<Op, OpI8>, int, float> ACC;
     const unsigned tiles = (unsigned)(((p.M + BM - 1) / BM) * (int64_t)((p.N + BN - 1) / BN));
     if (splits == 1) {
-        hipLaunchKernelGGL((tile_kernel<Op, T, BM, BN, WM, WN, false>), dim3(tiles), dim3(WM * WN * 64), 0, stream, p, 1);
+        hipLaunchKernelGGL((tile_kernel<Op, T, BM, BN, WM, WN, STAGES, false>), dim3(tiles), dim3(WM * WN * 64), 0, stream, p, 1);
         REXSC_CHECK_HIP(hipGetLastError());
         return REXSC_OK;
     }
     TileArgs q = p;
     q.y = workspace;
-    hipLaunchKernelGGL((tile_kernel<Op, ACC, BM, BN, WM, WN, true>), dim3(tiles * splits), dim3(WM * WN * 64), 0, stream, q, splits);
+    hipLaunchKernelGGL((tile_kernel<Op, ACC, BM, BN, WM, WN, STAGES, true>), dim3(tiles * splits), dim3(WM * WN * 64), 0, stream, q, splits);
     REXSC_CHECK_HIP(hipGetLastError());
     const size_t all = (size_t)p.M * p.N;
     hipLaunchKernelGGL((join_kernel<ACC, T>), dim3((unsigned)((all + 1023) / 1024)), dim3(256), 0, stream, p, (const ACC *)workspace,
@@ -325,9 +345,9 @@ int launch_one(const TileArgs &p, int splits, void *workspace, hipStream_t strea
 template <typename Op, typename T>
 int launch_size(const TileArgs &p, const TilePlan &pl, void *workspace, hipStream_t stream)
 {
-    if (pl.size == 256) return launch_one<Op, T, 256, 256, 2, 4>(p, pl.splits, workspace, stream);
-    if (pl.size == 128) return launch_one<Op, T, 128, 128, 2, 2>(p, pl.splits, workspace, stream);
-    return launch_one<Op, T, 64, 64, 2, 2>(p, pl.splits, workspace, stream);
+    if (pl.size == 256) return launch_one<Op, T, 256, 256, 2, 4, 2>(p, pl.splits, workspace, stream);
+    if (pl.size == 128) return launch_one<Op, T, 128, 128, 2, 2, 2>(p, pl.splits, workspace, stream);
+    return launch_one<Op, T, 64, 64, 2, 2, 4>(p, pl.splits, workspace, stream);
 }
 
 } // namespace
