@@ -719,9 +719,8 @@ def _same_device(what, first, *rest):
 def _rows_of(t):
     """t [..., K] as a matrix whose rows lie at one distance and whose elements are neighbours (a view where t has such
     a layout, else a copy)."""
-    t = t.detach()
     m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if m.stride(1) != 1 and m.shape[1] > 1 or (m.shape[0] > 1 and m.stride(0) < m.shape[1]):
+    if m.shape[1] > 1 and m.stride(1) != 1 or m.shape[0] > 1 and m.stride(0) < m.shape[1]:
         m = m.contiguous()
     return m
 
@@ -733,38 +732,42 @@ def _row_stride(m):
 def quantize_rows(x):
     """Rows of x [..., K] in 8 bits -> (q int8 of x's shape, scale float32 of x.shape[:-1]).  q's rows lie at a multiple
     of 128 bytes, padded with zeros."""
-    _require_cuda(x)
+    if not x.is_cuda:
+        _require_cuda(x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError("quantize_rows: expected rows of at least one element (got shape %s)" % (tuple(x.shape),))
     code = _dtype_code(x, "quantize_rows")
-    m = _rows_of(x)
+    m = _rows_of(x.detach())
     R, K = m.shape
     pad = -(-K // ROW_PAD) * ROW_PAD
-    with torch.cuda.device(x.device):
+    dev = x.get_device()
+    with _on(dev):
         q = torch.empty((R, pad), dtype=torch.int8, device=x.device)
-        scale = torch.empty(R, dtype=torch.float32, device=x.device)
-        rc = _lib.lib().rexsc_quantize_rows(_ptr(m), code, R, K, _row_stride(m), _ptr(q), pad, _ptr(scale), _stream())
-        _lib.check(rc, "rexsc_quantize_rows")
-    q = q[:, :K]
+        scale = torch.empty((R,), dtype=torch.float32, device=x.device)
+        rc = _lib.lib().rexsc_quantize_rows(m.data_ptr(), code, R, K, _row_stride(m), q.data_ptr(), pad, scale.data_ptr(),
+                                            _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "rexsc_quantize_rows")
+    if pad != K:
+        q = q[:, :K]
     if x.dim() != 2:
         q, scale = q.view(x.shape) if x.dim() > 2 else q[0], scale.view(x.shape[:-1])
     return q, scale
 
 
 def _operand8(t, what):
-    """int8 matrix as the product reads it: rows 16-byte aligned and readable to the next multiple of 16 bytes."""
+    """(int8 matrix as the product reads it, distance of its rows): rows 16-byte aligned and readable to the next
+    multiple of 16 bytes."""
     if t.dtype != torch.int8 or t.dim() != 2 or not 1 <= t.shape[1] <= MAX_K:
         raise RuntimeError("%s: expected an int8 matrix with 1 to %d columns (got %s %s)"
                            % (what, MAX_K, t.dtype, tuple(t.shape)))
     R, K = t.shape
-    fits = (K == 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0
-    if fits and R > 1:
-        fits = t.stride(0) % 16 == 0 and t.stride(0) >= K
-    if fits and K % 16:
-        last = t.storage_offset() + (R - 1) * t.stride(0) + -(-K // 16) * 16
-        fits = R == 0 or last <= t.untyped_storage().nbytes()
-    if fits:
-        return t, (t.stride(0) if R > 1 else -(-K // 16) * 16)
+    step, inner = t.stride()
+    if R <= 1:
+        step = -(-K // 16) * 16
+    if (inner == 1 or K == 1) and step % 16 == 0 and step >= K and t.data_ptr() % 16 == 0:
+        if K % 16 == 0 or R == 0 or t.storage_offset() + (R - 1) * step + -(-K // 16) * 16 <= t.untyped_storage().nbytes():
+            return t, step
     pad = -(-K // ROW_PAD) * ROW_PAD
     out = torch.empty((R, pad), dtype=torch.int8, device=t.device)[:, :K]
     out.copy_(t)  # what lies behind the K-th byte does not matter
@@ -775,136 +778,163 @@ def _scale_vector(s, n, device, what):
     if s.dtype != torch.float32 or s.numel() != n or s.device != device:
         raise RuntimeError("%s: expected %d float32 scales on %s (got %d %s on %s)"
                            % (what, n, device, s.numel(), s.dtype, s.device))
-    return s.detach().reshape(-1).contiguous()
+    return s if s.is_contiguous() else s.contiguous()
 
 
 def _bias_vector(bias, n, what):
     if bias is None:
         return None, _lib.F32
-    if bias.numel() != n or bias.dim() != 1:
+    if bias.dim() != 1 or bias.shape[0] != n:
         raise RuntimeError("%s: expected a bias of %d elements (got %s)" % (what, n, tuple(bias.shape)))
-    return bias.detach().contiguous(), _dtype_code(bias, what)
+    return bias if bias.is_contiguous() else bias.contiguous(), _dtype_code(bias, what)
+
+
+_NO_BYTES = ctypes.c_size_t(-1).value
 
 
 def _int8_space(L, d, what, device):
-    nbytes = L.rexsc_int8_workspace_bytes(ctypes.byref(d), what)
-    if nbytes == ctypes.c_size_t(-1).value:
+    """(workspace of a call or None, its bytes)"""
+    nbytes = L.rexsc_int8_workspace_bytes(d, what)
+    if nbytes == 0:
+        return None, 0
+    if nbytes == _NO_BYTES:
         _lib.check(-1, "rexsc_int8_linear (planning)")
-    return (_workspace(nbytes, device), nbytes) if nbytes else (None, 0)
+    return torch.empty((nbytes,), dtype=torch.uint8, device=device), nbytes
 
 
 def matmul_int8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
     """(a [M, K] int8 times b [N, K] int8 transposed, summed in int32) * a_scale[:, None] * b_scale + bias -> [M, N]."""
-    _require_cuda(a, b)
+    if not (a.is_cuda and b.is_cuda):
+        _require_cuda(a, b)
     _same_device("matmul_int8", a, b, bias)
     if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1]:
         raise RuntimeError("matmul_int8: expected int8 matrices [M, K] and [N, K], got %s and %s"
                            % (tuple(a.shape), tuple(b.shape)))
     M, K = a.shape
     N = b.shape[0]
-    a_scale = _scale_vector(a_scale, M, a.device, "matmul_int8")
-    b_scale = _scale_vector(b_scale, N, a.device, "matmul_int8")
+    device, dev = a.device, a.get_device()
+    a_scale = _scale_vector(a_scale, M, device, "matmul_int8")
+    b_scale = _scale_vector(b_scale, N, device, "matmul_int8")
     bias, bias_code = _bias_vector(bias, N, "matmul_int8")
     L = _lib.lib()
-    with torch.cuda.device(a.device):
+    with _on(dev):
         a, sa = _operand8(a, "matmul_int8")
         b, sb = _operand8(b, "matmul_int8")
-        d = _lib.Int8Desc(M, N, K, _dtype_code(out_dtype, "matmul_int8"), bias_code, _lib.F32, 0, 0, sa, sb)
-        y = torch.empty((M, N), dtype=out_dtype, device=a.device)
-        ws, nbytes = _int8_space(L, d, _lib.INT8_PRODUCT, a.device)
-        rc = L.rexsc_int8_product(ctypes.byref(d), _ptr(a), _ptr(a_scale), _ptr(b), _ptr(b_scale), _ptr(bias), _ptr(y),
-                                  _ptr(ws), nbytes, _stream())
-        _lib.check(rc, "rexsc_int8_product")
+        d = ctypes.byref(_lib.Int8Desc(M, N, K, _dtype_code(out_dtype, "matmul_int8"), bias_code, 0, 0, 0, sa, sb))
+        y = torch.empty((M, N), dtype=out_dtype, device=device)
+        ws, nbytes = _int8_space(L, d, _lib.INT8_PRODUCT, device)
+        rc = L.rexsc_int8_product(d, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), _addr(bias),
+                                  y.data_ptr(), _addr(ws), nbytes, _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "rexsc_int8_product")
     return y
 
 
 def int8_linear(x, wq, w_scale, bias=None):
     """x [..., K] float times the 8-bit weights wq [N, K] -> [..., N] in x's type; x's rows are taken to 8 bits inside."""
-    _require_cuda(x, wq)
+    if not (x.is_cuda and wq.is_cuda):
+        _require_cuda(x, wq)
     _same_device("linear_int8", x, wq, bias)
-    if wq.dim() != 2 or x.dim() < 1 or x.shape[-1] != wq.shape[1]:
+    shape = x.shape
+    if wq.dim() != 2 or len(shape) < 1 or shape[-1] != wq.shape[1]:
         raise RuntimeError("linear_int8: expected input [..., K] and weight [N, K], got %s and %s"
-                           % (tuple(x.shape), tuple(wq.shape)))
+                           % (tuple(shape), tuple(wq.shape)))
     code = _dtype_code(x, "linear_int8")
     m = _rows_of(x)
     M, K = m.shape
     N = wq.shape[0]
-    w_scale = _scale_vector(w_scale, N, x.device, "linear_int8")
+    device, dev = x.device, x.get_device()
+    w_scale = _scale_vector(w_scale, N, device, "linear_int8")
     bias, bias_code = _bias_vector(bias, N, "linear_int8")
     L = _lib.lib()
-    with torch.cuda.device(x.device):
+    with _on(dev):
         wq, sb = _operand8(wq, "linear_int8")
-        d = _lib.Int8Desc(M, N, K, code, bias_code, _lib.F32, 0, _row_stride(m), 0, sb)
-        y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
-        ws, nbytes = _int8_space(L, d, _lib.INT8_LINEAR, x.device)
-        rc = L.rexsc_int8_linear(ctypes.byref(d), _ptr(m), _ptr(wq), _ptr(w_scale), _ptr(bias), _ptr(y), _ptr(ws), nbytes,
-                                 _stream())
-        _lib.check(rc, "rexsc_int8_linear")
+        d = ctypes.byref(_lib.Int8Desc(M, N, K, code, bias_code, 0, 0, _row_stride(m), 0, sb))
+        y = torch.empty(shape[:-1] + (N,), dtype=x.dtype, device=device)
+        ws, nbytes = _int8_space(L, d, _lib.INT8_LINEAR, device)
+        rc = L.rexsc_int8_linear(d, m.data_ptr(), wq.data_ptr(), w_scale.data_ptr(), _addr(bias), y.data_ptr(), _addr(ws),
+                                 nbytes, _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "rexsc_int8_linear")
     return y
+
+
+def _dense_rows(g, n):
+    """g [..., n] as a dense matrix."""
+    if g.dim() != 2:
+        g = g.reshape(-1, n)
+    return g if g.is_contiguous() else g.contiguous()
 
 
 def int8_grad_input(g, wq, w_scale):
     """Straight-through gradient of the product with respect to its input: g [..., N] -> [..., K] in g's type."""
-    _require_cuda(g, wq)
+    if not (g.is_cuda and wq.is_cuda):
+        _require_cuda(g, wq)
     _same_device("linear_int8", g, wq, w_scale)
     code = _dtype_code(g, "linear_int8")
     N, K = wq.shape
-    gm = g.detach().reshape(-1, N).contiguous()
+    gm = _dense_rows(g, N)
+    device, dev = g.device, g.get_device()
     L = _lib.lib()
-    with torch.cuda.device(g.device):
+    with _on(dev):
         wq, sb = _operand8(wq, "linear_int8")
-        d = _lib.Int8Desc(gm.shape[0], N, K, code, _lib.F32, _lib.F32, 0, 0, 0, sb)
-        dx = torch.empty(g.shape[:-1] + (K,), dtype=g.dtype, device=g.device)
-        ws, nbytes = _int8_space(L, d, _lib.INT8_GRAD_INPUT, g.device)
-        rc = L.rexsc_int8_grad_input(ctypes.byref(d), _ptr(gm), _ptr(wq), _ptr(w_scale), _ptr(dx), _ptr(ws), nbytes,
-                                     _stream())
-        _lib.check(rc, "rexsc_int8_grad_input")
+        d = ctypes.byref(_lib.Int8Desc(gm.shape[0], N, K, code, 0, 0, 0, 0, 0, sb))
+        dx = torch.empty(g.shape[:-1] + (K,), dtype=g.dtype, device=device)
+        ws, nbytes = _int8_space(L, d, _lib.INT8_GRAD_INPUT, device)
+        rc = L.rexsc_int8_grad_input(d, gm.data_ptr(), wq.data_ptr(), w_scale.data_ptr(), dx.data_ptr(), _addr(ws), nbytes,
+                                     _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "rexsc_int8_grad_input")
     return dx
 
 
 def int8_grad_weight(g, xq, x_scale, weight_dtype=None, bias_dtype=None):
     """Straight-through gradients with respect to weight and bias: (dw [N, K] of weight_dtype, db [N] of bias_dtype);
     a type of None: not wanted."""
-    _require_cuda(g, xq)
+    if not (g.is_cuda and xq.is_cuda):
+        _require_cuda(g, xq)
     _same_device("linear_int8", g, xq, x_scale)
     code = _dtype_code(g, "linear_int8")
     N = g.shape[-1]
     M, K = xq.shape
-    gm = g.detach().reshape(M, N).contiguous()
+    gm = _dense_rows(g, N)
+    device, dev = g.device, g.get_device()
     L = _lib.lib()
-    with torch.cuda.device(g.device):
+    with _on(dev):
         xq, sa = _operand8(xq, "linear_int8")
-        mk = lambda shape, dt: torch.empty(shape, dtype=dt, device=g.device) if dt is not None else None
-        dw, db = mk((N, K), weight_dtype), mk((N,), bias_dtype)
-        d = _lib.Int8Desc(M, N, K, code, _dtype_code(bias_dtype or torch.float32, "linear_int8"),
-                          _dtype_code(weight_dtype or torch.float32, "linear_int8"), 0, 0, sa, 0)
-        ws, nbytes = _int8_space(L, d, _lib.INT8_GRAD_WEIGHT, g.device)
-        rc = L.rexsc_int8_grad_weight(ctypes.byref(d), _ptr(gm), _ptr(xq), _ptr(x_scale), _ptr(dw), _ptr(db), _ptr(ws),
-                                      nbytes, _stream())
-        _lib.check(rc, "rexsc_int8_grad_weight")
+        dw = torch.empty((N, K), dtype=weight_dtype, device=device) if weight_dtype is not None else None
+        db = torch.empty((N,), dtype=bias_dtype, device=device) if bias_dtype is not None else None
+        d = ctypes.byref(_lib.Int8Desc(M, N, K, code, 0 if bias_dtype is None else _dtype_code(bias_dtype, "linear_int8"),
+                                       0 if weight_dtype is None else _dtype_code(weight_dtype, "linear_int8"), 0, 0, sa, 0))
+        ws, nbytes = _int8_space(L, d, _lib.INT8_GRAD_WEIGHT, device)
+        rc = L.rexsc_int8_grad_weight(d, gm.data_ptr(), xq.data_ptr(), x_scale.data_ptr(), _addr(dw), _addr(db), _addr(ws),
+                                      nbytes, _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "rexsc_int8_grad_weight")
     return dw, db
 
 
 # ---- layer norm ----------------------------------------------------------------------------------
 
-def _norm_vectors(x, weight, bias):
-    """weight and bias as the kernels read them: one type for both, float32 or x's."""
-    dt = torch.float32
-    given = [t for t in (weight, bias) if t is not None]
-    for t in given:
-        if t.dim() != 1 or t.numel() != x.shape[-1]:
-            raise RuntimeError("layer_norm: expected weight and bias of %d elements (got %s)"
-                               % (x.shape[-1], tuple(t.shape)))
-        _dtype_code(t, "layer_norm")
-    if given and all(t.dtype == x.dtype for t in given):
-        dt = x.dtype
-    fit = lambda t: None if t is None else t.detach().to(dt).contiguous()
+def _norm_vectors(x, weight, bias, dtype=None):
+    """(weight, bias, their type) as the kernels read them: one type for both, float32 or x's (dtype: that one)."""
+    same = dtype is None
+    for t in (weight, bias):
+        if t is not None:
+            if t.dim() != 1 or t.shape[0] != x.shape[-1]:
+                raise RuntimeError("layer_norm: expected weight and bias of %d elements (got %s)"
+                                   % (x.shape[-1], tuple(t.shape)))
+            _dtype_code(t, "layer_norm")
+            same = same and t.dtype == x.dtype
+    dt = dtype or (x.dtype if same else torch.float32)
+    fit = lambda t: t if t is None or t.dtype == dt and t.is_contiguous() else t.detach().to(dt).contiguous()
     return fit(weight), fit(bias), dt
 
 
 def layer_norm_forward(x, weight, bias, eps, want_stats=True):
     """(y, mean, rstd) of a layer norm over the last dimension; mean and rstd float32 per row (None unless wanted)."""
-    _require_cuda(x)
+    if not x.is_cuda:
+        _require_cuda(x)
     _same_device("layer_norm", x, weight, bias)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError("layer_norm: expected rows of at least one element (got shape %s)" % (tuple(x.shape),))
@@ -912,46 +942,53 @@ def layer_norm_forward(x, weight, bias, eps, want_stats=True):
     w, b, wdt = _norm_vectors(x, weight, bias)
     m = _rows_of(x)
     R, D = m.shape
-    with torch.cuda.device(x.device):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean = torch.empty(R, dtype=torch.float32, device=x.device) if want_stats else None
-        rstd = torch.empty(R, dtype=torch.float32, device=x.device) if want_stats else None
-        d = _lib.NormDesc(code, _DTYPE_CODE[wdt], float(eps), R, D, _row_stride(m))
-        rc = _lib.lib().rexsc_layer_norm_forward(ctypes.byref(d), _ptr(m), _ptr(w), _ptr(b), _ptr(y), _ptr(mean),
-                                                 _ptr(rstd), _stream())
-        _lib.check(rc, "rexsc_layer_norm_forward")
+    device, dev = x.device, x.get_device()
+    with _on(dev):
+        y = torch.empty(x.shape, dtype=x.dtype, device=device)
+        mean = rstd = None
+        if want_stats:
+            stats = torch.empty((2, R), dtype=torch.float32, device=device)
+            mean, rstd = stats[0], stats[1]
+        d = _lib.NormDesc(code, _DTYPE_CODE[wdt], eps, R, D, _row_stride(m))
+        rc = _lib.lib().rexsc_layer_norm_forward(ctypes.byref(d), m.data_ptr(), _addr(w), _addr(b), y.data_ptr(), _addr(mean),
+                                                 _addr(rstd), _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "rexsc_layer_norm_forward")
     return y, mean, rstd
 
 
 def layer_norm_backward(grad_output, x, weight, mean, rstd, eps, need_x=True, weight_dtype=None, bias_dtype=None):
     """(dx in x's type, dw of weight_dtype, db of bias_dtype); a type of None: not wanted."""
-    _require_cuda(grad_output, x)
+    if not (grad_output.is_cuda and x.is_cuda):
+        _require_cuda(grad_output, x)
     _same_device("layer_norm", x, grad_output, weight)
     code = _dtype_code(x, "layer_norm")
-    w, _, _ = _norm_vectors(x, weight, None)
+    # the sums leave the kernel in float32 or in x's type; any other type is rounded once more
+    wanted = weight_dtype is not None or bias_dtype is not None
+    low = wanted and weight_dtype in (None, x.dtype) and bias_dtype in (None, x.dtype)
+    sum_dt = x.dtype if low else torch.float32
+    w = _norm_vectors(x, weight, None, sum_dt)[0]
     m = _rows_of(x)
     R, D = m.shape
-    g = grad_output.detach().to(x.dtype).reshape(R, D).contiguous()
-    # the sums leave the kernel in float32 or in x's type; any other type is rounded once more
-    wanted = [t for t in (weight_dtype, bias_dtype) if t is not None]
-    sum_dt = x.dtype if wanted and all(t == x.dtype for t in wanted) else torch.float32
-    if w is not None and w.dtype != sum_dt:
-        w = w.to(sum_dt)
+    g = grad_output if grad_output.dtype == x.dtype else grad_output.to(x.dtype)
+    g = _dense_rows(g, D)
+    device, dev = x.device, x.get_device()
     L = _lib.lib()
-    with torch.cuda.device(x.device):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        mk = lambda dt: torch.empty(D, dtype=sum_dt, device=x.device) if dt is not None else None
-        dw, db = mk(weight_dtype), mk(bias_dtype)
-        d = _lib.NormDesc(code, _DTYPE_CODE[sum_dt], float(eps), R, D, _row_stride(m))
-        ws = None
+    with _on(dev):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
+        dw = torch.empty((D,), dtype=sum_dt, device=device) if weight_dtype is not None else None
+        db = torch.empty((D,), dtype=sum_dt, device=device) if bias_dtype is not None else None
+        d = ctypes.byref(_lib.NormDesc(code, _DTYPE_CODE[sum_dt], eps, R, D, _row_stride(m)))
+        ws, nbytes = None, 0
         if wanted:
-            nbytes = L.rexsc_layer_norm_backward_workspace_bytes(ctypes.byref(d))
-            if nbytes == ctypes.c_size_t(-1).value:
+            nbytes = L.rexsc_layer_norm_backward_workspace_bytes(d)
+            if nbytes == _NO_BYTES:
                 _lib.check(-1, "rexsc_layer_norm_backward (planning)")
-            ws = _workspace(nbytes, x.device)
-        rc = L.rexsc_layer_norm_backward(ctypes.byref(d), _ptr(g), _ptr(m), _ptr(w), _ptr(mean), _ptr(rstd), _ptr(dx),
-                                         _ptr(dw), _ptr(db), _ptr(ws), ws.numel() if ws is not None else 0, _stream())
-        _lib.check(rc, "rexsc_layer_norm_backward")
+            ws = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+        rc = L.rexsc_layer_norm_backward(d, g.data_ptr(), m.data_ptr(), _addr(w), mean.data_ptr(), rstd.data_ptr(), _addr(dx),
+                                         _addr(dw), _addr(db), _addr(ws), nbytes, _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "rexsc_layer_norm_backward")
     if dw is not None and dw.dtype != weight_dtype:
         dw = dw.to(weight_dtype)
     if db is not None and db.dtype != bias_dtype:

@@ -1,6 +1,8 @@
 """AdamW over many tensors at once on the HIP kernels, with 32-bit or 8-bit states and the clamp of the weights that SC
 training applies after every step (utils_own.py:187-190) folded into it."""
 import ctypes
+import itertools
+import operator
 
 import torch
 
@@ -23,10 +25,19 @@ def _dense(t):
     return True
 
 
-def _like(p, t, what, dtype):
-    if t.dtype != dtype or t.device != p.device or t.numel() != p.numel():
-        raise RuntimeError("adamw_step: %s of a %s parameter on %s must be %s, as long and beside it (got %s %s on %s)"
-                           % (what, tuple(p.shape), p.device, dtype, t.dtype, tuple(t.shape), t.device))
+_T = torch.Tensor
+_PTR, _NUMEL, _DENSE, _DEV = _T.data_ptr, _T.numel, _T.is_contiguous, _T.get_device
+_DTYPE = operator.attrgetter("dtype")
+
+
+def _check_list(tensors, what, params, dtype, device, numels):
+    """All of one type, on one device and as long as the parameters (one pass in C per property: a step of a network
+    with many small tensors is bound by this)."""
+    if not (set(map(_DTYPE, tensors)) == {dtype} and set(map(_DEV, tensors)) == {device} and list(map(_NUMEL, tensors)) == numels):
+        for p, t, n in zip(params, tensors, numels):
+            if t.dtype != dtype or t.get_device() != device or t.numel() != n:
+                raise RuntimeError("adamw_step: %s of a %s %s parameter on %s must be %s, of %d elements and beside it (got %s %s "
+                                   "on %s)" % (what, tuple(p.shape), p.dtype, p.device, dtype, n, t.dtype, tuple(t.shape), t.device))
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_avg_sq_scales=None, *, step, lr, beta1=0.9,
@@ -51,34 +62,35 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_av
     if not params:
         return
     first = params[0]
-    _ops._require_cuda(first)
+    if not first.is_cuda:
+        _ops._require_cuda(first)
     code = _ops._dtype_code(first, "adamw_step")
-    state = E4M3 if eight else torch.float32
-    table = []
-    for i, p in enumerate(params):
-        g, m, v = grads[i], exp_avgs[i], exp_avg_sqs[i]
-        n = p.numel()
-        if p.dtype != first.dtype or p.device != first.device:
-            raise RuntimeError("adamw_step: parameters of one type on one device are wanted (got %s on %s and %s on %s)"
-                               % (first.dtype, first.device, p.dtype, p.device))
-        _like(p, g, "the gradient", p.dtype)
-        _like(p, m, "exp_avg", state)
-        _like(p, v, "exp_avg_sq", state)
-        if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
+    state, dev = E4M3 if eight else torch.float32, first.get_device()
+    numels = list(map(_NUMEL, params))
+    _check_list(params, "each parameter, as the first", params, first.dtype, dev, numels)
+    _check_list(grads, "the gradient", params, first.dtype, dev, numels)
+    _check_list(exp_avgs, "exp_avg", params, state, dev, numels)
+    _check_list(exp_avg_sqs, "exp_avg_sq", params, state, dev, numels)
+    if not (all(map(_DENSE, params)) and all(map(_DENSE, grads)) and all(map(_DENSE, exp_avgs)) and all(map(_DENSE, exp_avg_sqs))):
+        for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
+            if p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous():
+                continue
             same = p.stride() == g.stride() and (m.is_contiguous() and v.is_contiguous() if eight else
                                                  p.stride() == m.stride() == v.stride())
             if not (same and _dense(p)):
                 raise RuntimeError("adamw_step: a parameter, its gradient and its states must be dense and laid out alike "
                                    "(strides %s, %s, %s, %s)" % (p.stride(), g.stride(), m.stride(), v.stride()))
-        ms = vs = 0
-        if eight:
-            ms, vs = exp_avg_scales[i], exp_avg_sq_scales[i]
-            for s in (ms, vs):
-                if s.dtype != torch.float32 or s.device != p.device or not s.is_contiguous() or s.numel() != -(-n // BLOCK):
-                    raise RuntimeError("adamw_step: %d elements need %d float32 scales beside them (got %s %s on %s)"
-                                       % (n, -(-n // BLOCK), s.dtype, tuple(s.shape), s.device))
-            ms, vs = ms.data_ptr(), vs.data_ptr()
-        table += (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), ms, vs, n)
+    columns = [map(_PTR, params), map(_PTR, grads), map(_PTR, exp_avgs), map(_PTR, exp_avg_sqs)]
+    if eight:
+        blocks = [-(-n // BLOCK) for n in numels]
+        for scales, what in ((exp_avg_scales, "exp_avg_scale"), (exp_avg_sq_scales, "exp_avg_sq_scale")):
+            _check_list(scales, what, params, torch.float32, dev, blocks)
+            if not all(map(_DENSE, scales)):
+                raise RuntimeError("adamw_step: the scales of a state must be contiguous")
+        columns += [map(_PTR, exp_avg_scales), map(_PTR, exp_avg_sq_scales)]
+    else:
+        columns += [itertools.repeat(0), itertools.repeat(0)]
+    table = list(itertools.chain.from_iterable(zip(*columns, numels)))
     on_device = isinstance(step, torch.Tensor)
     if on_device and (step.dtype != torch.int64 or step.numel() != 1 or step.device != first.device):
         raise RuntimeError("adamw_step: a step held in a tensor is one int64 beside the parameters")
@@ -91,12 +103,13 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_av
     d = _lib.AdamwDesc(code, 8 if eight else 32, int(clamp is not None), float(lr), float(beta1), float(beta2), float(eps),
                        float(weight_decay), lo, hi, 0 if on_device else int(step))
     arr = (ctypes.c_int64 * len(table))(*table)
-    with torch.cuda.device(first.device):
-        coef = torch.empty(_lib.ADAMW_COEF_BYTES, dtype=torch.uint8, device=first.device) if on_device else None
-        rc = _lib.lib().rexsc_adamw_step(ctypes.byref(d), ctypes.cast(arr, ctypes.c_void_p), len(params),
-                                         _ops._ptr(step if on_device else None), _ops._ptr(grad_scale), _ops._ptr(found_inf),
-                                         _ops._ptr(coef), _ops._stream())
-        _lib.check(rc, "rexsc_adamw_step")
+    with _ops._on(dev):
+        coef = torch.empty((_lib.ADAMW_COEF_BYTES,), dtype=torch.uint8, device=first.device) if on_device else None
+        rc = _lib.lib().rexsc_adamw_step(ctypes.byref(d), ctypes.addressof(arr), len(params),
+                                         _ops._addr(step if on_device else None), _ops._addr(grad_scale),
+                                         _ops._addr(found_inf), _ops._addr(coef), _ops._raw_stream(dev))
+        if rc:
+            _lib.check(rc, "rexsc_adamw_step")
 
 
 class AdamW(torch.optim.Optimizer):
