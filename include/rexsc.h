@@ -316,7 +316,7 @@ typedef struct rexsc_int8_desc {
 } rexsc_int8_desc;
 
 /* What a workspace is for. */
-enum { REXSC_INT8_PRODUCT = 0, REXSC_INT8_LINEAR = 1, REXSC_INT8_GRAD_INPUT = 2, REXSC_INT8_GRAD_WEIGHT = 3 };
+enum { REXSC_INT8_PRODUCT = 0, REXSC_INT8_LINEAR = 1, REXSC_INT8_BACKWARD = 2 };
 /* Bytes of workspace a call needs (0: none).  (size_t)-1 and rexsc_last_error() if the descriptor is invalid. */
 size_t rexsc_int8_workspace_bytes(const rexsc_int8_desc *d, int what);
 
@@ -333,12 +333,12 @@ int rexsc_int8_linear(const rexsc_int8_desc *d, const void *x, const int8_t *b, 
 
 /* Straight-through gradients (the quantisation passes the gradient on, as QuantizeGrad's backward does,
  * utils_functional.py:117-123): dx[m][k] = sum_n g[m][n] b_scale[n] b[n][k] in d->dtype,
- * dw[n][k] = sum_m g[m][n] a_scale[m] a[m][k] in d->weight_dtype, db[n] = sum_m g[m][n] in d->bias_dtype (NULL: not
- * wanted; dw may be NULL too).  g: dense [M][N] of d->dtype, dx: dense [M][K], dw: dense [N][K]. */
-int rexsc_int8_grad_input(const rexsc_int8_desc *d, const void *g, const int8_t *b, const float *b_scale, void *dx,
-                          void *workspace, size_t workspace_bytes, rexsc_stream_t stream);
-int rexsc_int8_grad_weight(const rexsc_int8_desc *d, const void *g, const int8_t *a, const float *a_scale, void *dw,
-                           void *db, void *workspace, size_t workspace_bytes, rexsc_stream_t stream);
+ * dw[n][k] = sum_m g[m][n] a_scale[m] a[m][k] in d->weight_dtype, db[n] = sum_m g[m][n] in d->bias_dtype; any of the
+ * three may be NULL (a and a_scale are read for dw only, b and b_scale for dx only).  g: dense [M][N] of d->dtype,
+ * dx: dense [M][K], dw: dense [N][K].  A row of dx or dw whose sum takes in a NaN or an infinity is NaN. */
+int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, const int8_t *a, const float *a_scale, const int8_t *b,
+                        const float *b_scale, void *dx, void *dw, void *db, void *workspace, size_t workspace_bytes,
+                        rexsc_stream_t stream);
 
 /* ---- layer norm ----------------------------------------------------------------------------------
  * No counterpart in the reference.  y = (x - mean) * rstd * weight + bias over each row of `cols` elements, with

@@ -67,7 +67,7 @@ class AdamwDesc(_Desc):
 ADAMW_TENSOR_FIELDS = 7
 ADAMW_COEF_BYTES = 256            # REXSC_ADAMW_COEF_BYTES
 F32, F16, BF16 = 0, 1, 2          # REXSC_F32, ...
-INT8_PRODUCT, INT8_LINEAR, INT8_GRAD_INPUT, INT8_GRAD_WEIGHT = 0, 1, 2, 3  # REXSC_INT8_*
+INT8_PRODUCT, INT8_LINEAR, INT8_BACKWARD = 0, 1, 2  # REXSC_INT8_*
 
 
 class ProfileRecord(ctypes.Structure):
@@ -121,8 +121,7 @@ SIGNATURES = {
     "rexsc_int8_workspace_bytes": (_sz, [_i8d, _int]),
     "rexsc_int8_product": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "rexsc_int8_linear": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "rexsc_int8_grad_input": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "rexsc_int8_grad_weight": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "rexsc_int8_backward": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "rexsc_layer_norm_forward": (_int, [_nd, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "rexsc_layer_norm_backward_workspace_bytes": (_sz, [_nd]),
     "rexsc_layer_norm_backward": (_int, [_nd, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

@@ -866,52 +866,37 @@ def _dense_rows(g, n):
     return g if g.is_contiguous() else g.contiguous()
 
 
-def int8_grad_input(g, wq, w_scale):
-    """Straight-through gradient of the product with respect to its input: g [..., N] -> [..., K] in g's type."""
+def int8_backward(g, xq, x_scale, wq, w_scale, need_x, weight_dtype, bias_dtype):
+    """Straight-through gradients of y = x W^T + bias in 8 bits, given those of y: (dx [..., K] in g's type or None, dw [N, K]
+    of weight_dtype, db [N] of bias_dtype); a type of None: not wanted.  xq and x_scale are read for dw only."""
     if not (g.is_cuda and wq.is_cuda):
         _require_cuda(g, wq)
-    _same_device("linear_int8", g, wq, w_scale)
+    _same_device("linear_int8", g, wq, xq)
     code = _dtype_code(g, "linear_int8")
     N, K = wq.shape
     gm = _dense_rows(g, N)
+    M = gm.shape[0]
     device, dev = g.device, g.get_device()
     L = _lib.lib()
     with _on(dev):
-        wq, sb = _operand8(wq, "linear_int8")
-        d = ctypes.byref(_lib.Int8Desc(gm.shape[0], N, K, code, 0, 0, 0, 0, 0, sb))
-        dx = torch.empty(g.shape[:-1] + (K,), dtype=g.dtype, device=device)
-        ws, nbytes = _int8_space(L, d, _lib.INT8_GRAD_INPUT, device)
-        rc = L.rexsc_int8_grad_input(d, gm.data_ptr(), wq.data_ptr(), w_scale.data_ptr(), dx.data_ptr(), _addr(ws), nbytes,
-                                     _raw_stream(dev))
+        sa = sb = 0
+        dx = dw = db = None
+        if need_x:
+            wq, sb = _operand8(wq, "linear_int8")
+            dx = torch.empty(g.shape[:-1] + (K,), dtype=g.dtype, device=device)
+        if weight_dtype is not None:
+            xq, sa = _operand8(xq, "linear_int8")
+            dw = torch.empty((N, K), dtype=weight_dtype, device=device)
+        if bias_dtype is not None:
+            db = torch.empty((N,), dtype=bias_dtype, device=device)
+        d = ctypes.byref(_lib.Int8Desc(M, N, K, code, 0 if db is None else _dtype_code(db, "linear_int8"),
+                                       0 if dw is None else _dtype_code(dw, "linear_int8"), 0, 0, sa, sb))
+        ws, nbytes = _int8_space(L, d, _lib.INT8_BACKWARD, device)
+        rc = L.rexsc_int8_backward(d, gm.data_ptr(), _addr(xq), _addr(x_scale), wq.data_ptr(), w_scale.data_ptr(), _addr(dx),
+                                   _addr(dw), _addr(db), _addr(ws), nbytes, _raw_stream(dev))
         if rc:
-            _lib.check(rc, "rexsc_int8_grad_input")
-    return dx
-
-
-def int8_grad_weight(g, xq, x_scale, weight_dtype=None, bias_dtype=None):
-    """Straight-through gradients with respect to weight and bias: (dw [N, K] of weight_dtype, db [N] of bias_dtype);
-    a type of None: not wanted."""
-    if not (g.is_cuda and xq.is_cuda):
-        _require_cuda(g, xq)
-    _same_device("linear_int8", g, xq, x_scale)
-    code = _dtype_code(g, "linear_int8")
-    N = g.shape[-1]
-    M, K = xq.shape
-    gm = _dense_rows(g, N)
-    device, dev = g.device, g.get_device()
-    L = _lib.lib()
-    with _on(dev):
-        xq, sa = _operand8(xq, "linear_int8")
-        dw = torch.empty((N, K), dtype=weight_dtype, device=device) if weight_dtype is not None else None
-        db = torch.empty((N,), dtype=bias_dtype, device=device) if bias_dtype is not None else None
-        d = ctypes.byref(_lib.Int8Desc(M, N, K, code, 0 if bias_dtype is None else _dtype_code(bias_dtype, "linear_int8"),
-                                       0 if weight_dtype is None else _dtype_code(weight_dtype, "linear_int8"), 0, 0, sa, 0))
-        ws, nbytes = _int8_space(L, d, _lib.INT8_GRAD_WEIGHT, device)
-        rc = L.rexsc_int8_grad_weight(d, gm.data_ptr(), xq.data_ptr(), x_scale.data_ptr(), _addr(dw), _addr(db), _addr(ws),
-                                      nbytes, _raw_stream(dev))
-        if rc:
-            _lib.check(rc, "rexsc_int8_grad_weight")
-    return dw, db
+            _lib.check(rc, "rexsc_int8_backward")
+    return dx, dw, db
 
 
 # ---- layer norm ----------------------------------------------------------------------------------

@@ -5,11 +5,9 @@
 //   y[m][n] = (sum_k qa[m][k] qb[n][k]) sa[m] sb[n] + bias[n]            sum exact in int32
 //   dx[m][k] = sum_n (g[m][n] sb[n]) qb[n][k]     dw[n][k] = sum_m (g[m][n] sa[m]) qa[m][k]     db[n] = sum_m g[m][n]
 //
-// The gradients run on the bfloat16 matrix instructions: an int8 value is exact in bfloat16, and the float32 factor
-// g * s is split into bfloat16 pieces whose sum it is (8 bits each: three pieces hold all 24 bits and serve float32
-// results, two hold 16 and serve 16-bit results, whose own rounding is far coarser), so nothing but the float32
-// accumulation is rounded.  Pieces and transposed operands are laid out in the workspace first, which makes both
-// gradients the same product of two row-major operands as the forward pass.
+// The gradients run on the binary16 matrix instructions: an int8 value is exact in binary16, and the float32 factor
+// g * s is taken apart into binary16 pieces.  Pieces and transposed operands are laid out in the workspace first, which
+// makes both gradients the same product of two row-major operands as the forward pass.
 #include <stdlib.h>
 
 #include "few_rows.h"
@@ -127,79 +125,203 @@ void launch_quantize_t(const QuantArgs &p, hipStream_t s)
 }
 
 // ---- operands of the gradients ---------------------------------------------------------------------
-// v = sum of `pieces` bfloat16 values.  Each but the last keeps the leading 8 bits (truncated, so that nothing
-// overflows), the last is rounded.  Of an infinity or NaN the first piece is all.
-__device__ __forceinline__ void split(float v, int pieces, bf16_t (&out)[3])
+// Both gradients sum (gradient * scale) * int8.  An int8 value is exact in binary16, and the float32 factor v = g * s is
+// taken apart into binary16 pieces, each rounded to nearest (2^-11): v = h + l to 2^-22 of v.  A power of two per
+// row of the result keeps them in binary16's range: with the row's largest |v| between 2^14 and 2^15, a v below 2^-28
+// of that loses bits, and no more than 2^-40 of the largest.  It is multiplied back in the epilogue, exactly.
+// Results in float32 or float16 take both pieces, less of an error than the float32 additions of a few terms make;
+// results in bfloat16 take one: it is off by an eighth of what the gradient's own type and the result's round to.
+struct OperandArgs {
+    const void *g;                  // [M][N] dense
+    int M, N, K;
+    const float *a_scale, *b_scale;
+    const int8_t *a, *b;            // tokens [M][K], channels [N][K]
+    size_t a_stride, b_stride;
+    // for dx: pieces of g * b_scale, [pieces][M][ldn], with the rows' powers of two, and b transposed, [K][ldn]
+    f16_t *g_rows, *b_t;
+    float *g_rows_scale;
+    int pieces_x, ldn;
+    // for dw: pieces of (g * a_scale) transposed, [pieces][N][ldm], likewise, and a transposed, [K][ldm]
+    f16_t *g_cols, *a_t;
+    float *g_cols_scale;
+    int pieces_w, ldm;
+    // statistics of g's columns over each of `shares` runs of `share_rows` rows: sum of g and largest |g * a_scale|
+    float *sums;
+    unsigned *tops;
+    int shares, share_rows;
+    void *db;
+    int db_dtype;
+    // blocks of the first launch: rows of g, then tiles of b, then tiles of a, then the statistics
+    unsigned row_blocks, b_blocks, a_blocks, stat_blocks;
+};
+
+// Exponent e with top * 2^-e in [2^14, 2^15), or below where 2^e would not be a normal number; 0 for an empty row.
+__device__ __forceinline__ int piece_exponent(unsigned top)
 {
-    const bool finite = mag_bits(v) < 0x7f800000u;
+    return top == 0 ? 0 : max(ilogbf(__uint_as_float(top)) - 14, -126);
+}
+// What the row's sums are multiplied by: 2^e, or NaN where the row holds an infinity or a NaN.
+__device__ __forceinline__ float piece_scale(unsigned top, int e)
+{
+    return top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : ldexpf(1.f, e);
+}
+__device__ __forceinline__ void split(float v, unsigned top, int e, f16_t &high, f16_t &low)
+{
+    const float t = top >= 0x7f800000u ? 0.f : ldexpf(v, -e);
+    high = (f16_t)t;
+    low = (f16_t)(t - (float)high);
+}
+
+template <typename T, int V>
+__device__ void split_row(const OperandArgs &p, size_t row, unsigned (&lds)[16])
+{
+    const T *g = (const T *)p.g + row * (size_t)p.N;
+    unsigned t = 0;
+    for (int c = threadIdx.x * V; c < p.N; c += 256 * V) {
+        float v[V];
+        load_vec<V>(v, g + c);
 #pragma unroll
-    for (int i = 0; i < 3; i++) {
-        if (i >= pieces) break;
-        if (!finite) { out[i] = i == 0 ? (bf16_t)v : (bf16_t)0.f; continue; }
-        if (i + 1 == pieces) { out[i] = (bf16_t)v; break; }
-        const float head = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-        out[i] = (bf16_t)head;
-        v -= head;
+        for (int j = 0; j < V; j++) t = max(t, mag_bits(v[j] * p.b_scale[c + j]));
     }
+    t = row_top<256>(t, lds);
+    const int e = piece_exponent(t);
+    f16_t *high = p.g_rows + row * (size_t)p.ldn, *low = high + (size_t)p.M * p.ldn;
+    for (int c = threadIdx.x * V; c < p.ldn; c += 256 * V) { // ldn is a multiple of 64: whole vectors
+        float v[V] = {};
+        if (c < p.N) load_vec<V>(v, g + c);
+        typename VecOf<f16_t, V>::type h, l;
+        f16_t *hp = (f16_t *)&h, *lp = (f16_t *)&l;
+#pragma unroll
+        for (int j = 0; j < V; j++) split(c < p.N ? v[j] * p.b_scale[c + j] : 0.f, t, e, hp[j], lp[j]);
+        *(typename VecOf<f16_t, V>::type *)(high + c) = h;
+        if (p.pieces_x > 1) *(typename VecOf<f16_t, V>::type *)(low + c) = l;
+    }
+    if (threadIdx.x == 0) p.g_rows_scale[row] = piece_scale(t, e);
 }
 
-// g [rows][cols] -> out [pieces][rows][ld], elements times scale[column], columns from cols to ld zero.
-template <typename T>
-__global__ __launch_bounds__(256) void split_rows_kernel(const T *g, const float *scale, int cols, int ld, int pieces, bf16_t *out)
+// q [rows][cols] int8 -> out [cols][ld] binary16, positions from rows to ld zero; a 64 x 64 tile.  q's rows are 16-byte
+// aligned and readable to the next multiple of 16.
+__device__ void transpose_tile(const int8_t *q, size_t stride, int rows, int cols, int ld, f16_t *out, unsigned tile, int8_t (&lds)[64][68])
 {
-    const size_t row = blockIdx.x, rows = gridDim.x;
-    for (int c = threadIdx.x; c < ld; c += 256) {
-        bf16_t q[3];
-        split(c < cols ? (float)g[row * cols + c] * scale[c] : 0.f, pieces, q);
-        for (int i = 0; i < pieces; i++) out[(i * rows + row) * ld + c] = q[i];
+    const int across = ld / 64, r0 = (int)(tile % across) * 64, c0 = (int)(tile / across) * 64;
+    const int r = threadIdx.x / 4, c = threadIdx.x % 4 * 16;
+    int v[4] = {0, 0, 0, 0};
+    if (r0 + r < rows && c0 + c < cols) {
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        const i32x4 u = *(const i32x4 *)(q + (size_t)(r0 + r) * stride + c0 + c);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = u[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) *(int *)&lds[r][c + 4 * i] = v[i];
+    __syncthreads();
+    const int oc = threadIdx.x / 4, orow = threadIdx.x % 4 * 16;
+    if (c0 + oc >= cols) return;
+    f16_t *dst = out + (size_t)(c0 + oc) * ld + r0 + orow;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        typename VecOf<f16_t, 8>::type w;
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = (f16_t)(float)lds[orow + 8 * h + i][oc];
+        *(typename VecOf<f16_t, 8>::type *)(dst + 8 * h) = w;
     }
 }
 
-// g [rows][cols] -> out [pieces][cols][ld], elements times scale[row], positions from rows to ld zero; and the sums of
-// g's columns over this block's 64 rows to part[row block][cols].  out NULL: only the sums.
+// Sum of g and largest |g * a_scale| of 64 columns over one share of the rows.
 template <typename T>
-__global__ __launch_bounds__(256) void split_transposed_kernel(const T *g, const float *scale, int rows, int cols, int ld,
-                                                               int pieces, bf16_t *out, float *part)
+__device__ void column_stats(const OperandArgs &p, unsigned block, float (&ls)[4][64], unsigned (&lt)[4][64])
+{
+    const int share = (int)(block % p.shares), c = (int)(block / p.shares) * 64 + threadIdx.x % 64, part = threadIdx.x / 64;
+    const int begin = share * p.share_rows, end = min(p.M, begin + p.share_rows);
+    float s = 0.f;
+    unsigned t = 0;
+    if (c < p.N)
+#pragma unroll 8
+        for (int m = begin + part; m < end; m += 4) {
+            const float g = (float)((const T *)p.g)[(size_t)m * p.N + c];
+            s += g;
+            if (p.a_scale) t = max(t, mag_bits(g * p.a_scale[m]));
+        }
+    ls[part][threadIdx.x % 64] = s;
+    lt[part][threadIdx.x % 64] = t;
+    __syncthreads();
+    if (part == 0 && c < p.N) {
+#pragma unroll
+        for (int i = 1; i < 4; i++) {
+            s += ls[i][threadIdx.x];
+            t = max(t, lt[i][threadIdx.x]);
+        }
+        p.sums[(size_t)share * p.N + c] = s;
+        p.tops[(size_t)share * p.N + c] = t;
+    }
+}
+
+// All that the gradients' operands need of each other's results is the columns' statistics, so everything else is one
+// launch, told apart by the block's number.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void operands_kernel(OperandArgs p)
+{
+    __shared__ union {
+        unsigned top[16];
+        int8_t tile[64][68];
+        struct { float s[4][64]; unsigned t[4][64]; } stats;
+    } lds;
+    unsigned b = blockIdx.x;
+    if (b < p.row_blocks) return split_row<T, V>(p, b, lds.top);
+    b -= p.row_blocks;
+    if (b < p.b_blocks) return transpose_tile(p.b, p.b_stride, p.N, p.K, p.ldn, p.b_t, b, lds.tile);
+    b -= p.b_blocks;
+    if (b < p.a_blocks) return transpose_tile(p.a, p.a_stride, p.M, p.K, p.ldm, p.a_t, b, lds.tile);
+    b -= p.a_blocks;
+    column_stats<T>(p, b, lds.stats.s, lds.stats.t);
+}
+
+// The second launch: pieces of (g * a_scale) transposed, a 64 x 64 tile per block, and db from the shares' sums.
+template <typename T>
+__global__ __launch_bounds__(256) void transposed_pieces_kernel(OperandArgs p)
 {
     __shared__ float tile[64][65];
-    const int row_blocks = ld / 64;
-    const int r0 = (int)(blockIdx.x % row_blocks) * 64, c0 = (int)(blockIdx.x / row_blocks) * 64;
+    __shared__ unsigned top[64];
+    const int across = p.ldm / 64, m0 = (int)(blockIdx.x % across) * 64, n0 = (int)(blockIdx.x / across) * 64;
     const int tx = threadIdx.x % 64, ty = threadIdx.x / 64;
+    const int n = n0 + tx;
+#pragma unroll 4
     for (int i = ty; i < 64; i += 4) {
-        const int r = r0 + i, c = c0 + tx;
-        tile[i][tx] = r < rows && c < cols ? (float)g[(size_t)r * cols + c] : 0.f;
+        const int m = m0 + i;
+        tile[i][tx] = m < p.M && n < p.N ? (float)((const T *)p.g)[(size_t)m * p.N + n] * p.a_scale[m] : 0.f;
     }
-    __syncthreads();
-    if (part && ty == 0 && c0 + tx < cols) {
+    if (ty == 0) {
+        unsigned t = 0;
         float s = 0.f;
-        for (int i = 0; i < 64; i++) s += tile[i][tx];
-        part[(size_t)(r0 / 64) * cols + c0 + tx] = s;
-    }
-    if (!out) return;
-    const float sc = r0 + tx < rows ? scale[r0 + tx] : 0.f;
-    for (int i = ty; i < 64; i += 4) {
-        if (c0 + i >= cols) break;
-        bf16_t q[3];
-        split(r0 + tx < rows ? tile[tx][i] * sc : 0.f, pieces, q);
-        for (int j = 0; j < pieces; j++) out[((size_t)j * cols + c0 + i) * ld + r0 + tx] = q[j];
-    }
-}
-
-// q [rows][cols] int8 -> out [cols][ld] bfloat16, positions from rows to ld zero.
-__global__ __launch_bounds__(256) void transpose_i8_kernel(const int8_t *q, size_t stride, int rows, int cols, int ld, bf16_t *out)
-{
-    __shared__ int8_t tile[64][68];
-    const int row_blocks = ld / 64;
-    const int r0 = (int)(blockIdx.x % row_blocks) * 64, c0 = (int)(blockIdx.x / row_blocks) * 64;
-    const int tx = threadIdx.x % 64, ty = threadIdx.x / 64;
-    for (int i = ty; i < 64; i += 4) {
-        const int r = r0 + i, c = c0 + tx;
-        tile[i][tx] = r < rows && c < cols ? q[(size_t)r * stride + c] : (int8_t)0;
+        if (n < p.N)
+            for (int i = 0; i < p.shares; i++) {
+                t = max(t, p.tops[(size_t)i * p.N + n]);
+                s += p.sums[(size_t)i * p.N + n];
+            }
+        top[tx] = t;
+        if (m0 == 0 && n < p.N) {
+            p.g_cols_scale[n] = piece_scale(t, piece_exponent(t));
+            if (p.db) store_any(p.db, p.db_dtype, n, s);
+        }
     }
     __syncthreads();
-    for (int i = ty; i < 64; i += 4) {
-        if (c0 + i >= cols) break;
-        out[(size_t)(c0 + i) * ld + r0 + tx] = (bf16_t)(float)tile[tx][i];
+    const int on = threadIdx.x / 4, om = threadIdx.x % 4 * 16;
+    if (n0 + on >= p.N) return;
+    const unsigned t = top[on];
+    const int e = piece_exponent(t);
+    f16_t *high = p.g_cols + (size_t)(n0 + on) * p.ldm + m0 + om, *low = high + (size_t)p.N * p.ldm;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        typename VecOf<f16_t, 8>::type hv, lv;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            f16_t a, b;
+            split(tile[om + 8 * h + i][on], t, e, a, b);
+            hv[i] = a;
+            lv[i] = b;
+        }
+        *(typename VecOf<f16_t, 8>::type *)(high + 8 * h) = hv;
+        if (p.pieces_w > 1) *(typename VecOf<f16_t, 8>::type *)(low + 8 * h) = lv;
     }
 }
 
@@ -227,9 +349,13 @@ int check_rows8(const char *what, const void *q, int64_t stride, int K)
 }
 
 inline int64_t pad64(int64_t n) { return (n + 63) / 64 * 64; }
-inline int pieces_of(int dtype) { return dtype == REXSC_F32 ? 3 : 2; }
+inline int pieces_of(int dtype) { return dtype == REXSC_BF16 ? 1 : 2; }
 
-struct Space { size_t tokens, scales, pieces, transposed, part, product, total; };
+struct Space { size_t tokens, scales, g_rows, g_rows_scale, b_t, g_cols, g_cols_scale, a_t, sums, tops, product, total; };
+
+constexpr int MAX_SHARES = 32, SHARE_ROWS = 256; // runs of g's rows whose column statistics are taken apart
+int share_rows(int M) { return max(SHARE_ROWS, (M + MAX_SHARES - 1) / MAX_SHARES); }
+int shares(int M) { return (M + share_rows(M) - 1) / share_rows(M); }
 
 Space space(const rexsc_int8_desc *d, int what)
 {
@@ -243,17 +369,19 @@ Space space(const rexsc_int8_desc *d, int what)
         s.product = take(tile_product_workspace(d->M, d->N, d->K, 1));
         s.tokens = take(M * align_up(K, 128));
         s.scales = take(M * 4);
-    } else if (what == REXSC_INT8_GRAD_INPUT) {
-        const size_t ld = pad64(N);
-        s.product = take(tile_product_workspace(d->M, d->K, (int)ld * 2, pieces_of(d->dtype)));
-        s.pieces = take(M * ld * pieces_of(d->dtype) * 2);
-        s.transposed = take(K * ld * 2);
-    } else if (what == REXSC_INT8_GRAD_WEIGHT) {
-        const size_t ld = pad64(M);
-        s.product = take(tile_product_workspace(d->N, d->K, (int)ld * 2, pieces_of(d->weight_dtype)));
-        s.pieces = take(N * ld * pieces_of(d->weight_dtype) * 2);
-        s.transposed = take(K * ld * 2);
-        s.part = take(ld / 64 * N * 4);
+    } else if (M > 0 && N > 0) {
+        // dx and dw follow each other on the stream, so their partial results share a place
+        const size_t ldn = pad64(N), ldm = pad64(M);
+        const int px = pieces_of(d->dtype), pw = pieces_of(d->weight_dtype);
+        s.product = take(max(tile_product_workspace(d->M, d->K, (int)ldn * 2, px), tile_product_workspace(d->N, d->K, (int)ldm * 2, pw)));
+        s.g_rows = take(M * ldn * px * 2);
+        s.g_rows_scale = take(M * 4);
+        s.b_t = take(K * ldn * 2);
+        s.g_cols = take(N * ldm * pw * 2);
+        s.g_cols_scale = take(N * 4);
+        s.a_t = take(K * ldm * 2);
+        s.sums = take((size_t)shares(d->M) * N * 4);
+        s.tops = take((size_t)shares(d->M) * N * 4);
     }
     s.total = at;
     return s;
@@ -310,7 +438,7 @@ extern "C" int rexsc_quantize_rows(const void *x, int dtype, size_t rows, size_t
 extern "C" size_t rexsc_int8_workspace_bytes(const rexsc_int8_desc *d, int what)
 {
     if (check_int8(d)) return (size_t)-1;
-    if (what < REXSC_INT8_PRODUCT || what > REXSC_INT8_GRAD_WEIGHT) {
+    if (what < REXSC_INT8_PRODUCT || what > REXSC_INT8_BACKWARD) {
         set_error("int8 linear: no call has the number %d", what);
         return (size_t)-1;
     }
@@ -355,71 +483,87 @@ extern "C" int rexsc_int8_linear(const rexsc_int8_desc *d, const void *x, const 
     return product(d, q, (int64_t)stride, scale, b, b_scale, bias, y, (char *)workspace + s.product, stream);
 }
 
-extern "C" int rexsc_int8_grad_input(const rexsc_int8_desc *d, const void *g, const int8_t *b, const float *b_scale, void *dx,
-                                     void *workspace, size_t workspace_bytes, rexsc_stream_t stream_)
+extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, const int8_t *a, const float *a_scale,
+                                   const int8_t *b, const float *b_scale, void *dx, void *dw, void *db, void *workspace,
+                                   size_t workspace_bytes, rexsc_stream_t stream_)
 {
     hipStream_t stream = (hipStream_t)stream_;
     if (int rc = check_int8(d)) return rc;
-    if (d->M == 0) return REXSC_OK;
-    REXSC_CHECK_ARG(d->N >= 1, "int8 linear: a gradient needs at least one output channel");
-    if (int rc = check_rows8("channels", b, d->b_stride, d->K)) return rc;
-    REXSC_CHECK_ARG(g && b_scale && dx, "null pointer");
-    const Space s = space(d, REXSC_INT8_GRAD_INPUT);
+    if (!dx && !dw && !db) return REXSC_OK;
+    if (d->M == 0 || d->N == 0) { // sums over nothing: zeros, from the same kernels
+        auto zeros = [&](int rows, void *y, int dtype) {
+            const TileArgs t{nullptr, nullptr, 0, 0, rows, d->K, 0, 1, 0, nullptr, nullptr, nullptr, REXSC_F32, y};
+            return launch_tile_product(t, true, dtype, nullptr, "int8_backward_empty", stream);
+        };
+        if (dx && d->M > 0)
+            if (int rc = zeros(d->M, dx, d->dtype)) return rc;
+        if (dw && d->N > 0)
+            if (int rc = zeros(d->N, dw, d->weight_dtype)) return rc;
+        if (db && d->N > 0) return launch_column_sums(nullptr, 0, d->N, d->N, db, d->bias_dtype, stream);
+        return REXSC_OK;
+    }
+    REXSC_CHECK_ARG(g && (!dx || b_scale) && (!dw || a_scale), "null pointer");
+    REXSC_CHECK_ARG((uintptr_t)g % dtype_size(d->dtype) == 0, "int8 linear: the gradient is not aligned to its element");
+    if (dx)
+        if (int rc = check_rows8("channels", b, d->b_stride, d->K)) return rc;
+    if (dw)
+        if (int rc = check_rows8("tokens", a, d->a_stride, d->K)) return rc;
+    const Space s = space(d, REXSC_INT8_BACKWARD);
     if (int rc = check_space(s, workspace, workspace_bytes)) return rc;
-    bf16_t *pieces = (bf16_t *)((char *)workspace + s.pieces), *bt = (bf16_t *)((char *)workspace + s.transposed);
-    const int P = pieces_of(d->dtype), ld = (int)pad64(d->N);
-    {
-        ProfScope prof("int8_grad_operands", (double)d->M * d->N * (dtype_size(d->dtype) + 2.0 * P), stream);
-        REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL(split_rows_kernel<T>, dim3((unsigned)d->M), dim3(256), 0, stream,
-                                                        (const T *)g, b_scale, d->N, ld, P, pieces));
-        REXSC_CHECK_HIP(hipGetLastError());
-    }
-    {
-        ProfScope prof("int8_grad_operands", 3.0 * d->N * d->K, stream);
-        hipLaunchKernelGGL(transpose_i8_kernel, dim3((unsigned)((ld / 64) * ((d->K + 63) / 64))), dim3(256), 0, stream, b,
-                           (size_t)d->b_stride, d->N, d->K, ld, bt);
-        REXSC_CHECK_HIP(hipGetLastError());
-    }
-    const TileArgs p{(const char *)pieces, (const char *)bt, (size_t)ld * 2, (size_t)ld * 2, d->M, d->K, ld * 2, P,
-                     (size_t)d->M * ld * 2, nullptr, nullptr, nullptr, REXSC_F32, dx};
-    return launch_tile_product(p, true, d->dtype, (char *)workspace + s.product, "int8_grad_input", stream);
-}
+    auto at = [&](size_t o) { return (char *)workspace + o; };
 
-extern "C" int rexsc_int8_grad_weight(const rexsc_int8_desc *d, const void *g, const int8_t *a, const float *a_scale, void *dw,
-                                      void *db, void *workspace, size_t workspace_bytes, rexsc_stream_t stream_)
-{
-    hipStream_t stream = (hipStream_t)stream_;
-    if (int rc = check_int8(d)) return rc;
-    if (d->N == 0 || (!dw && !db)) return REXSC_OK;
-    const Space s = space(d, REXSC_INT8_GRAD_WEIGHT);
-    if (d->M > 0) {
-        if (dw)
-            if (int rc = check_rows8("tokens", a, d->a_stride, d->K)) return rc;
-        REXSC_CHECK_ARG(g && (a_scale || !dw), "null pointer");
-        if (int rc = check_space(s, workspace, workspace_bytes)) return rc;
-    }
-    bf16_t *pieces = (bf16_t *)((char *)workspace + s.pieces), *at = (bf16_t *)((char *)workspace + s.transposed);
-    float *part = (float *)((char *)workspace + s.part);
-    const int P = pieces_of(d->weight_dtype), ld = (int)pad64(d->M);
-    if (d->M > 0) {
-        ProfScope prof("int8_grad_operands", (double)d->M * d->N * (dtype_size(d->dtype) + (dw ? 2.0 * P : 0)), stream);
-        REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL(split_transposed_kernel<T>,
-                                                        dim3((unsigned)((ld / 64) * ((d->N + 63) / 64))), dim3(256), 0, stream,
-                                                        (const T *)g, a_scale, d->M, d->N, ld, P, dw ? pieces : nullptr,
-                                                        db ? part : nullptr));
+    OperandArgs p{};
+    p.g = g;
+    p.M = d->M; p.N = d->N; p.K = d->K;
+    p.a_scale = dw ? a_scale : nullptr;
+    p.b_scale = b_scale;
+    p.a = a; p.b = b;
+    p.a_stride = (size_t)d->a_stride; p.b_stride = (size_t)d->b_stride;
+    p.g_rows = (f16_t *)at(s.g_rows); p.b_t = (f16_t *)at(s.b_t); p.g_rows_scale = (float *)at(s.g_rows_scale);
+    p.g_cols = (f16_t *)at(s.g_cols); p.a_t = (f16_t *)at(s.a_t); p.g_cols_scale = (float *)at(s.g_cols_scale);
+    p.pieces_x = pieces_of(d->dtype); p.pieces_w = pieces_of(d->weight_dtype);
+    p.ldn = (int)pad64(d->N); p.ldm = (int)pad64(d->M);
+    p.sums = (float *)at(s.sums); p.tops = (unsigned *)at(s.tops);
+    p.shares = shares(d->M); p.share_rows = share_rows(d->M);
+    p.db = db; p.db_dtype = d->bias_dtype;
+    const uint64_t tiles_k = (uint64_t)((d->K + 63) / 64), tiles_n = (uint64_t)p.ldn / 64, tiles_m = (uint64_t)p.ldm / 64;
+    REXSC_CHECK_ARG((uint64_t)d->M + (tiles_n + tiles_m) * tiles_k + tiles_n * MAX_SHARES < (1ull << 31) && tiles_m * tiles_n < (1ull << 31),
+                    "int8 linear: %d x %d x %d is too large", d->M, d->N, d->K);
+    REXSC_CHECK_ARG((size_t)p.ldn * 2 < MAX_ROW_BYTES && (size_t)p.ldm * 2 < MAX_ROW_BYTES,
+                    "int8 linear: gradients of at most %zu tokens or channels", MAX_ROW_BYTES / 2 - 64);
+    p.row_blocks = dx ? (unsigned)d->M : 0;
+    p.b_blocks = dx ? (unsigned)(tiles_n * tiles_k) : 0;
+    p.a_blocks = dw ? (unsigned)(tiles_m * tiles_k) : 0;
+    p.stat_blocks = dw || db ? (unsigned)(p.shares * tiles_n) : 0;
+    {
+        const double es = (double)dtype_size(d->dtype), mn = (double)d->M * d->N, k = (double)d->K;
+        ProfScope prof("int8_backward_operands", (dx ? mn * (es + 2.0 * p.pieces_x) + 3.0 * k * d->N : 0.0) + (dw || db ? mn * es : 0.0) +
+                       (dw ? 3.0 * k * d->M : 0.0), stream);
+        const dim3 grid(p.row_blocks + p.b_blocks + p.a_blocks + p.stat_blocks);
+        const int V = d->dtype == REXSC_F32 ? 4 : 8;
+        if (d->N % V == 0 && (uintptr_t)g % 16 == 0)
+            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((operands_kernel<T, 16 / sizeof(T)>), grid, dim3(256), 0, stream, p));
+        else
+            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((operands_kernel<T, 1>), grid, dim3(256), 0, stream, p));
         REXSC_CHECK_HIP(hipGetLastError());
     }
-    if (db)
-        if (int rc = launch_column_sums(part, (size_t)ld / 64, d->N, d->N, db, d->bias_dtype, stream)) return rc;
-    if (!dw) return REXSC_OK;
-    if (d->M > 0) {
-        ProfScope prof("int8_grad_operands", 3.0 * d->M * d->K, stream);
-        hipLaunchKernelGGL(transpose_i8_kernel, dim3((unsigned)((ld / 64) * ((d->K + 63) / 64))), dim3(256), 0, stream, a,
-                           (size_t)d->a_stride, d->M, d->K, ld, at);
+    if (dw) {
+        ProfScope prof("int8_backward_pieces", (double)d->M * d->N * (dtype_size(d->dtype) + 2.0 * p.pieces_w), stream);
+        REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL(transposed_pieces_kernel<T>, dim3((unsigned)(tiles_m * tiles_n)), dim3(256), 0,
+                                                        stream, p));
         REXSC_CHECK_HIP(hipGetLastError());
+    } else if (db) {
+        if (int rc = launch_column_sums(p.sums, p.shares, d->N, d->N, db, d->bias_dtype, stream)) return rc;
     }
-    // without tokens the reduction is empty and the kernel writes zeros
-    const TileArgs p{(const char *)pieces, (const char *)at, (size_t)ld * 2, (size_t)ld * 2, d->N, d->K, ld * 2, P,
-                     (size_t)d->N * ld * 2, nullptr, nullptr, nullptr, REXSC_F32, dw};
-    return launch_tile_product(p, true, d->weight_dtype, (char *)workspace + s.product, "int8_grad_weight", stream);
+    if (dx) {
+        const TileArgs t{(const char *)p.g_rows, (const char *)p.b_t, (size_t)p.ldn * 2, (size_t)p.ldn * 2, d->M, d->K, p.ldn * 2,
+                         p.pieces_x, (size_t)d->M * p.ldn * 2, p.g_rows_scale, nullptr, nullptr, REXSC_F32, dx};
+        if (int rc = launch_tile_product(t, true, d->dtype, at(s.product), "int8_grad_input", stream)) return rc;
+    }
+    if (dw) {
+        const TileArgs t{(const char *)p.g_cols, (const char *)p.a_t, (size_t)p.ldm * 2, (size_t)p.ldm * 2, d->N, d->K, p.ldm * 2,
+                         p.pieces_w, (size_t)d->N * p.ldm * 2, p.g_cols_scale, nullptr, nullptr, REXSC_F32, dw};
+        if (int rc = launch_tile_product(t, true, d->weight_dtype, at(s.product), "int8_grad_weight", stream)) return rc;
+    }
+    return REXSC_OK;
 }

@@ -11,14 +11,14 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 
 struct OpI8 { typedef i32x4 acc; };
-struct OpBF16 { typedef f32x4 acc; };
+struct OpF16 { typedef f32x4 acc; };
 __device__ __forceinline__ i32x4 mma(OpI8, i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x4 mma(OpBF16, i32x4 a, i32x4 b, f32x4 c)
+__device__ __forceinline__ f32x4 mma(OpF16, i32x4 a, i32x4 b, f32x4 c)
 {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
 // Waits until at most N of this wave's loads into LDS are still on their way (they land in order), and until its reads
@@ -359,7 +359,7 @@ size_t tile_product_workspace(int M, int N, int kbytes, int pieces)
     return pl.splits > 1 ? (size_t)pl.splits * M * N * 4 : 0;
 }
 
-int launch_tile_product(const TileArgs &p, bool bf16, int out_dtype, void *workspace, const char *name, hipStream_t stream)
+int launch_tile_product(const TileArgs &p, bool f16, int out_dtype, void *workspace, const char *name, hipStream_t stream)
 {
     REXSC_CHECK_ARG(p.a_stride < MAX_ROW_BYTES && p.b_stride < MAX_ROW_BYTES,
                     "int8 linear: operand rows of %zu and %zu bytes, at most %zu are supported", p.a_stride, p.b_stride,
@@ -367,8 +367,8 @@ int launch_tile_product(const TileArgs &p, bool bf16, int out_dtype, void *works
     const TilePlan pl = tile_plan(p.M, p.N, p.kbytes, p.pieces);
     const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64);
     REXSC_CHECK_ARG(tiles * pl.splits < (1ll << 31), "int8 linear: result of %d x %d is too large", p.M, p.N);
-    ProfScope prof(name, 2.0 * p.M * p.N * (bf16 ? p.kbytes / 2 : p.kbytes) * p.pieces, stream);
-    if (bf16) REXSC_DTYPE_SWITCH(out_dtype, return (launch_size<OpBF16, T>(p, pl, workspace, stream)));
+    ProfScope prof(name, 2.0 * p.M * p.N * (f16 ? p.kbytes / 2 : p.kbytes) * p.pieces, stream);
+    if (f16) REXSC_DTYPE_SWITCH(out_dtype, return (launch_size<OpF16, T>(p, pl, workspace, stream)));
     else REXSC_DTYPE_SWITCH(out_dtype, return (launch_size<OpI8, T>(p, pl, workspace, stream)));
 }
 

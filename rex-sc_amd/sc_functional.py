@@ -739,13 +739,8 @@ class Linear_Int8_Grad(torch.autograd.Function):
         wq, ws, xq, xs = ctx.saved_tensors
         w_dtype, b_dtype = ctx.types
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = _ops.int8_grad_input(grad_output, wq, ws) if need_x else None
-        dw = db = None
-        if need_w:
-            dw, db = _ops.int8_grad_weight(grad_output, xq, xs, w_dtype, b_dtype if need_b else None)
-        elif need_b:
-            db = grad_output.reshape(-1, grad_output.shape[-1]).sum(0, dtype=torch.float32).to(b_dtype)
-        return dx, dw, db, None
+        return _ops.int8_backward(grad_output, xq, xs, wq, ws, need_x, w_dtype if need_w else None,
+                                  b_dtype if need_b else None) + (None,)
 
 
 def linear_int8(x, weight, bias=None, weight_scale=None):

@@ -251,9 +251,11 @@ def test_gradients(dt, wdt, m, n, k):
     xd, wd, gd = qx * sx.double()[:, None], qw * sw.double()[:, None], go.double()
 
     def close(got, want, size, terms, out):
-        # two pieces of the factor g * scale keep 16 bits of it: 2^-16 of every term; three keep all
-        pieces = 3 if out == torch.float32 else 2
-        tol = size * ((terms * pieces + 4) * 2.0 ** -23 + (2.0 ** -16 if pieces == 2 else 0.0))
+        # the factor g * scale is taken apart into binary16 pieces, each off by half a step of that type, eps / 2 = 2^-11:
+        # one, for bfloat16 results, leaves 2^-11 of a term, two, for the others, 2^-11 * 2^-11 = 2^-22.  Terms below
+        # 2^-28 of the row's largest: 2^-40 of that, nothing beside the additions' share of `size`.
+        pieces = 1 if out == torch.bfloat16 else 2
+        tol = size * ((terms * pieces + 4) * 2.0 ** -23 + 2.0 ** (-11 * pieces))
         tol = tol + _half(out) * (want.abs() + tol) + _floor(out)
         err = (got.cpu().double() - want).abs()
         assert got.dtype == out and (err <= tol).all(), "max error %g of its bound" % (err / tol).max()

@@ -39,13 +39,14 @@ def test_int8_workspace_and_refusals():
     none = ctypes.c_size_t(-1).value
     ws = lambda d, what: L.rexsc_int8_workspace_bytes(ctypes.byref(d), what)
     assert ws(_int8(M=1000, K=4096), _lib.INT8_LINEAR) >= 1000 * 4096 + 4000
-    assert ws(_int8(M=100, N=50, K=70), _lib.INT8_GRAD_INPUT) >= 100 * 64 * 3 * 2 + 70 * 64 * 2
-    assert ws(_int8(M=100, N=50, K=70, weight=2), _lib.INT8_GRAD_WEIGHT) >= 50 * 128 * 2 * 2 + 70 * 128 * 2
+    # both pieces of g for either gradient, and the transposed operands, in binary16
+    assert ws(_int8(M=100, N=50, K=70), _lib.INT8_BACKWARD) >= 2 * (2 * 100 * 64 + 70 * 64 + 2 * 50 * 128 + 70 * 128)
+    assert ws(_int8(M=0), _lib.INT8_BACKWARD) == ws(_int8(N=0), _lib.INT8_BACKWARD) == 0
     for d, text in ((_int8(K=0), "K must be"), (_int8(K=131072), "K must be"), (_int8(M=-1), "M -1"), (_int8(dtype=3), "dtypes"),
                     (_int8(bias=-1), "dtypes"), (_int8(weight=9), "dtypes"), (_int8(reserved=1), "reserved")):
-        for what in range(4):
+        for what in range(3):
             assert ws(d, what) == none and text in _error(L)
-    assert ws(_int8(), 4) == none and "number 4" in _error(L)
+    assert ws(_int8(), 3) == none and "number 3" in _error(L)
     d = _int8()
     d.struct_size -= 8
     assert ws(d, 0) == none and "struct_size" in _error(L)
@@ -68,11 +69,17 @@ def test_int8_calls_refuse():
     assert linear(big, ws=ODD, n=need) == -1 and "16-byte" in _error(L)
     assert linear(_int8(xs=31)) == -1 and "overlap" in _error(L)
     assert linear(_int8(), x=ctypes.c_void_p(3)) == -1 and "aligned" in _error(L)
-    gi = lambda d, ws=None, n=0: L.rexsc_int8_grad_input(ctypes.byref(d), FAKE, FAKE, FAKE, FAKE, ws, n, None)
-    gw = lambda d, ws=None, n=0: L.rexsc_int8_grad_weight(ctypes.byref(d), FAKE, FAKE, FAKE, FAKE, FAKE, ws, n, None)
-    assert gi(_int8()) == -2 and gw(_int8()) == -2
-    assert gi(_int8(N=0)) == -1 and "output channel" in _error(L)
-    assert gi(_int8(M=0, N=1)) == 0 and gw(_int8(N=0)) == 0
+    back = lambda d, g=FAKE, a=FAKE, b=FAKE, dx=FAKE, dw=FAKE, db=FAKE, ws=None, n=0: L.rexsc_int8_backward(
+        ctypes.byref(d), g, a, FAKE, b, FAKE, dx, dw, db, ws, n, None)
+    assert back(_int8()) == -2 and "workspace" in _error(L)
+    for d, kw, text in ((_int8(a=40), {}, "tokens"), (_int8(b=16), {}, "channels"), (_int8(), {"a": ODD}, "tokens"),
+                        (_int8(), {"b": None}, "null"), (_int8(), {"g": None}, "null"), (_int8(), {"g": ctypes.c_void_p(2)}, "aligned"),
+                        (_int8(M=4194304, N=1), {}, "at most")):
+        need = L.rexsc_int8_workspace_bytes(ctypes.byref(d), _lib.INT8_BACKWARD)
+        assert back(d, ws=FAKE, n=need, **kw) == -1 and text in _error(L), text
+    # what a gradient does not read is not checked; none wanted, or empty: nothing to do
+    assert back(_int8(a=40), dw=None) == -2 and back(_int8(b=16), dx=None) == -2
+    assert back(_int8(), dx=None, dw=None, db=None) == 0 and back(_int8(M=0, N=0)) == 0
     q = lambda rows, cols, stride, out=FAKE, x=FAKE, dt=0: L.rexsc_quantize_rows(x, dt, rows, cols, cols, out, stride, FAKE, None)
     assert q(0, 4, 16) == 0
     for args, text in (((2, 0, 16), "elements"), ((2, 20, 16), "int8 rows"), ((2, 20, 24), "int8 rows"), ((2, 4, 16, ODD), "int8 rows"),
