@@ -499,7 +499,7 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
             if (int rc = zeros(d->M, dx, d->dtype)) return rc;
         if (dw && d->N > 0)
             if (int rc = zeros(d->N, dw, d->weight_dtype)) return rc;
-        if (db && d->N > 0) return launch_column_sums(nullptr, 0, d->N, d->N, db, d->bias_dtype, stream);
+        if (db && d->N > 0) return launch_column_sums(nullptr, 0, d->N, d->N, db, nullptr, d->bias_dtype, stream);
         return REXSC_OK;
     }
     REXSC_CHECK_ARG(g && (!dx || b_scale) && (!dw || a_scale), "null pointer");
@@ -553,7 +553,7 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
                                                         stream, p));
         REXSC_CHECK_HIP(hipGetLastError());
     } else if (db) {
-        if (int rc = launch_column_sums(p.sums, p.shares, d->N, d->N, db, d->bias_dtype, stream)) return rc;
+        if (int rc = launch_column_sums(p.sums, p.shares, d->N, d->N, db, nullptr, d->bias_dtype, stream)) return rc;
     }
     if (dx) {
         const TileArgs t{(const char *)p.g_rows, (const char *)p.b_t, (size_t)p.ldn * 2, (size_t)p.ldn * 2, d->M, d->K, p.ldn * 2,

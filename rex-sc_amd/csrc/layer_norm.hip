@@ -4,10 +4,11 @@
 //   dx = r (gw - mean(gw) - h mean(gw h)),  gw = g w, h = (x - mu) r;   dw = sum_rows g h;   db = sum_rows g
 //
 // Bound by memory: forward reads x and writes y, backward reads x and g and writes dx, each once.  A row lives in the
-// registers of TPR threads (a wave, or a block of 256, 512 or 1024), at most 16 elements per thread, so the variance
+// registers of TPR threads (16 lanes, a wave, or a block of 256, 512 or 1024), at most 16 elements per thread (backward 32), so the variance
 // is taken around the true mean without a second read.  Blocks are persistent over rows: w and b (forward), w and the
 // two gradient sums (backward) stay in registers from row to row, since re-reading float32 w and b from L2 for every
-// 16-bit row would move more bytes than the row itself.  The next row is loaded before the current one is reduced.
+// 16-bit row would move more bytes than the row itself.  The next row is loaded before the current one is reduced
+// (where registers allow).
 // Rows longer than 16384 elements take the streaming kernels, which read the row again for each pass (from L2).
 #include "lowp.h"
 #include "profile.h"
@@ -33,7 +34,9 @@ template <int TPR, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float (*lds)[TPR / 64 + 1][N], int slot)
 {
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = wave_sum(v[i]);
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int s = (TPR < 64 ? TPR : 64) / 2; s; s >>= 1) v[i] += __shfl_xor(v[i], s, 64);
     if constexpr (TPR > 64) {
         const int wave = threadIdx.x / 64;
         if (threadIdx.x % 64 == 0)
@@ -51,13 +54,13 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*lds)[TPR / 64 + 1
 }
 
 template <typename T, int V, int NV, int TPR>
-__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_forward_kernel(NormParams p)
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_forward_kernel(NormParams p)
 {
-    constexpr int RPB = TPR == 64 ? 4 : 1;
+    constexpr int RPB = TPR <= 64 ? 256 / TPR : 1; // rows a block holds at once
     typedef typename VecOf<T, V>::type vec;
     __shared__ float lds[2][TPR / 64 + 1][1];
-    const int tid = TPR == 64 ? threadIdx.x % 64 : threadIdx.x;
-    const int sub = TPR == 64 ? threadIdx.x / 64 : 0;
+    const int tid = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x;
+    const int sub = TPR <= 64 ? threadIdx.x / TPR : 0;
     const float inv = 1.0f / (float)p.cols;
     float w[NV][V], b[NV][V];
 #pragma unroll
@@ -126,13 +129,13 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_forward_kernel(Nor
 }
 
 template <typename T, int V, int NV, int TPR>
-__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_backward_kernel(NormParams p)
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(NormParams p)
 {
-    constexpr int RPB = TPR == 64 ? 4 : 1;
+    constexpr int RPB = TPR <= 64 ? 256 / TPR : 1; // rows a block holds at once
     typedef typename VecOf<T, V>::type vec;
     __shared__ float lds[2][TPR / 64 + 1][2];
-    const int tid = TPR == 64 ? threadIdx.x % 64 : threadIdx.x;
-    const int sub = TPR == 64 ? threadIdx.x / 64 : 0;
+    const int tid = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x;
+    const int sub = TPR <= 64 ? threadIdx.x / TPR : 0;
     const float inv = 1.0f / (float)p.cols;
     float w[NV][V], dw[NV][V], db[NV][V];
 #pragma unroll
@@ -155,9 +158,11 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_backward_kernel(No
             cg[i] = c < p.cols ? *(const vec *)(sg + c) : vec{};
         }
     };
-    if (row < p.rows) fetch(row);
+    constexpr bool AHEAD = NV * (V == 1 ? 4 : V * sizeof(T)) <= 64; // registers for a row in flight beside the current one
+    if (AHEAD && row < p.rows) fetch(row);
     int slot = 0;
     for (; row < p.rows; row += step) {
+        if (!AHEAD) fetch(row);
         const float mu = p.mean[row], r = p.rstd[row];
         float h[NV][V], gw[NV][V], s[2] = {0.f, 0.f};
 #pragma unroll
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_backward_kernel(No
                 s[0] += gw[i][j];
                 s[1] = fmaf(gw[i][j], h[i][j], s[1]);
             }
-        if (row + step < p.rows) fetch(row + step);
+        if (AHEAD && row + step < p.rows) fetch(row + step);
         if (p.dx) {
             row_sum<TPR, 2>(s, lds, slot);
             slot ^= 1;
@@ -194,27 +199,26 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_backward_kernel(No
     }
     if (!p.part) return;
     float *out = p.part + (size_t)blockIdx.x * 2 * p.cols;
-    if constexpr (TPR == 64) {
-        // the block's four waves hold four sums of the same columns: joined in wave order
-        __shared__ float join[3][2][64 * NV * V];
+    if constexpr (RPB > 1) {
+        // the block's rows hold as many sums of the same columns: joined in their order
+        __shared__ float join[RPB - 1][2][TPR * NV * V];
         if (sub > 0)
 #pragma unroll
             for (int i = 0; i < NV; i++)
 #pragma unroll
                 for (int j = 0; j < V; j++) {
-                    join[sub - 1][0][(i * V + j) * 64 + tid] = dw[i][j];
-                    join[sub - 1][1][(i * V + j) * 64 + tid] = db[i][j];
+                    join[sub - 1][0][(i * V + j) * TPR + tid] = dw[i][j];
+                    join[sub - 1][1][(i * V + j) * TPR + tid] = db[i][j];
                 }
         __syncthreads();
         if (sub > 0) return;
-#pragma unroll
-        for (int k = 0; k < 3; k++)
+        for (int k = 0; k < RPB - 1; k++)
 #pragma unroll
             for (int i = 0; i < NV; i++)
 #pragma unroll
                 for (int j = 0; j < V; j++) {
-                    dw[i][j] += join[k][0][(i * V + j) * 64 + tid];
-                    db[i][j] += join[k][1][(i * V + j) * 64 + tid];
+                    dw[i][j] += join[k][0][(i * V + j) * TPR + tid];
+                    db[i][j] += join[k][1][(i * V + j) * TPR + tid];
                 }
     }
 #pragma unroll
@@ -305,26 +309,37 @@ __global__ __launch_bounds__(256) void norm_dw_stream_kernel(NormParams p)
 }
 
 // ---- column sums -----------------------------------------------------------------------------------
-// A block sums 32 columns, its eight row groups in turn over the rows and then joined in order.
-__global__ __launch_bounds__(256) void column_sums_kernel(const float *part, size_t rows, size_t cols, size_t ld, void *out,
-                                                          int out_dtype)
+// A block sums 16 columns: 64 row groups, each its rows in turn with eight loads in flight, joined in order.  Columns
+// from `cols` on (up to twice as many) go to out2.
+constexpr int CS_COLS = 16, CS_GROUPS = 64;
+__global__ __launch_bounds__(CS_COLS * CS_GROUPS) void column_sums_kernel(const float *part, size_t rows, size_t cols, size_t ld,
+                                                                          void *out, void *out2, int out_dtype)
 {
-    __shared__ float lds[8][33];
-    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-    const size_t c = (size_t)blockIdx.x * 32 + tx;
+    __shared__ float lds[CS_GROUPS][CS_COLS + 1];
+    const int tx = threadIdx.x % CS_COLS, ty = threadIdx.x / CS_COLS;
+    const size_t c = (size_t)blockIdx.x * CS_COLS + tx;
+    void *const dst = blockIdx.y ? out2 : out;
+    if (!dst) return;
+    const float *src = part + (blockIdx.y ? cols : 0) + c;
     float s = 0.f;
-    if (c < cols)
-        for (size_t r = ty; r < rows; r += 8) s += part[r * ld + c];
+    if (c < cols) {
+#pragma unroll 8
+        for (size_t r = ty; r < rows; r += CS_GROUPS) s += src[r * ld];
+    }
     lds[ty][tx] = s;
     __syncthreads();
-    if (ty == 0 && c < cols) {
-#pragma unroll
-        for (int k = 1; k < 8; k++) s += lds[k][tx];
-        store_any(out, out_dtype, c, s);
+    for (int half = CS_GROUPS / 2; half > 0; half /= 2) {
+        if (ty < half) lds[ty][tx] += lds[ty + half][tx];
+        __syncthreads();
     }
+    if (ty == 0 && c < cols) store_any(dst, out_dtype, c, lds[0][tx]);
 }
 
 // ---- host ------------------------------------------------------------------------------------------
+// Waves per CU of the persistent grids.  16384 x 8192 bfloat16: forward 110 us at 16, 142 at 8 and 126 at 32; backward
+// with its column sums 186 us at 8, 200 at 16, 229 at 32: more blocks, more partial sums to write and add.
+constexpr int FWD_WAVES = 16, BWD_WAVES = 8;
+
 struct NormPlan { int V, NV, TPR, grid; }; // TPR 0: streaming kernels
 
 int check_norm(const rexsc_norm_desc *d)
@@ -342,17 +357,18 @@ int check_norm(const rexsc_norm_desc *d)
 }
 
 // Vectors of 16 bytes where every row starts on one, else single elements; the fewest threads that hold a row at 16
-// elements each.  `per_cu`: blocks' worth of 64-lane waves to put on each of the 256 CUs.
-NormPlan norm_plan(const rexsc_norm_desc *d, bool aligned, int waves_per_cu)
+// elements each.  The backward pass holds a row of more than 8192 in 512 threads at 32 elements: with its five values
+// per element, 1024 threads have too few registers (8192 x 16384 bfloat16: 640 us with them spilled, against 178).
+NormPlan norm_plan(const rexsc_norm_desc *d, bool aligned, bool backward)
 {
     NormPlan pl{};
     const int VMAX = d->dtype == REXSC_F32 ? 4 : 8;
     pl.V = aligned && d->cols % VMAX == 0 && (d->x_stride % VMAX == 0 || d->rows <= 1) ? VMAX : 1;
-    pl.TPR = d->cols <= 64 * MAX_EPT ? 64 : d->cols <= 256 * MAX_EPT ? 256 : d->cols <= 512 * MAX_EPT ? 512
+    pl.TPR = d->cols <= 16 * MAX_EPT ? 16 : d->cols <= 64 * MAX_EPT ? 64 : d->cols <= 256 * MAX_EPT ? 256 : d->cols <= 512 * MAX_EPT ? 512
            : d->cols <= 1024 * MAX_EPT ? 1024 : 0;
-    const int64_t rpb = pl.TPR == 64 ? 4 : 1;
-    const int threads = pl.TPR == 0 ? STREAM_THREADS : pl.TPR == 64 ? 256 : pl.TPR;
-    const int64_t most = 256 * (int64_t)waves_per_cu * 64 / threads, want = (d->rows + rpb - 1) / rpb;
+    const int64_t rpb = pl.TPR && pl.TPR <= 64 ? 256 / pl.TPR : 1;
+    const int threads = pl.TPR == 0 ? STREAM_THREADS : pl.TPR <= 64 ? 256 : pl.TPR == 1024 && backward ? 512 : pl.TPR;
+    const int64_t most = 256 * (int64_t)(backward ? BWD_WAVES : FWD_WAVES) * 64 / threads, want = (d->rows + rpb - 1) / rpb;
     pl.grid = (int)(want < most ? want : most);
     if (pl.TPR) {
         const int64_t ept = (d->cols + pl.TPR - 1) / pl.TPR;
@@ -365,6 +381,7 @@ template <typename T, int V, int NV>
 void launch_fwd_tpr(const NormPlan &pl, const NormParams &p, hipStream_t s)
 {
     switch (pl.TPR) {
+    case 16: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 16>), dim3(pl.grid), dim3(256), 0, s, p); break;
     case 64: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 64>), dim3(pl.grid), dim3(256), 0, s, p); break;
     case 256: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 256>), dim3(pl.grid), dim3(256), 0, s, p); break;
     case 512: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 512>), dim3(pl.grid), dim3(512), 0, s, p); break;
@@ -375,10 +392,11 @@ template <typename T, int V, int NV>
 void launch_bwd_tpr(const NormPlan &pl, const NormParams &p, hipStream_t s)
 {
     switch (pl.TPR) {
+    case 16: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 16>), dim3(pl.grid), dim3(256), 0, s, p); break;
     case 64: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 64>), dim3(pl.grid), dim3(256), 0, s, p); break;
     case 256: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 256>), dim3(pl.grid), dim3(256), 0, s, p); break;
     case 512: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 512>), dim3(pl.grid), dim3(512), 0, s, p); break;
-    default: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 1024>), dim3(pl.grid), dim3(1024), 0, s, p); break;
+    default: hipLaunchKernelGGL((norm_backward_kernel<T, V, 2 * NV, 512>), dim3(pl.grid), dim3(512), 0, s, p); break;
     }
 }
 #define NORM_NV(FN)                                                                         \
@@ -396,11 +414,9 @@ void launch_bwd_tpr(const NormPlan &pl, const NormParams &p, hipStream_t s)
 template <typename T> void launch_fwd(const NormPlan &pl, const NormParams &p, hipStream_t s) { NORM_NV(launch_fwd_tpr); }
 template <typename T> void launch_bwd(const NormPlan &pl, const NormParams &p, hipStream_t s) { NORM_NV(launch_bwd_tpr); }
 
-constexpr int FWD_WAVES = 16, BWD_WAVES = 8; // waves per CU of the persistent grids
-
 int bwd_blocks(const rexsc_norm_desc *d)
 {
-    if (d->cols <= 1024 * MAX_EPT) return norm_plan(d, false, BWD_WAVES).grid;
+    if (d->cols <= 1024 * MAX_EPT) return norm_plan(d, false, true).grid;
     const int64_t shares = d->rows < 64 ? d->rows : 64;
     return (int)shares;
 }
@@ -412,11 +428,12 @@ bool aligned16(const void *a, const void *b, const void *c)
 
 } // namespace
 
-int launch_column_sums(const float *part, size_t rows, size_t cols, size_t ld, void *out, int out_dtype, hipStream_t stream)
+int launch_column_sums(const float *part, size_t rows, size_t cols, size_t ld, void *out, void *out2, int out_dtype,
+                       hipStream_t stream)
 {
-    ProfScope prof("column_sums", 4.0 * rows * cols, stream);
-    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, stream, part, rows, cols, ld,
-                       out, out_dtype);
+    ProfScope prof("column_sums", 4.0 * rows * cols * (out && out2 ? 2 : 1), stream);
+    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + CS_COLS - 1) / CS_COLS), out2 ? 2 : 1), dim3(CS_COLS * CS_GROUPS), 0,
+                       stream, part, rows, cols, ld, out, out2, out_dtype);
     REXSC_CHECK_HIP(hipGetLastError());
     return REXSC_OK;
 }
@@ -435,7 +452,7 @@ extern "C" int rexsc_layer_norm_forward(const rexsc_norm_desc *d, const void *x,
     REXSC_CHECK_ARG((mean == nullptr) == (rstd == nullptr), "layer norm: mean and rstd are given together or not at all");
     const size_t es = dtype_size(d->dtype);
     REXSC_CHECK_ARG((((uintptr_t)x | (uintptr_t)y) % es) == 0, "layer norm: a tensor is not aligned to its element");
-    const NormPlan pl = norm_plan(d, aligned16(x, y, nullptr), FWD_WAVES);
+    const NormPlan pl = norm_plan(d, aligned16(x, y, nullptr), false);
     const NormParams p{x, weight, bias, nullptr, y, nullptr, mean, rstd, nullptr, (size_t)d->rows, (size_t)d->x_stride,
                        (int)d->cols, d->weight_dtype, d->eps};
     ProfScope prof("layer_norm_forward", 2.0 * es * d->rows * d->cols, stream);
@@ -463,11 +480,8 @@ extern "C" int rexsc_layer_norm_backward(const rexsc_norm_desc *d, const void *g
     const size_t es = dtype_size(d->dtype), cols = (size_t)d->cols;
     const bool sums = dw || db;
     if (!dx && !sums) return REXSC_OK;
-    if (d->rows == 0) { // sums over no rows
-        if (dw) if (int rc = launch_column_sums(nullptr, 0, cols, cols, dw, d->weight_dtype, stream)) return rc;
-        if (db) if (int rc = launch_column_sums(nullptr, 0, cols, cols, db, d->weight_dtype, stream)) return rc;
-        return REXSC_OK;
-    }
+    if (d->rows == 0) // sums over no rows
+        return sums ? launch_column_sums(nullptr, 0, cols, cols, dw, db, d->weight_dtype, stream) : REXSC_OK;
     REXSC_CHECK_ARG(grad_out && x && mean && rstd, "null pointer");
     REXSC_CHECK_ARG((((uintptr_t)x | (uintptr_t)grad_out | (uintptr_t)dx) % es) == 0,
                     "layer norm: a tensor is not aligned to its element");
@@ -476,7 +490,7 @@ extern "C" int rexsc_layer_norm_backward(const rexsc_norm_desc *d, const void *g
         set_error("layer norm: workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
         return REXSC_ERR_WORKSPACE;
     }
-    const NormPlan pl = norm_plan(d, aligned16(x, grad_out, dx), BWD_WAVES);
+    const NormPlan pl = norm_plan(d, aligned16(x, grad_out, dx), true);
     const NormParams p{x, weight, nullptr, grad_out, nullptr, dx, const_cast<float *>(mean), const_cast<float *>(rstd),
                        sums ? (float *)workspace : nullptr, (size_t)d->rows, (size_t)d->x_stride, (int)d->cols,
                        d->weight_dtype, d->eps};
@@ -496,8 +510,5 @@ extern "C" int rexsc_layer_norm_backward(const rexsc_norm_desc *d, const void *g
         }
         REXSC_CHECK_HIP(hipGetLastError());
     }
-    const float *part = (const float *)workspace;
-    if (dw) if (int rc = launch_column_sums(part, blocks, cols, 2 * cols, dw, d->weight_dtype, stream)) return rc;
-    if (db) if (int rc = launch_column_sums(part + cols, blocks, cols, 2 * cols, db, d->weight_dtype, stream)) return rc;
-    return REXSC_OK;
+    return sums ? launch_column_sums((const float *)workspace, blocks, cols, 2 * cols, dw, db, d->weight_dtype, stream) : REXSC_OK;
 }

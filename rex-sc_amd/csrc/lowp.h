@@ -83,8 +83,10 @@ __device__ __forceinline__ unsigned wave_max(unsigned v)
 __device__ __forceinline__ unsigned mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // Column sums of partial results: out[c] = sum_r part[r][c] for `cols` columns of `rows` float32 rows at distance
-// `ld`, in a fixed order, rounded to out's type.  Launched by the operators that accumulate a weight's or bias's
-// gradient per block first (no atomics: the same inputs give the same bits).
-int launch_column_sums(const float *part, size_t rows, size_t cols, size_t ld, void *out, int out_dtype, hipStream_t stream);
+// `ld`, and out2[c] = sum_r part[r][cols + c] (either may be NULL), in a fixed order, rounded to out_dtype.  Launched by
+// the operators that accumulate a weight's or bias's gradient per block first (no atomics: the same inputs give the
+// same bits).
+int launch_column_sums(const float *part, size_t rows, size_t cols, size_t ld, void *out, void *out2, int out_dtype,
+                       hipStream_t stream);
 
 } // namespace rexsc

@@ -788,6 +788,7 @@ class Layer_Norm_Grad(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, var the biased variance.  x float32, float16
     or bfloat16, the result of the same type (also inside an autocast region); arithmetic in float32."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return Layer_Norm_Grad.apply(x, weight, bias, eps)
     return _ops.layer_norm_forward(x, weight, bias, eps, want_stats=False)[0]
