@@ -7,8 +7,10 @@
 // in its kernel arguments (nothing is copied to the device first, and a captured launch keeps its table), and a
 // workgroup finds the tensor its chunk belongs to by bisection over the chunks' running count.
 //
-// 8-bit states: a wave holds the 256 elements that share a scale, four per lane, so the block's maximum is a reduction
-// over the lanes and the conversion to and from e4m3 is the hardware's, two values an instruction.
+// 8-bit states: a wave holds two blocks of the 256 elements that share a scale, eight elements per lane, so a block's
+// maximum is a reduction over 32 lanes and the conversion to and from e4m3 is the hardware's, two values an instruction.
+// At 10 bytes an element the arithmetic counts as well: quotient and root are the hardware's approximations, good to one
+// step of float32, where correctly rounded ones would be some 20 instructions an element more.
 #include <math.h>
 
 #include "lowp.h"
@@ -19,7 +21,7 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int BLOCK = 256;                  // elements that share a scale
-constexpr int CHUNK = 4096;                 // elements a workgroup takes: four vectors of four per thread
+constexpr int CHUNK = 4096;                 // elements a workgroup takes
 constexpr float E4M3_MAX = 448.f;
 constexpr float E4M3_MIN = 0.001953125f;    // 2^-9, the smallest positive value
 constexpr float TINY = 7.888609052210118e-31f; // 2^-100: a block below it is stored as zeros (1 / scale stays finite)
@@ -62,10 +64,22 @@ __device__ __forceinline__ int find(const Table &t, unsigned c)
     return lo;
 }
 
+// Square root to one step, below the smallest normal number too.
+__device__ __forceinline__ float root(float v)
+{
+    const bool tiny = v < 7.888609052210118e-31f; // 2^-100
+    return __builtin_amdgcn_sqrtf(tiny ? v * 1.8446744073709552e19f : v) * (tiny ? 2.3283064365386963e-10f : 1.f); // 2^64, 2^-32
+}
+
 __device__ __forceinline__ float move(float p, float m, float root_v, const Hyper &h, const Coef &c)
 {
-    const float den = fmaf(root_v, c.inv_root_bc2, h.eps);
-    p = p * h.decay - c.step_size * (m / den);
+    // m / den; the reciprocal of a den above 2^126 would be lost, that of one below 2^-126 infinite
+    float den = fmaf(root_v, c.inv_root_bc2, h.eps);
+    const bool far = den > 1e37f, near = den < 1e-37f;
+    den = far ? den * 9.313225746154785e-10f : near ? den * 1073741824.f : den; // 2^-30, 2^30
+    float q = m * __builtin_amdgcn_rcpf(den);
+    q = far ? q * 9.313225746154785e-10f : near ? q * 1073741824.f : q;
+    p = fmaf(p, h.decay, -c.step_size * q);
     // a NaN stays one: both comparisons are false
     p = p < h.lo ? h.lo : p;
     return p > h.hi ? h.hi : p;
@@ -84,7 +98,7 @@ __device__ __forceinline__ void step32(T *p, const T *g, float *m, float *v, con
         const float gj = gf[j] * c.inv_grad_scale;
         mf[j] = fmaf(h.beta1, mf[j], h.one_minus_beta1 * gj);
         vf[j] = fmaf(h.beta2, vf[j], h.one_minus_beta2 * gj * gj);
-        pf[j] = move(pf[j], mf[j], sqrtf(vf[j]), h, c);
+        pf[j] = move(pf[j], mf[j], root(vf[j]), h, c);
     }
     store_vec<V>(p, pf);
     store_vec<V>(m, mf);
@@ -113,16 +127,27 @@ __global__ __launch_bounds__(THREADS) void adamw32_kernel(Table32 t, Hyper h)
     }
 }
 
-// Four values to e4m3 and back.
-__device__ __forceinline__ unsigned to_e4m3(const float (&v)[4])
+// Values to e4m3 and back, four to a word.
+template <int V>
+__device__ __forceinline__ void to_e4m3(unsigned (&q)[V / 4], const float (&v)[V])
 {
-    int q = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], q, true);
+#pragma unroll
+    for (int i = 0; i < V / 4; i++) {
+        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], 0, false);
+        q[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], lo, true);
+    }
 }
-__device__ __forceinline__ void from_e4m3(float (&v)[4], unsigned q)
+template <int V>
+__device__ __forceinline__ void from_e4m3(float (&v)[V], const unsigned (&q)[V / 4])
 {
-    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);
-    v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1];
+#pragma unroll
+    for (int i = 0; i < V / 4; i++) {
+        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[i], true);
+        v[4 * i] = a[0];
+        v[4 * i + 1] = a[1];
+        v[4 * i + 2] = b[0];
+        v[4 * i + 3] = b[1];
+    }
 }
 
 // Scale of a block whose largest magnitude has these bits, and what its elements are multiplied by.  A block with a
@@ -135,9 +160,54 @@ __device__ __forceinline__ void block_scale(unsigned top_bits, float &scale, flo
     else { scale = top / E4M3_MAX; inv = E4M3_MAX / top; }
 }
 
+constexpr int EPL = 8, LANES = BLOCK / EPL; // elements of a lane, lanes of a block
+
+__device__ __forceinline__ unsigned block_max(unsigned v)
+{
+#pragma unroll
+    for (int s = LANES / 2; s; s >>= 1) {
+        const unsigned o = (unsigned)__shfl_xor((int)v, s, 64);
+        v = v > o ? v : o;
+    }
+    return v;
+}
+
+struct State8 { float p[EPL], g[EPL]; unsigned m[EPL / 4], v[EPL / 4]; float ms, vs; };
+
+// The step of the eight elements of a lane, whose block its 32 lanes hold; afterwards x is what is to be stored.
+__device__ __forceinline__ void step8(State8 &x, const Hyper &h, const Coef &c)
+{
+    float m[EPL], r[EPL];
+    from_e4m3<EPL>(m, x.m);
+    from_e4m3<EPL>(r, x.v);
+    unsigned mt = 0, vt = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; j++) {
+        const float g = x.g[j] * c.inv_grad_scale, u = r[j] * x.vs;
+        m[j] = fmaf(h.beta1, m[j] * x.ms, h.one_minus_beta1 * g);
+        r[j] = root(fmaf(h.beta2, u * u, h.one_minus_beta2 * g * g));
+        x.p[j] = move(x.p[j], m[j], r[j], h, c);
+        mt = max(mt, mag_bits(m[j]));
+        vt = max(vt, mag_bits(r[j]));
+    }
+    float mi, vi;
+    block_scale(block_max(mt), x.ms, mi);
+    block_scale(block_max(vt), x.vs, vi);
+#pragma unroll
+    for (int j = 0; j < EPL; j++) {
+        // 448 / top * top may end one rounding above 448; of a lost block every element is 0 (times scale NaN)
+        m[j] = mi == 0.f ? 0.f : fminf(fmaxf(m[j] * mi, -E4M3_MAX), E4M3_MAX);
+        r[j] = vi == 0.f || r[j] == 0.f ? 0.f : fminf(fmaxf(r[j] * vi, E4M3_MIN), E4M3_MAX);
+    }
+    to_e4m3<EPL>(x.m, m);
+    to_e4m3<EPL>(x.v, r);
+}
+
 template <typename T>
 __global__ __launch_bounds__(THREADS) void adamw8_kernel(Table8 t, Hyper h)
 {
+    constexpr int ROUNDS = CHUNK / (THREADS * EPL);
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
     const Coef c = h.coef_dev ? *h.coef_dev : h.coef;
     if (c.skip != 0.f) return;
     const int k = find(t, blockIdx.x);
@@ -145,72 +215,63 @@ __global__ __launch_bounds__(THREADS) void adamw8_kernel(Table8 t, Hyper h)
     T *p = (T *)t.p[k];
     const T *g = (const T *)t.g[k];
     uint8_t *m = t.m[k], *v = t.v[k];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const bool aligned = (((uintptr_t)p | (uintptr_t)g) % (4 * sizeof(T)) | ((uintptr_t)m | (uintptr_t)v) % 4) == 0;
+    float *ms = t.ms[k], *vs = t.vs[k];
+    const bool aligned = (((uintptr_t)p | (uintptr_t)g) % 16 | ((uintptr_t)m | (uintptr_t)v) % 8) == 0;
+    State8 x[ROUNDS];
+    if (aligned && at + CHUNK <= n) { // the whole chunk is loaded before the first element is stepped
 #pragma unroll
-    for (int i = 0; i < CHUNK / BLOCK / (THREADS / 64); i++) {
-        const unsigned b0 = at + (unsigned)(i * (THREADS / 64) + wave) * BLOCK;
-        if (b0 >= n) continue; // wave-uniform
-        const unsigned e = b0 + lane * 4, block = b0 / BLOCK;
-        float pf[4], gf[4], mf[4], vf[4];
-        const bool whole = aligned && b0 + BLOCK <= n;
-        if (whole) {
-            load_vec<4>(pf, p + e);
-            load_vec<4>(gf, g + e);
-            from_e4m3(mf, *(const unsigned *)(m + e));
-            from_e4m3(vf, *(const unsigned *)(v + e));
-        } else {
-            unsigned mq = 0, vq = 0;
+        for (int i = 0; i < ROUNDS; i++) {
+            const unsigned e = at + (i * THREADS + threadIdx.x) * EPL;
+            load_vec<EPL>(x[i].p, p + e);
+            load_vec<EPL>(x[i].g, g + e);
+            const u32x2 a = *(const u32x2 *)(m + e), b = *(const u32x2 *)(v + e);
+            x[i].m[0] = a[0];
+            x[i].m[1] = a[1];
+            x[i].v[0] = b[0];
+            x[i].v[1] = b[1];
+            x[i].ms = ms[e / BLOCK];
+            x[i].vs = vs[e / BLOCK];
+        }
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool in = e + j < n;
-                pf[j] = in ? (float)p[e + j] : 0.f;
-                gf[j] = in ? (float)g[e + j] : 0.f;
-                mq |= in ? (unsigned)m[e + j] << (8 * j) : 0u;
-                vq |= in ? (unsigned)v[e + j] << (8 * j) : 0u;
+        for (int i = 0; i < ROUNDS; i++) {
+            const unsigned e = at + (i * THREADS + threadIdx.x) * EPL;
+            step8(x[i], h, c);
+            store_vec<EPL>(p + e, x[i].p);
+            *(u32x2 *)(m + e) = u32x2{x[i].m[0], x[i].m[1]};
+            *(u32x2 *)(v + e) = u32x2{x[i].v[0], x[i].v[1]};
+            if (threadIdx.x % LANES == 0) {
+                ms[e / BLOCK] = x[i].ms;
+                vs[e / BLOCK] = x[i].vs;
             }
-            from_e4m3(mf, mq);
-            from_e4m3(vf, vq);
         }
-        const float ms = t.ms[k][block], vs = t.vs[k][block];
-        float root[4];
-        unsigned mt = 0, vt = 0;
+        return;
+    }
+    for (int i = 0; i < ROUNDS; i++) {
+        const unsigned e = at + (i * THREADS + threadIdx.x) * EPL, block = e / BLOCK;
+        if (block * BLOCK >= n) continue; // all 32 lanes of a block
+        State8 &y = x[0];
+        y.m[0] = y.m[1] = y.v[0] = y.v[1] = 0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float gj = gf[j] * c.inv_grad_scale, u = vf[j] * vs;
-            mf[j] = fmaf(h.beta1, mf[j] * ms, h.one_minus_beta1 * gj);
-            root[j] = sqrtf(fmaf(h.beta2, u * u, h.one_minus_beta2 * gj * gj));
-            pf[j] = move(pf[j], mf[j], root[j], h, c);
-            mt = max(mt, mag_bits(mf[j]));
-            vt = max(vt, mag_bits(root[j]));
+        for (int j = 0; j < EPL; j++) { // elements behind the tensor are zeros, which change nothing in the block
+            const bool in = e + j < n;
+            y.p[j] = in ? (float)p[e + j] : 0.f;
+            y.g[j] = in ? (float)g[e + j] : 0.f;
+            y.m[j / 4] |= in ? (unsigned)m[e + j] << (8 * (j % 4)) : 0u;
+            y.v[j / 4] |= in ? (unsigned)v[e + j] << (8 * (j % 4)) : 0u;
         }
-        float ms_new, mi, vs_new, vi;
-        block_scale(wave_max(mt), ms_new, mi);
-        block_scale(wave_max(vt), vs_new, vi);
-        float mq[4], vq[4];
+        y.ms = ms[block];
+        y.vs = vs[block];
+        step8(y, h, c);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            // 448 / top * top may end one rounding above 448; of a lost block every element is 0 (times scale NaN)
-            mq[j] = mi == 0.f ? 0.f : fminf(fmaxf(mf[j] * mi, -E4M3_MAX), E4M3_MAX);
-            vq[j] = vi == 0.f || root[j] == 0.f ? 0.f : fminf(fmaxf(root[j] * vi, E4M3_MIN), E4M3_MAX);
-        }
-        const unsigned mw = to_e4m3(mq), vw = to_e4m3(vq);
-        if (whole) {
-            store_vec<4>(p + e, pf);
-            *(unsigned *)(m + e) = mw;
-            *(unsigned *)(v + e) = vw;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (e + j < n) {
-                    p[e + j] = (T)pf[j];
-                    m[e + j] = (uint8_t)(mw >> (8 * j));
-                    v[e + j] = (uint8_t)(vw >> (8 * j));
-                }
-        }
-        if (lane == 0) {
-            t.ms[k][block] = ms_new;
-            t.vs[k][block] = vs_new;
+        for (int j = 0; j < EPL; j++)
+            if (e + j < n) {
+                p[e + j] = (T)y.p[j];
+                m[e + j] = (uint8_t)(y.m[j / 4] >> (8 * (j % 4)));
+                v[e + j] = (uint8_t)(y.v[j / 4] >> (8 * (j % 4)));
+            }
+        if (threadIdx.x % LANES == 0) {
+            ms[block] = y.ms;
+            vs[block] = y.vs;
         }
     }
 }
