@@ -172,27 +172,42 @@ __device__ __forceinline__ void split(float v, unsigned top, int e, f16_t &high,
     low = (f16_t)(t - (float)high);
 }
 
+// V elements of a row of g times their channels' scales.
+template <int V, typename T>
+__device__ __forceinline__ void load_scaled(float (&v)[V], const T *g, const float *scale)
+{
+    load_vec<V>(v, g);
+#pragma unroll
+    for (int i = 0; i < V; i += V < 4 ? V : 4) {
+        float s[V < 4 ? V : 4];
+        load_vec<(V < 4 ? V : 4)>(s, scale + i);
+#pragma unroll
+        for (int j = 0; j < (V < 4 ? V : 4); j++) v[i + j] *= s[j];
+    }
+}
+
 template <typename T, int V>
 __device__ void split_row(const OperandArgs &p, size_t row, unsigned (&lds)[16])
 {
     const T *g = (const T *)p.g + row * (size_t)p.N;
     unsigned t = 0;
+#pragma unroll 2
     for (int c = threadIdx.x * V; c < p.N; c += 256 * V) {
         float v[V];
-        load_vec<V>(v, g + c);
+        load_scaled<V>(v, g + c, p.b_scale + c);
 #pragma unroll
-        for (int j = 0; j < V; j++) t = max(t, mag_bits(v[j] * p.b_scale[c + j]));
+        for (int j = 0; j < V; j++) t = max(t, mag_bits(v[j]));
     }
     t = row_top<256>(t, lds);
     const int e = piece_exponent(t);
     f16_t *high = p.g_rows + row * (size_t)p.ldn, *low = high + (size_t)p.M * p.ldn;
     for (int c = threadIdx.x * V; c < p.ldn; c += 256 * V) { // ldn is a multiple of 64: whole vectors
         float v[V] = {};
-        if (c < p.N) load_vec<V>(v, g + c);
+        if (c < p.N) load_scaled<V>(v, g + c, p.b_scale + c);
         typename VecOf<f16_t, V>::type h, l;
         f16_t *hp = (f16_t *)&h, *lp = (f16_t *)&l;
 #pragma unroll
-        for (int j = 0; j < V; j++) split(c < p.N ? v[j] * p.b_scale[c + j] : 0.f, t, e, hp[j], lp[j]);
+        for (int j = 0; j < V; j++) split(v[j], t, e, hp[j], lp[j]);
         *(typename VecOf<f16_t, V>::type *)(high + c) = h;
         if (p.pieces_x > 1) *(typename VecOf<f16_t, V>::type *)(low + c) = l;
     }
@@ -227,32 +242,44 @@ __device__ void transpose_tile(const int8_t *q, size_t stride, int rows, int col
     }
 }
 
-// Sum of g and largest |g * a_scale| of 64 columns over one share of the rows.
-template <typename T>
-__device__ void column_stats(const OperandArgs &p, unsigned block, float (&ls)[4][64], unsigned (&lt)[4][64])
+// Sum of g and largest |g * a_scale| of 64 columns over one share of the rows: 64 / V threads across, the rest down.
+template <typename T, int V>
+__device__ void column_stats(const OperandArgs &p, unsigned block, float (&ls)[32][64], unsigned (&lt)[32][64])
 {
-    const int share = (int)(block % p.shares), c = (int)(block / p.shares) * 64 + threadIdx.x % 64, part = threadIdx.x / 64;
-    const int begin = share * p.share_rows, end = min(p.M, begin + p.share_rows);
-    float s = 0.f;
-    unsigned t = 0;
-    if (c < p.N)
-#pragma unroll 8
-        for (int m = begin + part; m < end; m += 4) {
-            const float g = (float)((const T *)p.g)[(size_t)m * p.N + c];
-            s += g;
-            if (p.a_scale) t = max(t, mag_bits(g * p.a_scale[m]));
-        }
-    ls[part][threadIdx.x % 64] = s;
-    lt[part][threadIdx.x % 64] = t;
-    __syncthreads();
-    if (part == 0 && c < p.N) {
+    constexpr int ACROSS = 64 / V, DOWN = 256 / ACROSS; // 4 to 32 rows at once
+    const int share = (int)(block % p.shares), x = threadIdx.x % ACROSS * V, c = (int)(block / p.shares) * 64 + x;
+    const int y = threadIdx.x / ACROSS, begin = share * p.share_rows, end = min(p.M, begin + p.share_rows);
+    float s[V] = {};
+    unsigned t[V] = {};
+    if (c < p.N) // with V > 1, N is a multiple of V
+#pragma unroll 4
+        for (int m = begin + y; m < end; m += DOWN) {
+            float g[V];
+            load_vec<V>(g, (const T *)p.g + (size_t)m * p.N + c);
+            const float scale = p.a_scale ? p.a_scale[m] : 0.f;
 #pragma unroll
-        for (int i = 1; i < 4; i++) {
-            s += ls[i][threadIdx.x];
-            t = max(t, lt[i][threadIdx.x]);
+            for (int j = 0; j < V; j++) {
+                s[j] += g[j];
+                t[j] = max(t[j], mag_bits(g[j] * scale));
+            }
         }
-        p.sums[(size_t)share * p.N + c] = s;
-        p.tops[(size_t)share * p.N + c] = t;
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        ls[y][x + j] = s[j];
+        lt[y][x + j] = t[j];
+    }
+    __syncthreads();
+    const int n = (int)(block / p.shares) * 64 + threadIdx.x;
+    if (threadIdx.x < 64 && n < p.N) {
+        float sum = 0.f;
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < DOWN; i++) {
+            sum += ls[i][threadIdx.x];
+            top = max(top, lt[i][threadIdx.x]);
+        }
+        p.sums[(size_t)share * p.N + n] = sum;
+        p.tops[(size_t)share * p.N + n] = top;
     }
 }
 
@@ -264,7 +291,7 @@ __global__ __launch_bounds__(256) void operands_kernel(OperandArgs p)
     __shared__ union {
         unsigned top[16];
         int8_t tile[64][68];
-        struct { float s[4][64]; unsigned t[4][64]; } stats;
+        struct { float s[32][64]; unsigned t[32][64]; } stats;
     } lds;
     unsigned b = blockIdx.x;
     if (b < p.row_blocks) return split_row<T, V>(p, b, lds.top);
@@ -273,41 +300,51 @@ __global__ __launch_bounds__(256) void operands_kernel(OperandArgs p)
     b -= p.b_blocks;
     if (b < p.a_blocks) return transpose_tile(p.a, p.a_stride, p.M, p.K, p.ldm, p.a_t, b, lds.tile);
     b -= p.a_blocks;
-    column_stats<T>(p, b, lds.stats.s, lds.stats.t);
+    column_stats<T, V>(p, b, lds.stats.s, lds.stats.t);
 }
 
 // The second launch: pieces of (g * a_scale) transposed, a 64 x 64 tile per block, and db from the shares' sums.
-template <typename T>
+template <typename T, int V>
 __global__ __launch_bounds__(256) void transposed_pieces_kernel(OperandArgs p)
 {
+    constexpr int ACROSS = 64 / V, DOWN = 256 / ACROSS;
     __shared__ float tile[64][65];
-    __shared__ unsigned top[64];
+    __shared__ unsigned tops[4][64];
+    __shared__ float sums[4][64];
     const int across = p.ldm / 64, m0 = (int)(blockIdx.x % across) * 64, n0 = (int)(blockIdx.x / across) * 64;
-    const int tx = threadIdx.x % 64, ty = threadIdx.x / 64;
-    const int n = n0 + tx;
-#pragma unroll 4
-    for (int i = ty; i < 64; i += 4) {
-        const int m = m0 + i;
-        tile[i][tx] = m < p.M && n < p.N ? (float)((const T *)p.g)[(size_t)m * p.N + n] * p.a_scale[m] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 64; i += DOWN) {
+        const int r = i + threadIdx.x / ACROSS, m = m0 + r, c = threadIdx.x % ACROSS * V;
+        float v[V] = {};
+        if (m < p.M && n0 + c < p.N) load_vec<V>(v, (const T *)p.g + (size_t)m * p.N + n0 + c);
+        const float scale = m < p.M ? p.a_scale[m] : 0.f;
+#pragma unroll
+        for (int j = 0; j < V; j++) tile[r][c + j] = v[j] * scale;
     }
-    if (ty == 0) {
+    {
+        const int x = threadIdx.x % 64, y = threadIdx.x / 64, n = n0 + x;
         unsigned t = 0;
         float s = 0.f;
         if (n < p.N)
-            for (int i = 0; i < p.shares; i++) {
+#pragma unroll 4
+            for (int i = y; i < p.shares; i += 4) {
                 t = max(t, p.tops[(size_t)i * p.N + n]);
                 s += p.sums[(size_t)i * p.N + n];
             }
-        top[tx] = t;
-        if (m0 == 0 && n < p.N) {
-            p.g_cols_scale[n] = piece_scale(t, piece_exponent(t));
-            if (p.db) store_any(p.db, p.db_dtype, n, s);
-        }
+        tops[y][x] = t;
+        sums[y][x] = s;
     }
     __syncthreads();
+    auto top_of = [&](int x) { return max(max(tops[0][x], tops[1][x]), max(tops[2][x], tops[3][x])); };
+    if (m0 == 0 && threadIdx.x < 64 && n0 + threadIdx.x < p.N) {
+        const int x = threadIdx.x;
+        const unsigned t = top_of(x);
+        p.g_cols_scale[n0 + x] = piece_scale(t, piece_exponent(t));
+        if (p.db) store_any(p.db, p.db_dtype, n0 + x, ((sums[0][x] + sums[1][x]) + sums[2][x]) + sums[3][x]);
+    }
     const int on = threadIdx.x / 4, om = threadIdx.x % 4 * 16;
     if (n0 + on >= p.N) return;
-    const unsigned t = top[on];
+    const unsigned t = top_of(on);
     const int e = piece_exponent(t);
     f16_t *high = p.g_cols + (size_t)(n0 + on) * p.ldm + m0 + om, *low = high + (size_t)p.N * p.ldm;
 #pragma unroll
@@ -353,7 +390,7 @@ inline int pieces_of(int dtype) { return dtype == REXSC_BF16 ? 1 : 2; }
 
 struct Space { size_t tokens, scales, g_rows, g_rows_scale, b_t, g_cols, g_cols_scale, a_t, sums, tops, product, total; };
 
-constexpr int MAX_SHARES = 32, SHARE_ROWS = 256; // runs of g's rows whose column statistics are taken apart
+constexpr int MAX_SHARES = 32, SHARE_ROWS = 512; // runs of g's rows whose column statistics are taken apart
 int share_rows(int M) { return max(SHARE_ROWS, (M + MAX_SHARES - 1) / MAX_SHARES); }
 int shares(int M) { return (M + share_rows(M) - 1) / share_rows(M); }
 
@@ -535,13 +572,14 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
     p.b_blocks = dx ? (unsigned)(tiles_n * tiles_k) : 0;
     p.a_blocks = dw ? (unsigned)(tiles_m * tiles_k) : 0;
     p.stat_blocks = dw || db ? (unsigned)(p.shares * tiles_n) : 0;
+    // vectors of 16 bytes where every row of g starts on one (and the channels' scales)
+    const bool wide = d->N % (d->dtype == REXSC_F32 ? 4 : 8) == 0 && ((uintptr_t)g | (uintptr_t)b_scale) % 16 == 0;
     {
         const double es = (double)dtype_size(d->dtype), mn = (double)d->M * d->N, k = (double)d->K;
         ProfScope prof("int8_backward_operands", (dx ? mn * (es + 2.0 * p.pieces_x) + 3.0 * k * d->N : 0.0) + (dw || db ? mn * es : 0.0) +
                        (dw ? 3.0 * k * d->M : 0.0), stream);
         const dim3 grid(p.row_blocks + p.b_blocks + p.a_blocks + p.stat_blocks);
-        const int V = d->dtype == REXSC_F32 ? 4 : 8;
-        if (d->N % V == 0 && (uintptr_t)g % 16 == 0)
+        if (wide)
             REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((operands_kernel<T, 16 / sizeof(T)>), grid, dim3(256), 0, stream, p));
         else
             REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((operands_kernel<T, 1>), grid, dim3(256), 0, stream, p));
@@ -549,8 +587,11 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
     }
     if (dw) {
         ProfScope prof("int8_backward_pieces", (double)d->M * d->N * (dtype_size(d->dtype) + 2.0 * p.pieces_w), stream);
-        REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL(transposed_pieces_kernel<T>, dim3((unsigned)(tiles_m * tiles_n)), dim3(256), 0,
-                                                        stream, p));
+        const dim3 grid((unsigned)(tiles_m * tiles_n));
+        if (wide)
+            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((transposed_pieces_kernel<T, 16 / sizeof(T)>), grid, dim3(256), 0, stream, p));
+        else
+            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((transposed_pieces_kernel<T, 1>), grid, dim3(256), 0, stream, p));
         REXSC_CHECK_HIP(hipGetLastError());
     } else if (db) {
         if (int rc = launch_column_sums(p.sums, p.shares, d->N, d->N, db, nullptr, d->bias_dtype, stream)) return rc;
