@@ -163,8 +163,7 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(FewArgs g)
         float sa;
         if constexpr (FUSED) sa = row_scale(top[m]).scale;
         else sa = p.a_scale[m];
-        float y = (float)s * sa * p.b_scale[n];
-        if (p.bias) y += load_any(p.bias, p.bias_dtype, n);
+        const float y = fmaf((float)s * sa, p.b_scale[n], p.bias ? load_any(p.bias, p.bias_dtype, n) : 0.f);
         ((T *)p.y)[(size_t)m * p.N + n] = (T)y;
     }
 }

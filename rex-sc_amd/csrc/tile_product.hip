@@ -230,7 +230,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     if constexpr (SPLIT) v[e] = acc[r0 / 16 + i][j][e];
-                    else v[e] = (T)((float)acc[r0 / 16 + i][j][e] * sa * sb[j][e] + bias[j][e]);
+                    else v[e] = (T)fmaf((float)acc[r0 / 16 + i][j][e] * sa, sb[j][e], bias[j][e]);
                 }
                 *(__attribute__((address_space(3))) typename VecOf<T, 4>::type *)(mine + (i * 16 + lane % 16) * PITCH +
                                                                                   (j * 16 + lane / 16 * 4) * (int)sizeof(T)) = v;
@@ -274,11 +274,9 @@ __global__ __launch_bounds__(256) void join_kernel(TileArgs p, const ACC *part, 
             for (int e = 0; e < n; e++) s[e] += part[z * all + at + e];
     unsigned m = (unsigned)(at / p.N), c = (unsigned)(at - (size_t)m * p.N);
     for (int e = 0; e < n; e++) {
-        float v = (float)s[e];
-        if (p.a_scale) v *= p.a_scale[m];
-        if (p.b_scale) v *= p.b_scale[c];
-        if (p.bias) v += load_any(p.bias, p.bias_dtype, c);
-        ((T *)p.y)[at + e] = (T)v;
+        const float v = p.a_scale ? (float)s[e] * p.a_scale[m] : (float)s[e];
+        const float sb = p.b_scale ? p.b_scale[c] : 1.f, bias = p.bias ? load_any(p.bias, p.bias_dtype, c) : 0.f;
+        ((T *)p.y)[at + e] = (T)fmaf(v, sb, bias); // as the unsplit kernel rounds it
         if (++c == (unsigned)p.N) { c = 0; m++; }
     }
 }
