@@ -917,65 +917,74 @@ def _norm_vectors(x, weight, bias, dtype=None):
 
 
 def layer_norm_forward(x, weight, bias, eps, want_stats=True):
-    """(y, mean, rstd) of a layer norm over the last dimension; mean and rstd float32 per row (None unless wanted)."""
+    """(y, stats, desc, x as rows, weight as read): y the layer norm over the last dimension, stats float32 [2, rows] with
+    mean and 1 / standard deviation (None unless wanted); the rest is what the backward pass takes."""
     if not x.is_cuda:
         _require_cuda(x)
-    _same_device("layer_norm", x, weight, bias)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise RuntimeError("layer_norm: expected rows of at least one element (got shape %s)" % (tuple(x.shape),))
+    device, dev = x.device, x.get_device()
+    if (weight is not None and weight.get_device() != dev) or (bias is not None and bias.get_device() != dev):
+        _same_device("layer_norm", x, weight, bias)
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise RuntimeError("layer_norm: expected rows of at least one element (got shape %s)" % (tuple(shape),))
     code = _dtype_code(x, "layer_norm")
     w, b, wdt = _norm_vectors(x, weight, bias)
     m = _rows_of(x)
     R, D = m.shape
-    device, dev = x.device, x.get_device()
     with _on(dev):
-        y = torch.empty(x.shape, dtype=x.dtype, device=device)
-        mean = rstd = None
+        y = torch.empty(shape, dtype=x.dtype, device=device)
+        stats, mean, rstd = None, None, None
         if want_stats:
             stats = torch.empty((2, R), dtype=torch.float32, device=device)
-            mean, rstd = stats[0], stats[1]
+            mean = stats.data_ptr()
+            rstd = mean + 4 * R
         d = _lib.NormDesc(code, _DTYPE_CODE[wdt], eps, R, D, _row_stride(m))
-        rc = _lib.lib().rexsc_layer_norm_forward(ctypes.byref(d), m.data_ptr(), _addr(w), _addr(b), y.data_ptr(), _addr(mean),
-                                                 _addr(rstd), _raw_stream(dev))
+        rc = _lib.lib().rexsc_layer_norm_forward(ctypes.byref(d), m.data_ptr(), _addr(w), _addr(b), y.data_ptr(), mean, rstd,
+                                                 _raw_stream(dev))
         if rc:
             _lib.check(rc, "rexsc_layer_norm_forward")
-    return y, mean, rstd
+    return y, stats, d, m, w
 
 
-def layer_norm_backward(grad_output, x, weight, mean, rstd, eps, need_x=True, weight_dtype=None, bias_dtype=None):
-    """(dx in x's type, dw of weight_dtype, db of bias_dtype); a type of None: not wanted."""
-    if not (grad_output.is_cuda and x.is_cuda):
-        _require_cuda(grad_output, x)
-    _same_device("layer_norm", x, grad_output, weight)
-    code = _dtype_code(x, "layer_norm")
+def layer_norm_backward(grad_output, m, w, stats, d, need_x=True, weight_dtype=None, bias_dtype=None):
+    """(dx in x's type, dw of weight_dtype, db of bias_dtype) from what layer_norm_forward returned; a type of None: not
+    wanted."""
+    if not grad_output.is_cuda:
+        _require_cuda(grad_output)
+    device, dev = m.device, m.get_device()
+    if grad_output.get_device() != dev:
+        _same_device("layer_norm", m, grad_output)
+    R, D = m.shape
+    shape, dtype = grad_output.shape, m.dtype
+    g = grad_output if grad_output.dtype == dtype else grad_output.to(dtype)
+    g = _dense_rows(g, D)
     # the sums leave the kernel in float32 or in x's type; any other type is rounded once more
     wanted = weight_dtype is not None or bias_dtype is not None
-    low = wanted and weight_dtype in (None, x.dtype) and bias_dtype in (None, x.dtype)
-    sum_dt = x.dtype if low else torch.float32
-    w = _norm_vectors(x, weight, None, sum_dt)[0]
-    m = _rows_of(x)
-    R, D = m.shape
-    g = grad_output if grad_output.dtype == x.dtype else grad_output.to(x.dtype)
-    g = _dense_rows(g, D)
-    device, dev = x.device, x.get_device()
+    sum_dt = torch.float32
+    if wanted and dtype != sum_dt and weight_dtype in (None, dtype) and bias_dtype in (None, dtype):
+        sum_dt = dtype
+    if d.weight_dtype != _DTYPE_CODE[sum_dt]:
+        d = _lib.NormDesc(d.dtype, _DTYPE_CODE[sum_dt], d.eps, R, D, d.x_stride)
+        w = None if w is None else w.to(sum_dt)
     L = _lib.lib()
+    ref = ctypes.byref(d)
     with _on(dev):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
+        dx = torch.empty(shape, dtype=dtype, device=device) if need_x else None
         dw = torch.empty((D,), dtype=sum_dt, device=device) if weight_dtype is not None else None
         db = torch.empty((D,), dtype=sum_dt, device=device) if bias_dtype is not None else None
-        d = ctypes.byref(_lib.NormDesc(code, _DTYPE_CODE[sum_dt], eps, R, D, _row_stride(m)))
         ws, nbytes = None, 0
         if wanted:
-            nbytes = L.rexsc_layer_norm_backward_workspace_bytes(d)
+            nbytes = L.rexsc_layer_norm_backward_workspace_bytes(ref)
             if nbytes == _NO_BYTES:
                 _lib.check(-1, "rexsc_layer_norm_backward (planning)")
             ws = torch.empty((nbytes,), dtype=torch.uint8, device=device)
-        rc = L.rexsc_layer_norm_backward(d, g.data_ptr(), m.data_ptr(), _addr(w), mean.data_ptr(), rstd.data_ptr(), _addr(dx),
-                                         _addr(dw), _addr(db), _addr(ws), nbytes, _raw_stream(dev))
+        mean = stats.data_ptr()
+        rc = L.rexsc_layer_norm_backward(ref, g.data_ptr(), m.data_ptr(), _addr(w), mean, mean + 4 * R, _addr(dx), _addr(dw),
+                                         _addr(db), _addr(ws), nbytes, _raw_stream(dev))
         if rc:
             _lib.check(rc, "rexsc_layer_norm_backward")
-    if dw is not None and dw.dtype != weight_dtype:
+    if dw is not None and sum_dt != weight_dtype:
         dw = dw.to(weight_dtype)
-    if db is not None and db.dtype != bias_dtype:
+    if db is not None and sum_dt != bias_dtype:
         db = db.to(bias_dtype)
     return dx, dw, db

@@ -723,7 +723,6 @@ class Linear_Int8_Grad(torch.autograd.Function):
         else:
             wq, ws = weight, weight_scale
         ctx.types = (weight.dtype if weight_scale is None else None, None if bias is None else bias.dtype)
-        ctx.shape = x.shape
         if ctx.needs_input_grad[1]:  # the tokens are wanted in 8 bits again by the backward pass
             xq, xs = _ops.quantize_rows(x.reshape(-1, x.shape[-1]))
             y = _ops.matmul_int8(xq, xs, wq, ws, bias, x.dtype).view(x.shape[:-1] + (wq.shape[0],))
@@ -734,13 +733,20 @@ class Linear_Int8_Grad(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
-        wq, ws, xq, xs = ctx.saved_tensors
-        w_dtype, b_dtype = ctx.types
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        return _ops.int8_backward(grad_output, xq, xs, wq, ws, need_x, w_dtype if need_w else None,
-                                  b_dtype if need_b else None) + (None,)
+        return _linear_int8_once(ctx, grad_output) if torch.is_grad_enabled() else _linear_int8_backward(ctx, grad_output)
+
+
+def _linear_int8_backward(ctx, grad_output):
+    wq, ws, xq, xs = ctx.saved_tensors
+    w_dtype, b_dtype = ctx.types
+    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    dx, dw, db = _ops.int8_backward(grad_output, xq, xs, wq, ws, need_x, w_dtype if need_w else None,
+                                    b_dtype if need_b else None)
+    return dx, dw, db, None
+
+
+_linear_int8_once = torch.autograd.function.once_differentiable(_linear_int8_backward)
 
 
 def linear_int8(x, weight, bias=None, weight_scale=None):
@@ -770,19 +776,27 @@ class Layer_Norm_Grad(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _ops.layer_norm_forward(x, weight, bias, eps)
-        ctx.eps = eps
-        ctx.types = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, stats, desc, rows, w = _ops.layer_norm_forward(x, weight, bias, eps)
+        ctx.rest = (desc, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        ctx.save_for_backward(rows, w, stats)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
-        x, weight, mean, rstd = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        return _ops.layer_norm_backward(grad_output, x, weight, mean, rstd, ctx.eps, need_x,
-                                        ctx.types[0] if need_w else None, ctx.types[1] if need_b else None) + (None,)
+        # the wrapper that refuses a second derivative costs as much as the rest on a short row: only where one is asked for
+        return _layer_norm_once(ctx, grad_output) if torch.is_grad_enabled() else _layer_norm_backward(ctx, grad_output)
+
+
+def _layer_norm_backward(ctx, grad_output):
+    rows, w, stats = ctx.saved_tensors
+    desc, w_dtype, b_dtype = ctx.rest
+    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    dx, dw, db = _ops.layer_norm_backward(grad_output, rows, w, stats, desc, need_x, w_dtype if need_w else None,
+                                          b_dtype if need_b else None)
+    return dx, dw, db, None
+
+
+_layer_norm_once = torch.autograd.function.once_differentiable(_layer_norm_backward)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
