@@ -5,6 +5,7 @@ gets a RuntimeError -- there is no Python/CPU fallback.
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "librexsc.so")
@@ -23,6 +24,15 @@ class _Desc(ctypes.Structure):
 
     def key(self):
         return tuple(getattr(self, f[0]) for f in self._fields_)
+
+    @classmethod
+    def packed(cls, *args):
+        """The same descriptor as bytes, for calls where building the structure would be a good part of the call."""
+        if "_packer" not in cls.__dict__:
+            codes = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_double: "d"}
+            cls._packer = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_))
+            assert cls._packer.size == ctypes.sizeof(cls)
+        return cls._packer.pack(cls._packer.size, *args)
 
 
 class ConvDesc(_Desc):
@@ -79,7 +89,7 @@ _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
 _int = ctypes.c_int
 _u64 = ctypes.c_uint64
-_i8d, _nd = ctypes.POINTER(Int8Desc), ctypes.POINTER(NormDesc)
+_i8d = _nd = _ad = ctypes.c_void_p  # a reference to a descriptor, or a packed one
 
 # name -> (restype, argtypes); every symbol include/rexsc.h declares
 SIGNATURES = {
@@ -125,7 +135,7 @@ SIGNATURES = {
     "rexsc_layer_norm_forward": (_int, [_nd, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "rexsc_layer_norm_backward_workspace_bytes": (_sz, [_nd]),
     "rexsc_layer_norm_backward": (_int, [_nd, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "rexsc_adamw_step": (_int, [ctypes.POINTER(AdamwDesc), _vp, _sz, _vp, _vp, _vp, _vp, _vp]),
+    "rexsc_adamw_step": (_int, [_ad, _vp, _sz, _vp, _vp, _vp, _vp, _vp]),
     "rexsc_profile_begin": (_int, []),
     "rexsc_profile_end": (_int, [ctypes.POINTER(ProfileRecord), _int]),
     "rexsc_valu_probe": (_int, [_int, _int, _vp, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),

@@ -820,7 +820,7 @@ def matmul_int8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
     with _on(dev):
         a, sa = _operand8(a, "matmul_int8")
         b, sb = _operand8(b, "matmul_int8")
-        d = ctypes.byref(_lib.Int8Desc(M, N, K, _dtype_code(out_dtype, "matmul_int8"), bias_code, 0, 0, 0, sa, sb))
+        d = _lib.Int8Desc.packed(M, N, K, _dtype_code(out_dtype, "matmul_int8"), bias_code, 0, 0, 0, sa, sb)
         y = torch.empty((M, N), dtype=out_dtype, device=device)
         ws, nbytes = _int8_space(L, d, _lib.INT8_PRODUCT, device)
         rc = L.rexsc_int8_product(d, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), _addr(bias),
@@ -849,7 +849,7 @@ def int8_linear(x, wq, w_scale, bias=None):
     L = _lib.lib()
     with _on(dev):
         wq, sb = _operand8(wq, "linear_int8")
-        d = ctypes.byref(_lib.Int8Desc(M, N, K, code, bias_code, 0, 0, _row_stride(m), 0, sb))
+        d = _lib.Int8Desc.packed(M, N, K, code, bias_code, 0, 0, _row_stride(m), 0, sb)
         y = torch.empty(shape[:-1] + (N,), dtype=x.dtype, device=device)
         ws, nbytes = _int8_space(L, d, _lib.INT8_LINEAR, device)
         rc = L.rexsc_int8_linear(d, m.data_ptr(), wq.data_ptr(), w_scale.data_ptr(), _addr(bias), y.data_ptr(), _addr(ws),
@@ -889,8 +889,8 @@ def int8_backward(g, xq, x_scale, wq, w_scale, need_x, weight_dtype, bias_dtype)
             dw = torch.empty((N, K), dtype=weight_dtype, device=device)
         if bias_dtype is not None:
             db = torch.empty((N,), dtype=bias_dtype, device=device)
-        d = ctypes.byref(_lib.Int8Desc(M, N, K, code, 0 if db is None else _dtype_code(db, "linear_int8"),
-                                       0 if dw is None else _dtype_code(dw, "linear_int8"), 0, 0, sa, sb))
+        d = _lib.Int8Desc.packed(M, N, K, code, 0 if db is None else _dtype_code(db, "linear_int8"),
+                                 0 if dw is None else _dtype_code(dw, "linear_int8"), 0, 0, sa, sb)
         ws, nbytes = _int8_space(L, d, _lib.INT8_BACKWARD, device)
         rc = L.rexsc_int8_backward(d, gm.data_ptr(), _addr(xq), _addr(x_scale), wq.data_ptr(), w_scale.data_ptr(), _addr(dx),
                                    _addr(dw), _addr(db), _addr(ws), nbytes, _raw_stream(dev))
@@ -917,7 +917,7 @@ def _norm_vectors(x, weight, bias, dtype=None):
 
 
 def layer_norm_forward(x, weight, bias, eps, want_stats=True):
-    """(y, stats, desc, x as rows, weight as read): y the layer norm over the last dimension, stats float32 [2, rows] with
+    """(y, stats, rest, x as rows, weight as read): y the layer norm over the last dimension, stats float32 [2, rows] with
     mean and 1 / standard deviation (None unless wanted); the rest is what the backward pass takes."""
     if not x.is_cuda:
         _require_cuda(x)
@@ -938,15 +938,15 @@ def layer_norm_forward(x, weight, bias, eps, want_stats=True):
             stats = torch.empty((2, R), dtype=torch.float32, device=device)
             mean = stats.data_ptr()
             rstd = mean + 4 * R
-        d = _lib.NormDesc(code, _DTYPE_CODE[wdt], eps, R, D, _row_stride(m))
-        rc = _lib.lib().rexsc_layer_norm_forward(ctypes.byref(d), m.data_ptr(), _addr(w), _addr(b), y.data_ptr(), mean, rstd,
+        d = _lib.NormDesc.packed(code, _DTYPE_CODE[wdt], eps, R, D, _row_stride(m))
+        rc = _lib.lib().rexsc_layer_norm_forward(d, m.data_ptr(), _addr(w), _addr(b), y.data_ptr(), mean, rstd,
                                                  _raw_stream(dev))
         if rc:
             _lib.check(rc, "rexsc_layer_norm_forward")
-    return y, stats, d, m, w
+    return y, stats, (d, wdt, eps), m, w
 
 
-def layer_norm_backward(grad_output, m, w, stats, d, need_x=True, weight_dtype=None, bias_dtype=None):
+def layer_norm_backward(grad_output, m, w, stats, rest, need_x=True, weight_dtype=None, bias_dtype=None):
     """(dx in x's type, dw of weight_dtype, db of bias_dtype) from what layer_norm_forward returned; a type of None: not
     wanted."""
     if not grad_output.is_cuda:
@@ -963,23 +963,23 @@ def layer_norm_backward(grad_output, m, w, stats, d, need_x=True, weight_dtype=N
     sum_dt = torch.float32
     if wanted and dtype != sum_dt and weight_dtype in (None, dtype) and bias_dtype in (None, dtype):
         sum_dt = dtype
-    if d.weight_dtype != _DTYPE_CODE[sum_dt]:
-        d = _lib.NormDesc(d.dtype, _DTYPE_CODE[sum_dt], d.eps, R, D, d.x_stride)
+    d, wdt, eps = rest
+    if wdt != sum_dt:
+        d = _lib.NormDesc.packed(_DTYPE_CODE[dtype], _DTYPE_CODE[sum_dt], eps, R, D, _row_stride(m))
         w = None if w is None else w.to(sum_dt)
     L = _lib.lib()
-    ref = ctypes.byref(d)
     with _on(dev):
         dx = torch.empty(shape, dtype=dtype, device=device) if need_x else None
         dw = torch.empty((D,), dtype=sum_dt, device=device) if weight_dtype is not None else None
         db = torch.empty((D,), dtype=sum_dt, device=device) if bias_dtype is not None else None
         ws, nbytes = None, 0
         if wanted:
-            nbytes = L.rexsc_layer_norm_backward_workspace_bytes(ref)
+            nbytes = L.rexsc_layer_norm_backward_workspace_bytes(d)
             if nbytes == _NO_BYTES:
                 _lib.check(-1, "rexsc_layer_norm_backward (planning)")
             ws = torch.empty((nbytes,), dtype=torch.uint8, device=device)
         mean = stats.data_ptr()
-        rc = L.rexsc_layer_norm_backward(ref, g.data_ptr(), m.data_ptr(), _addr(w), mean, mean + 4 * R, _addr(dx), _addr(dw),
+        rc = L.rexsc_layer_norm_backward(d, g.data_ptr(), m.data_ptr(), _addr(w), mean, mean + 4 * R, _addr(dx), _addr(dw),
                                          _addr(db), _addr(ws), nbytes, _raw_stream(dev))
         if rc:
             _lib.check(rc, "rexsc_layer_norm_backward")

@@ -776,8 +776,8 @@ class Layer_Norm_Grad(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, stats, desc, rows, w = _ops.layer_norm_forward(x, weight, bias, eps)
-        ctx.rest = (desc, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        y, stats, rest, rows, w = _ops.layer_norm_forward(x, weight, bias, eps)
+        ctx.rest = (rest, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
         ctx.save_for_backward(rows, w, stats)
         return y
 
@@ -789,9 +789,9 @@ class Layer_Norm_Grad(torch.autograd.Function):
 
 def _layer_norm_backward(ctx, grad_output):
     rows, w, stats = ctx.saved_tensors
-    desc, w_dtype, b_dtype = ctx.rest
+    rest, w_dtype, b_dtype = ctx.rest
     need_x, need_w, need_b, _ = ctx.needs_input_grad
-    dx, dw, db = _ops.layer_norm_backward(grad_output, rows, w, stats, desc, need_x, w_dtype if need_w else None,
+    dx, dw, db = _ops.layer_norm_backward(grad_output, rows, w, stats, rest, need_x, w_dtype if need_w else None,
                                           b_dtype if need_b else None)
     return dx, dw, db, None
 

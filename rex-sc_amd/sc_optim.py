@@ -100,12 +100,12 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_av
         if t is not None and (not on_device or t.dtype != torch.float32 or t.numel() != 1 or t.device != first.device):
             raise RuntimeError("adamw_step: %s is one float32 beside the parameters, and needs the step in a tensor" % name)
     lo, hi = (0.0, 0.0) if clamp is None else (float(clamp[0]), float(clamp[1]))
-    d = _lib.AdamwDesc(code, 8 if eight else 32, int(clamp is not None), float(lr), float(beta1), float(beta2), float(eps),
+    d = _lib.AdamwDesc.packed(code, 8 if eight else 32, int(clamp is not None), float(lr), float(beta1), float(beta2), float(eps),
                        float(weight_decay), lo, hi, 0 if on_device else int(step))
     arr = (ctypes.c_int64 * len(table))(*table)
     with _ops._on(dev):
         coef = torch.empty((_lib.ADAMW_COEF_BYTES,), dtype=torch.uint8, device=first.device) if on_device else None
-        rc = _lib.lib().rexsc_adamw_step(ctypes.byref(d), ctypes.addressof(arr), len(params),
+        rc = _lib.lib().rexsc_adamw_step(d, ctypes.addressof(arr), len(params),
                                          _ops._addr(step if on_device else None), _ops._addr(grad_scale),
                                          _ops._addr(found_inf), _ops._addr(coef), _ops._raw_stream(dev))
         if rc:
