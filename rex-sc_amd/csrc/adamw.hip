@@ -385,7 +385,7 @@ extern "C" int rexsc_adamw_step(const rexsc_adamw_desc *d, const rexsc_adamw_ten
         return REXSC_OK;
     };
     constexpr int64_t PART = (int64_t)1 << 30;     // a longer tensor becomes several entries (32-bit offsets in the kernel)
-    constexpr uint64_t MAX_CHUNKS = 1u << 30;      // blocks of a launch
+    constexpr uint64_t MAX_CHUNKS = 1u << 23;      // blocks of a launch, which has fewer than 2^32 threads
     for (size_t i = 0; i < n_tensors; i++) {
         const rexsc_adamw_tensor &t = tensors[i];
         for (int64_t at = 0; at < t.numel; at += PART) {

@@ -171,6 +171,7 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(FewArgs g)
 template <int FM, typename T, typename X>
 int launch_u(const FewArgs &g, hipStream_t stream)
 {
+    REXSC_CHECK_ARG(g.p.N < (1 << 26), "int8 linear: %d output channels are more than a launch holds", g.p.N);
     const dim3 grid((unsigned)((g.p.N + 15) / 16));
     // a round that is longer than the row would load its first chunk over and over
     if (g.p.kbytes > 4 * UNIT) hipLaunchKernelGGL((few_rows_kernel<FM, 8, T, X>), grid, dim3(THREADS), 0, stream, g);

@@ -50,65 +50,74 @@ __device__ __forceinline__ unsigned row_top(unsigned t, unsigned (&lds)[16])
 template <typename T, int V, int TPR>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void quantize_rows_kernel(QuantArgs p)
 {
-    constexpr int NV = Q_EPT / V;
+    constexpr int NV = Q_EPT / V, RPB = TPR == 64 ? 4 : 1;
     typedef typename VecOf<T, V>::type vec;
-    __shared__ unsigned lds[16];
+    __shared__ unsigned lds[2][16];
     const int tid = TPR == 64 ? threadIdx.x % 64 : threadIdx.x;
-    const size_t row = TPR == 64 ? (size_t)blockIdx.x * 4 + threadIdx.x / 64 : blockIdx.x;
-    if (row >= p.rows) return; // TPR 64 only: a whole wave
-    const T *src = (const T *)p.x + row * p.x_stride;
-    vec v[NV];
+    int slot = 0;
+    for (size_t row = (size_t)blockIdx.x * RPB + (TPR == 64 ? threadIdx.x / 64 : 0); row < p.rows; row += (size_t)gridDim.x * RPB) {
+        const T *src = (const T *)p.x + row * p.x_stride;
+        vec v[NV];
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int c = (i * TPR + tid) * V;
-        v[i] = c < p.cols ? *(const vec *)(src + c) : vec{};
-    }
-    float x[NV][V];
-    unsigned t = 0;
-#pragma unroll
-    for (int i = 0; i < NV; i++)
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            if constexpr (V == 1) x[i][j] = (float)v[i];
-            else x[i][j] = (float)v[i][j];
-            t = max(t, mag_bits(x[i][j]));
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * TPR + tid) * V;
+            v[i] = c < p.cols ? *(const vec *)(src + c) : vec{};
         }
-    const RowScale rs = row_scale(row_top<TPR>(t, lds));
-    int8_t *dst = p.q + row * p.q_stride;
+        float x[NV][V];
+        unsigned t = 0;
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int c = (i * TPR + tid) * V;
-        if (c < p.cols) {
-            typename VecOf<int8_t, V>::type q;
-            if constexpr (V == 1) q = (int8_t)quant8(x[i][0], rs);
-            else
+        for (int i = 0; i < NV; i++)
 #pragma unroll
-                for (int j = 0; j < V; j++) q[j] = (int8_t)quant8(x[i][j], rs);
-            *(typename VecOf<int8_t, V>::type *)(dst + c) = q;
+            for (int j = 0; j < V; j++) {
+                if constexpr (V == 1) x[i][j] = (float)v[i];
+                else x[i][j] = (float)v[i][j];
+                t = max(t, mag_bits(x[i][j]));
+            }
+        const RowScale rs = row_scale(row_top<TPR>(t, lds[slot]));
+        slot ^= 1; // one barrier a row
+        int8_t *dst = p.q + row * p.q_stride;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * TPR + tid) * V;
+            if (c < p.cols) {
+                typename VecOf<int8_t, V>::type q;
+                if constexpr (V == 1) q = (int8_t)quant8(x[i][0], rs);
+                else
+#pragma unroll
+                    for (int j = 0; j < V; j++) q[j] = (int8_t)quant8(x[i][j], rs);
+                *(typename VecOf<int8_t, V>::type *)(dst + c) = q;
+            }
         }
+        for (size_t c = (size_t)p.cols + tid; c < p.q_stride; c += TPR) dst[c] = 0;
+        if (tid == 0) p.scale[row] = rs.scale;
     }
-    for (size_t c = (size_t)p.cols + tid; c < p.q_stride; c += TPR) dst[c] = 0;
-    if (tid == 0) p.scale[row] = rs.scale;
 }
 
 template <typename T>
 __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(QuantArgs p)
 {
-    __shared__ unsigned lds[16];
-    const T *src = (const T *)p.x + blockIdx.x * p.x_stride;
-    unsigned t = 0;
-    for (int c = threadIdx.x; c < p.cols; c += 1024) t = max(t, mag_bits((float)src[c]));
-    const RowScale rs = row_scale(row_top<1024>(t, lds));
-    int8_t *dst = p.q + blockIdx.x * p.q_stride;
-    for (size_t c = threadIdx.x; c < p.q_stride; c += 1024) dst[c] = c < (size_t)p.cols ? (int8_t)quant8((float)src[c], rs) : (int8_t)0;
-    if (threadIdx.x == 0) p.scale[blockIdx.x] = rs.scale;
+    __shared__ unsigned lds[2][16];
+    int slot = 0;
+    for (size_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T *src = (const T *)p.x + row * p.x_stride;
+        unsigned t = 0;
+        for (int c = threadIdx.x; c < p.cols; c += 1024) t = max(t, mag_bits((float)src[c]));
+        const RowScale rs = row_scale(row_top<1024>(t, lds[slot]));
+        slot ^= 1;
+        int8_t *dst = p.q + row * p.q_stride;
+        for (size_t c = threadIdx.x; c < p.q_stride; c += 1024) dst[c] = c < (size_t)p.cols ? (int8_t)quant8((float)src[c], rs) : (int8_t)0;
+        if (threadIdx.x == 0) p.scale[row] = rs.scale;
+    }
 }
 
 template <typename T, int V>
 void launch_quantize_v(const QuantArgs &p, hipStream_t s)
 {
-    const unsigned rows = (unsigned)p.rows;
-    if (p.cols <= 64 * Q_EPT) hipLaunchKernelGGL((quantize_rows_kernel<T, V, 64>), dim3((rows + 3) / 4), dim3(256), 0, s, p);
+    constexpr size_t MOST = 1u << 21; // blocks; a launch has fewer than 2^32 threads
+    const unsigned rows = (unsigned)(p.rows < MOST ? p.rows : MOST);
+    if (p.cols <= 64 * Q_EPT)
+        hipLaunchKernelGGL((quantize_rows_kernel<T, V, 64>), dim3((unsigned)((p.rows + 3) / 4 < MOST ? (p.rows + 3) / 4 : MOST)), dim3(256),
+                           0, s, p);
     else if (p.cols <= 256 * Q_EPT) hipLaunchKernelGGL((quantize_rows_kernel<T, V, 256>), dim3(rows), dim3(256), 0, s, p);
     else if (p.cols <= 1024 * Q_EPT) hipLaunchKernelGGL((quantize_rows_kernel<T, V, 1024>), dim3(rows), dim3(1024), 0, s, p);
     else hipLaunchKernelGGL(quantize_long_rows_kernel<T>, dim3(rows), dim3(1024), 0, s, p);
@@ -564,8 +573,9 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
     p.shares = shares(d->M); p.share_rows = share_rows(d->M);
     p.db = db; p.db_dtype = d->bias_dtype;
     const uint64_t tiles_k = (uint64_t)((d->K + 63) / 64), tiles_n = (uint64_t)p.ldn / 64, tiles_m = (uint64_t)p.ldm / 64;
-    REXSC_CHECK_ARG((uint64_t)d->M + (tiles_n + tiles_m) * tiles_k + tiles_n * MAX_SHARES < (1ull << 31) && tiles_m * tiles_n < (1ull << 31),
-                    "int8 linear: %d x %d x %d is too large", d->M, d->N, d->K);
+    // a launch has fewer than 2^32 threads
+    REXSC_CHECK_ARG((uint64_t)d->M + (tiles_n + tiles_m) * tiles_k + tiles_n * MAX_SHARES < (1ull << 24) && tiles_m * tiles_n < (1ull << 24),
+                    "int8 linear: gradients of %d x %d x %d are more than a launch holds", d->M, d->N, d->K);
     REXSC_CHECK_ARG((size_t)p.ldn * 2 < MAX_ROW_BYTES && (size_t)p.ldm * 2 < MAX_ROW_BYTES,
                     "int8 linear: gradients of at most %zu tokens or channels", MAX_ROW_BYTES / 2 - 64);
     p.row_blocks = dx ? (unsigned)d->M : 0;

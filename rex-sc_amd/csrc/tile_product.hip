@@ -364,7 +364,7 @@ int launch_tile_product(const TileArgs &p, bool f16, int out_dtype, void *worksp
                     MAX_ROW_BYTES - 1);
     const TilePlan pl = tile_plan(p.M, p.N, p.kbytes, p.pieces);
     const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64);
-    REXSC_CHECK_ARG(tiles * pl.splits < (1ll << 31), "int8 linear: result of %d x %d is too large", p.M, p.N);
+    REXSC_CHECK_ARG(tiles * pl.splits < (1ll << 23), "int8 linear: a result of %d x %d is more than a launch holds", p.M, p.N);
     ProfScope prof(name, 2.0 * p.M * p.N * (f16 ? p.kbytes / 2 : p.kbytes) * p.pieces, stream);
     if (f16) REXSC_DTYPE_SWITCH(out_dtype, return (launch_size<OpF16, T>(p, pl, workspace, stream)));
     else REXSC_DTYPE_SWITCH(out_dtype, return (launch_size<OpI8, T>(p, pl, workspace, stream)));

@@ -164,6 +164,13 @@ class Linear_Int8(nn.Linear):
             self.weight = None
         return self
 
+    def _apply(self, fn, *args, **kwargs):
+        scale = self.weight_scale
+        super(Linear_Int8, self)._apply(fn, *args, **kwargs)
+        if scale is not None and self.weight_scale.dtype != torch.float32:  # half() and the like: the scales stay float32
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
     def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
         if prefix + "weight_q" in state_dict and not self.frozen:  # a frozen layer's state into one that is not
             q, s = state_dict[prefix + "weight_q"], state_dict[prefix + "weight_scale"]

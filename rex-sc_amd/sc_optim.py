@@ -47,7 +47,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_av
     params, grads: lists of tensors of one type (float32, float16, bfloat16) on one device, each dense in memory and the
     gradient laid out like its parameter.  exp_avgs, exp_avg_sqs: float32 states laid out likewise, or, with the two
     lists of scales, 8-bit ones: float8_e4m3fn tensors of m / scale and sqrt(v) / scale, one float32 scale for each 256
-    elements in memory order.  step: the number of this step, from 1 on; or a device int64 tensor that holds the steps
+    elements in memory order.  The tensors of a call do not overlap, and a captured call keeps to theirs.  step: the number of this step, from 1 on; or a device int64 tensor that holds the steps
     taken, which the call advances on the stream (a captured call needs that).  clamp: (lo, hi) of the updated
     parameter.  grad_scale, found_inf: float32 device tensors of a gradient scaler, with a device step: gradients are
     divided by the one, and where the other is not 0 the step is left out."""
@@ -80,7 +80,10 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_av
             if not (same and _dense(p)):
                 raise RuntimeError("adamw_step: a parameter, its gradient and its states must be dense and laid out alike "
                                    "(strides %s, %s, %s, %s)" % (p.stride(), g.stride(), m.stride(), v.stride()))
-    columns = [map(_PTR, params), map(_PTR, grads), map(_PTR, exp_avgs), map(_PTR, exp_avg_sqs)]
+    where = list(map(_PTR, params))
+    if len(set(where)) != len(where) and len({a for a, n in zip(where, numels) if n}) != sum(map(bool, numels)):
+        raise RuntimeError("adamw_step: a parameter is given twice")
+    columns = [where, map(_PTR, grads), map(_PTR, exp_avgs), map(_PTR, exp_avg_sqs)]
     if eight:
         blocks = [-(-n // BLOCK) for n in numels]
         for scales, what in ((exp_avg_scales, "exp_avg_scale"), (exp_avg_sq_scales, "exp_avg_sq_scale")):
@@ -132,7 +135,10 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: clamp to (%r, %r)" % tuple(clamp))
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       clamp=clamp, capturable=capturable))
-        self._step_supports_amp_scaling = all(g["capturable"] for g in self.param_groups)
+
+    @property
+    def _step_supports_amp_scaling(self):  # torch.amp.GradScaler asks for it and then sets grad_scale and found_inf
+        return all(g["capturable"] for g in self.param_groups)
 
     def _new_state(self, p, group):
         if not _dense(p):

@@ -210,6 +210,36 @@ def test_many_tensors_and_unaligned_ones(bits):
             check(M[i], me, tm, torch.float32, "m")
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tensor_of_more_than_a_table_entry(bits):
+    """2^30 elements are one entry of a launch's table: the next ones are as right as the first."""
+    import sc_optim
+    n = (1 << 30) + 5000
+    p, g = torch.full((n,), 0.5, device="cuda", dtype=torch.bfloat16), torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    at = [0, 4097, (1 << 30) - 1, 1 << 30, (1 << 30) + 256, n - 1]
+    g[at] = 0.25
+    if bits == 32:
+        m, v, s = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda"), ()
+    else:
+        m, v = (torch.zeros(n, device="cuda", dtype=torch.uint8).view(E4M3) for _ in range(2))
+        s = tuple([torch.zeros(-(-n // 256), device="cuda")] for _ in range(2))
+    sc_optim.adamw_step([p], [g], [m], [v], *s, step=1, lr=0.125, weight_decay=0.0)
+    moved = p != 0.5
+    assert moved.sum().item() == len(at) and moved[at].all()
+    assert torch.equal(p[at].cpu(), torch.full((len(at),), 0.375, dtype=torch.bfloat16))  # the first move is lr
+    if bits == 8:
+        assert s[0][0].count_nonzero().item() == len({i // 256 for i in at})
+
+
+def test_a_parameter_given_twice_is_refused():
+    import sc_optim
+    t = lambda: torch.zeros(300, device="cuda")
+    p, e = t(), torch.zeros(0, device="cuda")
+    with pytest.raises(RuntimeError, match="twice"):
+        sc_optim.adamw_step([p, p], [t(), t()], [t(), t()], [t(), t()], step=1, lr=0.1)
+    sc_optim.adamw_step([e, e, p], [e, e, t()], [e, e, t()], [e, e, t()], step=1, lr=0.1)
+
+
 def test_step_on_the_device_scaler_and_capture():
     import sc_optim
     p0, g0, m0, v0 = tensors([(3000,)], torch.float32, 1)[0]

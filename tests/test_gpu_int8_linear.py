@@ -327,6 +327,60 @@ def test_gradient_of_an_infinite_and_a_nan_output_gradient():
     assert dw[[1, 3]].isfinite().all() and not dw[2].isfinite().any() and dw[0].isnan().all()
 
 
+# ---- every tile and share of the reduction ---------------------------------------------------------
+@pytest.mark.parametrize("tile", ["64", "128", "256"])
+@pytest.mark.parametrize("splits", ["1", "3", "16"])
+def test_forced_tiles_and_splits(tile, splits, monkeypatch):
+    """Integer sums do not depend on the plan; the gradients' float32 sums are exact here (integers, see above)."""
+    import sc_functional as F
+    monkeypatch.setenv("REXSC_TUNE_INT8_TILE", tile)
+    monkeypatch.setenv("REXSC_TUNE_INT8_SPLITS", splits)
+    g = torch.Generator().manual_seed(5)
+    for m, n, k in ((1, 1, 1), (3, 70, 129), (130, 259, 500), (257, 65, 2100), (300, 513, 127)):
+        print("forced", tile, splits, m, n, k, flush=True)
+        qa = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8)
+        qb = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8)
+        sa, sb, bias = torch.rand(m, generator=g), torch.rand(n, generator=g), torch.randn(n, generator=g)
+        for dt in (torch.float32, torch.bfloat16):
+            y = F.matmul_int8(qa.cuda(), sa.cuda(), qb.cuda(), sb.cuda(), bias.cuda(), dt)
+            _product_close(y, qa, sa, qb, sb, bias, dt)
+        x, w = torch.randint(-60, 61, (m, k), generator=g).float(), torch.randint(-60, 61, (n, k), generator=g).float()
+        x[:, 0], w[:, k - 1] = 127, -127
+        go = torch.randint(-8, 9, (m, n), generator=g).float()
+        xt, wt = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+        dx, dw = torch.autograd.grad(F.linear_int8(xt, wt), [xt, wt], go.cuda())
+        assert torch.equal(dx.cpu().double(), go.double() @ w.double())
+        assert torch.equal(dw.cpu().double(), go.double().t() @ x.double())
+
+
+def test_offsets_behind_32_bits():
+    """A result and an operand of more than 2^31 elements: the last rows are as right as the first."""
+    import sc_functional as F
+    m, n, k = 70001, 32776, 48
+    a = torch.randint(-128, 128, (m, k), device="cuda", dtype=torch.int8)
+    b = torch.randint(-128, 128, (n, k), device="cuda", dtype=torch.int8)
+    one = torch.ones(max(m, n), device="cuda")
+    y = F.matmul_int8(a, one[:m], b, one[:n], None, torch.bfloat16)
+    for r in (0, 40000, 65535, 65536, m - 1):
+        want = (a[r].cpu().double() @ b.cpu().double().t()).float().bfloat16()
+        assert torch.equal(y[r].cpu(), want), r
+    del y
+    x = torch.randn(1 << 19, 4100, device="cuda", dtype=torch.bfloat16)
+    q, s = F.quantize_rows(x)
+    for r in (0, 300000, (1 << 19) - 1):
+        qe, se = quantised(x[r])
+        assert torch.equal(q[r].cpu().double(), qe) and torch.equal(s[r].cpu(), se), r
+
+
+def test_more_rows_than_blocks():
+    import sc_functional as F
+    x = torch.randn((1 << 23) + 9, 3, device="cuda", dtype=torch.float16)
+    q, s = F.quantize_rows(x)
+    for sl in (slice(0, 1000), slice((1 << 23) - 500, None)):
+        qe, se = quantised(x[sl])
+        assert torch.equal(q[sl].cpu().double(), qe) and torch.equal(s[sl].cpu(), se)
+
+
 # ---- streams, graphs, threads --------------------------------------------------------------------
 def test_two_streams_at_once():
     import sc_functional as F
@@ -406,6 +460,17 @@ def test_layer_trains_freezes_and_reloads():
     xg = x.clone().requires_grad_(True)
     layer(xg).sum().backward()
     assert xg.grad.shape == x.shape
+
+
+def test_frozen_layer_in_half_precision():
+    from sc_layers import Linear_Int8
+    layer = Linear_Int8(70, 33, bias=False).cuda().freeze()
+    x = torch.randn(5, 70, device="cuda").half()
+    with torch.no_grad():
+        want = layer(x)
+        scale = layer.weight_scale.clone()
+        assert torch.equal(layer.half()(x), want) and torch.equal(layer.weight_scale, scale)
+        assert layer.weight_scale.dtype == torch.float32
 
 
 def test_autocast_region():

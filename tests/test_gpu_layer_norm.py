@@ -188,6 +188,22 @@ def test_captured_and_two_streams():
         assert all(torch.equal(a, b) for a, b in zip(r, want))  # no atomics: the same bits every time
 
 
+def test_offsets_behind_32_bits():
+    import sc_functional as F
+    x = torch.randn((1 << 21) + 3, 1032, device="cuda", dtype=torch.bfloat16)
+    w, b = torch.randn(1032, device="cuda"), torch.randn(1032, device="cuda")
+    xl = x.requires_grad_(True)
+    y = F.layer_norm(xl, w, b)
+    g = torch.zeros_like(y)
+    rows = [0, 5, 1 << 20, (1 << 21) + 2]
+    g[rows] = torch.randn(4, 1032, device="cuda").bfloat16()
+    dx, = torch.autograd.grad(y, [xl], g)
+    ref = reference(x.detach()[rows].cpu(), w.cpu(), b.cpu(), g[rows].cpu())
+    close(y.detach()[rows], ref["y"], torch.bfloat16, "y")
+    close(dx[rows], ref["dx"], torch.bfloat16, "dx")
+    assert not dx[6:1000].any()
+
+
 def test_layer():
     from sc_layers import LayerNorm
     import sc_functional as F
