@@ -284,7 +284,7 @@ __global__ __launch_bounds__(256) void join_kernel(TileArgs p, const ACC *part, 
 // ---- host ------------------------------------------------------------------------------------------
 constexpr int CUS = 256, MAX_SPLITS = 16;
 
-struct TilePlan { int size, splits; };
+struct TilePlan { int size, splits; }; // size: 256, 128, 64 (squares) or 32 (64 x 32)
 
 int tune(const char *name)
 {
@@ -307,8 +307,12 @@ TilePlan tile_plan(int M, int N, int kbytes, int pieces)
     const int64_t n256 = busiest(256), n128 = busiest(128), n64 = busiest(64);
     const double t256 = (double)n256, t128 = 0.61 * (double)(n128 / 2) + 0.44 * (double)(n128 % 2), t64 = 0.08 + 0.11 * (double)n64;
     TilePlan pl{t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64, 1};
-    if (const int t = tune("REXSC_TUNE_INT8_TILE")) pl.size = t == 256 || t == 128 ? t : 64;
-    const int64_t n = tiles(pl.size);
+    // 64 x 32 where that still leaves no CU two tiles: the weights are then read by twice as many (from cold weights
+    // 64 x 4096 x 4096: 11.4 us against 13.0; 256 x 4096 x 4096, two tiles for a CU: 15.8 against 13.5)
+    const int64_t halves = (int64_t)((M + 63) / 64) * ((N + 31) / 32);
+    if (pl.size == 64 && halves <= CUS) pl.size = 32;
+    if (const int t = tune("REXSC_TUNE_INT8_TILE")) pl.size = t == 256 || t == 128 || t == 32 ? t : 64;
+    const int64_t n = pl.size == 32 ? halves : tiles(pl.size);
     if (n > 0 && 4 * n <= CUS) {
         const int64_t fill = CUS / n, keep = steps / 8;
         pl.splits = (int)(fill < keep ? fill : keep);
@@ -345,6 +349,7 @@ int launch_size(const TileArgs &p, const TilePlan &pl, void *workspace, hipStrea
 {
     if (pl.size == 256) return launch_one<Op, T, 256, 256, 2, 4, 2>(p, pl.splits, workspace, stream);
     if (pl.size == 128) return launch_one<Op, T, 128, 128, 2, 2, 2>(p, pl.splits, workspace, stream);
+    if (pl.size == 32) return launch_one<Op, T, 64, 32, 2, 2, 4>(p, pl.splits, workspace, stream);
     return launch_one<Op, T, 64, 64, 2, 2, 4>(p, pl.splits, workspace, stream);
 }
 
@@ -363,7 +368,7 @@ int launch_tile_product(const TileArgs &p, bool f16, int out_dtype, void *worksp
                     "int8 linear: operand rows of %zu and %zu bytes, at most %zu are supported", p.a_stride, p.b_stride,
                     MAX_ROW_BYTES - 1);
     const TilePlan pl = tile_plan(p.M, p.N, p.kbytes, p.pieces);
-    const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64);
+    const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 31) / 32);
     REXSC_CHECK_ARG(tiles * pl.splits < (1ll << 23), "int8 linear: a result of %d x %d is more than a launch holds", p.M, p.N);
     ProfScope prof(name, 2.0 * p.M * p.N * (f16 ? p.kbytes / 2 : p.kbytes) * p.pieces, stream);
     if (f16) REXSC_DTYPE_SWITCH(out_dtype, return (launch_size<OpF16, T>(p, pl, workspace, stream)));

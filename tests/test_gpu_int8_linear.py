@@ -328,7 +328,7 @@ def test_gradient_of_an_infinite_and_a_nan_output_gradient():
 
 
 # ---- every tile and share of the reduction ---------------------------------------------------------
-@pytest.mark.parametrize("tile", ["64", "128", "256"])
+@pytest.mark.parametrize("tile", ["32", "64", "128", "256"])
 @pytest.mark.parametrize("splits", ["1", "3", "16"])
 def test_forced_tiles_and_splits(tile, splits, monkeypatch):
     """Integer sums do not depend on the plan; the gradients' float32 sums are exact here (integers, see above)."""
