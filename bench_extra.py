@@ -153,12 +153,13 @@ def config2_sc_linear(torch, dev):
     return out
 
 
-def _train_flavours(torch, dev, net, make_batch, batch, steps, lr, only=None):
+def _train_flavours(torch, dev, net, make_batch, batch, steps, lr, only=None, opt=None):
     """Training steps as utils_own.py:96-171 runs them: sync 1 / 3 / 2 in float32; only="autocast": sync 1 under
     float16 autocast with a gradient scaler instead (the reference's `torch_type != torch.float32` branch,
     :127-131,156-165); only="sync1": the float32 sync-1 flavour alone (for profiler runs)."""
     import torch.nn.functional as F
-    opt = torch.optim.Adam(net.parameters(), lr=lr, weight_decay=1e-4)
+    if opt is None:
+        opt = torch.optim.Adam(net.parameters(), lr=lr, weight_decay=1e-4)
     only_autocast = only == "autocast"
     scaler = torch.amp.GradScaler("cuda") if only_autocast else None
     out = {}
@@ -195,20 +196,31 @@ def _train_flavours(torch, dev, net, make_batch, batch, steps, lr, only=None):
     return out
 
 
-def config3_tinyconv_step(torch, dev, only=None):
+def config3_tinyconv_step(torch, dev, only=None, state_bits=None):
+    """state_bits: 32 or 8 takes the network with its 8-bit classifier and this package's AdamW with states of that many
+    bits, the weights held to their range in the step; None: the float classifier and torch's Adam."""
     from sc_models import TinyConvSC
     torch.manual_seed(3)
-    net = TinyConvSC(forward="or_3", err=6).to(dev)
+    net = TinyConvSC(forward="or_3", err=6, classifier="float" if state_bits is None else "int8").to(dev)
+    opt = None
+    if state_bits is not None:
+        import sc_optim
+        opt = sc_optim.AdamW(net.parameters(), lr=8e-3, weight_decay=1e-4, state_bits=state_bits, clamp=(-1, 0.999))
     g = torch.Generator().manual_seed(3)
 
     def make_batch(n):
         return (torch.randn(n, 3, 32, 32, generator=g).clamp(-1, 1).to(dev),
                 torch.randint(0, 10, (n,), generator=g).to(dev))
 
-    res = _train_flavours(torch, dev, net, make_batch, 256, 10, 8e-3, only)
+    res = _train_flavours(torch, dev, net, make_batch, 256, 10, 8e-3, only, opt)
     res["workload"] = ("TinyConv-style training step, batch 256, 3x32x32, conv3x3 3-32-32-pool-64-64-pool-fc10, "
-                       "OR-3, 64-bit streams, Adam")
+                       "OR-3, 64-bit streams, " + ("Adam" if state_bits is None else
+                                                   "LayerNorm + 8-bit fc, AdamW with %d-bit states" % state_bits))
     return res
+
+
+def config3_tinyconv_int8_adamw_step(torch, dev):
+    return {"states_%d_bit" % b: config3_tinyconv_step(torch, dev, only="sync1", state_bits=b) for b in (32, 8)}
 
 
 def config3_tinyconv_autocast_step(torch, dev):
@@ -408,6 +420,34 @@ def pointwise(torch, dev):
                      "hbm_frac_kernel_only": bpe * n / (kms * 1e-3) / HBM_PEAK if kms else None,
                      "hbm_frac_one_buffer_set": bpe * n / sec_one / HBM_PEAK}
         del sets, one
+        torch.cuda.empty_cache()
+    return res
+
+
+def linear8_operators(torch, dev):
+    """The 8-bit linear layer, layer norm and the AdamW step on the workloads of perf/operators.py: wall time of a call
+    among others (rotating through three sets of inputs), the library's kernels, bytes and operations that the call
+    cannot do without per second of wall time."""
+    import importlib.util
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "perf", "operators.py")
+    spec = importlib.util.spec_from_file_location("operator_workloads", path)
+    cases = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(cases)
+    cases.own = True
+    res = {}
+    for case in cases.listed():
+        states = [cases.prepare(case, seed) for seed in range(3)]
+        at = {"i": 0}
+
+        def call():
+            at["i"] += 1
+            return cases.run(states[at["i"] % 3])
+
+        need, sec = cases.work(case), _time(torch, call, 30, 6)
+        prof = _profile(torch, call, 6)
+        res[case["name"]] = {"us": sec * 1e6, "GB_per_s": need["bytes"] / sec / 1e9, "TFLOP_per_s": need["flops"] / sec / 1e12,
+                             "kernel_us": {k: [v["calls"], round(v["ms"] / v["calls"] * 1e3, 2)] for k, v in sorted(prof.items())}}
+        del states
         torch.cuda.empty_cache()
     return res
 
