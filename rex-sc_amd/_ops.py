@@ -859,6 +859,42 @@ def int8_linear(x, wq, w_scale, bias=None):
     return y
 
 
+def int8_linear_train(x, w, bias):
+    """int8_linear with a float weight, both operands' 8-bit forms kept for int8_backward: (y, xq, x_scale, wq, w_scale)."""
+    if not (x.is_cuda and w.is_cuda):
+        _require_cuda(x, w)
+    _same_device("linear_int8", x, w, bias)
+    shape = x.shape
+    K = shape[-1]
+    N = w.shape[0]
+    if not 1 <= K <= MAX_K:
+        raise RuntimeError("linear_int8: expected 1 to %d input features (got %d)" % (MAX_K, K))
+    code, w_code = _dtype_code(x, "linear_int8"), _dtype_code(w, "linear_int8")
+    xm, wm = _rows_of(x), _rows_of(w)
+    M = xm.shape[0]
+    pad = -(-K // ROW_PAD) * ROW_PAD
+    bias, bias_code = _bias_vector(bias, N, "linear_int8")
+    device, dev = x.device, x.get_device()
+    L = _lib.lib()
+    with _on(dev):
+        stream = _raw_stream(dev)
+        q = torch.empty((M + N, pad), dtype=torch.int8, device=device)
+        scales = torch.empty((M + N,), dtype=torch.float32, device=device)
+        xq, xs = q.data_ptr(), scales.data_ptr()
+        wq, ws = xq + M * pad, xs + 4 * M
+        rc = L.rexsc_quantize_rows(xm.data_ptr(), code, M, K, _row_stride(xm), xq, pad, xs, stream)
+        rc = rc or L.rexsc_quantize_rows(wm.data_ptr(), w_code, N, K, _row_stride(wm), wq, pad, ws, stream)
+        if rc:
+            _lib.check(rc, "rexsc_quantize_rows")
+        y = torch.empty(shape[:-1] + (N,), dtype=x.dtype, device=device)
+        d = _lib.Int8Desc.packed(M, N, K, code, bias_code, 0, 0, 0, pad, pad)
+        space, nbytes = _int8_space(L, d, _lib.INT8_PRODUCT, device)
+        rc = L.rexsc_int8_product(d, xq, xs, wq, ws, _addr(bias), y.data_ptr(), _addr(space), nbytes, stream)
+        if rc:
+            _lib.check(rc, "rexsc_int8_product")
+    return y, q[:M, :K], scales[:M], q[M:, :K], scales[M:]
+
+
 def _dense_rows(g, n):
     """g [..., n] as a dense matrix."""
     if g.dim() != 2:

@@ -297,7 +297,8 @@ int tune(const char *name)
 // 64 x 64, up to five side by side, 0.08 + 0.11 n.  E.g. 2048 x 4096: 37 us in 128s against 52 in 256s and 58 in 64s;
 // 4096 x 4096: 59 in 256s against 69 in 128s; 512 x 4096: 19 in 64s against 26 in 128s.
 // The reduction is split over blocks only where the result has tiles for at most a quarter of the CUs and each share
-// keeps 8 steps: the partial results cost a second launch.  300 x 300 x 16384: 16 us in 8 shares against 37 in one;
+// keeps 8 steps of 48 at least: the partial results cost a second launch (256 x 10 x 4096, 32 steps: 9.0 us in one
+// share, 7.8 in four, less than the launch's host time).  300 x 300 x 16384: 16 us in 8 shares against 37 in one;
 // with more tiles, splitting lost in each case measured (128 x 4096 x 4096: 14 us against 16 in two shares).
 TilePlan tile_plan(int M, int N, int kbytes, int pieces)
 {
@@ -313,7 +314,7 @@ TilePlan tile_plan(int M, int N, int kbytes, int pieces)
     if (pl.size == 64 && halves <= CUS) pl.size = 32;
     if (const int t = tune("REXSC_TUNE_INT8_TILE")) pl.size = t == 256 || t == 128 || t == 32 ? t : 64;
     const int64_t n = pl.size == 32 ? halves : tiles(pl.size);
-    if (n > 0 && 4 * n <= CUS) {
+    if (n > 0 && 4 * n <= CUS && steps >= 48) {
         const int64_t fill = CUS / n, keep = steps / 8;
         pl.splits = (int)(fill < keep ? fill : keep);
     }

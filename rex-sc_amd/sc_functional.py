@@ -718,16 +718,12 @@ class Linear_Int8_Grad(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, weight_scale):
-        if weight_scale is None:
-            wq, ws = _ops.quantize_rows(weight)
-        else:
-            wq, ws = weight, weight_scale
         ctx.types = (weight.dtype if weight_scale is None else None, None if bias is None else bias.dtype)
         if ctx.needs_input_grad[1]:  # the tokens are wanted in 8 bits again by the backward pass
-            xq, xs = _ops.quantize_rows(x.reshape(-1, x.shape[-1]))
-            y = _ops.matmul_int8(xq, xs, wq, ws, bias, x.dtype).view(x.shape[:-1] + (wq.shape[0],))
+            y, xq, xs, wq, ws = _ops.int8_linear_train(x, weight, bias)
             ctx.save_for_backward(wq, ws, xq, xs)
         else:
+            wq, ws = _ops.quantize_rows(weight) if weight_scale is None else (weight, weight_scale)
             y = _ops.int8_linear(x, wq, ws, bias)
             ctx.save_for_backward(wq, ws, None, None)
         return y

@@ -1,6 +1,6 @@
 """AdamW over many tensors at once on the HIP kernels, with 32-bit or 8-bit states and the clamp of the weights that SC
 training applies after every step (utils_own.py:187-190) folded into it."""
-import ctypes
+import array
 import itertools
 import operator
 
@@ -93,7 +93,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_av
         columns += [map(_PTR, exp_avg_scales), map(_PTR, exp_avg_sq_scales)]
     else:
         columns += [itertools.repeat(0), itertools.repeat(0)]
-    table = list(itertools.chain.from_iterable(zip(*columns, numels)))
+    table = array.array("q", itertools.chain.from_iterable(zip(*columns, numels)))
     on_device = isinstance(step, torch.Tensor)
     if on_device and (step.dtype != torch.int64 or step.numel() != 1 or step.device != first.device):
         raise RuntimeError("adamw_step: a step held in a tensor is one int64 beside the parameters")
@@ -105,10 +105,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_av
     lo, hi = (0.0, 0.0) if clamp is None else (float(clamp[0]), float(clamp[1]))
     d = _lib.AdamwDesc.packed(code, 8 if eight else 32, int(clamp is not None), float(lr), float(beta1), float(beta2), float(eps),
                        float(weight_decay), lo, hi, 0 if on_device else int(step))
-    arr = (ctypes.c_int64 * len(table))(*table)
     with _ops._on(dev):
         coef = torch.empty((_lib.ADAMW_COEF_BYTES,), dtype=torch.uint8, device=first.device) if on_device else None
-        rc = _lib.lib().rexsc_adamw_step(d, ctypes.addressof(arr), len(params),
+        rc = _lib.lib().rexsc_adamw_step(d, table.buffer_info()[0], len(params),
                                          _ops._addr(step if on_device else None), _ops._addr(grad_scale),
                                          _ops._addr(found_inf), _ops._addr(coef), _ops._raw_stream(dev))
         if rc:
