@@ -36,6 +36,11 @@ __device__ __forceinline__ void reads_done()
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
+__device__ __forceinline__ void meet()
+{
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory"); // the barrier alone does not keep the compiler from reading memory before it
+}
 
 // Bytes of a 16-byte chunk at offset k that lie before `end`; the rest become 0.
 __device__ __forceinline__ i32x4 keep_before(i32x4 v, int k, int end)
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
             if (i < total) fetch(lds + i * BUF);
         if (total >= STAGES) loads_left<(STAGES - 1) * (LA + LB)>();
         else loads_left<0>();
-        __builtin_amdgcn_s_barrier();
+        meet();
         if (tail && total == 1) clear_tail(base);
 #pragma unroll
         for (int i = 0; i < FM; i++) fa[0][i] = *(const lds_i32x4 *)(base + at_a[0] + i * 16 * KSTEP);
@@ -187,7 +192,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
             if (STAGES > 2 && s + STAGES - 1 < total) loads_left<(STAGES - 2) * (LA + LB)>();
             else loads_left<0>();
             reads_done();
-            __builtin_amdgcn_s_barrier();
+            meet();
             const int next = cur + BUF < STAGES * BUF ? cur + BUF : 0;
             if (tail && s + 2 == total) clear_tail(base + next);
             if (s + STAGES < total) fetch(lds + cur);

@@ -112,6 +112,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_av
                                          _ops._addr(found_inf), _ops._addr(coef), _ops._raw_stream(dev))
         if rc:
             _lib.check(rc, "rexsc_adamw_step")
+    # for autograd's check of tensors changed between a forward and its backward pass
+    torch.autograd.graph.increment_version(params)
 
 
 class AdamW(torch.optim.Optimizer):

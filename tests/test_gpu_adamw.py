@@ -231,6 +231,17 @@ def test_a_tensor_of_more_than_a_table_entry(bits):
         assert s[0][0].count_nonzero().item() == len({i // 256 for i in at})
 
 
+def test_a_step_between_forward_and_backward_is_noticed():
+    import sc_optim
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    opt = sc_optim.AdamW([p], lr=0.1)
+    y = (p * p).sum()
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_a_parameter_given_twice_is_refused():
     import sc_optim
     t = lambda: torch.zeros(300, device="cuda")
