@@ -6,6 +6,8 @@
 // 32-bit states, 16 with 8-bit states, 10 with bfloat16 tensors and 8-bit states.  One launch takes a table of tensors
 // in its kernel arguments (nothing is copied to the device first, and a captured launch keeps its table), and a
 // workgroup finds the tensor its chunk belongs to by bisection over the chunks' running count.
+// Measured: 11.7 M float32 values in 62 tensors, 32-bit states, 59-70 us (5.6-4.7 TB/s, part of them still in the
+// memory-side cache); 268 M bfloat16 values, 8-bit states, 524 us (5.1 TB/s); a copy of 1 GiB reaches 5.1 TB/s.
 //
 // 8-bit states: a wave holds two blocks of the 256 elements that share a scale, eight elements per lane, so a block's
 // maximum is a reduction over 32 lanes and the conversion to and from e4m3 is the hardware's, two values an instruction.

@@ -6,6 +6,8 @@
 // wave has UNROLL loads in flight before the first is used.  The waves' int32 sums, exact in any order, are joined
 // through LDS.  With one or two tokens (M K <= 8192) the block takes them to 8 bits itself, while its first weights are on their way:
 // a launch of its own would cost more than every block's reading the few kilobytes again.
+// Measured with weights from memory: 1 x 4096 x 4096 5.9 us from int8 tokens, 8.0 us from float ones (with the rows'
+// own launch 9.0); 1 x 16384 x 4096 14.4 us (4.7 TB/s of weights).
 #include <stdlib.h>
 
 #include <type_traits>

@@ -22,7 +22,8 @@ constexpr int MAX_K = 131071; // 128 * 128 * K < 2^31
 
 // ---- rows to 8 bits ------------------------------------------------------------------------------
 // Bound by memory: x is read once.  A row lives in the registers of TPR threads (a wave, or a block of 256 or 1024), 16
-// elements a thread at most, all its loads in flight together; rows longer than 16384 are read twice.
+// elements a thread at most, all its loads in flight together; rows longer than 16384 are read twice.  8192 x 4096
+// bfloat16: 24 us (4.2 TB/s of reads and writes); one row of 4096: 3 us, the launch and one round trip to memory.
 constexpr int Q_EPT = 16;
 
 struct QuantArgs {
@@ -293,7 +294,8 @@ __device__ void column_stats(const OperandArgs &p, unsigned block, float (&ls)[3
 }
 
 // All that the gradients' operands need of each other's results is the columns' statistics, so everything else is one
-// launch, told apart by the block's number.
+// launch, told apart by the block's number.  Bound by memory: g twice, int8 in and binary16 out for both transposes, g's
+// rows out; 8192 x 4096 x 4096 with bfloat16 g: 352 MB in 68 us (5.2 TB/s), the second launch 201 MB in 38 us (5.3).
 template <typename T, int V>
 __global__ __launch_bounds__(256) void operands_kernel(OperandArgs p)
 {

@@ -1,6 +1,5 @@
-// Element types of the operators that take float32, float16 or bfloat16 tensors, and the wave / block reductions
-// they share.  Arithmetic is float32 throughout: a 16-bit tensor is widened on the load and rounded once, half to
-// even, on the store.
+// Element types of the operators that take float32, float16 or bfloat16 tensors, and what they share.  Arithmetic is
+// float32 throughout: a 16-bit tensor is widened on the load and rounded once, half to even, on the store.
 #pragma once
 #include "rexsc_common.h"
 
@@ -61,13 +60,7 @@ __device__ __forceinline__ void store_any(void *p, int dtype, size_t i, float v)
     else ((bf16_t *)p)[i] = (bf16_t)v;
 }
 
-// Sums and maxima over the 64 lanes, the result in every lane.  The order of the additions is fixed.
-__device__ __forceinline__ float wave_sum(float v)
-{
-#pragma unroll
-    for (int s = 32; s; s >>= 1) v += __shfl_xor(v, s, 64);
-    return v;
-}
+// Maximum over the 64 lanes, the result in every lane.
 __device__ __forceinline__ unsigned wave_max(unsigned v)
 {
 #pragma unroll

@@ -1,4 +1,12 @@
 // Product of two row-major operands: c[m][n] = sum_k a[m][k] b[n][k].
+//
+// Bound by the matrix pipe where the result is large, by reading b where it is not.  A tile's operands go to LDS by
+// direct loads, whole steps ahead, and from there to registers half a step ahead of the matrix instruction.  256 x 256
+// outputs per block of eight waves is the largest tile whose accumulators (128 a lane) leave room for two sets of
+// fragments, and a step of 128 bytes the longest of which two fit LDS; it reads 64 KB from L2 for 8.4 M products.
+// Measured, int8: 8192^3 402-422 us (2.6-2.7 POP/s), 8192 x 16384 x 4096 463-480 us (2.3), 8192 x 4096 x 4096 108-115 us;
+// the library's int8 product reaches 2.24 POP/s at 8192^3 and 1.85 at 8192 x 16384 x 4096.  binary16, 4096 x 4096 x 8192
+// in two pieces: 400 us (1.37 PFLOP/s).  The matrix pipe is busy 0.69 of the cycles, at 1.8-1.95 GHz.
 #include <stdlib.h>
 
 #include <type_traits>
