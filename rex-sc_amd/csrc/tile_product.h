@@ -9,7 +9,7 @@ struct TileArgs {
     const char *a, *b;              // y[m][n] = sum_piece sum_k a[piece][m][k] b[n][k]
     size_t a_stride, b_stride;      // bytes, multiples of 16; below MAX_ROW_BYTES
     int M, N;
-    int kbytes;                     // length of a reduction row; rows are readable to the next multiple of 16 bytes
+    int kbytes;                     // length of a reduction row, 0: y is zeros; rows are readable to the next multiple of 16 bytes
     int pieces;                     // a is this many matrices, one behind the other, all multiplied by the same b
     size_t piece_stride;            // bytes
     const float *a_scale, *b_scale; // NULL: 1

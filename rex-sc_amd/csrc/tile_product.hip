@@ -37,7 +37,8 @@ __device__ __forceinline__ void loads_left()
 {
     static_assert(N < 64, "the counter has six bits");
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14); // vmcnt(N), no wait for the other counters
+    asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ void reads_done()
 {
@@ -61,14 +62,22 @@ __device__ __forceinline__ i32x4 keep_before(i32x4 v, int k, int end)
     return v;
 }
 
+// The same value, which the compiler takes for a new one: what is computed from it is not kept in registers from
+// before.
+__device__ __forceinline__ int again(int v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
 
-// 16 bytes per lane from base + lane offset + offset to LDS, at dst + 16 * lane.
-__device__ __forceinline__ void load_to_lds(const char *base, unsigned lane_offset, unsigned offset, char *dst)
+// 16 bytes per lane from base + offset to LDS, at dst + 16 * lane; zeros where the offset is not below `bytes`.
+__device__ __forceinline__ void load_to_lds(const char *base, unsigned bytes, unsigned offset, char *dst)
 {
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, 0x7fffffff, 0x00027000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)dst, 16, lane_offset, offset, 0, 0);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, (int)bytes, 0x00027000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)dst, 16, offset, 0, 0, 0);
 }
 
 constexpr int KSTEP = 128;          // bytes of the reduction per step
@@ -89,71 +98,96 @@ __device__ __forceinline__ void tile_of(unsigned bid, int tiles_m, int tiles_n, 
     const unsigned t = x * per + (x < extra ? x : extra) + i;
     const unsigned group = (unsigned)(GROUP_M * tiles_n), g = t / group, r = t % group;
     const int left = tiles_m - (int)g * GROUP_M, rows = left < GROUP_M ? left : GROUP_M;
-    tm = (int)g * GROUP_M + (int)(r % rows);
-    tn = (int)(r / rows);
+    tm = __builtin_amdgcn_readfirstlane((int)g * GROUP_M + (int)(r % rows)); // (divided in vector registers)
+    tn = __builtin_amdgcn_readfirstlane((int)(r / rows));
 }
 
 // SPLIT: the grid holds `splits` times the tiles, and a block sums only its share of the steps, into a partial result
 // of the accumulator's type (T) that join_kernel finishes.
-template <typename Op, typename T, int BM, int BN, int WM, int WN, int STAGES, bool SPLIT>
+// STREAM: the grid holds a block per CU, and a block takes every gridDim.x-th tile.  Its steps are one stream over all
+// its tiles: the next tile's first steps are fetched while the last one's are multiplied, and its first fragments wait in
+// registers while the finished tile is stored, from LDS of its own.
+template <typename Op, typename T, int BM, int BN, int WM, int WN, int STAGES, bool SPLIT, bool STREAM>
 __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int splits)
 {
+    static_assert(!(SPLIT && STREAM), "");
     constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
     constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES; // loads of 8 rows x 128 bytes per wave and step
     static_assert(LA * WAVES * 8 == BM && LB * WAVES * 8 == BN, "tile rows must divide among the waves");
     constexpr int BUF = (BM + BN) * KSTEP;
-    __shared__ __attribute__((aligned(1024))) char lds[STAGES * BUF];
+    // the tile on its way out: COLS x CR elements per wave, behind the buffers (STREAM) or in their place
+    constexpr int COLS = BN / WN, ROWS = BM / WM, RB = COLS * (int)sizeof(T), PART = STREAM ? 16 : sizeof(T) == 4 ? 32 : 64;
+    constexpr int CR = ROWS < PART ? ROWS : PART, SHARE = CR * RB;
+    static_assert(WAVES * SHARE <= STAGES * BUF, "the waves' shares fit the buffers");
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * BUF + (STREAM ? WAVES * SHARE : 0)];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    int tm, tn;
+    const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
     const int share = SPLIT ? (int)(blockIdx.x % splits) : 0;
-    tile_of(SPLIT ? blockIdx.x / splits : blockIdx.x, (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, tm, tn);
-    const int m0 = tm * BM, n0 = tn * BN;
-    const int last_m = p.M - 1 - m0, last_n = p.N - 1 - n0; // rows behind the operand's last read that one again
+    unsigned tile = SPLIT ? blockIdx.x / splits : blockIdx.x;
 
-    // per load: where this lane's row begins, and its chunk, the same for all loads since their rows lie 16 apart (the
-    // LDS side of a load is fixed: 16 bytes per lane in lane order)
+    // A wave's loads are 8 * WAVES rows apart, so that a lane takes the same chunk in all of them (the LDS side of a load
+    // is fixed: 16 bytes per lane in lane order).  Rows behind the operand's last lie behind the descriptor's range.
     static_assert(WAVES % 2 == 0, "loads of one wave must be 16 rows apart");
-    unsigned offa[LA], offb[LB];
-#pragma unroll
-    for (int i = 0; i < LA; i++) {
-        const int r = (i * WAVES + wave) * 8 + lane / 8;
-        offa[i] = (unsigned)(r < last_m ? r : last_m) * (unsigned)p.a_stride;
-    }
-#pragma unroll
-    for (int i = 0; i < LB; i++) {
-        const int r = (i * WAVES + wave) * 8 + lane / 8;
-        offb[i] = (unsigned)(r < last_n ? r : last_n) * (unsigned)p.b_stride;
-    }
+    const char *base_a, *base_b;
+    unsigned bytes_a, bytes_b;
+    auto seek = [&](unsigned t) __attribute__((always_inline)) {
+        int tm, tn;
+        tile_of(t, tiles_m, tiles_n, tm, tn);
+        const int m0 = tm * BM, n0 = tn * BN;
+        base_a = p.a + (size_t)m0 * p.a_stride;
+        base_b = p.b + (size_t)n0 * p.b_stride;
+        bytes_a = (unsigned)(p.M - m0 < BM ? p.M - m0 : BM) * (unsigned)p.a_stride;
+        bytes_b = (unsigned)(p.N - n0 < BN ? p.N - n0 : BN) * (unsigned)p.b_stride;
+    };
+    seek(tile);
     const unsigned chunk = (unsigned)swizzle(wave * 8 + lane / 8, lane % 8) * 16;
-    const char *base_a = p.a + (size_t)m0 * p.a_stride, *base_b = p.b + (size_t)n0 * p.b_stride;
-    const int steps = (p.kbytes + KSTEP - 1) / KSTEP, every = steps * p.pieces;
+    unsigned offa[LA], offb[LB]; // this lane's chunk in each load
+#pragma unroll
+    for (int i = 0; i < LA; i++) offa[i] = (unsigned)((i * WAVES + wave) * 8 + lane / 8) * (unsigned)p.a_stride + chunk;
+#pragma unroll
+    for (int i = 0; i < LB; i++) offb[i] = (unsigned)((i * WAVES + wave) * 8 + lane / 8) * (unsigned)p.b_stride + chunk;
+    const int steps = p.kbytes > KSTEP ? (p.kbytes + KSTEP - 1) / KSTEP : 1, every = steps * p.pieces; // (an empty sum: a step of zeros)
     const int begin = SPLIT ? (int)((int64_t)every * share / splits) : 0;
     const int total = (SPLIT ? (int)((int64_t)every * (share + 1) / splits) : every) - begin;
     if constexpr (SPLIT) base_a += (size_t)(begin / steps) * p.piece_stride;
 
-    unsigned k = SPLIT ? (unsigned)(begin % steps) * KSTEP : 0; // byte offset in the row of the step that is fetched next
+    // what is fetched next: the byte offset in the row, the tile, and the steps that this tile still has
+    unsigned k = SPLIT ? (unsigned)(begin % steps) * KSTEP : 0, ahead = tile;
+    int left = total;
+    const unsigned all = STREAM ? (unsigned)tiles_m * (unsigned)tiles_n : 0;
     auto fetch = [&](char *buf) __attribute__((always_inline)) {
+        if (left == 0) return;
+        auto load = [&](unsigned beyond) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < LA; i++) load_to_lds(base_a + k, bytes_a - k, offa[i] | beyond, buf + (i * WAVES + wave) * 1024);
+#pragma unroll
+            for (int i = 0; i < LB; i++)
+                load_to_lds(base_b + k, bytes_b - k, offb[i] | beyond, buf + BM * KSTEP + (i * WAVES + wave) * 1024);
+        };
         // a chunk behind the row's end is put outside of the descriptor's range and arrives as zeros
-        const unsigned c = k + chunk < (unsigned)p.kbytes ? chunk : 0x80000000u;
-#pragma unroll
-        for (int i = 0; i < LA; i++) load_to_lds(base_a, c + offa[i], k, buf + (i * WAVES + wave) * 1024);
-#pragma unroll
-        for (int i = 0; i < LB; i++) load_to_lds(base_b, c + offb[i], k, buf + BM * KSTEP + (i * WAVES + wave) * 1024);
+        if (k + KSTEP <= (unsigned)p.kbytes) load(0);
+        else load(k + chunk < (unsigned)p.kbytes ? 0 : 0x80000000u);
         k += KSTEP;
         if (k >= (unsigned)p.kbytes) { k = 0; base_a += p.piece_stride; }
+        left--;
+        if (STREAM && left == 0) {
+            ahead += gridDim.x;
+            if (ahead < all) { left = total; seek(ahead); }
+        }
     };
     // int8 rows whose last chunk is not full: what stands behind the row may be anything, and becomes 0 in a's tile
     const int tail = begin + total == every ? p.kbytes % 16 : 0;
+    const int clear_at = !tail ? -1 : total == 1 ? 0 : total - 2; // the step before the one with that chunk
     auto clear_tail = [&](lds_char *buf) __attribute__((always_inline)) {
         const int c = p.kbytes % KSTEP / 16;
-        for (int r = threadIdx.x; r < BM; r += WAVES * 64) {
+        for (int r = wave * 64 + again(lane); r < BM; r += WAVES * 64) {
             lds_i32x4 *at = (lds_i32x4 *)(buf + r * KSTEP + swizzle(r, c) * 16);
             *at = keep_before(*at, 0, tail);
         }
         __syncthreads();
     };
 
-    const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+    const int wm = wave / WN * ROWS, wn = wave % WN * COLS;
     typename Op::acc acc[FM][FN] = {};
     i32x4 fa[2][FM], fb[2][FN]; // fragments of the half step that is multiplied and of the next one
     // Rows 16 apart lie at the same place of the swizzle, and the second half's chunks 64 bytes across it, so a
@@ -176,25 +210,54 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    // The factors of the wave's rows and columns, one of each per lane, on their way while the tile is multiplied.  What
+    // lies behind the last row or column, and a vector that is not there, reads 0.
+    constexpr int SA = (ROWS + 63) / 64;
+    const bool wide_bias = p.bias_dtype == REXSC_F32;
+    int sa_lane[SA] = {}, sb_lane = 0, bias_lane = 0;
+    short bias16_lane = 0;
+    auto load_factors = [&](int m, int n) __attribute__((always_inline)) {
+        if constexpr (SPLIT) return;
+        const int l = again(lane);
+        const int rows = m < p.M ? (p.M - m < ROWS ? p.M - m : ROWS) : 0, cols = n < p.N ? (p.N - n < COLS ? p.N - n : COLS) : 0;
+        auto part = [](const void *v, int first, int count, int size) __attribute__((always_inline)) {
+            return __builtin_amdgcn_make_buffer_rsrc((char *)const_cast<void *>(v) + (size_t)first * size, 0, v ? count * size : 0,
+                                                     0x00027000);
+        };
+#pragma unroll
+        for (int i = 0; i < SA; i++)
+            sa_lane[i] = __builtin_amdgcn_raw_buffer_load_b32(part(p.a_scale, m, rows, 4), (i * 64 + l) * 4, 0, 0);
+        sb_lane = __builtin_amdgcn_raw_buffer_load_b32(part(p.b_scale, n, cols, 4), l * 4, 0, 0);
+        bias_lane = __builtin_amdgcn_raw_buffer_load_b32(part(wide_bias ? p.bias : nullptr, n, cols, 4), l * 4, 0, 0);
+        bias16_lane = __builtin_amdgcn_raw_buffer_load_b16(part(wide_bias ? nullptr : p.bias, n, cols, 2), l * 2, 0, 0);
+    };
+
     // STAGES buffers in a ring.  A step's second half is read while its first is multiplied; then, with every wave's
     // fragments of this buffer in registers and the next buffer filled, one barrier, behind which this buffer is filled
     // anew, STAGES steps ahead, and the first half of the next is read while the second half is multiplied.  (Behind
     // the last step that reads what is not used.)
-    if (total > 0) {
-        fetch(lds);
 #pragma unroll
-        for (int i = 1; i < STAGES; i++)
-            if (i < total) fetch(lds + i * BUF);
-        if (total >= STAGES) loads_left<(STAGES - 1) * (LA + LB)>();
-        else loads_left<0>();
-        meet();
-        if (tail && total == 1) clear_tail(base);
+    for (int i = 0; i < STAGES; i++) fetch(lds + i * BUF);
+    if (!STREAM && total >= STAGES) loads_left<(STAGES - 1) * (LA + LB)>();
+    else loads_left<0>();
+    meet();
+    if (tail && total == 1) clear_tail(base);
+    T *const y = (T *)p.y + (SPLIT ? (size_t)share * p.M * p.N : 0);
+    const size_t pitch = (size_t)p.N * sizeof(T);
+    const bool wide = pitch % 16 == 0 && (uintptr_t)y % 16 == 0 && pitch < 0x80000000u / CR;
+    lds_char *const mine = base + (STREAM ? STAGES * BUF : 0) + wave * SHARE;
+    int cur = 0;
+    do {
+        int tm, tn;
+        tile_of(tile, tiles_m, tiles_n, tm, tn);
+        const int first_m = tm * BM + wm, first_n = tn * BN + wn;
+        load_factors(first_m, first_n);
 #pragma unroll
-        for (int i = 0; i < FM; i++) fa[0][i] = *(const lds_i32x4 *)(base + at_a[0] + i * 16 * KSTEP);
+        for (int i = 0; i < FM; i++) fa[0][i] = *(const lds_i32x4 *)(base + cur + at_a[0] + i * 16 * KSTEP);
 #pragma unroll
-        for (int j = 0; j < FN; j++) fb[0][j] = *(const lds_i32x4 *)(base + at_b[0] + j * 16 * KSTEP);
-        int cur = 0;
-        for (int s = 0; s < total; s++) {
+        for (int j = 0; j < FN; j++) fb[0][j] = *(const lds_i32x4 *)(base + cur + at_b[0] + j * 16 * KSTEP);
+        int s = 0;
+        do {
             multiply(std::integral_constant<int, 0>{}, base + cur);
             // the loads of steps s + 2 ... s + STAGES - 1 may still be on their way (towards the end there are fewer)
             if (STAGES > 2 && s + STAGES - 1 < total) loads_left<(STAGES - 2) * (LA + LB)>();
@@ -202,70 +265,82 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
             reads_done();
             meet();
             const int next = cur + BUF < STAGES * BUF ? cur + BUF : 0;
-            if (tail && s + 2 == total) clear_tail(base + next);
-            if (s + STAGES < total) fetch(lds + cur);
+            if (s == clear_at) clear_tail(base + next);
+            fetch(lds + cur);
             __builtin_amdgcn_sched_barrier(0);
             cur = next;
             multiply(std::integral_constant<int, 1>{}, base + cur);
-        }
-    }
+        } while (++s < total);
 
-    // Epilogue.  b was the first operand, so a lane holds four neighbouring columns n of one row m: written like that, a
-    // store would touch 16 rows with 8 bytes each.  The wave turns its part of the tile round in LDS (its own share, so
-    // one barrier in all) and stores 16 bytes per lane along the rows.  The rows' pitch is 16 bytes off a multiple of
-    // the banks, which spreads the 16 rows of a write over all of them.
-    constexpr int COLS = BN / WN, ROWS = BM / WM, VEC = 16 / sizeof(T), PITCH = COLS * sizeof(T) + 16;
-    constexpr int PART = sizeof(T) == 4 ? 32 : 64, CR = ROWS < PART ? ROWS : PART; // rows that are turned at a time
-    static_assert(WAVES * CR * PITCH <= STAGES * BUF, "the waves' shares fit the buffers");
-    const int first_n = n0 + wn;
-    float sb[FN][4], bias[FN][4];
+        // Epilogue.  b was the first operand, so a lane holds four neighbouring columns n of one row m: written like
+        // that, a store would touch 16 rows with 8 bytes each.  The wave turns its part of the tile round in LDS (its own
+        // share) and stores 16 bytes per lane along the rows.  The 16-byte chunks of a row are permuted by its number,
+        // which spreads the 16 rows of a write over all banks.
+        const int l = again(lane);
+        auto place = [&](int r, int byte) { return r * RB + ((byte / 16 ^ r * RB / 256) & (RB / 16 - 1)) * 16 + byte % 16; };
+        const float bias_f = wide_bias ? __builtin_bit_cast(float, bias_lane)
+                             : p.bias_dtype == REXSC_F16 ? (float)__builtin_bit_cast(f16_t, bias16_lane)
+                                                         : __builtin_bit_cast(float, (int)bias16_lane << 16);
+        const float sb_f = p.b_scale ? __builtin_bit_cast(float, sb_lane) : 1.f;
+        float sa_f[SA], sb[FN][4], bias[FN][4];
 #pragma unroll
-    for (int j = 0; j < FN; j++)
+        for (int i = 0; i < SA; i++) sa_f[i] = p.a_scale ? __builtin_bit_cast(float, sa_lane[i]) : 1.f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int n = first_n + j * 16 + lane / 16 * 4 + e, c = n < p.N ? n : p.N - 1;
-            sb[j][e] = !SPLIT && p.b_scale ? p.b_scale[c] : 1.f;
-            bias[j][e] = !SPLIT && p.bias ? load_any(p.bias, p.bias_dtype, c) : 0.f;
-        }
-    __syncthreads();
-    lds_char *const mine = base + wave * (CR * PITCH);
-    T *const y = (T *)p.y + (SPLIT ? (size_t)share * p.M * p.N : 0);
-    const bool wide = ((size_t)p.N * sizeof(T) % 16 == 0) && ((uintptr_t)y % 16 == 0);
+        for (int j = 0; j < FN; j++)
 #pragma unroll
-    for (int r0 = 0; r0 < ROWS; r0 += CR) {
+            for (int e = 0; e < 4; e++) {
+                const int c = j * 16 + l / 16 * 4 + e;
+                sb[j][e] = __shfl(sb_f, c, 64);
+                bias[j][e] = __shfl(bias_f, c, 64);
+            }
+        if (!STREAM) __syncthreads(); // the buffers are the waves' shares from here on
 #pragma unroll
-        for (int i = 0; i < CR / 16; i++) {
-            const int m = m0 + wm + r0 + i * 16 + lane % 16;
-            const float sa = !SPLIT && p.a_scale ? p.a_scale[m < p.M ? m : p.M - 1] : 1.f;
+        for (int r0 = 0; r0 < ROWS; r0 += CR) {
 #pragma unroll
-            for (int j = 0; j < FN; j++) {
-                typename VecOf<T, 4>::type v;
+            for (int i = 0; i < CR / 16; i++) {
+                const float sa = __shfl(sa_f[(r0 + i * 16) / 64], (r0 + i * 16) % 64 + l % 16, 64);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if constexpr (SPLIT) v[e] = acc[r0 / 16 + i][j][e];
-                    else v[e] = (T)fmaf((float)acc[r0 / 16 + i][j][e] * sa, sb[j][e], bias[j][e]);
+                for (int j = 0; j < FN; j++) {
+                    typename VecOf<T, 4>::type v;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if constexpr (SPLIT) v[e] = acc[r0 / 16 + i][j][e];
+                        else v[e] = (T)fmaf((float)acc[r0 / 16 + i][j][e] * sa, sb[j][e], bias[j][e]);
+                    }
+                    *(__attribute__((address_space(3))) typename VecOf<T, 4>::type *)(mine + place(i * 16 + l % 16, (j * 16 + l / 16 * 4) *
+                                                                                                                  (int)sizeof(T))) = v;
                 }
-                *(__attribute__((address_space(3))) typename VecOf<T, 4>::type *)(mine + (i * 16 + lane % 16) * PITCH +
-                                                                                  (j * 16 + lane / 16 * 4) * (int)sizeof(T)) = v;
             }
-        }
-        const int rows = p.M - (m0 + wm + r0); // of this part, that exist
-        T *out = y + (size_t)(m0 + wm + r0) * p.N + first_n;
-        if (wide) {
+            const int rows = p.M - (first_m + r0) < CR ? p.M - (first_m + r0) : CR; // of this part, that exist
+            T *out = y + (size_t)(first_m + r0) * p.N + first_n;
+            if (wide) {
+                // rows that do not exist lie behind the descriptor's range, and so do a lane's columns if they do not exist
+                constexpr int LANES = RB / 16; // that store a row
+                const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+                    out, 0, rows > 0 && first_n < p.N ? (int)((rows - 1) * pitch + (size_t)(p.N - first_n) * sizeof(T)) : 0, 0x00027000);
+                unsigned to = (unsigned)(l / LANES) * (unsigned)pitch + (unsigned)(l % LANES) * 16;
+                if (first_n + l % LANES * 16 / (int)sizeof(T) >= p.N) to = 0x80000000u;
 #pragma unroll
-            for (int t = 0; t < CR * COLS / VEC / 64; t++) {
-                const int at = t * 64 + lane, r = at / (COLS / VEC), c = at % (COLS / VEC) * VEC;
-                const i32x4 v = *(const lds_i32x4 *)(mine + r * PITCH + c * (int)sizeof(T));
-                if (r < rows && first_n + c < p.N) *(i32x4 *)(out + (size_t)r * p.N + c) = v;
-            }
-        } else {
-            for (int t = 0; t < CR * COLS / 64; t++) {
-                const int at = t * 64 + lane, r = at / COLS, c = at % COLS;
-                if (r < rows && first_n + c < p.N)
-                    out[(size_t)r * p.N + c] = *(const __attribute__((address_space(3))) T *)(mine + r * PITCH + c * (int)sizeof(T));
+                for (int t = 0; t < SHARE / 1024; t++) {
+                    const i32x4 v = *(const lds_i32x4 *)(mine + place(t * (64 / LANES) + l / LANES, l % LANES * 16));
+                    __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, to + (unsigned)(t * (64 / LANES)) * (unsigned)pitch, 0, 0);
+                }
+            } else {
+#pragma nounroll
+                for (int t = 0; t < CR * COLS / 64; t++) {
+                    const int at = t * 64 + l, r = at / COLS, c = at % COLS;
+                    if (r < rows && first_n + c < p.N)
+                        out[(size_t)r * p.N + c] = *(const __attribute__((address_space(3))) T *)(mine + place(r, c * (int)sizeof(T)));
+                }
             }
         }
-    }
+        if (!STREAM) break;
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) acc[i][j] = typename Op::acc{};
+        tile += gridDim.x;
+    } while (tile < all);
 }
 
 // y = (sum of the partial results, in order) * scales + bias; ACC: int or float.  Four elements per thread.
@@ -342,14 +417,15 @@ int launch_one(const TileArgs &p, int splits, void *workspace, hipStream_t strea
 {
     typedef std::conditional_t<std::is_same_v<Op, OpI8>, int, float> ACC;
     const unsigned tiles = (unsigned)(((p.M + BM - 1) / BM) * (int64_t)((p.N + BN - 1) / BN));
+    constexpr bool STREAM = BM == 256;
     if (splits == 1) {
-        hipLaunchKernelGGL((tile_kernel<Op, T, BM, BN, WM, WN, STAGES, false>), dim3(tiles), dim3(WM * WN * 64), 0, stream, p, 1);
+        hipLaunchKernelGGL((tile_kernel<Op, T, BM, BN, WM, WN, STAGES, false, STREAM>), dim3(STREAM && tiles > CUS ? CUS : tiles), dim3(WM * WN * 64), 0, stream, p, 1);
         REXSC_CHECK_HIP(hipGetLastError());
         return REXSC_OK;
     }
     TileArgs q = p;
     q.y = workspace;
-    hipLaunchKernelGGL((tile_kernel<Op, ACC, BM, BN, WM, WN, STAGES, true>), dim3(tiles * splits), dim3(WM * WN * 64), 0, stream, q, splits);
+    hipLaunchKernelGGL((tile_kernel<Op, ACC, BM, BN, WM, WN, STAGES, true, false>), dim3(tiles * splits), dim3(WM * WN * 64), 0, stream, q, splits);
     REXSC_CHECK_HIP(hipGetLastError());
     const size_t all = (size_t)p.M * p.N;
     hipLaunchKernelGGL((join_kernel<ACC, T>), dim3((unsigned)((all + 1023) / 1024)), dim3(256), 0, stream, p, (const ACC *)workspace,

@@ -372,6 +372,31 @@ def test_offsets_behind_32_bits():
         assert torch.equal(q[r].cpu().double(), qe) and torch.equal(s[r].cpu(), se), r
 
 
+@pytest.mark.parametrize("dt,n", [(torch.bfloat16, 4104), (torch.float16, 4101), (torch.float32, 4100), (torch.float32, 4099)])
+@pytest.mark.parametrize("k", [1, 100, 128, 129, 300, 513])
+def test_more_large_tiles_than_blocks(dt, n, k, monkeypatch):
+    """A block goes on from tile to tile: each tile's rows, columns and factors must be its own, whatever the number of
+    steps (one, two, an odd number) and wherever the last tiles end."""
+    import sc_functional as F
+    m = 4353
+    print("tiles", dt, m, n, k, flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(n + k)
+    pitch = max(128, -(-k // 128) * 128)
+    a, b = (torch.randint(-127, 128, (r, pitch), device="cuda", dtype=torch.int8, generator=gen)[:, :k] for r in (m, n))
+    sa, sb = (torch.rand(r, device="cuda", generator=gen) + 0.5 for r in (m, n))
+    bias = torch.randn(n, device="cuda", generator=gen).to(dt)
+    monkeypatch.setenv("REXSC_TUNE_INT8_TILE", "256")
+    y = F.matmul_int8(a, sa, b, sb, bias, out_dtype=dt)
+    prod = (a.double() @ b.double().t().contiguous()) * sa.double()[:, None] * sb.double()
+    want = prod + bias.double()
+    tol = 4 * U * prod.abs() + U * want.abs() + _half(dt) * want.abs() * (1 + 2 ** -8) + _floor(dt) + 2.0 ** -126
+    # what half a step of the type beyond its largest number reaches is rounded to infinity
+    limit = torch.finfo(dt).max * (1 + _half(dt) / 2)
+    over = want.abs() - tol >= limit
+    assert torch.equal(y[over].double(), want[over].sign() * torch.inf)
+    assert (((y.double() - want).abs() <= tol) | (want.abs() + tol >= limit)).all()
+
+
 def test_more_rows_than_blocks():
     import sc_functional as F
     x = torch.randn((1 << 23) + 9, 3, device="cuda", dtype=torch.float16)
