@@ -2,10 +2,11 @@
 //
 // The weights are read once, straight into the matrix instruction's first operand: a load takes 64 bytes of 16 weight
 // rows, two loads of a wave a cache line of each, and the eight waves of a block take neighbouring lines of the same
-// rows, so a row is read in runs of 1024 bytes.  There is nothing to share in LDS (each weight is used by one wave), and nothing to wait for but memory: a
-// wave has UNROLL loads in flight before the first is used.  The waves' int32 sums, exact in any order, are joined
-// through LDS.  With one or two tokens (M K <= 8192) the block takes them to 8 bits itself, while its first weights are on their way:
-// a launch of its own would cost more than every block's reading the few kilobytes again.
+// rows, so a row is read in runs of 1024 bytes.  There is nothing to share in LDS (each weight is used by one wave), and
+// nothing to wait for but memory: a wave has UNROLL loads in flight before the first is used.  The waves' int32 sums,
+// exact in any order, are joined through LDS.  With few tokens (M K <= 8192) the block takes them to 8 bits itself, while
+// its first weights are on their way: a launch of its own would cost more than every block's reading the few kilobytes
+// again.
 // Measured with weights from memory: 1 x 4096 x 4096 5.9 us from int8 tokens, 8.0 us from float ones (with the rows'
 // own launch 9.0); 1 x 16384 x 4096 14.4 us (4.7 TB/s of weights).
 #include <stdlib.h>

@@ -4,7 +4,7 @@
 // direct loads, whole steps ahead, and from there to registers half a step ahead of the matrix instruction.  256 x 256
 // outputs per block of eight waves is the largest tile whose accumulators (128 a lane) leave room for two sets of
 // fragments, and a step of 128 bytes the longest of which two fit LDS; it reads 64 KB from L2 for 8.4 M products.
-// Measured, int8: 8192^3 402-422 us (2.6-2.7 POP/s), 8192 x 16384 x 4096 463-480 us (2.3), 8192 x 4096 x 4096 108-115 us;
+// Measured, int8: 8192^3 398-404 us (2.7 POP/s), 8192 x 16384 x 4096 450-484 us (2.3-2.4), 8192 x 4096 x 4096 108-113 us;
 // the library's int8 product reaches 2.24 POP/s at 8192^3 and 1.85 at 8192 x 16384 x 4096.  binary16, 4096 x 4096 x 8192
 // in two pieces: 400 us (1.37 PFLOP/s).  The matrix pipe is busy 0.69 of the cycles, at 1.8-1.95 GHz.
 #include <stdlib.h>
@@ -105,12 +105,13 @@ __device__ __forceinline__ void tile_of(unsigned bid, int tiles_m, int tiles_n, 
 // SPLIT: the grid holds `splits` times the tiles, and a block sums only its share of the steps, into a partial result
 // of the accumulator's type (T) that join_kernel finishes.
 // STREAM: the grid holds a block per CU, and a block takes every gridDim.x-th tile.  Its steps are one stream over all
-// its tiles: the next tile's first steps are fetched while the last one's are multiplied, and its first fragments wait in
-// registers while the finished tile is stored, from LDS of its own.
+// its tiles: the next tile's first steps are fetched while the last one's are multiplied and while the finished tile is
+// stored, from LDS of its own.  Against a block per tile, in turn: 8192 x 16384 x 4096 468 -> 451 us, 8192 x 4096 x 4096
+// 114 -> 109, 8192 x 16384 x 1024 165 -> 146-153.
 template <typename Op, typename T, int BM, int BN, int WM, int WN, int STAGES, bool SPLIT, bool STREAM>
 __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int splits)
 {
-    static_assert(!(SPLIT && STREAM), "");
+    static_assert(!(SPLIT && STREAM), "a split tile is one of its own");
     constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
     constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES; // loads of 8 rows x 128 bytes per wave and step
     static_assert(LA * WAVES * 8 == BM && LB * WAVES * 8 == BN, "tile rows must divide among the waves");
@@ -146,7 +147,8 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
     for (int i = 0; i < LA; i++) offa[i] = (unsigned)((i * WAVES + wave) * 8 + lane / 8) * (unsigned)p.a_stride + chunk;
 #pragma unroll
     for (int i = 0; i < LB; i++) offb[i] = (unsigned)((i * WAVES + wave) * 8 + lane / 8) * (unsigned)p.b_stride + chunk;
-    const int steps = p.kbytes > KSTEP ? (p.kbytes + KSTEP - 1) / KSTEP : 1, every = steps * p.pieces; // (an empty sum: a step of zeros)
+    const int steps = p.kbytes > KSTEP ? (p.kbytes + KSTEP - 1) / KSTEP : 1; // (an empty sum: a step of zeros)
+    const int every = steps * p.pieces;
     const int begin = SPLIT ? (int)((int64_t)every * share / splits) : 0;
     const int total = (SPLIT ? (int)((int64_t)every * (share + 1) / splits) : every) - begin;
     if constexpr (SPLIT) base_a += (size_t)(begin / steps) * p.piece_stride;
@@ -307,8 +309,8 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
                         if constexpr (SPLIT) v[e] = acc[r0 / 16 + i][j][e];
                         else v[e] = (T)fmaf((float)acc[r0 / 16 + i][j][e] * sa, sb[j][e], bias[j][e]);
                     }
-                    *(__attribute__((address_space(3))) typename VecOf<T, 4>::type *)(mine + place(i * 16 + l % 16, (j * 16 + l / 16 * 4) *
-                                                                                                                  (int)sizeof(T))) = v;
+                    const int to = place(i * 16 + l % 16, (j * 16 + l / 16 * 4) * (int)sizeof(T));
+                    *(__attribute__((address_space(3))) typename VecOf<T, 4>::type *)(mine + to) = v;
                 }
             }
             const int rows = p.M - (first_m + r0) < CR ? p.M - (first_m + r0) : CR; // of this part, that exist
@@ -417,9 +419,10 @@ int launch_one(const TileArgs &p, int splits, void *workspace, hipStream_t strea
 {
     typedef std::conditional_t<std::is_same_v<Op, OpI8>, int, float> ACC;
     const unsigned tiles = (unsigned)(((p.M + BM - 1) / BM) * (int64_t)((p.N + BN - 1) / BN));
-    constexpr bool STREAM = BM == 256;
+    constexpr bool STREAM = BM == 256; // of the smaller ones a CU holds several, which hide each other's ends
     if (splits == 1) {
-        hipLaunchKernelGGL((tile_kernel<Op, T, BM, BN, WM, WN, STAGES, false, STREAM>), dim3(STREAM && tiles > CUS ? CUS : tiles), dim3(WM * WN * 64), 0, stream, p, 1);
+        const unsigned blocks = STREAM && tiles > CUS ? CUS : tiles;
+        hipLaunchKernelGGL((tile_kernel<Op, T, BM, BN, WM, WN, STAGES, false, STREAM>), dim3(blocks), dim3(WM * WN * 64), 0, stream, p, 1);
         REXSC_CHECK_HIP(hipGetLastError());
         return REXSC_OK;
     }
