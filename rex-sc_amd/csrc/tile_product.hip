@@ -6,7 +6,7 @@
 // fragments, and a step of 128 bytes the longest of which two fit LDS; it reads 64 KB from L2 for 8.4 M products.
 // Measured, int8: 8192^3 398-404 us (2.7 POP/s), 8192 x 16384 x 4096 450-484 us (2.3-2.4), 8192 x 4096 x 4096 108-113 us;
 // the library's int8 product reaches 2.24 POP/s at 8192^3 and 1.85 at 8192 x 16384 x 4096.  binary16, 4096 x 4096 x 8192
-// in two pieces: 400 us (1.37 PFLOP/s).  The matrix pipe is busy 0.69 of the cycles, at 1.8-1.95 GHz.
+// in two pieces: 394-407 us (1.35-1.4 PFLOP/s).  The matrix pipe is busy 0.71 of the cycles, at 1.7-1.9 GHz.
 #include <stdlib.h>
 
 #include <type_traits>
