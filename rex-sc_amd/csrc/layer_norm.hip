@@ -4,11 +4,11 @@
 //   dx = r (gw - mean(gw) - h mean(gw h)),  gw = g w, h = (x - mu) r;   dw = sum_rows g h;   db = sum_rows g
 //
 // Bound by memory: forward reads x and writes y, backward reads x and g and writes dx, each once.  A row lives in the
-// registers of TPR threads (16 lanes, a wave, or a block of 256, 512 or 1024), at most 16 elements per thread (backward 32), so the variance
-// is taken around the true mean without a second read.  Blocks are persistent over rows: w and b (forward), w and the
-// two gradient sums (backward) stay in registers from row to row, since re-reading float32 w and b from L2 for every
-// 16-bit row would move more bytes than the row itself.  The next row is loaded before the current one is reduced
-// (where registers allow).
+// registers of TPR threads (16 lanes, a wave, or a block of 256, 512 or 1024), at most 16 elements per thread (backward
+// 32), so the variance is taken around the true mean without a second read.  Blocks are persistent over rows: w and b
+// (forward), w and the two gradient sums (backward) stay in registers from row to row, since re-reading float32 w and b
+// from L2 for every 16-bit row would move more bytes than the row itself.  The next row is loaded before the current one
+// is reduced (where registers allow).
 // Rows longer than 16384 elements take the streaming kernels, which read the row again for each pass (from L2).
 // Measured: 16384 x 8192 bfloat16 forward 99 us (5.4 TB/s), backward 184 + 8 us for the sums (4.4 TB/s of x, g and dx);
 // 524288 x 128 forward 50 us (5.4), backward 88 us; a copy of 1 GiB reaches 5.1 TB/s.
@@ -319,22 +319,25 @@ __global__ __launch_bounds__(CS_COLS * CS_GROUPS) void column_sums_kernel(const 
 {
     __shared__ float lds[CS_GROUPS][CS_COLS + 1];
     const int tx = threadIdx.x % CS_COLS, ty = threadIdx.x / CS_COLS;
-    const size_t c = (size_t)blockIdx.x * CS_COLS + tx;
     void *const dst = blockIdx.y ? out2 : out;
     if (!dst) return;
-    const float *src = part + (blockIdx.y ? cols : 0) + c;
-    float s = 0.f;
-    if (c < cols) {
+    for (size_t c0 = (size_t)blockIdx.x * CS_COLS; c0 < cols; c0 += (size_t)gridDim.x * CS_COLS) {
+        const size_t c = c0 + tx;
+        const float *src = part + (blockIdx.y ? cols : 0) + c;
+        float s = 0.f;
+        if (c < cols) {
 #pragma unroll 8
-        for (size_t r = ty; r < rows; r += CS_GROUPS) s += src[r * ld];
-    }
-    lds[ty][tx] = s;
-    __syncthreads();
-    for (int half = CS_GROUPS / 2; half > 0; half /= 2) {
-        if (ty < half) lds[ty][tx] += lds[ty + half][tx];
+            for (size_t r = ty; r < rows; r += CS_GROUPS) s += src[r * ld];
+        }
+        lds[ty][tx] = s;
+        __syncthreads();
+        for (int half = CS_GROUPS / 2; half > 0; half /= 2) {
+            if (ty < half) lds[ty][tx] += lds[ty + half][tx];
+            __syncthreads();
+        }
+        if (ty == 0 && c < cols) store_any(dst, out_dtype, c, lds[0][tx]);
         __syncthreads();
     }
-    if (ty == 0 && c < cols) store_any(dst, out_dtype, c, lds[0][tx]);
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -419,7 +422,8 @@ template <typename T> void launch_bwd(const NormPlan &pl, const NormParams &p, h
 int bwd_blocks(const rexsc_norm_desc *d)
 {
     if (d->cols <= 1024 * MAX_EPT) return norm_plan(d, false, true).grid;
-    const int64_t shares = d->rows < 64 ? d->rows : 64;
+    int64_t shares = d->rows < 64 ? d->rows : 64;
+    while ((d->cols + 255) / 256 * shares >= 1 << 23) shares /= 2; // a launch has fewer than 2^32 threads
     return (int)shares;
 }
 
@@ -434,7 +438,9 @@ int launch_column_sums(const float *part, size_t rows, size_t cols, size_t ld, v
                        hipStream_t stream)
 {
     ProfScope prof("column_sums", 4.0 * rows * cols * (out && out2 ? 2 : 1), stream);
-    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + CS_COLS - 1) / CS_COLS), out2 ? 2 : 1), dim3(CS_COLS * CS_GROUPS), 0,
+    constexpr size_t MOST = 1u << 20; // blocks; a launch has fewer than 2^32 threads
+    const size_t blocks = (cols + CS_COLS - 1) / CS_COLS;
+    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)(blocks < MOST ? blocks : MOST), out2 ? 2 : 1), dim3(CS_COLS * CS_GROUPS), 0,
                        stream, part, rows, cols, ld, out, out2, out_dtype);
     REXSC_CHECK_HIP(hipGetLastError());
     return REXSC_OK;

@@ -204,6 +204,36 @@ def test_offsets_behind_32_bits():
     assert not dx[6:1000].any()
 
 
+def test_rows_longer_than_a_launch_of_column_sums():
+    """More columns than a launch has 16-column blocks, and so many that the rows' shares of the weight gradients are
+    fewer than the rows."""
+    import sc_functional as F
+    for rows, d in ((2, (1 << 25) + 17), (70, (1 << 25) + 3)):
+        print("rows", rows, d, flush=True)
+        gen = torch.Generator(device="cuda").manual_seed(rows)
+        dt = torch.float32 if rows == 2 else torch.bfloat16
+        x, g = (torch.randn(rows, d, device="cuda", generator=gen).to(dt) for _ in range(2))
+        w, b = (torch.randn(d, device="cuda", generator=gen).requires_grad_() for _ in range(2))
+        x.requires_grad_()
+        y = F.layer_norm(x, w, b)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+        with torch.no_grad():
+            mu = torch.stack([r.double().mean() for r in x])[:, None]
+            var = torch.stack([(r.double() - m).square().mean() for r, m in zip(x, mu)])[:, None]
+            r = (var + 1e-5).rsqrt()
+            depth = d // 1024 + 22
+            for part in (slice(0, 3000), slice(d - 3000, d)):
+                xs, gs, ws = x[:, part].double(), g[:, part].double(), w[part].double()
+                h = (xs - mu) * r
+                e = U * (r * (xs.abs() + mu.abs() + depth) + (depth + 8) * h.abs())  # mean|x| of a normal row is below 1
+                ref = {"y": (h * ws + b[part].double(), e * ws.abs() + 2 * U * (2 * (h * ws).abs() + b[part].double().abs())),
+                       "dw": ((gs * h).sum(0), (gs.abs() * e).sum(0) + (rows + 8) * U * (gs * h).abs().sum(0)),
+                       "db": (gs.sum(0), (rows + 8) * U * gs.abs().sum(0))}
+                for name, got in (("y", y[:, part]), ("dw", dw[part]), ("db", db[part])):
+                    close(got, tuple(t.cpu() for t in ref[name]), got.dtype, "%s %d" % (name, rows))
+        del x, g, y, dx
+
+
 def test_layer():
     from sc_layers import LayerNorm
     import sc_functional as F
