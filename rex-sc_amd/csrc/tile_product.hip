@@ -461,8 +461,10 @@ int launch_tile_product(const TileArgs &p, bool f16, int out_dtype, void *worksp
                     "int8 linear: operand rows of %zu and %zu bytes, at most %zu are supported", p.a_stride, p.b_stride,
                     MAX_ROW_BYTES - 1);
     const TilePlan pl = tile_plan(p.M, p.N, p.kbytes, p.pieces);
-    const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 31) / 32);
-    REXSC_CHECK_ARG(tiles * pl.splits < (1ll << 23), "int8 linear: a result of %d x %d is more than a launch holds", p.M, p.N);
+    // tiles are counted in 32 bits, and a launch has fewer than 2^32 threads (256 x 256 tiles, unsplit: 256 blocks)
+    const int64_t rows = pl.size == 32 ? 64 : pl.size, tiles = ((p.M + rows - 1) / rows) * (((int64_t)p.N + pl.size - 1) / pl.size);
+    REXSC_CHECK_ARG(tiles * pl.splits < (pl.size == 256 && pl.splits == 1 ? 1ll << 31 : 1ll << 23),
+                    "int8 linear: a result of %d x %d is more than a launch holds", p.M, p.N);
     ProfScope prof(name, 2.0 * p.M * p.N * (f16 ? p.kbytes / 2 : p.kbytes) * p.pieces, stream);
     if (f16) REXSC_DTYPE_SWITCH(out_dtype, return (launch_size<OpF16, T>(p, pl, workspace, stream)));
     else REXSC_DTYPE_SWITCH(out_dtype, return (launch_size<OpI8, T>(p, pl, workspace, stream)));

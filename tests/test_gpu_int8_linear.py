@@ -372,6 +372,19 @@ def test_offsets_behind_32_bits():
         assert torch.equal(q[r].cpu().double(), qe) and torch.equal(s[r].cpu(), se), r
 
 
+def test_result_of_more_tiles_than_a_launch_of_small_ones():
+    """131072 x 131104 (34 GB): more 64 x 32 tiles than a launch of them could have."""
+    import sc_functional as F
+    m, n, k = 1 << 17, (1 << 17) + 32, 16
+    a = torch.randint(-128, 128, (m, k), device="cuda", dtype=torch.int8)
+    b = torch.randint(-128, 128, (n, k), device="cuda", dtype=torch.int8)
+    one = torch.ones(n, device="cuda")
+    y = F.matmul_int8(a, one[:m], b, one, None, torch.bfloat16)
+    for r in (0, 255, 256, 65535, 100000, m - 1):
+        want = (a[r].cpu().double() @ b.cpu().double().t()).float().bfloat16()
+        assert torch.equal(y[r].cpu(), want), r
+
+
 @pytest.mark.parametrize("dt,n", [(torch.bfloat16, 4104), (torch.float16, 4101), (torch.float32, 4100), (torch.float32, 4099)])
 @pytest.mark.parametrize("k", [1, 100, 128, 129, 300, 513])
 def test_more_large_tiles_than_blocks(dt, n, k, monkeypatch):
