@@ -47,10 +47,11 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_av
     params, grads: lists of tensors of one type (float32, float16, bfloat16) on one device, each dense in memory and the
     gradient laid out like its parameter.  exp_avgs, exp_avg_sqs: float32 states laid out likewise, or, with the two
     lists of scales, 8-bit ones: float8_e4m3fn tensors of m / scale and sqrt(v) / scale, one float32 scale for each 256
-    elements in memory order.  The tensors of a call do not overlap, and a captured call keeps to theirs.  step: the number of this step, from 1 on; or a device int64 tensor that holds the steps
-    taken, which the call advances on the stream (a captured call needs that).  clamp: (lo, hi) of the updated
-    parameter.  grad_scale, found_inf: float32 device tensors of a gradient scaler, with a device step: gradients are
-    divided by the one, and where the other is not 0 the step is left out."""
+    elements in memory order.  The tensors of a call do not overlap, and a captured call keeps to theirs.  step: the
+    number of this step, from 1 on; or a device int64 tensor that holds the steps taken, which the call advances on the
+    stream (a captured call needs that).  clamp: (lo, hi) of the updated parameter.  grad_scale, found_inf: float32
+    device tensors of a gradient scaler, with a device step: gradients are divided by the one, and where the other is
+    not 0 the step is left out."""
     eight = exp_avg_scales is not None
     lists = [params, grads, exp_avgs, exp_avg_sqs]
     if eight != (exp_avg_sq_scales is not None):
@@ -186,14 +187,16 @@ class AdamW(torch.optim.Optimizer):
                 if group["capturable"]:
                     key = (p.dtype, p.device)
                 else:
-                    state["step"] += 1
+                    state["step"] = int(state["step"]) + 1  # (a tensor's where the group was capturable before)
                     key = (p.dtype, p.device, state["step"])
                 sets.setdefault(key, []).append((p, state))
             for key, members in sets.items():
                 if group["capturable"]:
-                    step = next((s["step"] for _, s in members if "step" in s), None)
-                    if step is None:
-                        step = torch.zeros(1, dtype=torch.int64, device=key[1])
+                    step = next((s["step"] for _, s in members if "step" in s), 0)
+                    if not isinstance(step, torch.Tensor):  # the first step, or a group that was not capturable before
+                        if step and torch.cuda.is_current_stream_capturing():
+                            raise RuntimeError("AdamW: a group that becomes capturable needs an eager step before a captured one")
+                        step = torch.full((1,), step, dtype=torch.int64, device=key[1])
                     for _, s in members:
                         s["step"] = step
                 else:

@@ -320,6 +320,22 @@ def test_optimizer_class_follows_the_function(bits):
         assert again.state[copies[0]]["exp_avg"].dtype == E4M3
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_group_that_becomes_capturable_and_back_keeps_its_count(bits):
+    import sc_optim
+    torch.manual_seed(1)
+    ps, qs = ([torch.nn.Parameter(torch.ones(n, device="cuda")) for n in (300, 7)] for _ in range(2))
+    a, b = (sc_optim.AdamW(v, lr=0.1, state_bits=bits) for v in (ps, qs))
+    for capturable in (False, False, True, True, False, False, True):
+        a.param_groups[0]["capturable"] = capturable
+        for p, q in zip(ps, qs):
+            p.grad = torch.randn_like(p)
+            q.grad = p.grad.clone()
+        a.step(), b.step()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs)), capturable
+    assert all(int(a.state[p]["step"]) == 7 for p in ps)
+
+
 def test_gradient_scaler_leaves_out_a_step_without_a_synchronisation():
     import sc_optim
     p, q = (torch.nn.Parameter(torch.ones(300, device="cuda")) for _ in range(2))
