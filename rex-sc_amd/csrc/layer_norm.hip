@@ -130,7 +130,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_forward_kernel(Nor
     }
 }
 
-template <typename T, int V, int NV, int TPR>
+// RAGGED: rows begin anywhere and end inside a vector.
+template <typename T, int V, int NV, int TPR, bool RAGGED = false>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(NormParams p)
 {
     constexpr int RPB = TPR <= 64 ? 256 / TPR : 1; // rows a block holds at once
@@ -156,8 +157,13 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(No
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (i * TPR + tid) * V;
-            cx[i] = c < p.cols ? *(const vec *)(sx + c) : vec{};
-            cg[i] = c < p.cols ? *(const vec *)(sg + c) : vec{};
+            if constexpr (RAGGED) {
+                cx[i] = load_some<T, V>(sx + c, p.cols - c);
+                cg[i] = load_some<T, V>(sg + c, p.cols - c);
+            } else {
+                cx[i] = c < p.cols ? *(const vec *)(sx + c) : vec{};
+                cg[i] = c < p.cols ? *(const vec *)(sg + c) : vec{};
+            }
         }
     };
     constexpr bool AHEAD = NV * (V == 1 ? 4 : V * sizeof(T)) <= 64; // registers for a row in flight beside the current one
@@ -174,7 +180,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(No
                 float xv, gv;
                 if constexpr (V == 1) { xv = (float)cx[i]; gv = (float)cg[i]; }
                 else { xv = (float)cx[i][j]; gv = (float)cg[i][j]; }
-                h[i][j] = (i * TPR + tid) * V < p.cols ? (xv - mu) * r : 0.f; // beyond the row: g is 0, h must be finite
+                // beyond the row: g is 0, h must be finite
+                h[i][j] = (i * TPR + tid) * V + (RAGGED ? j : 0) < p.cols ? (xv - mu) * r : 0.f;
                 dw[i][j] = fmaf(gv, h[i][j], dw[i][j]);
                 db[i][j] += gv;
                 gw[i][j] = gv * w[i][j];
@@ -194,7 +201,8 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(No
                     float o[V];
 #pragma unroll
                     for (int j = 0; j < V; j++) o[j] = r * (gw[i][j] - m0 - h[i][j] * m1);
-                    store_vec<V>(dst + c, o);
+                    if constexpr (RAGGED) store_some<T, V>(dst + c, o, p.cols - c);
+                    else store_vec<V>(dst + c, o);
                 }
             }
         }
@@ -226,9 +234,9 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(No
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int c = (i * TPR + tid) * V;
-        if (c < p.cols)
 #pragma unroll
-            for (int j = 0; j < V; j++) {
+        for (int j = 0; j < V; j++)
+            if (c + (RAGGED ? j : 0) < p.cols) {
                 out[c + j] = dw[i][j];
                 out[p.cols + c + j] = db[i][j];
             }
@@ -361,9 +369,12 @@ int check_norm(const rexsc_norm_desc *d)
     return REXSC_OK;
 }
 
-// Vectors of 16 bytes where every row starts on one, else single elements; the fewest threads that hold a row at 16
-// elements each.  The backward pass holds a row of more than 8192 in 512 threads at 32 elements: with its five values
-// per element, 1024 threads have too few registers (8192 x 16384 bfloat16: 640 us with them spilled, against 178).
+// Vectors of 16 bytes where every row starts on one, else single elements (vectors that lie anywhere are slower in 16
+// bits: 16388 x 4095 bfloat16 forward 101 us against 60, backward 203 against 102; in float32 the two are alike); the
+// fewest threads that hold a row at 16 elements each.  The backward pass holds a row of more than 8192 in 512 threads at
+// 32 elements: with its five values per element, 1024 threads have too few registers (8192 x 16384 bfloat16: 640 us with
+// them spilled, against 178).  There single elements need too many as well, and vectors that lie anywhere are taken
+// (5591 x 12001 bfloat16: 161 us against 459).
 NormPlan norm_plan(const rexsc_norm_desc *d, bool aligned, bool backward)
 {
     NormPlan pl{};
@@ -401,7 +412,13 @@ void launch_bwd_tpr(const NormPlan &pl, const NormParams &p, hipStream_t s)
     case 64: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 64>), dim3(pl.grid), dim3(256), 0, s, p); break;
     case 256: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 256>), dim3(pl.grid), dim3(256), 0, s, p); break;
     case 512: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 512>), dim3(pl.grid), dim3(512), 0, s, p); break;
-    default: hipLaunchKernelGGL((norm_backward_kernel<T, V, 2 * NV, 512>), dim3(pl.grid), dim3(512), 0, s, p); break;
+    default:
+        if constexpr (V == 1) {
+            constexpr int W = 16 / sizeof(T);
+            hipLaunchKernelGGL((norm_backward_kernel<T, W, 32 / W, 512, true>), dim3(pl.grid), dim3(512), 0, s, p);
+        } else {
+            hipLaunchKernelGGL((norm_backward_kernel<T, V, 2 * NV, 512>), dim3(pl.grid), dim3(512), 0, s, p);
+        }
     }
 }
 #define NORM_NV(FN)                                                                         \

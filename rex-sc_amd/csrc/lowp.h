@@ -21,6 +21,36 @@ inline bool dtype_ok(int dtype) { return dtype == REXSC_F32 || dtype == REXSC_F1
 
 template <typename T, int V> struct VecOf { typedef T type __attribute__((ext_vector_type(V))); };
 template <typename T> struct VecOf<T, 1> { typedef T type; };
+// The same, aligned to its element only: one load or store of as many bytes wherever it lies.
+template <typename T, int V> struct LooseVecOf { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
+
+// The first n of V elements from p on, zeros behind them.
+template <typename T, int V>
+__device__ __forceinline__ typename VecOf<T, V>::type load_some(const T *p, int n)
+{
+    typename VecOf<T, V>::type v{};
+    if (n >= V) v = *(const typename LooseVecOf<T, V>::type *)p;
+    else if (n > 0) {
+#pragma unroll
+        for (int i = 0; i < V - 1; i++)
+            if (i < n) v[i] = p[i];
+    }
+    return v;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_some(T *p, const float (&v)[V], int n)
+{
+    if (n >= V) {
+        typename LooseVecOf<T, V>::type w;
+#pragma unroll
+        for (int i = 0; i < V; i++) w[i] = (T)v[i];
+        *(typename LooseVecOf<T, V>::type *)p = w;
+    } else if (n > 0) {
+#pragma unroll
+        for (int i = 0; i < V - 1; i++)
+            if (i < n) p[i] = (T)v[i];
+    }
+}
 
 // V consecutive elements, widened.  p is aligned to V * sizeof(T).
 template <int V, typename T>
