@@ -4,11 +4,10 @@
 //   dx = r (gw - mean(gw) - h mean(gw h)),  gw = g w, h = (x - mu) r;   dw = sum_rows g h;   db = sum_rows g
 //
 // Bound by memory: forward reads x and writes y, backward reads x and g and writes dx, each once.  A row lives in the
-// registers of TPR threads (16 lanes, a wave, or a block of 256, 512 or 1024), at most 16 elements per thread (backward
-// 32), so the variance is taken around the true mean without a second read.  Blocks are persistent over rows: w and b
-// (forward), w and the two gradient sums (backward) stay in registers from row to row, since re-reading float32 w and b
-// from L2 for every 16-bit row would move more bytes than the row itself.  The next row is loaded before the current one
-// is reduced (where registers allow).
+// registers of TPR threads (16 lanes, a wave, or a block of 128 to 1024), so the variance is taken around the true mean
+// without a second read.  Blocks are persistent over rows: w and b (forward), w and the two gradient sums (backward)
+// stay in registers from row to row, since re-reading float32 w and b from L2 for every 16-bit row would move more bytes
+// than the row itself.  The next row is loaded before the current one is reduced (where registers allow).
 // Rows longer than 16384 elements take the streaming kernels, which read the row again for each pass (from L2).
 // Measured: 16384 x 8192 bfloat16 forward 99 us (5.4 TB/s), backward 184 + 8 us for the sums (4.4 TB/s of x, g and dx);
 // 524288 x 128 forward 50 us (5.4), backward 88 us; a copy of 1 GiB reaches 5.1 TB/s.
@@ -18,7 +17,7 @@
 namespace rexsc {
 namespace {
 
-constexpr int MAX_EPT = 16;         // elements of a row per thread
+constexpr int LONGEST = 1024 * 16;  // row that is held in registers
 constexpr int STREAM_THREADS = 1024;
 
 struct NormParams {
@@ -166,7 +165,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(No
             }
         }
     };
-    constexpr bool AHEAD = NV * (V == 1 ? 4 : V * sizeof(T)) <= 64; // registers for a row in flight beside the current one
+    constexpr bool AHEAD = NV * V * (int)sizeof(T) <= 64; // registers for a row in flight beside the current one
     if (AHEAD && row < p.rows) fetch(row);
     int slot = 0;
     for (; row < p.rows; row += step) {
@@ -222,6 +221,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(No
                 }
         __syncthreads();
         if (sub > 0) return;
+#pragma nounroll
         for (int k = 0; k < RPB - 1; k++)
 #pragma unroll
             for (int i = 0; i < NV; i++)
@@ -370,75 +370,118 @@ int check_norm(const rexsc_norm_desc *d)
 }
 
 // Vectors of 16 bytes where every row starts on one, else single elements (vectors that lie anywhere are slower in 16
-// bits: 16388 x 4095 bfloat16 forward 101 us against 60, backward 203 against 102; in float32 the two are alike); the
-// fewest threads that hold a row at 16 elements each.  The backward pass holds a row of more than 8192 in 512 threads at
-// 32 elements: with its five values per element, 1024 threads have too few registers (8192 x 16384 bfloat16: 640 us with
-// them spilled, against 178).  There single elements need too many as well, and vectors that lie anywhere are taken
-// (5591 x 12001 bfloat16: 161 us against 459).
+// bits: 16388 x 4095 bfloat16 forward 101 us against 60, backward 203 against 102; in float32 the two are alike).
+//
+// A row is held by the fewest threads that have it at 20 elements each (forward in 16 bits 24): rows of a wave need no
+// barrier, and 128 or 256 threads of which a part has nothing still wait for each other.  At 16 elements, bfloat16, the
+// width that has just outgrown a wave took twice as long: 64527 x 1040 backward 175 us against 86, 60952 x 1101 214
+// against 90, 33537 x 2001 137 against 96, 7281 x 9216 forward 80 against 61.  In float32, with half the elements for
+// the same bytes, that gains for a wave only (32263 x 1040 backward 102 us against 85; 16768 x 2001 in 128 threads 89
+// against 86 in 256, 6553 x 5120 forward 54 in 256 against 50 in 512), and forward rows of 8193 to 10240 (3727 x 9001
+// 60 us in 1024 threads, 53 in 512).
+//
+// The backward pass holds a row of more than 8192 in 512 threads at 32 elements: with its five values per element, 1024
+// threads have too few registers (8192 x 16384 bfloat16: 640 us with them spilled, against 178).  There single elements
+// need too many as well, and vectors that lie anywhere are taken (5591 x 12001 bfloat16: 161 us against 459).
 NormPlan norm_plan(const rexsc_norm_desc *d, bool aligned, bool backward)
 {
     NormPlan pl{};
-    const int VMAX = d->dtype == REXSC_F32 ? 4 : 8;
+    const bool f32 = d->dtype == REXSC_F32;
+    const int VMAX = f32 ? 4 : 8, most = f32 || backward ? 20 : 24;
     pl.V = aligned && d->cols % VMAX == 0 && (d->x_stride % VMAX == 0 || d->rows <= 1) ? VMAX : 1;
-    pl.TPR = d->cols <= 16 * MAX_EPT ? 16 : d->cols <= 64 * MAX_EPT ? 64 : d->cols <= 256 * MAX_EPT ? 256 : d->cols <= 512 * MAX_EPT ? 512
-           : d->cols <= 1024 * MAX_EPT ? 1024 : 0;
+    pl.TPR = d->cols <= 16 * 16                        ? 16
+             : d->cols <= 64 * most                    ? 64
+             : d->cols <= 128 * most && !f32           ? 128
+             : d->cols <= 256 * (f32 ? 16 : most)      ? 256
+             : d->cols <= 512 * (backward ? 16 : most) ? 512
+             : d->cols <= LONGEST                      ? 1024
+                                                       : 0;
     const int64_t rpb = pl.TPR && pl.TPR <= 64 ? 256 / pl.TPR : 1;
     const int threads = pl.TPR == 0 ? STREAM_THREADS : pl.TPR <= 64 ? 256 : pl.TPR == 1024 && backward ? 512 : pl.TPR;
-    const int64_t most = 256 * (int64_t)(backward ? BWD_WAVES : FWD_WAVES) * 64 / threads, want = (d->rows + rpb - 1) / rpb;
-    pl.grid = (int)(want < most ? want : most);
+    const int64_t full = 256 * (int64_t)(backward ? BWD_WAVES : FWD_WAVES) * 64 / threads, want = (d->rows + rpb - 1) / rpb;
+    pl.grid = (int)(want < full ? want : full);
     if (pl.TPR) {
-        const int64_t ept = (d->cols + pl.TPR - 1) / pl.TPR;
-        pl.NV = pl.V == 8 ? (ept <= 8 ? 1 : 2) : pl.V == 4 ? (ept <= 8 ? 2 : 4) : (ept <= 4 ? 4 : 16);
+        const int ept = (int)((d->cols + pl.TPR - 1) / pl.TPR);
+        pl.NV = pl.V > 1 ? (ept + pl.V - 1) / pl.V : (ept + 3) / 4 * 4;
     }
     return pl;
 }
 
-template <typename T, int V, int NV>
-void launch_fwd_tpr(const NormPlan &pl, const NormParams &p, hipStream_t s)
+// The numbers of threads per row that come with room for EPT elements in each, see norm_plan.
+constexpr bool takes(int tpr, int ept, bool f32)
 {
-    switch (pl.TPR) {
-    case 16: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 16>), dim3(pl.grid), dim3(256), 0, s, p); break;
-    case 64: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 64>), dim3(pl.grid), dim3(256), 0, s, p); break;
-    case 256: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 256>), dim3(pl.grid), dim3(256), 0, s, p); break;
-    case 512: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 512>), dim3(pl.grid), dim3(512), 0, s, p); break;
-    default: hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, 1024>), dim3(pl.grid), dim3(1024), 0, s, p); break;
+    return tpr == 16     ? ept <= 16
+           : tpr == 64   ? ept > 4
+           : tpr == 128  ? ept > 8 && !f32
+           : tpr == 256  ? ept > 4 && (ept <= 16 || !f32)
+           : tpr == 512  ? ept > 8
+                         : ept > 8 && ept <= 16;
+}
+template <typename T, int V, int NV, int TPR>
+bool launch_fwd_if(const NormPlan &pl, const NormParams &p, hipStream_t s)
+{
+    if constexpr (takes(TPR, V * NV, sizeof(T) == 4)) {
+        if (pl.TPR != TPR) return false;
+        hipLaunchKernelGGL((norm_forward_kernel<T, V, NV, TPR>), dim3(pl.grid), dim3(TPR <= 64 ? 256 : TPR), 0, s, p);
+        return true;
     }
+    return false;
+}
+template <typename T, int V, int NV, int TPR>
+bool launch_bwd_if(const NormPlan &pl, const NormParams &p, hipStream_t s)
+{
+    if constexpr (takes(TPR, V * NV, sizeof(T) == 4) && (TPR < 512 || V * NV <= 16)) {
+        if (pl.TPR != TPR) return false;
+        hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, TPR>), dim3(pl.grid), dim3(TPR <= 64 ? 256 : TPR), 0, s, p);
+        return true;
+    }
+    return false;
 }
 template <typename T, int V, int NV>
-void launch_bwd_tpr(const NormPlan &pl, const NormParams &p, hipStream_t s)
+bool launch_fwd_tpr(const NormPlan &pl, const NormParams &p, hipStream_t s)
 {
-    switch (pl.TPR) {
-    case 16: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 16>), dim3(pl.grid), dim3(256), 0, s, p); break;
-    case 64: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 64>), dim3(pl.grid), dim3(256), 0, s, p); break;
-    case 256: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 256>), dim3(pl.grid), dim3(256), 0, s, p); break;
-    case 512: hipLaunchKernelGGL((norm_backward_kernel<T, V, NV, 512>), dim3(pl.grid), dim3(512), 0, s, p); break;
-    default:
-        if constexpr (V == 1) {
-            constexpr int W = 16 / sizeof(T);
-            hipLaunchKernelGGL((norm_backward_kernel<T, W, 32 / W, 512, true>), dim3(pl.grid), dim3(512), 0, s, p);
-        } else {
-            hipLaunchKernelGGL((norm_backward_kernel<T, V, 2 * NV, 512>), dim3(pl.grid), dim3(512), 0, s, p);
-        }
-    }
+    return launch_fwd_if<T, V, NV, 16>(pl, p, s) || launch_fwd_if<T, V, NV, 64>(pl, p, s) || launch_fwd_if<T, V, NV, 128>(pl, p, s) ||
+           launch_fwd_if<T, V, NV, 256>(pl, p, s) || launch_fwd_if<T, V, NV, 512>(pl, p, s) || launch_fwd_if<T, V, NV, 1024>(pl, p, s);
+}
+template <typename T, int V, int NV>
+bool launch_bwd_tpr(const NormPlan &pl, const NormParams &p, hipStream_t s)
+{
+    return launch_bwd_if<T, V, NV, 16>(pl, p, s) || launch_bwd_if<T, V, NV, 64>(pl, p, s) || launch_bwd_if<T, V, NV, 128>(pl, p, s) ||
+           launch_bwd_if<T, V, NV, 256>(pl, p, s) || launch_bwd_if<T, V, NV, 512>(pl, p, s);
 }
 #define NORM_NV(FN)                                                                         \
     do {                                                                                    \
         if constexpr (sizeof(T) == 4) {                                                     \
+            if (pl.V == 4 && pl.NV == 1) return FN<T, 4, 1>(pl, p, s);                      \
             if (pl.V == 4 && pl.NV == 2) return FN<T, 4, 2>(pl, p, s);                      \
-            if (pl.V == 4) return FN<T, 4, 4>(pl, p, s);                                    \
+            if (pl.V == 4 && pl.NV == 3) return FN<T, 4, 3>(pl, p, s);                      \
+            if (pl.V == 4 && pl.NV == 4) return FN<T, 4, 4>(pl, p, s);                      \
+            if (pl.V == 4) return FN<T, 4, 5>(pl, p, s);                                    \
         } else {                                                                            \
             if (pl.V == 8 && pl.NV == 1) return FN<T, 8, 1>(pl, p, s);                      \
-            if (pl.V == 8) return FN<T, 8, 2>(pl, p, s);                                    \
+            if (pl.V == 8 && pl.NV == 2) return FN<T, 8, 2>(pl, p, s);                      \
+            if (pl.V == 8) return FN<T, 8, 3>(pl, p, s);                                    \
+            if (pl.NV == 24) return FN<T, 1, 24>(pl, p, s);                                 \
         }                                                                                   \
         if (pl.NV == 4) return FN<T, 1, 4>(pl, p, s);                                       \
-        return FN<T, 1, 16>(pl, p, s);                                                      \
+        if (pl.NV == 8) return FN<T, 1, 8>(pl, p, s);                                       \
+        if (pl.NV == 12) return FN<T, 1, 12>(pl, p, s);                                     \
+        if (pl.NV == 16) return FN<T, 1, 16>(pl, p, s);                                     \
+        return FN<T, 1, 20>(pl, p, s);                                                      \
     } while (0)
-template <typename T> void launch_fwd(const NormPlan &pl, const NormParams &p, hipStream_t s) { NORM_NV(launch_fwd_tpr); }
-template <typename T> void launch_bwd(const NormPlan &pl, const NormParams &p, hipStream_t s) { NORM_NV(launch_bwd_tpr); }
+template <typename T> bool launch_fwd(const NormPlan &pl, const NormParams &p, hipStream_t s) { NORM_NV(launch_fwd_tpr); }
+template <typename T> bool launch_bwd(const NormPlan &pl, const NormParams &p, hipStream_t s)
+{
+    constexpr int W = 16 / sizeof(T);
+    if (pl.TPR < 1024) NORM_NV(launch_bwd_tpr);
+    if (pl.V > 1) hipLaunchKernelGGL((norm_backward_kernel<T, W, 32 / W, 512>), dim3(pl.grid), dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((norm_backward_kernel<T, W, 32 / W, 512, true>), dim3(pl.grid), dim3(512), 0, s, p);
+    return true;
+}
 
 int bwd_blocks(const rexsc_norm_desc *d)
 {
-    if (d->cols <= 1024 * MAX_EPT) return norm_plan(d, false, true).grid;
+    if (d->cols <= LONGEST) return norm_plan(d, false, true).grid;
     int64_t shares = d->rows < 64 ? d->rows : 64;
     while ((d->cols + 255) / 256 * shares >= 1 << 23) shares /= 2; // a launch has fewer than 2^32 threads
     return (int)shares;
@@ -485,7 +528,7 @@ extern "C" int rexsc_layer_norm_forward(const rexsc_norm_desc *d, const void *x,
         REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL(norm_forward_stream_kernel<T>, dim3(pl.grid), dim3(STREAM_THREADS), 0,
                                                         stream, p));
     else
-        REXSC_DTYPE_SWITCH(d->dtype, launch_fwd<T>(pl, p, stream));
+        REXSC_DTYPE_SWITCH(d->dtype, REXSC_CHECK_ARG(launch_fwd<T>(pl, p, stream), "layer norm: no kernel for rows of %d", p.cols));
     REXSC_CHECK_HIP(hipGetLastError());
     return REXSC_OK;
 }
@@ -531,7 +574,7 @@ extern "C" int rexsc_layer_norm_backward(const rexsc_norm_desc *d, const void *g
                                                                 dim3((unsigned)((cols + 255) / 256), blocks), dim3(256), 0,
                                                                 stream, p));
         } else {
-            REXSC_DTYPE_SWITCH(d->dtype, launch_bwd<T>(pl, p, stream));
+            REXSC_DTYPE_SWITCH(d->dtype, REXSC_CHECK_ARG(launch_bwd<T>(pl, p, stream), "layer norm: no kernel for rows of %d", p.cols));
         }
         REXSC_CHECK_HIP(hipGetLastError());
     }

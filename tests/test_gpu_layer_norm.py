@@ -82,6 +82,13 @@ def test_forward_and_gradients(dt, wdt, rows, d):
     assert torch.equal(F.layer_norm(x.cuda(), w.cuda(), b.cuda()), y.detach())
 
 
+@pytest.mark.parametrize("dt,wdt", [(torch.float32, torch.float32), (torch.float16, torch.float32), (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("d", [256, 257, 264, 1032, 1101, 1280, 1281, 1288, 1536, 1537, 2001, 2560, 2561, 2568, 3060, 3080, 4104,
+                               5120, 5121, 5128, 6144, 6145, 8193, 8200, 9001, 10240, 10241, 12001, 12288, 12289, 16383])
+def test_widths_around_the_numbers_of_threads(dt, wdt, d):
+    test_forward_and_gradients(dt, wdt, 3, d)
+
+
 @pytest.mark.parametrize("d", [48, 1003, 5000])
 def test_without_weight_or_bias_and_partial_gradients(d):
     import sc_functional as F
