@@ -10,6 +10,8 @@
 // makes both gradients the same product of two row-major operands as the forward pass.
 #include <stdlib.h>
 
+#include <type_traits>
+
 #include "few_rows.h"
 #include "profile.h"
 #include "quant8.h"
@@ -21,11 +23,13 @@ namespace {
 constexpr int MAX_K = 131071; // 128 * 128 * K < 2^31
 
 // ---- rows to 8 bits ------------------------------------------------------------------------------
-// Bound by memory: x is read once.  A row lives in the registers of TPR threads (a wave, or a block of 256 or 1024), 16
-// elements a thread at most, all its loads in flight together; rows longer than 16384 are read twice.  8192 x 4096
-// bfloat16: 24 us (4.2 TB/s of reads and writes); one row of 4096: 3 us, the launch and one round trip to memory.
-constexpr int Q_EPT = 16;
-
+// Bound by memory: x is read once, in vectors of 16 bytes wherever they lie (RAGGED: rows that begin anywhere and end
+// inside one).  A row lives in the registers of TPR threads, all its loads in flight together; rows longer than 16384 are
+// read twice.  8192 x 4096 bfloat16: 24 us (4.2 TB/s of reads and writes); one row of 4096: 3 us, the launch and one round
+// trip to memory.  Single elements take longer where rows are not aligned, most of it for storing single bytes (bfloat16
+// 16376 x 4098 193 us against 48, float32 72 against 28).  TPR is the smallest number with at most 24 elements a thread:
+// with more threads, of which a part has nothing, all wait for each other (at 16 elements: 43690 x 1536 bfloat16 55 us
+// against 35, 13107 x 5120 71 against 34; 65536 x 100 in a wave each 22, in 16 lanes 11).
 struct QuantArgs {
     const void *x;
     int8_t *q;
@@ -38,7 +42,12 @@ struct QuantArgs {
 template <int TPR>
 __device__ __forceinline__ unsigned row_top(unsigned t, unsigned (&lds)[16])
 {
-    t = wave_max(t);
+    if constexpr (TPR < 64) {
+#pragma unroll
+        for (int s = TPR / 2; s; s >>= 1) t = max(t, (unsigned)__shfl_xor((int)t, s, 64));
+    } else {
+        t = wave_max(t);
+    }
     if constexpr (TPR > 64) {
         if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = t;
         __syncthreads();
@@ -48,21 +57,22 @@ __device__ __forceinline__ unsigned row_top(unsigned t, unsigned (&lds)[16])
     return t;
 }
 
-template <typename T, int V, int TPR>
-__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void quantize_rows_kernel(QuantArgs p)
+template <typename T, int NV, int TPR, bool RAGGED>
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void quantize_rows_kernel(QuantArgs p)
 {
-    constexpr int NV = Q_EPT / V, RPB = TPR == 64 ? 4 : 1;
+    constexpr int V = 16 / sizeof(T), RPB = TPR <= 64 ? 256 / TPR : 1;
     typedef typename VecOf<T, V>::type vec;
     __shared__ unsigned lds[2][16];
-    const int tid = TPR == 64 ? threadIdx.x % 64 : threadIdx.x;
+    const int tid = TPR <= 64 ? threadIdx.x % TPR : threadIdx.x;
     int slot = 0;
-    for (size_t row = (size_t)blockIdx.x * RPB + (TPR == 64 ? threadIdx.x / 64 : 0); row < p.rows; row += (size_t)gridDim.x * RPB) {
+    for (size_t row = (size_t)blockIdx.x * RPB + (TPR <= 64 ? threadIdx.x / TPR : 0); row < p.rows; row += (size_t)gridDim.x * RPB) {
         const T *src = (const T *)p.x + row * p.x_stride;
         vec v[NV];
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (i * TPR + tid) * V;
-            v[i] = c < p.cols ? *(const vec *)(src + c) : vec{};
+            if constexpr (RAGGED) v[i] = load_some<T, V>(src + c, p.cols - c);
+            else v[i] = c < p.cols ? *(const vec *)(src + c) : vec{};
         }
         float x[NV][V];
         unsigned t = 0;
@@ -70,8 +80,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void quantize_rows_kernel(Qu
         for (int i = 0; i < NV; i++)
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                if constexpr (V == 1) x[i][j] = (float)v[i];
-                else x[i][j] = (float)v[i][j];
+                x[i][j] = (float)v[i][j];
                 t = max(t, mag_bits(x[i][j]));
             }
         const RowScale rs = row_scale(row_top<TPR>(t, lds[slot]));
@@ -81,11 +90,9 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void quantize_rows_kernel(Qu
         for (int i = 0; i < NV; i++) {
             const int c = (i * TPR + tid) * V;
             if (c < p.cols) {
-                typename VecOf<int8_t, V>::type q;
-                if constexpr (V == 1) q = (int8_t)quant8(x[i][0], rs);
-                else
+                typename VecOf<int8_t, V>::type q; // zeros behind the row's end, within its padding
 #pragma unroll
-                    for (int j = 0; j < V; j++) q[j] = (int8_t)quant8(x[i][j], rs);
+                for (int j = 0; j < V; j++) q[j] = (int8_t)quant8(x[i][j], rs);
                 *(typename VecOf<int8_t, V>::type *)(dst + c) = q;
             }
         }
@@ -111,27 +118,51 @@ __global__ __launch_bounds__(1024) void quantize_long_rows_kernel(QuantArgs p)
     }
 }
 
-template <typename T, int V>
-void launch_quantize_v(const QuantArgs &p, hipStream_t s)
+template <typename T, int NV, bool RAGGED>
+void launch_quantize_nv(const QuantArgs &p, int tpr, hipStream_t s)
 {
+    constexpr int EPT = NV * (16 / sizeof(T));
     constexpr size_t MOST = 1u << 21; // blocks; a launch has fewer than 2^32 threads
-    const unsigned rows = (unsigned)(p.rows < MOST ? p.rows : MOST);
-    if (p.cols <= 64 * Q_EPT)
-        hipLaunchKernelGGL((quantize_rows_kernel<T, V, 64>), dim3((unsigned)((p.rows + 3) / 4 < MOST ? (p.rows + 3) / 4 : MOST)), dim3(256),
-                           0, s, p);
-    else if (p.cols <= 256 * Q_EPT) hipLaunchKernelGGL((quantize_rows_kernel<T, V, 256>), dim3(rows), dim3(256), 0, s, p);
-    else if (p.cols <= 1024 * Q_EPT) hipLaunchKernelGGL((quantize_rows_kernel<T, V, 1024>), dim3(rows), dim3(1024), 0, s, p);
-    else hipLaunchKernelGGL(quantize_long_rows_kernel<T>, dim3(rows), dim3(1024), 0, s, p);
+    const size_t rpb = tpr <= 64 ? 256 / tpr : 1, want = (p.rows + rpb - 1) / rpb;
+    const dim3 blocks((unsigned)(want < MOST ? want : MOST));
+    if (tpr == 64) hipLaunchKernelGGL((quantize_rows_kernel<T, NV, 64, RAGGED>), blocks, dim3(256), 0, s, p);
+    if constexpr (EPT <= 16) {
+        if (tpr == 16) hipLaunchKernelGGL((quantize_rows_kernel<T, NV, 16, RAGGED>), blocks, dim3(256), 0, s, p);
+    }
+    if constexpr (EPT > 8) {
+        if (tpr == 128) hipLaunchKernelGGL((quantize_rows_kernel<T, NV, 128, RAGGED>), blocks, dim3(128), 0, s, p);
+        if (tpr == 256) hipLaunchKernelGGL((quantize_rows_kernel<T, NV, 256, RAGGED>), blocks, dim3(256), 0, s, p);
+        if (tpr == 512) hipLaunchKernelGGL((quantize_rows_kernel<T, NV, 512, RAGGED>), blocks, dim3(512), 0, s, p);
+    }
+    if constexpr (EPT == 16) {
+        if (tpr == 1024) hipLaunchKernelGGL((quantize_rows_kernel<T, NV, 1024, RAGGED>), blocks, dim3(1024), 0, s, p);
+    }
 }
 
-// Vectors of 16 bytes where every row of x starts on one (and its int8 row, a multiple of 16 bytes, on V).
 template <typename T>
 void launch_quantize_t(const QuantArgs &p, hipStream_t s)
 {
     constexpr int V = 16 / sizeof(T);
-    const bool aligned = (uintptr_t)p.x % 16 == 0 && p.cols % V == 0 && (p.x_stride % V == 0 || p.rows == 1);
-    if (aligned) launch_quantize_v<T, V>(p, s);
-    else launch_quantize_v<T, 1>(p, s);
+    if (p.cols > 1024 * 16) {
+        constexpr size_t MOST = 1u << 21;
+        hipLaunchKernelGGL(quantize_long_rows_kernel<T>, dim3((unsigned)(p.rows < MOST ? p.rows : MOST)), dim3(1024), 0, s, p);
+        return;
+    }
+    const int tpr = p.cols <= 16 * 16    ? 16
+                    : p.cols <= 64 * 24  ? 64
+                    : p.cols <= 128 * 24 ? 128
+                    : p.cols <= 256 * 24 ? 256
+                    : p.cols <= 512 * 24 ? 512
+                                         : 1024;
+    const int ept = (p.cols + tpr - 1) / tpr;
+    auto launch = [&](auto nv) {
+        constexpr int NV = nv;
+        if ((uintptr_t)p.x % 16 == 0 && p.cols % V == 0 && (p.x_stride % V == 0 || p.rows == 1)) launch_quantize_nv<T, NV, false>(p, tpr, s);
+        else launch_quantize_nv<T, NV, true>(p, tpr, s);
+    };
+    if (ept <= 8) launch(std::integral_constant<int, 8 / V>{});
+    else if (ept <= 16) launch(std::integral_constant<int, 16 / V>{});
+    else launch(std::integral_constant<int, 24 / V>{});
 }
 
 // ---- operands of the gradients ---------------------------------------------------------------------

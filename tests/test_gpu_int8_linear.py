@@ -60,6 +60,26 @@ def test_quantize_rows_is_exact(dt, rows, k):
     assert not pad.any(), "the rows' padding is not zero"
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("k", [4, 8, 31, 255, 256, 257, 264, 520, 1101, 1536, 1537, 1544, 2001, 3060, 3080, 4098, 5001, 6144, 6145,
+                               6152, 8193, 9001, 12288, 12289, 12296, 16383])
+def test_quantize_rows_around_the_numbers_of_threads(dt, k):
+    """Also of a matrix inside another one: rows that begin anywhere, beside elements that must not be read as theirs."""
+    import sc_functional as F
+    print("quantize", dt, k, flush=True)
+    g = torch.Generator().manual_seed(k)
+    whole = torch.randn(19, k + 11, generator=g).to(dt)
+    whole[:, :3] = 1e4
+    whole[:, k + 3:] = -1e4
+    gpu = whole.cuda()
+    for x, y in ((whole[:, 3:k + 3], gpu[:, 3:k + 3]), (whole[:, 8:].contiguous(), gpu[:, 8:].contiguous())):
+        q, s = F.quantize_rows(y)
+        qe, se = quantised(x)
+        assert torch.equal(q.cpu().double(), qe) and torch.equal(s.cpu(), se)
+        pad = q.as_strided((19, q.stride(0)), (q.stride(0), 1))[:, y.shape[1]:]
+        assert not pad.any(), "the rows' padding is not zero"
+
+
 def test_quantize_rows_ties_and_extremes():
     import sc_functional as F
     # max 127: 127 x / max = x, so every half-integer is a tie
