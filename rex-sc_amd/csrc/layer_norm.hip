@@ -200,8 +200,14 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(No
                     float o[V];
 #pragma unroll
                     for (int j = 0; j < V; j++) o[j] = r * (gw[i][j] - m0 - h[i][j] * m1);
-                    if constexpr (RAGGED) store_some<T, V>(dst + c, o, p.cols - c);
-                    else store_vec<V>(dst + c, o);
+                    if constexpr (RAGGED) {
+                        vec t;
+#pragma unroll
+                        for (int j = 0; j < V; j++) t[j] = (T)o[j];
+                        store_some<T, V>(dst + c, t, p.cols - c);
+                    } else {
+                        store_vec<V>(dst + c, o);
+                    }
                 }
             }
         }

@@ -38,17 +38,13 @@ __device__ __forceinline__ typename VecOf<T, V>::type load_some(const T *p, int 
     return v;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_some(T *p, const float (&v)[V], int n)
+__device__ __forceinline__ void store_some(T *p, typename VecOf<T, V>::type v, int n)
 {
-    if (n >= V) {
-        typename LooseVecOf<T, V>::type w;
-#pragma unroll
-        for (int i = 0; i < V; i++) w[i] = (T)v[i];
-        *(typename LooseVecOf<T, V>::type *)p = w;
-    } else if (n > 0) {
+    if (n >= V) *(typename LooseVecOf<T, V>::type *)p = v;
+    else if (n > 0) {
 #pragma unroll
         for (int i = 0; i < V - 1; i++)
-            if (i < n) p[i] = (T)v[i];
+            if (i < n) p[i] = v[i];
     }
 }
 

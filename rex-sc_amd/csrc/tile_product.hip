@@ -328,11 +328,14 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
                     __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, to + (unsigned)(t * (64 / LANES)) * (unsigned)pitch, 0, 0);
                 }
             } else {
+                // the same wherever the rows begin; the vector that a row's end cuts is stored by elements
+                constexpr int LANES = RB / 16, VEC = 16 / sizeof(T);
+                const int left = p.N - first_n - l % LANES * VEC;
 #pragma nounroll
-                for (int t = 0; t < CR * COLS / 64; t++) {
-                    const int at = t * 64 + l, r = at / COLS, c = at % COLS;
-                    if (r < rows && first_n + c < p.N)
-                        out[(size_t)r * p.N + c] = *(const __attribute__((address_space(3))) T *)(mine + place(r, c * (int)sizeof(T)));
+                for (int t = 0; t < SHARE / 1024; t++) {
+                    const int r = t * (64 / LANES) + l / LANES;
+                    const i32x4 v = *(const lds_i32x4 *)(mine + place(r, l % LANES * 16));
+                    if (r < rows) store_some<T, VEC>(out + (size_t)r * p.N + l % LANES * VEC, __builtin_bit_cast(typename VecOf<T, VEC>::type, v), left);
                 }
             }
         }
