@@ -27,7 +27,7 @@ constexpr int MAX_K = 131071; // 128 * 128 * K < 2^31
 // inside one).  A row lives in the registers of TPR threads, all its loads in flight together; rows longer than 16384 are
 // read twice.  8192 x 4096 bfloat16: 24 us (4.2 TB/s of reads and writes); one row of 4096: 3 us, the launch and one round
 // trip to memory.  Single elements take longer where rows are not aligned, most of it for storing single bytes (bfloat16
-// 16376 x 4098 193 us against 48, float32 72 against 28).  TPR is the smallest number with at most 24 elements a thread:
+// 16376 x 4098 193 us against 46, float32 72 against 28).  TPR is the smallest number with at most 24 elements a thread:
 // with more threads, of which a part has nothing, all wait for each other (at 16 elements: 43690 x 1536 bfloat16 55 us
 // against 35, 13107 x 5120 71 against 34; 65536 x 100 in a wave each 22, in 16 lanes 11).
 struct QuantArgs {
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void quantize_rows_kernel(Qu
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (i * TPR + tid) * V;
-            if constexpr (RAGGED) v[i] = load_some<T, V>(src + c, p.cols - c);
+            if constexpr (RAGGED) v[i] = load_some<T, V>(src + c, p.cols - c, c);
             else v[i] = c < p.cols ? *(const vec *)(src + c) : vec{};
         }
         float x[NV][V];
@@ -213,29 +213,41 @@ __device__ __forceinline__ void split(float v, unsigned top, int e, f16_t &high,
     low = (f16_t)(t - (float)high);
 }
 
-// V elements of a row of g times their channels' scales.
-template <int V, typename T>
-__device__ __forceinline__ void load_scaled(float (&v)[V], const T *g, const float *scale)
+// The first n of V = 16 / sizeof(T) elements of a row from its element c on, zeros behind them.  RAGGED: they lie
+// anywhere, and n may be less than V; else n is at least V or at most 0.
+template <bool RAGGED, typename T, int V>
+__device__ __forceinline__ void load_row(float (&v)[V], const T *row, int c, int n)
 {
-    load_vec<V>(v, g);
+    typename VecOf<T, V>::type u{};
+    if constexpr (RAGGED) u = load_some<T, V>(row + c, n, c);
+    else if (n > 0) u = *(const typename VecOf<T, V>::type *)(row + c);
 #pragma unroll
-    for (int i = 0; i < V; i += V < 4 ? V : 4) {
-        float s[V < 4 ? V : 4];
-        load_vec<(V < 4 ? V : 4)>(s, scale + i);
+    for (int j = 0; j < V; j++) v[j] = (float)u[j];
+}
+// The same of a row of g times their channels' scales.
+template <bool RAGGED, typename T, int V>
+__device__ __forceinline__ void load_scaled(float (&v)[V], const T *g, const float *scale, int c, int n)
+{
+    load_row<RAGGED>(v, g, c, n);
 #pragma unroll
-        for (int j = 0; j < (V < 4 ? V : 4); j++) v[i + j] *= s[j];
+    for (int i = 0; i < V; i += 4) {
+        float s[4];
+        load_row<RAGGED>(s, scale, c + i, n - i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[i + j] *= s[j];
     }
 }
 
-template <typename T, int V>
+template <typename T, bool RAGGED>
 __device__ void split_row(const OperandArgs &p, size_t row, unsigned (&lds)[16])
 {
+    constexpr int V = 16 / sizeof(T);
     const T *g = (const T *)p.g + row * (size_t)p.N;
     unsigned t = 0;
 #pragma unroll 2
     for (int c = threadIdx.x * V; c < p.N; c += 256 * V) {
         float v[V];
-        load_scaled<V>(v, g + c, p.b_scale + c);
+        load_scaled<RAGGED>(v, g, p.b_scale, c, p.N - c);
 #pragma unroll
         for (int j = 0; j < V; j++) t = max(t, mag_bits(v[j]));
     }
@@ -243,8 +255,8 @@ __device__ void split_row(const OperandArgs &p, size_t row, unsigned (&lds)[16])
     const int e = piece_exponent(t);
     f16_t *high = p.g_rows + row * (size_t)p.ldn, *low = high + (size_t)p.M * p.ldn;
     for (int c = threadIdx.x * V; c < p.ldn; c += 256 * V) { // ldn is a multiple of 64: whole vectors
-        float v[V] = {};
-        if (c < p.N) load_scaled<V>(v, g + c, p.b_scale + c);
+        float v[V];
+        load_scaled<RAGGED>(v, g, p.b_scale, c, p.N - c);
         typename VecOf<f16_t, V>::type h, l;
         f16_t *hp = (f16_t *)&h, *lp = (f16_t *)&l;
 #pragma unroll
@@ -284,19 +296,19 @@ __device__ void transpose_tile(const int8_t *q, size_t stride, int rows, int col
 }
 
 // Sum of g and largest |g * a_scale| of 64 columns over one share of the rows: 64 / V threads across, the rest down.
-template <typename T, int V>
+template <typename T, bool RAGGED>
 __device__ void column_stats(const OperandArgs &p, unsigned block, float (&ls)[32][64], unsigned (&lt)[32][64])
 {
-    constexpr int ACROSS = 64 / V, DOWN = 256 / ACROSS; // 4 to 32 rows at once
+    constexpr int V = 16 / sizeof(T), ACROSS = 64 / V, DOWN = 256 / ACROSS; // 16 or 32 rows at once
     const int share = (int)(block % p.shares), x = threadIdx.x % ACROSS * V, c = (int)(block / p.shares) * 64 + x;
     const int y = threadIdx.x / ACROSS, begin = share * p.share_rows, end = min(p.M, begin + p.share_rows);
     float s[V] = {};
     unsigned t[V] = {};
-    if (c < p.N) // with V > 1, N is a multiple of V
+    if (c < p.N)
 #pragma unroll 4
         for (int m = begin + y; m < end; m += DOWN) {
             float g[V];
-            load_vec<V>(g, (const T *)p.g + (size_t)m * p.N + c);
+            load_row<RAGGED>(g, (const T *)p.g + (size_t)m * p.N, c, p.N - c);
             const float scale = p.a_scale ? p.a_scale[m] : 0.f;
 #pragma unroll
             for (int j = 0; j < V; j++) {
@@ -327,7 +339,7 @@ __device__ void column_stats(const OperandArgs &p, unsigned block, float (&ls)[3
 // All that the gradients' operands need of each other's results is the columns' statistics, so everything else is one
 // launch, told apart by the block's number.  Bound by memory: g twice, int8 in and binary16 out for both transposes, g's
 // rows out; 8192 x 4096 x 4096 with bfloat16 g: 352 MB in 68 us (5.2 TB/s), the second launch 201 MB in 38 us (5.3).
-template <typename T, int V>
+template <typename T, bool RAGGED>
 __global__ __launch_bounds__(256) void operands_kernel(OperandArgs p)
 {
     __shared__ union {
@@ -336,20 +348,20 @@ __global__ __launch_bounds__(256) void operands_kernel(OperandArgs p)
         struct { float s[32][64]; unsigned t[32][64]; } stats;
     } lds;
     unsigned b = blockIdx.x;
-    if (b < p.row_blocks) return split_row<T, V>(p, b, lds.top);
+    if (b < p.row_blocks) return split_row<T, RAGGED>(p, b, lds.top);
     b -= p.row_blocks;
     if (b < p.b_blocks) return transpose_tile(p.b, p.b_stride, p.N, p.K, p.ldn, p.b_t, b, lds.tile);
     b -= p.b_blocks;
     if (b < p.a_blocks) return transpose_tile(p.a, p.a_stride, p.M, p.K, p.ldm, p.a_t, b, lds.tile);
     b -= p.a_blocks;
-    column_stats<T, V>(p, b, lds.stats.s, lds.stats.t);
+    column_stats<T, RAGGED>(p, b, lds.stats.s, lds.stats.t);
 }
 
 // The second launch: pieces of (g * a_scale) transposed, a 64 x 64 tile per block, and db from the shares' sums.
-template <typename T, int V>
+template <typename T, bool RAGGED>
 __global__ __launch_bounds__(256) void transposed_pieces_kernel(OperandArgs p)
 {
-    constexpr int ACROSS = 64 / V, DOWN = 256 / ACROSS;
+    constexpr int V = 16 / sizeof(T), ACROSS = 64 / V, DOWN = 256 / ACROSS;
     __shared__ float tile[64][65];
     __shared__ unsigned tops[4][64];
     __shared__ float sums[4][64];
@@ -357,8 +369,8 @@ __global__ __launch_bounds__(256) void transposed_pieces_kernel(OperandArgs p)
 #pragma unroll
     for (int i = 0; i < 64; i += DOWN) {
         const int r = i + threadIdx.x / ACROSS, m = m0 + r, c = threadIdx.x % ACROSS * V;
-        float v[V] = {};
-        if (m < p.M && n0 + c < p.N) load_vec<V>(v, (const T *)p.g + (size_t)m * p.N + n0 + c);
+        float v[V];
+        load_row<RAGGED>(v, (const T *)p.g + (size_t)m * p.N, n0 + c, m < p.M ? p.N - n0 - c : 0);
         const float scale = m < p.M ? p.a_scale[m] : 0.f;
 #pragma unroll
         for (int j = 0; j < V; j++) tile[r][c + j] = v[j] * scale;
@@ -615,7 +627,8 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
     p.b_blocks = dx ? (unsigned)(tiles_n * tiles_k) : 0;
     p.a_blocks = dw ? (unsigned)(tiles_m * tiles_k) : 0;
     p.stat_blocks = dw || db ? (unsigned)(p.shares * tiles_n) : 0;
-    // vectors of 16 bytes where every row of g starts on one (and the channels' scales)
+    // whether every row of g starts on a vector of 16 bytes, and the channels' scales (8192 tokens, 4095 channels, bfloat16, by single
+    // elements: 99 and 62 us for both launches, in vectors wherever they lie 89 and 40)
     const bool wide = d->N % (d->dtype == REXSC_F32 ? 4 : 8) == 0 && ((uintptr_t)g | (uintptr_t)b_scale) % 16 == 0;
     {
         const double es = (double)dtype_size(d->dtype), mn = (double)d->M * d->N, k = (double)d->K;
@@ -623,18 +636,18 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
                        (dw ? 3.0 * k * d->M : 0.0), stream);
         const dim3 grid(p.row_blocks + p.b_blocks + p.a_blocks + p.stat_blocks);
         if (wide)
-            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((operands_kernel<T, 16 / sizeof(T)>), grid, dim3(256), 0, stream, p));
+            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((operands_kernel<T, false>), grid, dim3(256), 0, stream, p));
         else
-            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((operands_kernel<T, 1>), grid, dim3(256), 0, stream, p));
+            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((operands_kernel<T, true>), grid, dim3(256), 0, stream, p));
         REXSC_CHECK_HIP(hipGetLastError());
     }
     if (dw) {
         ProfScope prof("int8_backward_pieces", (double)d->M * d->N * (dtype_size(d->dtype) + 2.0 * p.pieces_w), stream);
         const dim3 grid((unsigned)(tiles_m * tiles_n));
         if (wide)
-            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((transposed_pieces_kernel<T, 16 / sizeof(T)>), grid, dim3(256), 0, stream, p));
+            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((transposed_pieces_kernel<T, false>), grid, dim3(256), 0, stream, p));
         else
-            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((transposed_pieces_kernel<T, 1>), grid, dim3(256), 0, stream, p));
+            REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((transposed_pieces_kernel<T, true>), grid, dim3(256), 0, stream, p));
         REXSC_CHECK_HIP(hipGetLastError());
     } else if (db) {
         if (int rc = launch_column_sums(p.sums, p.shares, d->N, d->N, db, nullptr, d->bias_dtype, stream)) return rc;
