@@ -156,9 +156,9 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(No
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (i * TPR + tid) * V;
-            if constexpr (RAGGED) { // (shifting the last vector takes registers that are not there: 181 us at 5591 x 12001)
-                cx[i] = load_some<T, V>(sx + c, p.cols - c, 0);
-                cg[i] = load_some<T, V>(sg + c, p.cols - c, 0);
+            if constexpr (RAGGED) { // (by one shifted load: registers that are not there, 181 us against 160 at 5591 x 12001)
+                cx[i] = load_some<T, V>(sx + c, p.cols - c);
+                cg[i] = load_some<T, V>(sg + c, p.cols - c);
             } else {
                 cx[i] = c < p.cols ? *(const vec *)(sx + c) : vec{};
                 cg[i] = c < p.cols ? *(const vec *)(sg + c) : vec{};

@@ -24,12 +24,25 @@ template <typename T> struct VecOf<T, 1> { typedef T type; };
 // The same, aligned to its element only: one load or store of as many bytes wherever it lies.
 template <typename T, int V> struct LooseVecOf { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
 
-// The first n of the V elements from p on, zeros behind them; `before` elements in front of p may be read.  Where fewer
-// than V are left the vector that ends with the last one is read and shifted down: one load all the same.
+// The first n of the V elements from p on, zeros behind them.
+template <typename T, int V>
+__device__ __forceinline__ typename VecOf<T, V>::type load_some(const T *p, int n)
+{
+    typename VecOf<T, V>::type v{};
+    if (n >= V) v = *(const typename LooseVecOf<T, V>::type *)p;
+    else if (n > 0) {
+#pragma unroll
+        for (int i = 0; i < V - 1; i++)
+            if (i < n) v[i] = p[i];
+    }
+    return v;
+}
+// The same where `before` elements in front of p may be read: where fewer than V are left, the vector that ends with the
+// last one is read and shifted down, one load all the same.
 template <typename T, int V>
 __device__ __forceinline__ typename VecOf<T, V>::type load_some(const T *p, int n, int before)
 {
-    static_assert(V * sizeof(T) == 16, "");
+    static_assert(V * sizeof(T) == 16, "shifted as a 128-bit integer");
     typename VecOf<T, V>::type v{};
     const int back = n < V ? V - n : 0;
     if (n > 0 && back <= before) {
