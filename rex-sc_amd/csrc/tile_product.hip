@@ -377,7 +377,7 @@ __global__ __launch_bounds__(256) void join_kernel(TileArgs p, const ACC *part, 
 // ---- host ------------------------------------------------------------------------------------------
 constexpr int CUS = 256, MAX_SPLITS = 16;
 
-struct TilePlan { int size, splits; }; // size: 256, 128, 64 (squares) or 32 (64 x 32)
+struct TilePlan { int size, splits; bool alone; }; // size: 256, 128, 64 (squares) or 32 (64 x 32)
 
 int tune(const char *name)
 {
@@ -386,7 +386,8 @@ int tune(const char *name)
 }
 
 // Tile size by what a launch takes when its busiest CU gets n tiles, in units of one 256 x 256 tile (measured at
-// K = 4096 int8, 57 us each): one block of 256 x 256 per CU, n; two of 128 x 128 side by side 0.61, a single one 0.44;
+// K = 4096 int8, 57 us each): one block of 256 x 256 per CU, n; two of 128 x 128 side by side 0.61, a single one 0.44, or
+// 0.37 where no CU gets two and it may take eight waves and four buffers (1024 x 4096: 21 us against 26);
 // 64 x 64, up to five side by side, 0.08 + 0.11 n.  E.g. 2048 x 4096: 37 us in 128s against 52 in 256s and 58 in 64s;
 // 4096 x 4096: 59 in 256s against 69 in 128s; 512 x 4096: 19 in 64s against 26 in 128s.
 // The reduction is split over blocks only where the result has tiles for at most a quarter of the CUs and each share
@@ -399,8 +400,8 @@ TilePlan tile_plan(int M, int N, int kbytes, int pieces)
     auto tiles = [&](int b) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b); };
     auto busiest = [&](int b) { return (tiles(b) + CUS - 1) / CUS; };
     const int64_t n256 = busiest(256), n128 = busiest(128), n64 = busiest(64);
-    const double t256 = (double)n256, t128 = 0.61 * (double)(n128 / 2) + 0.44 * (double)(n128 % 2), t64 = 0.08 + 0.11 * (double)n64;
-    TilePlan pl{t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64, 1};
+    const double t256 = (double)n256, t128 = n128 == 1 ? 0.37 : 0.61 * (double)(n128 / 2) + 0.44 * (double)(n128 % 2), t64 = 0.08 + 0.11 * (double)n64;
+    TilePlan pl{t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64, 1, n128 == 1};
     // 64 x 32 where that still leaves no CU two tiles: the weights are then read by twice as many (from cold weights
     // 64 x 4096 x 4096: 11.4 us against 13.0; 256 x 4096 x 4096, two tiles for a CU: 15.8 against 13.5)
     const int64_t halves = (int64_t)((M + 63) / 64) * ((N + 31) / 32);
@@ -444,6 +445,7 @@ template <typename Op, typename T>
 int launch_size(const TileArgs &p, const TilePlan &pl, void *workspace, hipStream_t stream)
 {
     if (pl.size == 256) return launch_one<Op, T, 256, 256, 2, 4, 2>(p, pl.splits, workspace, stream);
+    if (pl.size == 128 && pl.alone) return launch_one<Op, T, 128, 128, 2, 4, 4>(p, pl.splits, workspace, stream);
     if (pl.size == 128) return launch_one<Op, T, 128, 128, 2, 2, 2>(p, pl.splits, workspace, stream);
     if (pl.size == 32) return launch_one<Op, T, 64, 32, 2, 2, 4>(p, pl.splits, workspace, stream);
     return launch_one<Op, T, 64, 64, 2, 2, 4>(p, pl.splits, workspace, stream);

@@ -430,6 +430,20 @@ def test_more_large_tiles_than_blocks(dt, n, k, monkeypatch):
     assert (((y.double() - want).abs() <= tol) | (want.abs() + tol >= limit)).all()
 
 
+@pytest.mark.parametrize("m,n", [(4353, 4100), (1100, 900)])
+@pytest.mark.parametrize("k", [100, 385, 1100])
+def test_tiles_of_128_alone_on_a_cu_and_not(m, n, k, monkeypatch):
+    import sc_functional as F
+    gen = torch.Generator(device="cuda").manual_seed(m + k)
+    pitch = -(-k // 128) * 128
+    a, b = (torch.randint(-127, 128, (r, pitch), device="cuda", dtype=torch.int8, generator=gen)[:, :k] for r in (m, n))
+    sa, sb = (torch.rand(r, device="cuda", generator=gen) + 0.5 for r in (m, n))
+    monkeypatch.setenv("REXSC_TUNE_INT8_TILE", "128")
+    y = F.matmul_int8(a, sa, b, sb, None)
+    want = (a.double() @ b.double().t().contiguous()) * sa.double()[:, None] * sb.double()
+    assert ((y.double() - want).abs() <= 5 * U * want.abs() + 2.0 ** -126).all()
+
+
 def test_more_rows_than_blocks():
     import sc_functional as F
     x = torch.randn((1 << 23) + 9, 3, device="cuda", dtype=torch.float16)
