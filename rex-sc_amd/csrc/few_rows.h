@@ -10,9 +10,9 @@ bool few_rows_takes(int M, int N); // whether it is the faster one
 // y = a b^T of int8 operands with their epilogue, as TileArgs says (one piece).
 int launch_few_rows(const TileArgs &p, int out_dtype, hipStream_t stream);
 
-// The same from float tokens x [M][K] (rows x_stride elements apart), taken to 8 bits in every block: where M K is
+// The same from float tokens x [M][K] (rows x_stride elements apart), taken to 8 bits in every block: where M K and N are
 // small and the rows begin on 16 bytes.
-bool few_rows_fuses(int M, int K, const void *x, size_t x_stride, int dtype);
+bool few_rows_fuses(int M, int N, int K, const void *x, size_t x_stride, int dtype);
 int launch_few_rows_fused(const TileArgs &p, const void *x, size_t x_stride, int dtype, hipStream_t stream);
 
 } // namespace rexsc

@@ -4,7 +4,7 @@
 // rows, two loads of a wave a cache line of each, and the eight waves of a block take neighbouring lines of the same
 // rows, so a row is read in runs of 1024 bytes.  There is nothing to share in LDS (each weight is used by one wave), and
 // nothing to wait for but memory: a wave has UNROLL loads in flight before the first is used.  The waves' int32 sums,
-// exact in any order, are joined through LDS.  With few tokens (M K <= 8192) the block takes them to 8 bits itself, while
+// exact in any order, are joined through LDS.  With few tokens the block takes them to 8 bits itself, while
 // its first weights are on their way: a launch of its own would cost more than every block's reading the few kilobytes
 // again.
 // Measured with weights from memory: 1 x 4096 x 4096 5.9 us from int8 tokens, 8.0 us from float ones (with the rows'
@@ -25,7 +25,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr int WAVES = 8, THREADS = WAVES * 64;
 constexpr int LOADS = 8;                   // of 64 bytes of 16 rows that a wave has in flight, at most
 constexpr int UNIT = WAVES * 64;           // bytes of a row that the block's waves take with one load each
-constexpr int FUSED_ELEMS = 8192, FUSED_ROWS = 16; // tokens x K, and tokens, that a block takes to 8 bits by itself
+constexpr int FUSED_ROWS = 16;             // tokens that a block takes to 8 bits by itself, at most
 
 __device__ __forceinline__ i32x4 keep_before(i32x4 v, int n) // the first n bytes (n may be anything)
 {
@@ -43,13 +43,14 @@ struct FewArgs {
     size_t x_stride;
 };
 
-// A block makes 16 channels.  FM: fragments of 16 tokens; U0: loads per wave of the first round; X: type of the tokens, or int8_t: already in 8 bits.
-template <int FM, int U0, typename T, typename X>
+// A block makes 16 channels.  FM: fragments of 16 tokens; U0: loads per wave of the first round; X: type of the tokens, or
+// int8_t: already in 8 bits; ELEMS: float elements that the block has room for.
+template <int FM, int U0, typename T, typename X, int ELEMS>
 __global__ __launch_bounds__(THREADS) void few_rows_kernel(FewArgs g)
 {
-    constexpr bool FUSED = sizeof(X) > 1;
+    constexpr bool FUSED = ELEMS > 0;
     const TileArgs &p = g.p;
-    __shared__ __attribute__((aligned(16))) int8_t tokens[FUSED ? FUSED_ELEMS + FUSED_ROWS * 80 : 16];
+    __shared__ __attribute__((aligned(16))) int8_t tokens[FUSED ? ELEMS + FUSED_ROWS * 80 : 16];
     __shared__ int sums[WAVES][FM][256];
     __shared__ unsigned top[FUSED ? FUSED_ROWS : 1];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
@@ -73,8 +74,8 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(FewArgs g)
 
     const int pitch = (K + 63) / 64 * 64 + 16; // of a token in LDS
     if constexpr (FUSED) {
-        // M K <= FUSED_ELEMS elements in vectors of 16 bytes, SLOTS per thread; rows begin on one
-        constexpr int V = 16 / sizeof(X), SLOTS = FUSED_ELEMS / V / THREADS;
+        // M K <= ELEMS elements in vectors of 16 bytes, SLOTS per thread; rows begin on one
+        constexpr int V = 16 / sizeof(X), SLOTS = ELEMS / V / THREADS;
         typedef typename VecOf<X, V>::type vec;
         const int per = K / V, all = p.M * per;
         vec v[SLOTS];
@@ -171,15 +172,15 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(FewArgs g)
     }
 }
 
-template <int FM, typename T, typename X>
+template <int FM, typename T, typename X, int ELEMS>
 int launch_u(const FewArgs &g, hipStream_t stream)
 {
     REXSC_CHECK_ARG(g.p.N < (1 << 26), "int8 linear: %d output channels are more than a launch holds", g.p.N);
     const dim3 grid((unsigned)((g.p.N + 15) / 16));
     // a round that is longer than the row would load its first chunk over and over
-    if (g.p.kbytes > 4 * UNIT) hipLaunchKernelGGL((few_rows_kernel<FM, 8, T, X>), grid, dim3(THREADS), 0, stream, g);
-    else if (g.p.kbytes > 2 * UNIT) hipLaunchKernelGGL((few_rows_kernel<FM, 4, T, X>), grid, dim3(THREADS), 0, stream, g);
-    else hipLaunchKernelGGL((few_rows_kernel<FM, 2, T, X>), grid, dim3(THREADS), 0, stream, g);
+    if (g.p.kbytes > 4 * UNIT) hipLaunchKernelGGL((few_rows_kernel<FM, 8, T, X, ELEMS>), grid, dim3(THREADS), 0, stream, g);
+    else if (g.p.kbytes > 2 * UNIT) hipLaunchKernelGGL((few_rows_kernel<FM, 4, T, X, ELEMS>), grid, dim3(THREADS), 0, stream, g);
+    else hipLaunchKernelGGL((few_rows_kernel<FM, 2, T, X, ELEMS>), grid, dim3(THREADS), 0, stream, g);
     REXSC_CHECK_HIP(hipGetLastError());
     return REXSC_OK;
 }
@@ -187,9 +188,9 @@ int launch_u(const FewArgs &g, hipStream_t stream)
 template <typename T>
 int launch_fm(const FewArgs &g, hipStream_t stream)
 {
-    if (g.p.M <= 16) return launch_u<1, T, int8_t>(g, stream);
-    if (g.p.M <= 32) return launch_u<2, T, int8_t>(g, stream);
-    return launch_u<3, T, int8_t>(g, stream);
+    if (g.p.M <= 16) return launch_u<1, T, int8_t, 0>(g, stream);
+    if (g.p.M <= 32) return launch_u<2, T, int8_t, 0>(g, stream);
+    return launch_u<3, T, int8_t, 0>(g, stream);
 }
 
 double work(const TileArgs &p) { return 2.0 * p.M * p.N * p.kbytes; }
@@ -208,18 +209,23 @@ int launch_few_rows(const TileArgs &p, int out_dtype, hipStream_t stream)
 // but 37 x 11003 x 4099 27 us here and 15 in tiles, 16 x 16384 x 4096 19 and 17.5.
 bool few_rows_takes(int M, int N) { return M <= 8 || (M <= FEW_ROWS && N < 64 * 128); }
 
-bool few_rows_fuses(int M, int K, const void *x, size_t x_stride, int dtype)
+// Every block of 16 channels takes the tokens to 8 bits again, which hides behind the weights and saves a launch while a
+// CU has few blocks: 13.7 us a call against 16 from 1 x 2048 x 1000 to 1 x 4096 x 16384 in 16 bits; 4 x 4096 x 4096, with
+// twice the elements, 13.9 against 16.0.  With more blocks or longer rows it costs more than it saves (float32 1 x 4096 x
+// 32768 35 us against 32 and 2 x 2048 x 32768 33 against 18; 1 x 16384 x 4096 27 against 23.5).
+bool few_rows_fuses(int M, int N, int K, const void *x, size_t x_stride, int dtype)
 {
-    const size_t es = dtype_size(dtype);
-    return M <= FUSED_ROWS && (int64_t)M * K <= FUSED_ELEMS && (size_t)K * es % 16 == 0 && (uintptr_t)x % 16 == 0 &&
-           (M == 1 || x_stride * es % 16 == 0);
+    const size_t es = dtype_size(dtype), elems = (size_t)M * K, out = (size_t)N * es;
+    const bool pays = elems <= 8192 ? out <= 32768 : elems <= 16384 && K <= 8192 && out <= 16384;
+    return M <= FUSED_ROWS && pays && (size_t)K * es % 16 == 0 && (uintptr_t)x % 16 == 0 && (M == 1 || x_stride * es % 16 == 0);
 }
 
 int launch_few_rows_fused(const TileArgs &p, const void *x, size_t x_stride, int dtype, hipStream_t stream)
 {
     ProfScope prof("int8_linear_few", work(p), stream);
     const FewArgs g{p, x, x_stride};
-    REXSC_DTYPE_SWITCH(dtype, return (launch_u<1, T, T>(g, stream)));
+    if (p.M * p.kbytes <= 8192) REXSC_DTYPE_SWITCH(dtype, return (launch_u<1, T, T, 8192>(g, stream)));
+    REXSC_DTYPE_SWITCH(dtype, return (launch_u<1, T, T, 16384>(g, stream)));
 }
 
 } // namespace rexsc

@@ -562,7 +562,7 @@ extern "C" int rexsc_int8_linear(const rexsc_int8_desc *d, const void *x, const 
                     "int8 linear: x is not aligned to its element, or its rows overlap (distance %lld)", (long long)d->x_stride);
     const Space s = space(d, REXSC_INT8_LINEAR);
     if (int rc = check_space(s, workspace, workspace_bytes)) return rc;
-    if (few_rows_fuses(d->M, d->K, x, (size_t)d->x_stride, d->dtype)) {
+    if (few_rows_fuses(d->M, d->N, d->K, x, (size_t)d->x_stride, d->dtype)) {
         const TileArgs p{nullptr, (const char *)b, 0, (size_t)d->b_stride, d->M, d->N, d->K, 1, 0, nullptr, b_scale, bias,
                          d->bias_dtype, y};
         return launch_few_rows_fused(p, x, (size_t)d->x_stride, d->dtype, stream);

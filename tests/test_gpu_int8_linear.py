@@ -444,6 +444,14 @@ def test_tiles_of_128_alone_on_a_cu_and_not(m, n, k, monkeypatch):
     assert ((y.double() - want).abs() <= 5 * U * want.abs() + 2.0 ** -126).all()
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 24, 8192), (2, 24, 4096), (2, 24, 4104), (2, 24, 8192), (16, 24, 1024), (16, 40, 520), (16, 40, 512),
+                                   (3, 24, 5000), (1, 24, 8200), (2, 4096, 600), (2, 4104, 600), (2, 8200, 600), (2, 16392, 600),
+                                   (4, 4104, 2056), (4, 8200, 2056)])
+def test_serving_around_the_fused_sizes(dt, m, n, k):
+    test_linear_int8_serving(dt, m, n, k)
+
+
 def test_more_rows_than_blocks():
     import sc_functional as F
     x = torch.randn((1 << 23) + 9, 3, device="cuda", dtype=torch.float16)
