@@ -369,7 +369,7 @@ __global__ __launch_bounds__(256) void join_kernel(TileArgs p, const ACC *part, 
     for (int e = 0; e < n; e++) {
         const float v = p.a_scale ? (float)s[e] * p.a_scale[m] : (float)s[e];
         const float sb = p.b_scale ? p.b_scale[c] : 1.f, bias = p.bias ? load_any(p.bias, p.bias_dtype, c) : 0.f;
-        ((T *)p.y)[at + e] = (T)fmaf(v, sb, bias); // as the unsplit kernel rounds it
+        ((T *)p.y)[at + e] = (T)fmaf(v, sb, bias); // as in the unsplit kernel
         if (++c == (unsigned)p.N) { c = 0; m++; }
     }
 }

@@ -40,6 +40,16 @@ def _product_close(y, qa, sa, qb, sb, bias, dt):
     assert y.dtype == dt and (err <= tol).all(), "max error %g of its bound" % (err / tol).max()
 
 
+def _close_or_over(y, prod, want, dt):
+    """_product_close's bound on the device; what half a step of the type beyond its largest number reaches is rounded to
+    infinity."""
+    tol = 4 * U * prod.abs() + U * want.abs() + _half(dt) * want.abs() * (1 + 2 ** -8) + _floor(dt) + 2.0 ** -126
+    limit = torch.finfo(dt).max * (1 + _half(dt) / 2)
+    over = want.abs() - tol >= limit
+    assert torch.equal(y[over].double(), want[over].sign() * torch.inf)
+    assert (((y.double() - want).abs() <= tol) | (want.abs() + tol >= limit)).all()
+
+
 # ---- rows to 8 bits ------------------------------------------------------------------------------
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("rows,k", [(1, 1), (3, 7), (5, 64), (17, 1000), (4, 4096), (2, 4099), (3, 8192), (2, 16384),
@@ -422,12 +432,7 @@ def test_more_large_tiles_than_blocks(dt, n, k, monkeypatch):
     y = F.matmul_int8(a, sa, b, sb, bias, out_dtype=dt)
     prod = (a.double() @ b.double().t().contiguous()) * sa.double()[:, None] * sb.double()
     want = prod + bias.double()
-    tol = 4 * U * prod.abs() + U * want.abs() + _half(dt) * want.abs() * (1 + 2 ** -8) + _floor(dt) + 2.0 ** -126
-    # what half a step of the type beyond its largest number reaches is rounded to infinity
-    limit = torch.finfo(dt).max * (1 + _half(dt) / 2)
-    over = want.abs() - tol >= limit
-    assert torch.equal(y[over].double(), want[over].sign() * torch.inf)
-    assert (((y.double() - want).abs() <= tol) | (want.abs() + tol >= limit)).all()
+    _close_or_over(y, prod, want, dt)
 
 
 @pytest.mark.parametrize("m,n", [(4353, 4100), (1100, 900)])
@@ -450,6 +455,32 @@ def test_tiles_of_128_alone_on_a_cu_and_not(m, n, k, monkeypatch):
                                    (4, 4104, 2056), (4, 8200, 2056)])
 def test_serving_around_the_fused_sizes(dt, m, n, k):
     test_linear_int8_serving(dt, m, n, k)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("m,n", [(3, 33), (70, 65), (70, 1001), (130, 1002), (300, 130), (700, 5003)])
+def test_nothing_is_written_behind_a_result(dt, m, n, monkeypatch):
+    """The result lies inside a larger buffer whose rest must stay as it was, from the kernel's own entry."""
+    import _lib
+    import _ops
+    gen = torch.Generator(device="cuda").manual_seed(m * n)
+    a, b = (torch.randint(-127, 128, (r, 128), device="cuda", dtype=torch.int8, generator=gen) for r in (m, n))
+    sa, sb = (torch.rand(r, device="cuda", generator=gen) + 0.5 for r in (m, n))
+    # (a kernel may round the last multiply-add to the type at once or by way of float32, so two of them are a step of the
+    # type apart where the value lies within a float32 rounding of a tie: each is held to the bound, not to another)
+    want = (a.double() @ b.double().t().contiguous()) * sa.double()[:, None] * sb.double()
+    for tile in ("", "32", "64", "128", "256"):
+        monkeypatch.setenv("REXSC_TUNE_INT8_TILE", tile) if tile else monkeypatch.delenv("REXSC_TUNE_INT8_TILE", raising=False)
+        for before in (8, 5, 2):  # elements in front of the result: aligned to 16 bytes, or to an element only
+            whole = torch.full((before + m * n + 512,), 7.0, device="cuda", dtype=dt)
+            d = _lib.Int8Desc.packed(m, n, 128, _ops._dtype_code(dt, ""), 0, 0, 0, 0, 128, 128)
+            ws, nbytes = _ops._int8_space(_lib.lib(), d, _lib.INT8_PRODUCT, a.device)
+            rc = _lib.lib().rexsc_int8_product(d, a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(), None,
+                                               whole.data_ptr() + before * whole.element_size(), _ops._addr(ws), nbytes,
+                                               _ops._raw_stream(0))
+            _lib.check(rc, "rexsc_int8_product")
+            _close_or_over(whole[before:before + m * n].view(m, n), want, want, dt)
+            assert (whole[:before] == 7).all() and (whole[before + m * n:] == 7).all(), (tile, before)
 
 
 def test_more_rows_than_blocks():

@@ -89,6 +89,25 @@ def test_widths_around_the_numbers_of_threads(dt, wdt, d):
     test_forward_and_gradients(dt, wdt, 3, d)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("d", [37, 250, 1101, 1536, 2001, 5001, 8200, 9001, 12288, 16383])
+def test_rows_inside_another_matrix(dt, d):
+    """Rows that begin anywhere, beside elements that must neither be read as theirs nor written."""
+    import sc_functional as F
+    gen = torch.Generator().manual_seed(d)
+    whole = torch.randn(5, d + 11, generator=gen).to(dt)
+    whole[:, :3], whole[:, d + 3:] = 1e4, -1e4
+    w, b = 1 + 0.2 * torch.randn(d, generator=gen), torch.randn(d, generator=gen)
+    g = torch.randn(5, d, generator=gen).to(dt)
+    x = whole.cuda()[:, 3:d + 3].requires_grad_()
+    leaves = [x, w.cuda().requires_grad_(), b.cuda().requires_grad_()]
+    y = F.layer_norm(*leaves)
+    ref = reference(whole[:, 3:d + 3], w, b, g)
+    close(y, ref["y"], dt, "y")
+    for name, got, t in zip(("dx", "dw", "db"), torch.autograd.grad(y, leaves, g.cuda()), (dt, torch.float32, torch.float32)):
+        close(got, ref[name], t, name)
+
+
 @pytest.mark.parametrize("d", [48, 1003, 5000])
 def test_without_weight_or_bias_and_partial_gradients(d):
     import sc_functional as F
