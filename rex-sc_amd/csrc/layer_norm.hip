@@ -156,7 +156,12 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(No
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (i * TPR + tid) * V;
-            if constexpr (RAGGED) { // (by one shifted load: registers that are not there, 181 us against 160 at 5591 x 12001)
+            // the vector that the row's end cuts: one shifted load where there are registers for it (5591 x 12001 bfloat16:
+            // 140 us against 152 by elements; with 32 elements a thread 181 against 160, in float32 97 against 93)
+            if constexpr (RAGGED && sizeof(T) == 2 && NV * V <= 24) {
+                cx[i] = load_some<T, V>(sx + c, p.cols - c, c);
+                cg[i] = load_some<T, V>(sg + c, p.cols - c, c);
+            } else if constexpr (RAGGED) {
                 cx[i] = load_some<T, V>(sx + c, p.cols - c);
                 cg[i] = load_some<T, V>(sg + c, p.cols - c);
             } else {
@@ -386,9 +391,10 @@ int check_norm(const rexsc_norm_desc *d)
 // against 86 in 256, 6553 x 5120 forward 54 in 256 against 50 in 512), and forward rows of 8193 to 10240 (3727 x 9001
 // 60 us in 1024 threads, 53 in 512).
 //
-// The backward pass holds a row of more than 8192 in 512 threads at 32 elements: with its five values per element, 1024
-// threads have too few registers (8192 x 16384 bfloat16: 640 us with them spilled, against 178).  There single elements
-// need too many as well, and vectors that lie anywhere are taken (5591 x 12001 bfloat16: 161 us against 459).
+// The backward pass holds a row of more than 8192 in 512 threads at 24 or 32 elements: with its five values per element,
+// 1024 threads have too few registers (8192 x 16384 bfloat16: 640 us with them spilled, against 178; 5591 x 12001 at 12
+// elements 162 against 140).  There single elements need too many as well, and vectors that lie anywhere are taken
+// (5591 x 12001 bfloat16: 459 us by single elements).
 NormPlan norm_plan(const rexsc_norm_desc *d, bool aligned, bool backward)
 {
     NormPlan pl{};
@@ -480,7 +486,10 @@ template <typename T> bool launch_bwd(const NormPlan &pl, const NormParams &p, h
 {
     constexpr int W = 16 / sizeof(T);
     if (pl.TPR < 1024) NORM_NV(launch_bwd_tpr);
-    if (pl.V > 1) hipLaunchKernelGGL((norm_backward_kernel<T, W, 32 / W, 512>), dim3(pl.grid), dim3(512), 0, s, p);
+    const bool shorter = p.cols <= 512 * 24;
+    if (pl.V > 1 && shorter) hipLaunchKernelGGL((norm_backward_kernel<T, W, 24 / W, 512>), dim3(pl.grid), dim3(512), 0, s, p);
+    else if (pl.V > 1) hipLaunchKernelGGL((norm_backward_kernel<T, W, 32 / W, 512>), dim3(pl.grid), dim3(512), 0, s, p);
+    else if (shorter) hipLaunchKernelGGL((norm_backward_kernel<T, W, 24 / W, 512, true>), dim3(pl.grid), dim3(512), 0, s, p);
     else hipLaunchKernelGGL((norm_backward_kernel<T, W, 32 / W, 512, true>), dim3(pl.grid), dim3(512), 0, s, p);
     return true;
 }
