@@ -102,14 +102,15 @@ __device__ __forceinline__ void tile_of(unsigned bid, int tiles_m, int tiles_n, 
     tn = __builtin_amdgcn_readfirstlane((int)(r / rows));
 }
 
+// The tiles first ... end - 1 of the order.
 // SPLIT: the grid holds `splits` times the tiles, and a block sums only its share of the steps, into a partial result
-// of the accumulator's type (T) that join_kernel finishes.
+// of the accumulator's type (T), a tile of its own, that join_kernel finishes.
 // STREAM: the grid holds a block per CU, and a block takes every gridDim.x-th tile.  Its steps are one stream over all
 // its tiles: the next tile's first steps are fetched while the last one's are multiplied and while the finished tile is
 // stored, from LDS of its own.  Against a block per tile, in turn: 8192 x 16384 x 4096 468 -> 451 us, 8192 x 4096 x 4096
 // 114 -> 109, 8192 x 16384 x 1024 165 -> 146-153.
 template <typename Op, typename T, int BM, int BN, int WM, int WN, int STAGES, bool SPLIT, bool STREAM>
-__global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int splits)
+__global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int splits, unsigned first, unsigned end)
 {
     static_assert(!(SPLIT && STREAM), "a split tile is one of its own");
     constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
     const int share = SPLIT ? (int)(blockIdx.x % splits) : 0;
-    unsigned tile = SPLIT ? blockIdx.x / splits : blockIdx.x;
+    unsigned tile = first + (SPLIT ? blockIdx.x / splits : blockIdx.x);
 
     // A wave's loads are 8 * WAVES rows apart, so that a lane takes the same chunk in all of them (the LDS side of a load
     // is fixed: 16 bytes per lane in lane order).  Rows behind the operand's last lie behind the descriptor's range.
@@ -156,7 +157,6 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
     // what is fetched next: the byte offset in the row, the tile, and the steps that this tile still has
     unsigned k = SPLIT ? (unsigned)(begin % steps) * KSTEP : 0, ahead = tile;
     int left = total;
-    const unsigned all = STREAM ? (unsigned)tiles_m * (unsigned)tiles_n : 0;
     auto fetch = [&](char *buf) __attribute__((always_inline)) {
         if (left == 0) return;
         auto load = [&](unsigned beyond) __attribute__((always_inline)) {
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
         left--;
         if (STREAM && left == 0) {
             ahead += gridDim.x;
-            if (ahead < all) { left = total; seek(ahead); }
+            if (ahead < end) { left = total; seek(ahead); }
         }
     };
     // int8 rows whose last chunk is not full: what stands behind the row may be anything, and becomes 0 in a's tile
@@ -244,8 +244,9 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
     else loads_left<0>();
     meet();
     if (tail && total == 1) clear_tail(base);
-    T *const y = (T *)p.y + (SPLIT ? (size_t)share * p.M * p.N : 0);
-    const size_t pitch = (size_t)p.N * sizeof(T);
+    const int height = SPLIT ? BM : p.M, width = SPLIT ? BN : p.N;
+    T *const y = (T *)p.y + (SPLIT ? ((size_t)share * (end - first) + (tile - first)) * (BM * BN) : 0);
+    const size_t pitch = (size_t)width * sizeof(T);
     const bool wide = pitch % 16 == 0 && (uintptr_t)y % 16 == 0 && pitch < 0x80000000u / CR;
     lds_char *const mine = base + (STREAM ? STAGES * BUF : 0) + wave * SHARE;
     int cur = 0;
@@ -296,6 +297,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
                 bias[j][e] = __shfl(bias_f, c, 64);
             }
         if (!STREAM) __syncthreads(); // the buffers are the waves' shares from here on
+        const int row0 = SPLIT ? wm : first_m, col0 = SPLIT ? wn : first_n;
 #pragma unroll
         for (int r0 = 0; r0 < ROWS; r0 += CR) {
 #pragma unroll
@@ -313,15 +315,15 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
                     *(__attribute__((address_space(3))) typename VecOf<T, 4>::type *)(mine + to) = v;
                 }
             }
-            const int rows = p.M - (first_m + r0) < CR ? p.M - (first_m + r0) : CR; // of this part, that exist
-            T *out = y + (size_t)(first_m + r0) * p.N + first_n;
+            const int rows = height - (row0 + r0) < CR ? height - (row0 + r0) : CR; // of this part, that exist
+            T *out = y + (size_t)(row0 + r0) * width + col0;
             if (wide) {
                 // rows that do not exist lie behind the descriptor's range, and so do a lane's columns if they do not exist
                 constexpr int LANES = RB / 16; // that store a row
                 const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
-                    out, 0, rows > 0 && first_n < p.N ? (int)((rows - 1) * pitch + (size_t)(p.N - first_n) * sizeof(T)) : 0, 0x00027000);
+                    out, 0, rows > 0 && col0 < width ? (int)((rows - 1) * pitch + (size_t)(width - col0) * sizeof(T)) : 0, 0x00027000);
                 unsigned to = (unsigned)(l / LANES) * (unsigned)pitch + (unsigned)(l % LANES) * 16;
-                if (first_n + l % LANES * 16 / (int)sizeof(T) >= p.N) to = 0x80000000u;
+                if (col0 + l % LANES * 16 / (int)sizeof(T) >= width) to = 0x80000000u;
 #pragma unroll
                 for (int t = 0; t < SHARE / 1024; t++) {
                     const i32x4 v = *(const lds_i32x4 *)(mine + place(t * (64 / LANES) + l / LANES, l % LANES * 16));
@@ -330,12 +332,12 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
             } else {
                 // the same wherever the rows begin; the vector that a row's end cuts is stored by elements
                 constexpr int LANES = RB / 16, VEC = 16 / sizeof(T);
-                const int left = p.N - first_n - l % LANES * VEC;
+                const int left = width - col0 - l % LANES * VEC;
 #pragma nounroll
                 for (int t = 0; t < SHARE / 1024; t++) {
                     const int r = t * (64 / LANES) + l / LANES;
                     const i32x4 v = *(const lds_i32x4 *)(mine + place(r, l % LANES * 16));
-                    if (r < rows) store_some<T, VEC>(out + (size_t)r * p.N + l % LANES * VEC, __builtin_bit_cast(typename VecOf<T, VEC>::type, v), left);
+                    if (r < rows) store_some<T, VEC>(out + (size_t)r * width + l % LANES * VEC, __builtin_bit_cast(typename VecOf<T, VEC>::type, v), left);
                 }
             }
         }
@@ -345,39 +347,46 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(TileArgs p, int spli
 #pragma unroll
             for (int j = 0; j < FN; j++) acc[i][j] = typename Op::acc{};
         tile += gridDim.x;
-    } while (tile < all);
+    } while (tile < end);
 }
 
-// y = (sum of the partial results, in order) * scales + bias; ACC: int or float.  Four elements per thread.
+// y = (sum of the partial results, in order) * scales + bias of `count` tiles from `first` on; ACC: int or float.  Four
+// elements of a row per thread.
 template <typename ACC, typename T>
-__global__ __launch_bounds__(256) void join_kernel(TileArgs p, const ACC *part, int splits)
+__global__ __launch_bounds__(256) void join_kernel(TileArgs p, const ACC *part, int splits, unsigned first, unsigned count, int bm, int bn)
 {
-    const size_t all = (size_t)p.M * p.N, at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (at >= all) return;
+    const unsigned per = (unsigned)(bm * bn) / 1024, local = blockIdx.x / per;
+    const int at = (int)(blockIdx.x % per * 1024 + threadIdx.x * 4);
+    int tm, tn;
+    tile_of(first + local, (p.M + bm - 1) / bm, (p.N + bn - 1) / bn, tm, tn);
+    const int m = tm * bm + at / bn, n = tn * bn + at % bn;
+    if (m >= p.M || n >= p.N) return;
     ACC s[4] = {};
-    const int n = all - at < 4 ? (int)(all - at) : 4;
-    if (n == 4 && all % 4 == 0)
-        for (int z = 0; z < splits; z++) {
-            const typename VecOf<ACC, 4>::type v = *(const typename VecOf<ACC, 4>::type *)(part + z * all + at);
+    for (int z = 0; z < splits; z++) {
+        const typename VecOf<ACC, 4>::type v = *(const typename VecOf<ACC, 4>::type *)(part + ((size_t)z * count + local) * (bm * bn) + at);
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[e] += v[e];
-        }
-    else
-        for (int z = 0; z < splits; z++)
-            for (int e = 0; e < n; e++) s[e] += part[z * all + at + e];
-    unsigned m = (unsigned)(at / p.N), c = (unsigned)(at - (size_t)m * p.N);
-    for (int e = 0; e < n; e++) {
-        const float v = p.a_scale ? (float)s[e] * p.a_scale[m] : (float)s[e];
-        const float sb = p.b_scale ? p.b_scale[c] : 1.f, bias = p.bias ? load_any(p.bias, p.bias_dtype, c) : 0.f;
-        ((T *)p.y)[at + e] = (T)fmaf(v, sb, bias); // as in the unsplit kernel
-        if (++c == (unsigned)p.N) { c = 0; m++; }
+        for (int e = 0; e < 4; e++) s[e] += v[e];
     }
+    const float sa = p.a_scale ? p.a_scale[m] : 1.f;
+    T *out = (T *)p.y + (size_t)m * p.N + n;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (n + e < p.N) {
+            const float sb = p.b_scale ? p.b_scale[n + e] : 1.f, bias = p.bias ? load_any(p.bias, p.bias_dtype, n + e) : 0.f;
+            out[e] = (T)fmaf((float)s[e] * sa, sb, bias); // as in the unsplit kernel
+        }
 }
 
 // ---- host ------------------------------------------------------------------------------------------
 constexpr int CUS = 256, MAX_SPLITS = 16;
+constexpr double REST_US = 16, REST_TILE_US = 0.12; // of splitting the last tiles, and of each partial result; see tile_plan
 
-struct TilePlan { int size, splits; bool alone; }; // size: 256, 128, 64 (squares) or 32 (64 x 32)
+struct TilePlan {
+    int size;        // 256, 128, 64 (squares) or 32 (64 x 32)
+    int splits;      // shares of the reduction
+    bool alone;      // no CU gets two 128 x 128 tiles
+    int rest_splits; // 256: shares for the tiles behind the last full round, 0 where they are a round like the others
+};
 
 int tune(const char *name)
 {
@@ -394,14 +403,26 @@ int tune(const char *name)
 // keeps 8 steps of 48 at least: the partial results cost a second launch (256 x 10 x 4096, 32 steps: 9.0 us in one
 // share, 7.8 in four, less than the launch's host time).  300 x 300 x 16384: 16 us in 8 shares against 37 in one;
 // with more tiles, splitting lost in each case measured (128 x 4096 x 4096: 14 us against 16 in two shares).
+// 256 x 256 tiles behind the last full round of the CUs would leave most of them idle for a round: where the time says
+// so, these are split over up to eight shares.  That costs two launches and the partial results, 256 KB each that are
+// written and read (REST_US, REST_TILE_US).  In turn: 4200 x 4200 x 16384 294 -> 247 us, 8192 x 4098 x 4096 153 -> 143,
+// the training form of the latter 1143 -> 981; 8192 x 4400 x 4096, 32 steps for 64 tiles, stays as it is at 146.
 TilePlan tile_plan(int M, int N, int kbytes, int pieces)
 {
     const int steps = (kbytes + KSTEP - 1) / KSTEP * pieces;
     auto tiles = [&](int b) { return (int64_t)((M + b - 1) / b) * ((N + b - 1) / b); };
     auto busiest = [&](int b) { return (tiles(b) + CUS - 1) / CUS; };
     const int64_t n256 = busiest(256), n128 = busiest(128), n64 = busiest(64);
-    const double t256 = (double)n256, t128 = n128 == 1 ? 0.37 : 0.61 * (double)(n128 / 2) + 0.44 * (double)(n128 % 2), t64 = 0.08 + 0.11 * (double)n64;
-    TilePlan pl{t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64, 1, n128 == 1};
+    const int64_t rest = tiles(256) % CUS;
+    int rest_splits = 0;
+    double t256 = (double)n256;
+    if (n256 > 1 && rest > 0)
+        for (int n = 2; n <= 8 && n * rest <= CUS && steps / n >= 8; n++) {
+            const double t = (double)(n256 - 1) + 1.0 / n + (REST_US + REST_TILE_US * (double)(n * rest)) / (57.0 / 32 * steps);
+            if (t < t256) { t256 = t; rest_splits = n; }
+        }
+    const double t128 = n128 == 1 ? 0.37 : 0.61 * (double)(n128 / 2) + 0.44 * (double)(n128 % 2), t64 = 0.08 + 0.11 * (double)n64;
+    TilePlan pl{t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64, 1, n128 == 1, 0};
     // 64 x 32 where that still leaves no CU two tiles: the weights are then read by twice as many (from cold weights
     // 64 x 4096 x 4096: 11.4 us against 13.0; 256 x 4096 x 4096, two tiles for a CU: 15.8 against 13.5)
     const int64_t halves = (int64_t)((M + 63) / 64) * ((N + 31) / 32);
@@ -413,30 +434,36 @@ TilePlan tile_plan(int M, int N, int kbytes, int pieces)
         pl.splits = (int)(fill < keep ? fill : keep);
     }
     if (const int t = tune("REXSC_TUNE_INT8_SPLITS")) pl.splits = t;
+    else if (pl.size == 256 && pl.splits == 1) pl.rest_splits = rest_splits;
     pl.splits = pl.splits > steps ? steps : pl.splits > MAX_SPLITS ? MAX_SPLITS : pl.splits;
     if (pl.splits < 1) pl.splits = 1;
     return pl;
 }
 
 template <typename Op, typename T, int BM, int BN, int WM, int WN, int STAGES>
-int launch_one(const TileArgs &p, int splits, void *workspace, hipStream_t stream)
+int launch_one(const TileArgs &p, const TilePlan &pl, void *workspace, hipStream_t stream)
 {
     typedef std::conditional_t<std::is_same_v<Op, OpI8>, int, float> ACC;
     const unsigned tiles = (unsigned)(((p.M + BM - 1) / BM) * (int64_t)((p.N + BN - 1) / BN));
     constexpr bool STREAM = BM == 256; // of the smaller ones a CU holds several, which hide each other's ends
-    if (splits == 1) {
-        const unsigned blocks = STREAM && tiles > CUS ? CUS : tiles;
-        hipLaunchKernelGGL((tile_kernel<Op, T, BM, BN, WM, WN, STAGES, false, STREAM>), dim3(blocks), dim3(WM * WN * 64), 0, stream, p, 1);
+    unsigned whole = pl.splits > 1 ? 0 : tiles;
+    if (STREAM && pl.rest_splits > 1) whole = tiles / CUS * CUS;
+    if (whole > 0) {
+        const unsigned blocks = STREAM && whole > CUS ? CUS : whole;
+        hipLaunchKernelGGL((tile_kernel<Op, T, BM, BN, WM, WN, STAGES, false, STREAM>), dim3(blocks), dim3(WM * WN * 64), 0, stream, p, 1,
+                           0u, whole);
         REXSC_CHECK_HIP(hipGetLastError());
-        return REXSC_OK;
     }
+    if (whole == tiles) return REXSC_OK;
+    const unsigned count = tiles - whole;
+    const int splits = whole > 0 ? pl.rest_splits : pl.splits;
     TileArgs q = p;
     q.y = workspace;
-    hipLaunchKernelGGL((tile_kernel<Op, ACC, BM, BN, WM, WN, STAGES, true, false>), dim3(tiles * splits), dim3(WM * WN * 64), 0, stream, q, splits);
+    hipLaunchKernelGGL((tile_kernel<Op, ACC, BM, BN, WM, WN, STAGES, true, false>), dim3(count * splits), dim3(WM * WN * 64), 0, stream, q,
+                       splits, whole, tiles);
     REXSC_CHECK_HIP(hipGetLastError());
-    const size_t all = (size_t)p.M * p.N;
-    hipLaunchKernelGGL((join_kernel<ACC, T>), dim3((unsigned)((all + 1023) / 1024)), dim3(256), 0, stream, p, (const ACC *)workspace,
-                       splits);
+    hipLaunchKernelGGL((join_kernel<ACC, T>), dim3(count * (BM * BN / 1024)), dim3(256), 0, stream, p, (const ACC *)workspace, splits,
+                       whole, count, BM, BN);
     REXSC_CHECK_HIP(hipGetLastError());
     return REXSC_OK;
 }
@@ -444,11 +471,11 @@ int launch_one(const TileArgs &p, int splits, void *workspace, hipStream_t strea
 template <typename Op, typename T>
 int launch_size(const TileArgs &p, const TilePlan &pl, void *workspace, hipStream_t stream)
 {
-    if (pl.size == 256) return launch_one<Op, T, 256, 256, 2, 4, 2>(p, pl.splits, workspace, stream);
-    if (pl.size == 128 && pl.alone) return launch_one<Op, T, 128, 128, 2, 4, 4>(p, pl.splits, workspace, stream);
-    if (pl.size == 128) return launch_one<Op, T, 128, 128, 2, 2, 2>(p, pl.splits, workspace, stream);
-    if (pl.size == 32) return launch_one<Op, T, 64, 32, 2, 2, 4>(p, pl.splits, workspace, stream);
-    return launch_one<Op, T, 64, 64, 2, 2, 4>(p, pl.splits, workspace, stream);
+    if (pl.size == 256) return launch_one<Op, T, 256, 256, 2, 4, 2>(p, pl, workspace, stream);
+    if (pl.size == 128 && pl.alone) return launch_one<Op, T, 128, 128, 2, 4, 4>(p, pl, workspace, stream);
+    if (pl.size == 128) return launch_one<Op, T, 128, 128, 2, 2, 2>(p, pl, workspace, stream);
+    if (pl.size == 32) return launch_one<Op, T, 64, 32, 2, 2, 4>(p, pl, workspace, stream);
+    return launch_one<Op, T, 64, 64, 2, 2, 4>(p, pl, workspace, stream);
 }
 
 } // namespace
@@ -457,7 +484,9 @@ size_t tile_product_workspace(int M, int N, int kbytes, int pieces)
 {
     if (M == 0 || N == 0) return 0;
     const TilePlan pl = tile_plan(M, N, kbytes, pieces);
-    return pl.splits > 1 ? (size_t)pl.splits * M * N * 4 : 0;
+    const int64_t bm = pl.size == 32 ? 64 : pl.size, tiles = ((M + bm - 1) / bm) * (((int64_t)N + pl.size - 1) / pl.size);
+    const int64_t parts = pl.splits > 1 ? tiles * pl.splits : tiles % CUS * pl.rest_splits; // tiles of partial results
+    return (size_t)(parts * bm * pl.size) * 4;
 }
 
 int launch_tile_product(const TileArgs &p, bool f16, int out_dtype, void *workspace, const char *name, hipStream_t stream)

@@ -435,6 +435,39 @@ def test_more_large_tiles_than_blocks(dt, n, k, monkeypatch):
     _close_or_over(y, prod, want, dt)
 
 
+@pytest.mark.parametrize("dt,n", [(torch.bfloat16, 4104), (torch.float16, 4101), (torch.float32, 4099)])
+@pytest.mark.parametrize("k", [8192, 8205])
+def test_last_tiles_split_over_the_reduction(dt, n, k, monkeypatch):
+    """4353 x 4100 is one round of 256 tiles and 50 more, which are summed in shares."""
+    import sc_functional as F
+    m = 4353
+    gen = torch.Generator(device="cuda").manual_seed(n + k)
+    pitch = -(-k // 128) * 128
+    a, b = (torch.randint(-127, 128, (r, pitch), device="cuda", dtype=torch.int8, generator=gen)[:, :k] for r in (m, n))
+    sa, sb = ((torch.rand(r, device="cuda", generator=gen) + 0.5) / 100 for r in (m, n))
+    bias = torch.randn(n, device="cuda", generator=gen).to(dt)
+    monkeypatch.setenv("REXSC_TUNE_INT8_TILE", "256")
+    y = F.matmul_int8(a, sa, b, sb, bias, out_dtype=dt)
+    prod = (a.double() @ b.double().t().contiguous()) * sa.double()[:, None] * sb.double()
+    _close_or_over(y, prod, prod + bias.double(), dt)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_gradients_whose_last_tiles_are_split(dt, monkeypatch):
+    """As test_gradients_of_integers_are_exact, dx of 306 tiles and 66 or 33 steps."""
+    import sc_functional as F
+    m, n, k = 4353, 2100, 4100
+    monkeypatch.setenv("REXSC_TUNE_INT8_TILE", "256")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    ints = lambda top, *shape: torch.randint(-top, top + 1, shape, device="cuda", generator=g).float()
+    x, w, go = ints(60, m, k), ints(60, n, k), ints(8, m, n)
+    x[:, 0], w[:, k - 1] = 127, -127
+    xt, wt = x.to(dt).requires_grad_(True), w.clone().requires_grad_(True)
+    dx, dw = torch.autograd.grad(F.linear_int8(xt, wt), [xt, wt], go.to(dt))
+    assert torch.equal(dx, (go.double() @ w.double()).float().to(dt))
+    assert torch.equal(dw.double(), go.double().t().contiguous() @ x.double())
+
+
 @pytest.mark.parametrize("m,n", [(4353, 4100), (1100, 900)])
 @pytest.mark.parametrize("k", [100, 385, 1100])
 def test_tiles_of_128_alone_on_a_cu_and_not(m, n, k, monkeypatch):
