@@ -1013,7 +1013,8 @@ def layer_norm_backward(grad_output, m, w, stats, rest, need_x=True, weight_dtyp
             nbytes = L.rexsc_layer_norm_backward_workspace_bytes(d)
             if nbytes == _NO_BYTES:
                 _lib.check(-1, "rexsc_layer_norm_backward (planning)")
-            ws = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+            if nbytes:
+                ws = torch.empty((nbytes,), dtype=torch.uint8, device=device)
         mean = stats.data_ptr()
         rc = L.rexsc_layer_norm_backward(d, g.data_ptr(), m.data_ptr(), _addr(w), mean, mean + 4 * R, _addr(dx), _addr(dw),
                                          _addr(db), _addr(ws), nbytes, _raw_stream(dev))

@@ -254,6 +254,62 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void norm_backward_kernel(No
     }
 }
 
+// ---- few short rows ------------------------------------------------------------------------------
+// The whole backward pass in one launch: a wave per row for dx, and blocks of 16 columns that take dw and db over all
+// rows, 16 groups of them joined in order.  x and g are read three times, but from L2, and a launch, an allocation and the
+// partial sums are saved, which is what such a call's time goes to.
+constexpr int SMALL_ROWS = 512, SMALL_COLS = 2048;
+template <typename T>
+__global__ __launch_bounds__(256) void norm_backward_small_kernel(NormParams p, void *dw_out, void *db_out, unsigned row_blocks)
+{
+    __shared__ float lds[2][16][17];
+    const T *const x = (const T *)p.x, *const g = (const T *)p.g;
+    if (blockIdx.x < row_blocks) {
+        const size_t row = (size_t)blockIdx.x * 4 + threadIdx.x / 64;
+        if (row >= p.rows) return;
+        const int lane = threadIdx.x % 64;
+        const T *sx = x + row * p.x_stride, *sg = g + row * (size_t)p.cols;
+        const float mu = p.mean[row], r = p.rstd[row], inv = 1.0f / (float)p.cols;
+        float s[2] = {0.f, 0.f};
+#pragma unroll 4
+        for (int c = lane; c < p.cols; c += 64) {
+            const float gw = (float)sg[c] * (p.w ? load_any(p.w, p.w_dtype, c) : 1.f);
+            s[0] += gw;
+            s[1] = fmaf(gw, ((float)sx[c] - mu) * r, s[1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int o = 32; o; o >>= 1) s[i] += __shfl_xor(s[i], o, 64);
+        const float m0 = s[0] * inv, m1 = s[1] * inv;
+        T *dst = (T *)p.dx + row * (size_t)p.cols;
+#pragma unroll 4
+        for (int c = lane; c < p.cols; c += 64) {
+            const float gw = (float)sg[c] * (p.w ? load_any(p.w, p.w_dtype, c) : 1.f);
+            dst[c] = (T)(r * (gw - m0 - ((float)sx[c] - mu) * r * m1));
+        }
+        return;
+    }
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, c = (int)(blockIdx.x - row_blocks) * 16 + tx;
+    float dw = 0.f, db = 0.f;
+    if (c < p.cols)
+#pragma unroll 4
+        for (size_t row = ty; row < p.rows; row += 16) {
+            const float gv = (float)g[row * (size_t)p.cols + c];
+            dw = fmaf(gv, ((float)x[row * p.x_stride + c] - p.mean[row]) * p.rstd[row], dw);
+            db += gv;
+        }
+    lds[0][ty][tx] = dw;
+    lds[1][ty][tx] = db;
+    __syncthreads();
+    if (ty > 1 || c >= p.cols) return;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) sum += lds[ty][i][tx];
+    void *const out = ty ? db_out : dw_out;
+    if (out) store_any(out, p.w_dtype, c, sum);
+}
+
 // ---- rows of any length --------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(STREAM_THREADS) void norm_forward_stream_kernel(NormParams p)
@@ -494,6 +550,8 @@ template <typename T> bool launch_bwd(const NormPlan &pl, const NormParams &p, h
     return true;
 }
 
+bool small_backward(const rexsc_norm_desc *d) { return d->rows <= SMALL_ROWS && d->cols <= SMALL_COLS; }
+
 int bwd_blocks(const rexsc_norm_desc *d)
 {
     if (d->cols <= LONGEST) return norm_plan(d, false, true).grid;
@@ -551,6 +609,7 @@ extern "C" int rexsc_layer_norm_forward(const rexsc_norm_desc *d, const void *x,
 extern "C" size_t rexsc_layer_norm_backward_workspace_bytes(const rexsc_norm_desc *d)
 {
     if (check_norm(d)) return (size_t)-1;
+    if (small_backward(d)) return 0;
     return (size_t)bwd_blocks(d) * 2 * (size_t)d->cols * sizeof(float);
 }
 
@@ -568,6 +627,16 @@ extern "C" int rexsc_layer_norm_backward(const rexsc_norm_desc *d, const void *g
     REXSC_CHECK_ARG(grad_out && x && mean && rstd, "null pointer");
     REXSC_CHECK_ARG((((uintptr_t)x | (uintptr_t)grad_out | (uintptr_t)dx) % es) == 0,
                     "layer norm: a tensor is not aligned to its element");
+    if (small_backward(d)) {
+        const NormParams p{x, weight, nullptr, grad_out, nullptr, dx, const_cast<float *>(mean), const_cast<float *>(rstd), nullptr,
+                           (size_t)d->rows, (size_t)d->x_stride, (int)d->cols, d->weight_dtype, d->eps};
+        const unsigned row_blocks = dx ? (unsigned)((d->rows + 3) / 4) : 0, col_blocks = sums ? (unsigned)((cols + 15) / 16) : 0;
+        ProfScope prof("layer_norm_backward", (dx ? 3.0 : 2.0) * es * d->rows * d->cols, stream);
+        REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL(norm_backward_small_kernel<T>, dim3(row_blocks + col_blocks), dim3(256), 0, stream,
+                                                        p, dw, db, row_blocks));
+        REXSC_CHECK_HIP(hipGetLastError());
+        return REXSC_OK;
+    }
     const size_t need = rexsc_layer_norm_backward_workspace_bytes(d);
     if (sums && (!workspace || workspace_bytes < need)) {
         set_error("layer norm: workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
