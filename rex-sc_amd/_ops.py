@@ -674,9 +674,11 @@ def calib_stats(a_bit, a_act, win_lo, win_hi):
 # ---- 8-bit linear layer --------------------------------------------------------------------------
 
 # These calls are short enough on the GPU for the host's share to count: pointers go over as plain integers, the stream
-# as the raw handle, and the current device is switched only where it is another one.
+# as the raw handle, the current device is switched only where it is another one, and sizes are given to torch.empty one
+# by one (1.7 us against 2.5 for a tuple and 7 for a torch.Size).
 _DTYPE_CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice  # (where there is a CUDA tensor, the device is initialised)
 
 
 class _SameDevice:
@@ -692,7 +694,7 @@ _same = _SameDevice()
 
 def _on(index):
     """Context in which device `index` is the current one."""
-    return _same if torch.cuda.current_device() == index else torch.cuda.device(index)
+    return _same if _current_device() == index else torch.cuda.device(index)
 
 
 def _addr(t):
@@ -742,8 +744,8 @@ def quantize_rows(x):
     pad = -(-K // ROW_PAD) * ROW_PAD
     dev = x.get_device()
     with _on(dev):
-        q = torch.empty((R, pad), dtype=torch.int8, device=x.device)
-        scale = torch.empty((R,), dtype=torch.float32, device=x.device)
+        q = torch.empty(R, pad, dtype=torch.int8, device=x.device)
+        scale = torch.empty(R, dtype=torch.float32, device=x.device)
         rc = _lib.lib().rexsc_quantize_rows(m.data_ptr(), code, R, K, _row_stride(m), q.data_ptr(), pad, scale.data_ptr(),
                                             _raw_stream(dev))
         if rc:
@@ -769,7 +771,7 @@ def _operand8(t, what):
         if K % 16 == 0 or R == 0 or t.storage_offset() + (R - 1) * step + -(-K // 16) * 16 <= t.untyped_storage().nbytes():
             return t, step
     pad = -(-K // ROW_PAD) * ROW_PAD
-    out = torch.empty((R, pad), dtype=torch.int8, device=t.device)[:, :K]
+    out = torch.empty(R, pad, dtype=torch.int8, device=t.device)[:, :K]
     out.copy_(t)  # what lies behind the K-th byte does not matter
     return out, pad
 
@@ -799,7 +801,7 @@ def _int8_space(L, d, what, device):
         return None, 0
     if nbytes == _NO_BYTES:
         _lib.check(-1, "rexsc_int8_linear (planning)")
-    return torch.empty((nbytes,), dtype=torch.uint8, device=device), nbytes
+    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
 
 
 def matmul_int8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
@@ -821,7 +823,7 @@ def matmul_int8(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
         a, sa = _operand8(a, "matmul_int8")
         b, sb = _operand8(b, "matmul_int8")
         d = _lib.Int8Desc.packed(M, N, K, _dtype_code(out_dtype, "matmul_int8"), bias_code, 0, 0, 0, sa, sb)
-        y = torch.empty((M, N), dtype=out_dtype, device=device)
+        y = torch.empty(M, N, dtype=out_dtype, device=device)
         ws, nbytes = _int8_space(L, d, _lib.INT8_PRODUCT, device)
         rc = L.rexsc_int8_product(d, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), _addr(bias),
                                   y.data_ptr(), _addr(ws), nbytes, _raw_stream(dev))
@@ -850,7 +852,7 @@ def int8_linear(x, wq, w_scale, bias=None):
     with _on(dev):
         wq, sb = _operand8(wq, "linear_int8")
         d = _lib.Int8Desc.packed(M, N, K, code, bias_code, 0, 0, _row_stride(m), 0, sb)
-        y = torch.empty(shape[:-1] + (N,), dtype=x.dtype, device=device)
+        y = torch.empty(*shape[:-1], N, dtype=x.dtype, device=device)
         ws, nbytes = _int8_space(L, d, _lib.INT8_LINEAR, device)
         rc = L.rexsc_int8_linear(d, m.data_ptr(), wq.data_ptr(), w_scale.data_ptr(), _addr(bias), y.data_ptr(), _addr(ws),
                                  nbytes, _raw_stream(dev))
@@ -878,15 +880,15 @@ def int8_linear_train(x, w, bias):
     L = _lib.lib()
     with _on(dev):
         stream = _raw_stream(dev)
-        q = torch.empty((M + N, pad), dtype=torch.int8, device=device)
-        scales = torch.empty((M + N,), dtype=torch.float32, device=device)
+        q = torch.empty(M + N, pad, dtype=torch.int8, device=device)
+        scales = torch.empty(M + N, dtype=torch.float32, device=device)
         xq, xs = q.data_ptr(), scales.data_ptr()
         wq, ws = xq + M * pad, xs + 4 * M
         rc = L.rexsc_quantize_rows(xm.data_ptr(), code, M, K, _row_stride(xm), xq, pad, xs, stream)
         rc = rc or L.rexsc_quantize_rows(wm.data_ptr(), w_code, N, K, _row_stride(wm), wq, pad, ws, stream)
         if rc:
             _lib.check(rc, "rexsc_quantize_rows")
-        y = torch.empty(shape[:-1] + (N,), dtype=x.dtype, device=device)
+        y = torch.empty(*shape[:-1], N, dtype=x.dtype, device=device)
         d = _lib.Int8Desc.packed(M, N, K, code, bias_code, 0, 0, 0, pad, pad)
         space, nbytes = _int8_space(L, d, _lib.INT8_PRODUCT, device)
         rc = L.rexsc_int8_product(d, xq, xs, wq, ws, _addr(bias), y.data_ptr(), _addr(space), nbytes, stream)
@@ -919,12 +921,12 @@ def int8_backward(g, xq, x_scale, wq, w_scale, need_x, weight_dtype, bias_dtype)
         dx = dw = db = None
         if need_x:
             wq, sb = _operand8(wq, "linear_int8")
-            dx = torch.empty(g.shape[:-1] + (K,), dtype=g.dtype, device=device)
+            dx = torch.empty(*g.shape[:-1], K, dtype=g.dtype, device=device)
         if weight_dtype is not None:
             xq, sa = _operand8(xq, "linear_int8")
-            dw = torch.empty((N, K), dtype=weight_dtype, device=device)
+            dw = torch.empty(N, K, dtype=weight_dtype, device=device)
         if bias_dtype is not None:
-            db = torch.empty((N,), dtype=bias_dtype, device=device)
+            db = torch.empty(N, dtype=bias_dtype, device=device)
         d = _lib.Int8Desc.packed(M, N, K, code, 0 if db is None else _dtype_code(db, "linear_int8"),
                                  0 if dw is None else _dtype_code(dw, "linear_int8"), 0, 0, sa, sb)
         ws, nbytes = _int8_space(L, d, _lib.INT8_BACKWARD, device)
@@ -968,10 +970,10 @@ def layer_norm_forward(x, weight, bias, eps, want_stats=True):
     m = _rows_of(x)
     R, D = m.shape
     with _on(dev):
-        y = torch.empty(shape, dtype=x.dtype, device=device)
+        y = torch.empty(*shape, dtype=x.dtype, device=device)
         stats, mean, rstd = None, None, None
         if want_stats:
-            stats = torch.empty((2, R), dtype=torch.float32, device=device)
+            stats = torch.empty(2, R, dtype=torch.float32, device=device)
             mean = stats.data_ptr()
             rstd = mean + 4 * R
         d = _lib.NormDesc.packed(code, _DTYPE_CODE[wdt], eps, R, D, _row_stride(m))
@@ -1005,16 +1007,16 @@ def layer_norm_backward(grad_output, m, w, stats, rest, need_x=True, weight_dtyp
         w = None if w is None else w.to(sum_dt)
     L = _lib.lib()
     with _on(dev):
-        dx = torch.empty(shape, dtype=dtype, device=device) if need_x else None
-        dw = torch.empty((D,), dtype=sum_dt, device=device) if weight_dtype is not None else None
-        db = torch.empty((D,), dtype=sum_dt, device=device) if bias_dtype is not None else None
+        dx = torch.empty(*shape, dtype=dtype, device=device) if need_x else None
+        dw = torch.empty(D, dtype=sum_dt, device=device) if weight_dtype is not None else None
+        db = torch.empty(D, dtype=sum_dt, device=device) if bias_dtype is not None else None
         ws, nbytes = None, 0
         if wanted:
             nbytes = L.rexsc_layer_norm_backward_workspace_bytes(d)
             if nbytes == _NO_BYTES:
                 _lib.check(-1, "rexsc_layer_norm_backward (planning)")
             if nbytes:
-                ws = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         mean = stats.data_ptr()
         rc = L.rexsc_layer_norm_backward(d, g.data_ptr(), m.data_ptr(), _addr(w), mean, mean + 4 * R, _addr(dx), _addr(dw),
                                          _addr(db), _addr(ws), nbytes, _raw_stream(dev))

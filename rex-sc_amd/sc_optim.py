@@ -107,7 +107,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales=None, exp_av
     d = _lib.AdamwDesc.packed(code, 8 if eight else 32, int(clamp is not None), float(lr), float(beta1), float(beta2), float(eps),
                        float(weight_decay), lo, hi, 0 if on_device else int(step))
     with _ops._on(dev):
-        coef = torch.empty((_lib.ADAMW_COEF_BYTES,), dtype=torch.uint8, device=first.device) if on_device else None
+        coef = torch.empty(_lib.ADAMW_COEF_BYTES, dtype=torch.uint8, device=first.device) if on_device else None
         rc = _lib.lib().rexsc_adamw_step(d, table.buffer_info()[0], len(params),
                                          _ops._addr(step if on_device else None), _ops._addr(grad_scale),
                                          _ops._addr(found_inf), _ops._addr(coef), _ops._raw_stream(dev))

@@ -108,6 +108,12 @@ def test_rows_inside_another_matrix(dt, d):
         close(got, ref[name], t, name)
 
 
+@pytest.mark.parametrize("dt,wdt", [(torch.float32, torch.float32), (torch.float16, torch.float32), (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("rows,d", [(511, 33), (512, 2048), (513, 33), (512, 2049), (4, 2047), (15, 16), (17, 17), (100, 1), (1, 2048)])
+def test_around_the_backward_pass_in_one_launch(dt, wdt, rows, d):
+    test_forward_and_gradients(dt, wdt, rows, d)
+
+
 @pytest.mark.parametrize("d", [48, 1003, 5000])
 def test_without_weight_or_bias_and_partial_gradients(d):
     import sc_functional as F

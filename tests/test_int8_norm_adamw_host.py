@@ -100,10 +100,13 @@ def test_layer_norm_refusals():
         assert fwd(d, **kw) == -1 and text in _error(L), text
     assert fwd(D(rows=0), x=None, y=None) == 0
     bytes_ = L.rexsc_layer_norm_backward_workspace_bytes
-    assert bytes_(ctypes.byref(D())) >= 2 * 8 * 4 and bytes_(ctypes.byref(D(cols=0))) == ctypes.c_size_t(-1).value
+    many = D(rows=513)  # up to 512 short rows need no partial sums
+    assert bytes_(ctypes.byref(many)) >= 2 * 8 * 4 and bytes_(ctypes.byref(D())) == 0
+    assert bytes_(ctypes.byref(D(cols=2049, xs=2049))) >= 2 * 2049 * 4
+    assert bytes_(ctypes.byref(D(cols=0))) == ctypes.c_size_t(-1).value
     bwd = lambda d, g=FAKE, dx=FAKE, dw=FAKE, ws=None, n=0: L.rexsc_layer_norm_backward(
         ctypes.byref(d), g, FAKE, FAKE, FAKE, FAKE, dx, dw, None, ws, n, None)
-    assert bwd(D()) == -2 and "workspace" in _error(L)
+    assert bwd(many) == -2 and "workspace" in _error(L)
     assert bwd(D(), g=None) == -1 and "null" in _error(L)
     assert bwd(D(), dx=None, dw=None) == 0
 
