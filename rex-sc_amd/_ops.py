@@ -862,7 +862,8 @@ def int8_linear(x, wq, w_scale, bias=None):
 
 
 def int8_linear_train(x, w, bias):
-    """int8_linear with a float weight, both operands' 8-bit forms kept for int8_backward: (y, xq, x_scale, wq, w_scale)."""
+    """int8_linear with a float weight, both operands' 8-bit forms kept for int8_train_backward: (y, q, scales), the
+    rows of x and behind them those of w in one matrix of rows padded to 128 bytes."""
     if not (x.is_cuda and w.is_cuda):
         _require_cuda(x, w)
     _same_device("linear_int8", x, w, bias)
@@ -894,7 +895,7 @@ def int8_linear_train(x, w, bias):
         rc = L.rexsc_int8_product(d, xq, xs, wq, ws, _addr(bias), y.data_ptr(), _addr(space), nbytes, stream)
         if rc:
             _lib.check(rc, "rexsc_int8_product")
-    return y, q[:M, :K], scales[:M], q[M:, :K], scales[M:]
+    return y, q, scales
 
 
 def _dense_rows(g, n):
@@ -904,37 +905,46 @@ def _dense_rows(g, n):
     return g if g.is_contiguous() else g.contiguous()
 
 
-def int8_backward(g, xq, x_scale, wq, w_scale, need_x, weight_dtype, bias_dtype):
-    """Straight-through gradients of y = x W^T + bias in 8 bits, given those of y: (dx [..., K] in g's type or None, dw [N, K]
-    of weight_dtype, db [N] of bias_dtype); a type of None: not wanted.  xq and x_scale are read for dw only."""
-    if not (g.is_cuda and wq.is_cuda):
-        _require_cuda(g, wq)
-    _same_device("linear_int8", g, wq, xq)
+def _int8_gradients(g, N, K, a, a_stride, a_scale, b, b_stride, b_scale, need_x, weight_dtype, bias_dtype):
+    """(dx [..., K] in g's type or None, dw [N, K] of weight_dtype, db [N] of bias_dtype) from addresses of the operands' 8-bit
+    forms; a type of None: not wanted.  a (the tokens) is read for dw only."""
     code = _dtype_code(g, "linear_int8")
-    N, K = wq.shape
     gm = _dense_rows(g, N)
-    M = gm.shape[0]
     device, dev = g.device, g.get_device()
     L = _lib.lib()
     with _on(dev):
-        sa = sb = 0
-        dx = dw = db = None
-        if need_x:
-            wq, sb = _operand8(wq, "linear_int8")
-            dx = torch.empty(*g.shape[:-1], K, dtype=g.dtype, device=device)
-        if weight_dtype is not None:
-            xq, sa = _operand8(xq, "linear_int8")
-            dw = torch.empty(N, K, dtype=weight_dtype, device=device)
-        if bias_dtype is not None:
-            db = torch.empty(N, dtype=bias_dtype, device=device)
-        d = _lib.Int8Desc.packed(M, N, K, code, 0 if db is None else _dtype_code(db, "linear_int8"),
-                                 0 if dw is None else _dtype_code(dw, "linear_int8"), 0, 0, sa, sb)
+        dx = torch.empty(*g.shape[:-1], K, dtype=g.dtype, device=device) if need_x else None
+        dw = torch.empty(N, K, dtype=weight_dtype, device=device) if weight_dtype is not None else None
+        db = torch.empty(N, dtype=bias_dtype, device=device) if bias_dtype is not None else None
+        d = _lib.Int8Desc.packed(gm.shape[0], N, K, code, 0 if db is None else _dtype_code(db, "linear_int8"),
+                                 0 if dw is None else _dtype_code(dw, "linear_int8"), 0, 0, a_stride, b_stride)
         ws, nbytes = _int8_space(L, d, _lib.INT8_BACKWARD, device)
-        rc = L.rexsc_int8_backward(d, gm.data_ptr(), _addr(xq), _addr(x_scale), wq.data_ptr(), w_scale.data_ptr(), _addr(dx),
-                                   _addr(dw), _addr(db), _addr(ws), nbytes, _raw_stream(dev))
+        rc = L.rexsc_int8_backward(d, gm.data_ptr(), a, a_scale, b, b_scale, _addr(dx), _addr(dw), _addr(db), _addr(ws), nbytes,
+                                   _raw_stream(dev))
         if rc:
             _lib.check(rc, "rexsc_int8_backward")
     return dx, dw, db
+
+
+def int8_backward(g, wq, w_scale, need_x, bias_dtype):
+    """Straight-through gradients of y = x W^T + bias with 8-bit weights, given those of y: (dx, db), see _int8_gradients."""
+    if not (g.is_cuda and wq.is_cuda):
+        _require_cuda(g, wq)
+    _same_device("linear_int8", g, wq)
+    N, K = wq.shape
+    with _on(g.get_device()):
+        wq, stride = _operand8(wq, "linear_int8")
+    dx, _, db = _int8_gradients(g, N, K, None, 0, None, wq.data_ptr(), stride, w_scale.data_ptr(), need_x, None, bias_dtype)
+    return dx, db
+
+
+def int8_train_backward(g, q, scales, N, K, need_x, weight_dtype, bias_dtype):
+    """The gradients of int8_linear_train: (dx, dw, db), see _int8_gradients."""
+    if g.get_device() != q.get_device():
+        _same_device("linear_int8", g, q)
+    R, pad = q.shape
+    a, a_scale = q.data_ptr(), scales.data_ptr()
+    return _int8_gradients(g, N, K, a, pad, a_scale, a + (R - N) * pad, pad, a_scale + (R - N) * 4, need_x, weight_dtype, bias_dtype)
 
 
 # ---- layer norm ----------------------------------------------------------------------------------

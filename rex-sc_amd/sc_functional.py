@@ -718,14 +718,14 @@ class Linear_Int8_Grad(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, weight_scale):
-        ctx.types = (weight.dtype if weight_scale is None else None, None if bias is None else bias.dtype)
-        if ctx.needs_input_grad[1]:  # the tokens are wanted in 8 bits again by the backward pass
-            y, xq, xs, wq, ws = _ops.int8_linear_train(x, weight, bias)
-            ctx.save_for_backward(wq, ws, xq, xs)
+        ctx.rest = (*weight.shape, weight.dtype, None if bias is None else bias.dtype)
+        ctx.trains = ctx.needs_input_grad[1]
+        if ctx.trains:  # the tokens are wanted in 8 bits again by the backward pass
+            y, *saved = _ops.int8_linear_train(x, weight, bias)
         else:
-            wq, ws = _ops.quantize_rows(weight) if weight_scale is None else (weight, weight_scale)
-            y = _ops.int8_linear(x, wq, ws, bias)
-            ctx.save_for_backward(wq, ws, None, None)
+            saved = _ops.quantize_rows(weight) if weight_scale is None else (weight, weight_scale)
+            y = _ops.int8_linear(x, *saved, bias)
+        ctx.save_for_backward(*saved)
         return y
 
     @staticmethod
@@ -734,12 +734,14 @@ class Linear_Int8_Grad(torch.autograd.Function):
 
 
 def _linear_int8_backward(ctx, grad_output):
-    wq, ws, xq, xs = ctx.saved_tensors
-    w_dtype, b_dtype = ctx.types
+    q, scales = ctx.saved_tensors
+    n, k, w_dtype, b_dtype = ctx.rest
     need_x, need_w, need_b, _ = ctx.needs_input_grad
-    dx, dw, db = _ops.int8_backward(grad_output, xq, xs, wq, ws, need_x, w_dtype if need_w else None,
-                                    b_dtype if need_b else None)
-    return dx, dw, db, None
+    b_dtype = b_dtype if need_b else None
+    if ctx.trains:
+        return (*_ops.int8_train_backward(grad_output, q, scales, n, k, need_x, w_dtype if need_w else None, b_dtype), None)
+    dx, db = _ops.int8_backward(grad_output, q, scales, need_x, b_dtype)
+    return dx, None, db, None
 
 
 _linear_int8_once = torch.autograd.function.once_differentiable(_linear_int8_backward)
