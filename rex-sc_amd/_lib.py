@@ -4,6 +4,7 @@ The library is the only compute path: if it is missing, or an entry point fails,
 gets a RuntimeError -- there is no Python/CPU fallback.
 """
 import ctypes
+import functools
 import os
 import struct
 
@@ -25,14 +26,14 @@ class _Desc(ctypes.Structure):
     def key(self):
         return tuple(getattr(self, f[0]) for f in self._fields_)
 
-    @classmethod
-    def packed(cls, *args):
-        """The same descriptor as bytes, for calls where building the structure would be a good part of the call."""
-        if "_packer" not in cls.__dict__:
-            codes = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_double: "d"}
-            cls._packer = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_))
-            assert cls._packer.size == ctypes.sizeof(cls)
-        return cls._packer.pack(cls._packer.size, *args)
+
+def _packer(cls):
+    """Function that makes the same descriptor as bytes, for calls where building the structure would be a good part of the
+    call; arguments as the structure's."""
+    codes = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_double: "d"}
+    s = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_))
+    assert s.size == ctypes.sizeof(cls)
+    return functools.partial(s.pack, s.size)
 
 
 class ConvDesc(_Desc):
@@ -71,6 +72,8 @@ class AdamwDesc(_Desc):
         (n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "clamp_lo", "clamp_hi")] + [
         ("step", ctypes.c_int64)]
 
+
+Int8Desc.packed, NormDesc.packed, AdamwDesc.packed = map(_packer, (Int8Desc, NormDesc, AdamwDesc))
 
 # rexsc_adamw_tensor is seven 8-byte fields (param, grad, exp_avg, exp_avg_sq, their scales, numel): a table of them is
 # handed over as one array of integers

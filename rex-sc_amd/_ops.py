@@ -721,6 +721,8 @@ def _same_device(what, first, *rest):
 def _rows_of(t):
     """t [..., K] as a matrix whose rows lie at one distance and whose elements are neighbours (a view where t has such
     a layout, else a copy)."""
+    if t.is_contiguous():
+        return t if t.dim() == 2 else t.view(-1, t.shape[-1])
     m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     if m.shape[1] > 1 and m.stride(1) != 1 or m.shape[0] > 1 and m.stride(0) < m.shape[1]:
         m = m.contiguous()
@@ -951,6 +953,11 @@ def int8_train_backward(g, q, scales, N, K, need_x, weight_dtype, bias_dtype):
 
 def _norm_vectors(x, weight, bias, dtype=None):
     """(weight, bias, their type) as the kernels read them: one type for both, float32 or x's (dtype: that one)."""
+    if dtype is None and weight is not None and bias is not None:  # the usual case in few calls
+        dt = weight.dtype
+        if (dt == bias.dtype and (dt == torch.float32 or dt == x.dtype) and weight.dim() == 1 and bias.dim() == 1
+                and weight.numel() == bias.numel() == x.shape[-1] and weight.is_contiguous() and bias.is_contiguous()):
+            return weight, bias, dt
     same = dtype is None
     for t in (weight, bias):
         if t is not None:
