@@ -369,7 +369,10 @@ int rexsc_layer_norm_backward(const rexsc_norm_desc *d, const void *grad_out, co
  * in float32, p rounded to its type.  state_bits 32: m and v are float32.  state_bits 8: they are e4m3 values (one
  * sign, four exponent, three mantissa bits; largest 448) with one float32 scale for every 256 consecutive elements,
  *   m = value * scale with scale = max |m| / 448,   sqrt(v) = value * scale with scale = max sqrt(v) / 448,
- * the update using m and v as computed, before they are rounded to 8 bits.  A positive v never becomes 0 there: its
+ * the update using m and v as computed, before they are rounded to 8 bits.  What is stored is defined bit for bit: each
+ * operation of b1 (value scale) + (1 - b1) g and of b2 (value scale)^2 + (1 - b2) (g g) is rounded to float32, the root
+ * correctly; the scale is the largest magnitude times the float32 nearest to 1 / 448; a value is the e4m3 number nearest
+ * to the float32 quotient of m, or of the root, and the scale, ties to even.  A positive v never becomes 0 there: its
  * root is at least the smallest value, 2^-9, so that no element is divided by eps alone.  A block whose largest
  * magnitude is below 2^-100 is stored as zeros; a block that takes in a NaN or an infinity is lost as a whole. */
 typedef struct rexsc_adamw_tensor {

@@ -7,12 +7,13 @@
 // in its kernel arguments (nothing is copied to the device first, and a captured launch keeps its table), and a
 // workgroup finds the tensor its chunk belongs to by bisection over the chunks' running count.
 // Measured: 11.7 M float32 values in 62 tensors, 32-bit states, 59-70 us (5.6-4.7 TB/s, part of them still in the
-// memory-side cache); 268 M bfloat16 values, 8-bit states, 524 us (5.1 TB/s); a copy of 1 GiB reaches 5.1 TB/s.
+// memory-side cache); 268 M bfloat16 values, 8-bit states, 515 us (5.2 TB/s); a copy of 1 GiB reaches 5.1 TB/s.
 //
 // 8-bit states: a wave holds two blocks of the 256 elements that share a scale, eight elements per lane, so a block's
 // maximum is a reduction over 32 lanes and the conversion to and from e4m3 is the hardware's, two values an instruction.
-// At 10 bytes an element the arithmetic counts as well: quotient and root are the hardware's approximations, good to one
-// step of float32, where correctly rounded ones would be some 20 instructions an element more.
+// At 10 bytes an element the arithmetic counts as well: the update's quotient and root are the hardware's approximations,
+// good to one step of float32, where correctly rounded ones would be some 20 instructions an element more.  What is stored
+// in 8 bits is decided as the definition has it all the same (store8).
 #include <math.h>
 
 #include "lowp.h"
@@ -27,6 +28,7 @@ constexpr int CHUNK = 4096;                 // elements a workgroup takes
 constexpr float E4M3_MAX = 448.f;
 constexpr float E4M3_MIN = 0.001953125f;    // 2^-9, the smallest positive value
 constexpr float TINY = 7.888609052210118e-31f; // 2^-100: a block below it is stored as zeros (1 / scale stays finite)
+constexpr float EPS = 9.5367431640625e-07f;    // 2^-20, see store8
 
 struct Coef { float step_size, inv_root_bc2, inv_grad_scale, skip; };
 
@@ -152,14 +154,16 @@ __device__ __forceinline__ void from_e4m3(float (&v)[V], const unsigned (&q)[V /
     }
 }
 
-// Scale of a block whose largest magnitude has these bits, and what its elements are multiplied by.  A block with a
-// NaN or an infinity gets scale NaN, which its elements then become.
-__device__ __forceinline__ void block_scale(unsigned top_bits, float &scale, float &inv)
+// A block's scale, from the bits of its largest magnitude, and its reciprocal from below and from above, see store8.  A
+// block with a NaN or an infinity gets scale NaN, which its elements then become.
+struct BlockScale { float scale, low, high; };
+__device__ __forceinline__ BlockScale block_scale(unsigned top_bits)
 {
     const float top = __uint_as_float(top_bits);
-    if (top_bits >= 0x7f800000u) { scale = __uint_as_float(0x7fc00000u); inv = 0.f; }
-    else if (top < TINY) { scale = 0.f; inv = 0.f; }
-    else { scale = top / E4M3_MAX; inv = E4M3_MAX / top; }
+    if (top_bits >= 0x7f800000u) return BlockScale{__uint_as_float(0x7fc00000u), 0.f, 0.f};
+    if (top < TINY) return BlockScale{0.f, 0.f, 0.f};
+    const float scale = top * (1.0f / E4M3_MAX), inv = 1.0f / scale;
+    return BlockScale{scale, inv * (1.0f - EPS), inv * (1.0f + EPS)};
 }
 
 constexpr int EPL = 8, LANES = BLOCK / EPL; // elements of a lane, lanes of a block
@@ -176,33 +180,64 @@ __device__ __forceinline__ unsigned block_max(unsigned v)
 
 struct State8 { float p[EPL], g[EPL]; unsigned m[EPL / 4], v[EPL / 4]; float ms, vs; };
 
+// The e4m3 numbers nearest to the float32 quotients t / scale.  They are what a quotient of t and the reciprocal is
+// rounded to unless a midpoint of the e4m3 grid lies within the approximations' error, so it is taken from below and from
+// above, a step of 2^-20 apart that covers them (root 2^-23; reciprocal, product, and the definition's own quotient and
+// root, 2^-24 each), and only a lane whose values come out differently divides (one in a few hundred).  The largest
+// quotient is 448 but for that step, which rounds to 448.  ROOT: t is the square, `approx` its root, and a root that is
+// not 0 is stored as 2^-9 at least.
+template <bool ROOT>
+__device__ __forceinline__ void store8(unsigned (&q)[EPL / 4], const float (&t)[EPL], const float (&approx)[EPL], const BlockScale &s)
+{
+    float low[EPL], high[EPL];
+#pragma unroll
+    for (int j = 0; j < EPL; j++) {
+        low[j] = approx[j] * s.low;
+        high[j] = approx[j] * s.high;
+        if constexpr (ROOT) {
+            low[j] = t[j] == 0.f ? 0.f : fmaxf(low[j], E4M3_MIN);
+            high[j] = t[j] == 0.f ? 0.f : fmaxf(high[j], E4M3_MIN);
+        }
+    }
+    unsigned other[EPL / 4], differ = s.scale != s.scale;
+    to_e4m3<EPL>(q, low);
+    to_e4m3<EPL>(other, high);
+#pragma unroll
+    for (int i = 0; i < EPL / 4; i++) differ |= q[i] ^ other[i];
+    if (differ) {
+#pragma unroll
+        for (int j = 0; j < EPL; j++) {
+            float v = (ROOT ? sqrtf(t[j]) : t[j]) / s.scale;
+            if constexpr (ROOT) v = t[j] == 0.f ? 0.f : fmaxf(v, E4M3_MIN);
+            // of a lost block every element is 0 (times scale NaN)
+            low[j] = s.scale != s.scale ? 0.f : fminf(fmaxf(v, -E4M3_MAX), E4M3_MAX);
+        }
+        to_e4m3<EPL>(q, low);
+    }
+}
+
 // The step of the eight elements of a lane, whose block its 32 lanes hold; afterwards x is what is to be stored.
 __device__ __forceinline__ void step8(State8 &x, const Hyper &h, const Coef &c)
 {
-    float m[EPL], r[EPL];
+    float m[EPL], v[EPL], r[EPL];
     from_e4m3<EPL>(m, x.m);
-    from_e4m3<EPL>(r, x.v);
+    from_e4m3<EPL>(v, x.v);
     unsigned mt = 0, vt = 0;
 #pragma unroll
     for (int j = 0; j < EPL; j++) {
-        const float g = x.g[j] * c.inv_grad_scale, u = r[j] * x.vs;
-        m[j] = fmaf(h.beta1, m[j] * x.ms, h.one_minus_beta1 * g);
-        r[j] = root(fmaf(h.beta2, u * u, h.one_minus_beta2 * g * g));
+        const float g = x.g[j] * c.inv_grad_scale, u = v[j] * x.vs;
+        m[j] = m[j] * x.ms * h.beta1 + g * h.one_minus_beta1;
+        v[j] = u * u * h.beta2 + g * g * h.one_minus_beta2;
+        r[j] = root(v[j]);
         x.p[j] = move(x.p[j], m[j], r[j], h, c);
         mt = max(mt, mag_bits(m[j]));
-        vt = max(vt, mag_bits(r[j]));
+        vt = max(vt, mag_bits(v[j]));
     }
-    float mi, vi;
-    block_scale(block_max(mt), x.ms, mi);
-    block_scale(block_max(vt), x.vs, vi);
-#pragma unroll
-    for (int j = 0; j < EPL; j++) {
-        // 448 / top * top may end one rounding above 448; of a lost block every element is 0 (times scale NaN)
-        m[j] = mi == 0.f ? 0.f : fminf(fmaxf(m[j] * mi, -E4M3_MAX), E4M3_MAX);
-        r[j] = vi == 0.f || r[j] == 0.f ? 0.f : fminf(fmaxf(r[j] * vi, E4M3_MIN), E4M3_MAX);
-    }
-    to_e4m3<EPL>(x.m, m);
-    to_e4m3<EPL>(x.v, r);
+    const BlockScale ms = block_scale(block_max(mt)), vs = block_scale(mag_bits(sqrtf(__uint_as_float(block_max(vt)))));
+    x.ms = ms.scale;
+    x.vs = vs.scale;
+    store8<false>(x.m, m, m, ms);
+    store8<true>(x.v, v, r, vs);
 }
 
 template <typename T>

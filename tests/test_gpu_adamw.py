@@ -367,3 +367,45 @@ def test_agrees_with_torch_adamw():
         q.grad = p.grad.clone()
         a.step(), b.step()
     assert (p - q).abs().max().item() <= 20 * (16 * U * 1.0 + 64 * U * 1e-2 * 10)
+
+
+# ---- stored states, bit for bit -------------------------------------------------------------------
+def stored8(t, least):
+    """(values, scales) of a float32 tensor of whole blocks as the header defines them: scale = the block's largest
+    magnitude times the float32 nearest to 1 / 448, value = the e4m3 number nearest to the float32 quotient.  Quotients
+    are taken in 64 bits and rounded to float32, which is the float32 quotient (53 bits are more than 2 x 24 + 2)."""
+    b = t.view(-1, 256)
+    scale = b.abs().amax(1) * torch.tensor(1.0 / 448, dtype=torch.float32, device=t.device)
+    q = (b.double() / torch.where(scale > 0, scale, 1.0).double()[:, None]).float()
+    if least:
+        q = torch.where(q > 0, q.clamp(min=2.0 ** -9), q)
+    return q.clamp(-448, 448).to(E4M3).view(-1), scale
+
+
+@pytest.mark.parametrize("dt,n,far", [(torch.bfloat16, 1 << 26, 1.0), (torch.float32, (1 << 24) + 256, 1.0), (torch.float32, 1 << 20, 8.0)])
+def test_stored_8_bit_states_are_the_definitions(dt, n, far):
+    """Two steps in a row: each operation of m = b1 m + (1 - b1) g and v = b2 v + (1 - b2) g^2 is rounded to float32, and
+    values and scales are then decided as defined, next to a midpoint of the e4m3 grid too.  A value that went the other
+    way there would be its block's largest a step later and take the scale of 256 elements with it."""
+    import sc_optim
+    print("stored", dt, n, far, flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    rand = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    size = torch.exp(far * rand(n // 256))
+    size[::97] = 0  # blocks that nothing has reached yet
+    size = size.repeat_interleave(256)
+    f = lambda v: torch.tensor(v, dtype=torch.float32, device="cuda")
+    b1, a1, b2, a2 = f(H["beta1"]), f(1 - H["beta1"]), f(H["beta2"]), f(1 - H["beta2"])
+    p = (rand(n) * 0.05).to(dt)
+    (M, MS), (V, VS) = stored8(rand(n) * 3e-4 * size, False), stored8((rand(n) * 1e-3 * size).abs(), True)
+    m, ms, v, vs = M.clone(), MS.clone(), V.clone(), VS.clone()
+    for step in (42, 43):
+        g = (rand(n) * 1e-3 * size).to(dt)
+        sc_optim.adamw_step([p], [g], [M], [V], [MS], [VS], step=step, **H)
+        back = lambda q, s: (q.float().view(-1, 256) * s[:, None]).view(-1)
+        gf, u = g.float(), back(v, vs)
+        m, ms = stored8(back(m, ms) * b1 + gf * a1, False)
+        v, vs = stored8(((u * u * b2 + gf * gf * a2).double().sqrt()).float(), True)
+        wrong = {name: int((a.float() != b.float()).sum()) for name, a, b in (("m", M, m), ("its scale", MS, ms), ("root", V, v), ("its scale ", VS, vs))}
+        assert not any(wrong.values()), (step, wrong)
+        assert p.isfinite().all()
