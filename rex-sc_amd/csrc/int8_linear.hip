@@ -170,22 +170,24 @@ void launch_quantize_t(const QuantArgs &p, hipStream_t s)
 // taken apart into binary16 pieces, each rounded to nearest (2^-11): v = h + l to 2^-22 of v.  A power of two per
 // row of the result keeps them in binary16's range: with the row's largest |v| between 2^14 and 2^15, a v below 2^-28
 // of that loses bits, and no more than 2^-40 of the largest.  It is multiplied back in the epilogue, exactly.
-// Results in float32 or float16 take both pieces, less of an error than the float32 additions of a few terms make;
-// results in bfloat16 take one: it is off by an eighth of what the gradient's own type and the result's round to.
+// That is less of an error than the float32 additions of a few terms make.  Results in bfloat16 take both pieces too: one
+// would be off by 2^-12 of each term, which shows where terms cancel (8192 x 4096 x 4096 with bfloat16 dx: a training
+// step's call of 865 us with one piece of it, 1062 with both).
+constexpr int PIECES = 2;
 struct OperandArgs {
     const void *g;                  // [M][N] dense
     int M, N, K;
     const float *a_scale, *b_scale;
     const int8_t *a, *b;            // tokens [M][K], channels [N][K]
     size_t a_stride, b_stride;
-    // for dx: pieces of g * b_scale, [pieces][M][ldn], with the rows' powers of two, and b transposed, [K][ldn]
+    // for dx: pieces of g * b_scale, [PIECES][M][ldn], with the rows' powers of two, and b transposed, [K][ldn]
     f16_t *g_rows, *b_t;
     float *g_rows_scale;
-    int pieces_x, ldn;
-    // for dw: pieces of (g * a_scale) transposed, [pieces][N][ldm], likewise, and a transposed, [K][ldm]
+    int ldn;
+    // for dw: pieces of (g * a_scale) transposed, [PIECES][N][ldm], likewise, and a transposed, [K][ldm]
     f16_t *g_cols, *a_t;
     float *g_cols_scale;
-    int pieces_w, ldm;
+    int ldm;
     // statistics of g's columns over each of `shares` runs of `share_rows` rows: sum of g and largest |g * a_scale|
     float *sums;
     unsigned *tops;
@@ -262,7 +264,7 @@ __device__ void split_row(const OperandArgs &p, size_t row, unsigned (&lds)[16])
 #pragma unroll
         for (int j = 0; j < V; j++) split(v[j], t, e, hp[j], lp[j]);
         *(typename VecOf<f16_t, V>::type *)(high + c) = h;
-        if (p.pieces_x > 1) *(typename VecOf<f16_t, V>::type *)(low + c) = l;
+        *(typename VecOf<f16_t, V>::type *)(low + c) = l;
     }
     if (threadIdx.x == 0) p.g_rows_scale[row] = piece_scale(t, e);
 }
@@ -412,7 +414,7 @@ __global__ __launch_bounds__(256) void transposed_pieces_kernel(OperandArgs p)
             lv[i] = b;
         }
         *(typename VecOf<f16_t, 8>::type *)(high + 8 * h) = hv;
-        if (p.pieces_w > 1) *(typename VecOf<f16_t, 8>::type *)(low + 8 * h) = lv;
+        *(typename VecOf<f16_t, 8>::type *)(low + 8 * h) = lv;
     }
 }
 
@@ -440,7 +442,6 @@ int check_rows8(const char *what, const void *q, int64_t stride, int K)
 }
 
 inline int64_t pad64(int64_t n) { return (n + 63) / 64 * 64; }
-inline int pieces_of(int dtype) { return dtype == REXSC_BF16 ? 1 : 2; }
 
 struct Space { size_t tokens, scales, g_rows, g_rows_scale, b_t, g_cols, g_cols_scale, a_t, sums, tops, product, total; };
 
@@ -463,12 +464,11 @@ Space space(const rexsc_int8_desc *d, int what)
     } else if (M > 0 && N > 0) {
         // dx and dw follow each other on the stream, so their partial results share a place
         const size_t ldn = pad64(N), ldm = pad64(M);
-        const int px = pieces_of(d->dtype), pw = pieces_of(d->weight_dtype);
-        s.product = take(max(tile_product_workspace(d->M, d->K, (int)ldn * 2, px), tile_product_workspace(d->N, d->K, (int)ldm * 2, pw)));
-        s.g_rows = take(M * ldn * px * 2);
+        s.product = take(max(tile_product_workspace(d->M, d->K, (int)ldn * 2, PIECES), tile_product_workspace(d->N, d->K, (int)ldm * 2, PIECES)));
+        s.g_rows = take(M * ldn * PIECES * 2);
         s.g_rows_scale = take(M * 4);
         s.b_t = take(K * ldn * 2);
-        s.g_cols = take(N * ldm * pw * 2);
+        s.g_cols = take(N * ldm * PIECES * 2);
         s.g_cols_scale = take(N * 4);
         s.a_t = take(K * ldm * 2);
         s.sums = take((size_t)shares(d->M) * N * 4);
@@ -612,7 +612,6 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
     p.a_stride = (size_t)d->a_stride; p.b_stride = (size_t)d->b_stride;
     p.g_rows = (f16_t *)at(s.g_rows); p.b_t = (f16_t *)at(s.b_t); p.g_rows_scale = (float *)at(s.g_rows_scale);
     p.g_cols = (f16_t *)at(s.g_cols); p.a_t = (f16_t *)at(s.a_t); p.g_cols_scale = (float *)at(s.g_cols_scale);
-    p.pieces_x = pieces_of(d->dtype); p.pieces_w = pieces_of(d->weight_dtype);
     p.ldn = (int)pad64(d->N); p.ldm = (int)pad64(d->M);
     p.sums = (float *)at(s.sums); p.tops = (unsigned *)at(s.tops);
     p.shares = shares(d->M); p.share_rows = share_rows(d->M);
@@ -632,7 +631,7 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
     const bool wide = d->N % (d->dtype == REXSC_F32 ? 4 : 8) == 0 && ((uintptr_t)g | (uintptr_t)b_scale) % 16 == 0;
     {
         const double es = (double)dtype_size(d->dtype), mn = (double)d->M * d->N, k = (double)d->K;
-        ProfScope prof("int8_backward_operands", (dx ? mn * (es + 2.0 * p.pieces_x) + 3.0 * k * d->N : 0.0) + (dw || db ? mn * es : 0.0) +
+        ProfScope prof("int8_backward_operands", (dx ? mn * (es + 2.0 * PIECES) + 3.0 * k * d->N : 0.0) + (dw || db ? mn * es : 0.0) +
                        (dw ? 3.0 * k * d->M : 0.0), stream);
         const dim3 grid(p.row_blocks + p.b_blocks + p.a_blocks + p.stat_blocks);
         if (wide)
@@ -642,7 +641,7 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
         REXSC_CHECK_HIP(hipGetLastError());
     }
     if (dw) {
-        ProfScope prof("int8_backward_pieces", (double)d->M * d->N * (dtype_size(d->dtype) + 2.0 * p.pieces_w), stream);
+        ProfScope prof("int8_backward_pieces", (double)d->M * d->N * (dtype_size(d->dtype) + 2.0 * PIECES), stream);
         const dim3 grid((unsigned)(tiles_m * tiles_n));
         if (wide)
             REXSC_DTYPE_SWITCH(d->dtype, hipLaunchKernelGGL((transposed_pieces_kernel<T, false>), grid, dim3(256), 0, stream, p));
@@ -654,12 +653,12 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
     }
     if (dx) {
         const TileArgs t{(const char *)p.g_rows, (const char *)p.b_t, (size_t)p.ldn * 2, (size_t)p.ldn * 2, d->M, d->K, p.ldn * 2,
-                         p.pieces_x, (size_t)d->M * p.ldn * 2, p.g_rows_scale, nullptr, nullptr, REXSC_F32, dx};
+                         PIECES, (size_t)d->M * p.ldn * 2, p.g_rows_scale, nullptr, nullptr, REXSC_F32, dx};
         if (int rc = launch_tile_product(t, true, d->dtype, at(s.product), "int8_grad_input", stream)) return rc;
     }
     if (dw) {
         const TileArgs t{(const char *)p.g_cols, (const char *)p.a_t, (size_t)p.ldm * 2, (size_t)p.ldm * 2, d->N, d->K, p.ldm * 2,
-                         p.pieces_w, (size_t)d->N * p.ldm * 2, p.g_cols_scale, nullptr, nullptr, REXSC_F32, dw};
+                         PIECES, (size_t)d->N * p.ldm * 2, p.g_cols_scale, nullptr, nullptr, REXSC_F32, dw};
         if (int rc = launch_tile_product(t, true, d->weight_dtype, at(s.product), "int8_grad_weight", stream)) return rc;
     }
     return REXSC_OK;

@@ -626,3 +626,28 @@ def test_autocast_region():
         assert y.dtype == dt and torch.equal(y.detach(), F.linear_int8(x.to(dt), w.detach()))
         dw, = torch.autograd.grad(y.float().sum(), [w])
         assert dw.dtype == torch.float32
+
+
+@pytest.mark.parametrize("wdt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(4, 2, 16), (70, 34, 129), (256, 10, 1024)])
+def test_bfloat16_gradients_are_sums_of_float32_factors(wdt, m, n, k):
+    """Terms that cancel to a part in 256 of their size: what the factor g * scale is held in shows there.  Two binary16
+    pieces are off by 2^-22 of a term, each of the additions of both by at most 2^-23 of the terms' magnitudes, and the
+    sum is rounded once."""
+    import sc_functional as F
+    g = torch.Generator().manual_seed(m + n + k)
+    pairs = lambda r, c: (torch.randn(r // 2, c, generator=g) * 3).repeat_interleave(2, 0)
+    x, w = pairs(m, k).bfloat16(), pairs(n, k).to(wdt)
+    go = torch.randn(m // 2, n // 2, generator=g).bfloat16().float()
+    near = (go * (1 + 2.0 ** -7)).bfloat16().float()
+    # rows and columns in pairs of opposite sign, one of four a step of bfloat16 beside the others
+    go = torch.stack([torch.stack([near, -go], -1), torch.stack([-go, go], -1)], 1).reshape(m, n).bfloat16()
+    xt, wt = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    dx, dw = torch.autograd.grad(F.linear_int8(xt, wt), [xt, wt], go.cuda())
+    (qx, sx), (qw, sw) = quantised(x), quantised(w)
+    xd, wd, gd = qx * sx.double()[:, None], qw * sw.double()[:, None], go.double()
+    for got, want, size, terms, out in ((dx, gd @ wd, gd.abs() @ wd.abs(), n, torch.bfloat16), (dw, gd.t() @ xd, gd.abs().t() @ xd.abs(), m, wdt)):
+        tol = size * ((terms * 2 + 4) * 2.0 ** -23 + 2.0 ** -22)
+        tol = tol + _half(out) * (want.abs() + tol) + _floor(out)
+        err = (got.cpu().double() - want).abs()
+        assert (err <= tol).all(), "max error %g of its bound" % (err / tol).max()
