@@ -936,6 +936,7 @@ def int8_backward(g, wq, w_scale, need_x, bias_dtype):
     N, K = wq.shape
     with _on(g.get_device()):
         wq, stride = _operand8(wq, "linear_int8")
+        w_scale = _scale_vector(w_scale, N, g.device, "linear_int8")
     dx, _, db = _int8_gradients(g, N, K, None, 0, None, wq.data_ptr(), stride, w_scale.data_ptr(), need_x, None, bias_dtype)
     return dx, db
 

@@ -651,3 +651,19 @@ def test_bfloat16_gradients_are_sums_of_float32_factors(wdt, m, n, k):
         tol = tol + _half(out) * (want.abs() + tol) + _floor(out)
         err = (got.cpu().double() - want).abs()
         assert (err <= tol).all(), "max error %g of its bound" % (err / tol).max()
+
+
+@pytest.mark.parametrize("n", [30, 64, 1000])
+def test_gradient_with_scales_of_any_layout(n):
+    """Scales out of a table of several per channel, and one for all channels expanded: as their dense copies."""
+    import sc_functional as F
+    x0, wq = torch.randn(20, 70, device="cuda"), F.quantize_rows(torch.randn(n, 70, device="cuda"))[0]
+    table, go = torch.rand(n, 3, device="cuda") + 0.1, torch.randn(20, n, device="cuda")
+
+    def both(scale):
+        x = x0.clone().requires_grad_(True)
+        y = F.linear_int8(x, wq, None, weight_scale=scale)
+        return y.detach(), torch.autograd.grad(y, [x], go)[0]
+
+    for scale in (table[:, 1], table[:, :1], table[:1, 0].expand(n), table[0, 2].expand(n), table[:, 0].flip(0)):
+        assert all(torch.equal(a, b) for a, b in zip(both(scale), both(scale.contiguous())))
