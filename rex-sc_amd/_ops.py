@@ -1014,12 +1014,14 @@ def layer_norm_backward(grad_output, m, w, stats, rest, need_x=True, weight_dtyp
     shape, dtype = grad_output.shape, m.dtype
     g = grad_output if grad_output.dtype == dtype else grad_output.to(dtype)
     g = _dense_rows(g, D)
-    # the sums leave the kernel in float32 or in x's type; any other type is rounded once more
+    # the sums leave the kernel in float32 or in x's type, which is that of the weight as it is read too (so a float32
+    # weight keeps them in float32); any other type is rounded once more
+    d, wdt, eps = rest
     wanted = weight_dtype is not None or bias_dtype is not None
     sum_dt = torch.float32
-    if wanted and dtype != sum_dt and weight_dtype in (None, dtype) and bias_dtype in (None, dtype):
+    if (wanted and dtype != sum_dt and weight_dtype in (None, dtype) and bias_dtype in (None, dtype)
+            and (w is None or wdt == dtype)):
         sum_dt = dtype
-    d, wdt, eps = rest
     if wdt != sum_dt:
         d = _lib.NormDesc.packed(_DTYPE_CODE[dtype], _DTYPE_CODE[sum_dt], eps, R, D, _row_stride(m))
         w = None if w is None else w.to(sum_dt)

@@ -284,3 +284,19 @@ def test_layer():
         assert layer(x).dtype == torch.float32
     with pytest.raises(RuntimeError, match="shape"):
         LayerNorm(9).cuda()(x)
+
+
+@pytest.mark.parametrize("rows,d", [(5, 100), (600, 264), (3, 4096), (2, 17000)])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_partial_gradients_of_mixed_types(dt, rows, d):
+    """A float32 weight is used as it is whichever gradients are asked for, also where only those of 16 bits are."""
+    import sc_functional as F
+    gen = torch.Generator().manual_seed(d)
+    x, w, b = torch.randn(rows, d, generator=gen).to(dt), 1 + 0.3 * torch.randn(d, generator=gen), torch.randn(d, generator=gen).to(dt)
+    g = torch.randn(rows, d, generator=gen).to(dt)
+    ref = reference(x, w, b, g)
+    for mask in range(1, 8):
+        leaves = [t.cuda().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((x, w, b))]
+        named = [(n, t) for n, t in zip(("dx", "dw", "db"), leaves) if t.requires_grad]
+        for (n, t), got in zip(named, torch.autograd.grad(F.layer_norm(*leaves), [t for _, t in named], g.cuda())):
+            close(got, ref[n], t.dtype, "%s %d" % (n, mask))
