@@ -409,3 +409,20 @@ def test_stored_8_bit_states_are_the_definitions(dt, n, far):
         wrong = {name: int((a.float() != b.float()).sum()) for name, a, b in (("m", M, m), ("its scale", MS, ms), ("root", V, v), ("its scale ", VS, vs))}
         assert not any(wrong.values()), (step, wrong)
         assert p.isfinite().all()
+
+
+@pytest.mark.parametrize("n", [1 << 20, 1001])
+def test_32_bit_states_root_and_quotient_are_correctly_rounded(n):
+    """With betas, eps and decay 0 and lr 1 a parameter of 0 becomes -g / sqrt(g^2), a handful of operations that are each
+    rounded to nearest: 64 bits rounded to float32 are the float32 root and quotient."""
+    import sc_optim
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    m0 = torch.randn(n, generator=gen, device="cuda")
+    g = torch.randn(n, generator=gen, device="cuda") * torch.exp(6 * torch.randn(n, generator=gen, device="cuda"))
+    p, m, v = torch.zeros(n, device="cuda"), m0.clone(), torch.zeros(n, device="cuda")
+    sc_optim.adamw_step([p], [g], [m], [v], step=1, lr=1.0, beta1=0.5, beta2=0.0, eps=0.0, weight_decay=0.0)
+    half = torch.tensor(0.5, device="cuda")
+    m1, v1 = m0 * half + g * half, g * g
+    assert torch.equal(m, m1) and torch.equal(v, v1)
+    q = (m1.double() / v1.double().sqrt().float().double()).float()
+    assert torch.equal(p, -(q * 2))  # lr / (1 - 1/2)
