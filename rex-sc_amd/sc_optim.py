@@ -161,6 +161,25 @@ class AdamW(torch.optim.Optimizer):
             for k, v in state_dict["state"].get(i, {}).items():
                 if isinstance(v, torch.Tensor):
                     self.state[p][k] = v.to(device=p.device, copy=True)
+        for group in self.param_groups:  # each parameter has a copy of the count now: one for all again
+            if group["capturable"]:
+                for key in {(p.dtype, p.device) for p in group["params"]}:
+                    self._share_step(group, key)
+
+    def _share_step(self, group, key):
+        """The step count that the parameters of `group` with this type and device share on the device, held by every
+        state there is from now on, also of those that have no gradient at the moment."""
+        states = [self.state[p] for p in group["params"] if (p.dtype, p.device) == key and self.state.get(p)]
+        held = [s["step"] for s in states if "step" in s]
+        if held and isinstance(held[0], torch.Tensor) and all(t is held[0] for t in held):
+            step = held[0]
+        else:  # the first step, a loaded state, or a group that was not capturable before
+            if held and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: a group that becomes capturable needs an eager step before a captured one")
+            step = torch.full((1,), max(map(int, held), default=0), dtype=torch.int64, device=key[1])
+        for s in states:
+            s["step"] = step
+        return step
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -192,13 +211,9 @@ class AdamW(torch.optim.Optimizer):
                 sets.setdefault(key, []).append((p, state))
             for key, members in sets.items():
                 if group["capturable"]:
-                    step = next((s["step"] for _, s in members if "step" in s), 0)
-                    if not isinstance(step, torch.Tensor):  # the first step, or a group that was not capturable before
-                        if step and torch.cuda.is_current_stream_capturing():
-                            raise RuntimeError("AdamW: a group that becomes capturable needs an eager step before a captured one")
-                        step = torch.full((1,), step, dtype=torch.int64, device=key[1])
-                    for _, s in members:
-                        s["step"] = step
+                    step = members[0][1].get("step")
+                    if not isinstance(step, torch.Tensor) or any(s.get("step") is not step for _, s in members):
+                        step = self._share_step(group, key)
                 else:
                     step = key[2]
                 grads = [p.grad if p.grad.stride() == p.stride() else torch.empty_like(p).copy_(p.grad) for p, _ in members]

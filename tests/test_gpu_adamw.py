@@ -426,3 +426,28 @@ def test_32_bit_states_root_and_quotient_are_correctly_rounded(n):
     assert torch.equal(m, m1) and torch.equal(v, v1)
     q = (m1.double() / v1.double().sqrt().float().double()).float()
     assert torch.equal(p, -(q * 2))  # lr / (1 - 1/2)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_reloaded_capturable_optimiser_goes_on_as_the_first_one(bits):
+    import sc_optim
+    torch.manual_seed(4)
+    make = lambda: [torch.nn.Parameter(torch.ones(n, device="cuda")) for n in (300, 7)]
+    a, b = (sc_optim.AdamW(make(), lr=0.1, state_bits=bits, capturable=True) for _ in range(2))
+    step = lambda which: [opt.step() for opt in (a, b) if set_gradients(opt, which)]
+
+    def set_gradients(opt, which):
+        for i, p in enumerate(opt.param_groups[0]["params"]):
+            p.grad = grads[i].clone() if i in which else None
+        return True
+
+    for which in ((0, 1), (0, 1), (1,), (1,), (0, 1), (0,), (0, 1)):
+        grads = [torch.randn(n, device="cuda") for n in (300, 7)]
+        step(which)
+        fresh = sc_optim.AdamW([torch.nn.Parameter(p.detach().clone()) for p in b.param_groups[0]["params"]], lr=0.1,
+                               state_bits=bits, capturable=True)
+        if which != (1,):  # else the next step is one of the reloaded optimiser too
+            fresh.load_state_dict(b.state_dict())
+            b = fresh
+        for p, q in zip(a.param_groups[0]["params"], b.param_groups[0]["params"]):
+            assert torch.equal(p, q) and a.state[p]["step"].item() == b.state[q]["step"].item(), which

@@ -185,3 +185,45 @@ def test_operand_layouts():
     d = sc_optim._dense
     assert d(torch.zeros(3, 4)) and d(torch.zeros(3, 4).t()) and d(torch.zeros(2, 3, 4, 5).contiguous(memory_format=torch.channels_last))
     assert not d(torch.zeros(3, 8)[:, :4]) and not d(torch.zeros(1, 4).expand(3, 4)) and d(torch.zeros(0, 4))
+
+
+def test_a_reloaded_capturable_optimiser_has_one_step_count(monkeypatch):
+    """Every parameter of a capturable group, with a gradient at the moment or without, counts the same steps after a
+    reload, after a change of `capturable`, and when it joins late.  (The kernel's part, advancing a device count, is
+    done by the test.)"""
+    import sc_optim
+
+    def advance(params, *lists, step, **rest):
+        if isinstance(step, torch.Tensor):
+            step += 1
+        seen.append(int(step))
+
+    seen = []
+    monkeypatch.setattr(sc_optim, "adamw_step", advance)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    make = lambda: [torch.nn.Parameter(torch.ones(3)) for _ in range(3)]
+
+    def step(opt, which):
+        for i, p in enumerate(opt.param_groups[0]["params"]):
+            p.grad = torch.ones(3) if i in which else None
+        opt.step()
+
+    first = sc_optim.AdamW(make(), capturable=True)
+    for _ in range(5):
+        step(first, (0, 1))
+    again = sc_optim.AdamW(make(), capturable=True)
+    again.load_state_dict(first.state_dict())
+    for which in ((1,), (1,), (1,), (0, 1), (0, 1, 2), (2,), (0,)):
+        step(again, which)
+    assert seen == [1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12]
+    counts = [again.state[p]["step"] for p in again.param_groups[0]["params"]]
+    assert all(c is counts[0] for c in counts) and int(first.state[first.param_groups[0]["params"][0]]["step"]) == 5
+    # a count on the host becomes the group's: parameters without a gradient at that moment count on too
+    seen.clear()
+    late = sc_optim.AdamW(make(), capturable=False)
+    for _ in range(4):
+        step(late, (0, 1, 2))
+    late.param_groups[0]["capturable"] = True
+    for which in ((1,), (1,), (0, 1, 2)):
+        step(late, which)
+    assert seen == [1, 2, 3, 4, 5, 6, 7]
