@@ -14,6 +14,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 import _ops
 import fixed_extension_cuda
@@ -699,6 +700,14 @@ def linear_generic(activation, weight, **kwargs):
 
 
 # ---- 8-bit linear layer, layer norm --------------------------------------------------------------
+def _refuse_tangents(what, *tensors):
+    """Forward mode: a dual tensor need not require a gradient, and a kernel's result would lose its tangent silently."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("%s has no forward-mode derivative" % what)
+
+
 def quantize_rows(x):
     """Rows of x [..., K] in 8 bits with a scale each: q = nearest(127 x / max|row|), ties to even and decided exactly,
     scale = max|row| / 127 -> (q int8 of x's shape, scale float32 of x.shape[:-1]).  A row of zeros has scale 0; a row
@@ -752,7 +761,7 @@ def linear_int8(x, weight, bias=None, weight_scale=None):
     scale per row, W is either float [N, K], taken to int8 with a scale per output channel on every call (training), or
     int8 [N, K] with weight_scale [N], as quantize_rows returns them (serving).  The sum over K <= 131071 is exact; y
     has x's type.  Gradients pass straight through the quantisation.  Inside an autocast region x is cast to the
-    region's type first, as nn.functional.linear does."""
+    region's type first, as nn.functional.linear does.  Forward-mode derivatives are refused."""
     lowp = _autocast_dtype()
     if lowp is not None and x.is_cuda and x.dtype != lowp:
         x = x.to(lowp)
@@ -762,6 +771,7 @@ def linear_int8(x, weight, bias=None, weight_scale=None):
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError("linear_int8: expected input [..., K] and weight [N, K], got %s and %s"
                          % (tuple(x.shape), tuple(weight.shape)))
+    _refuse_tangents("linear_int8", x, weight, bias, weight_scale)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return Linear_Int8_Grad.apply(x, weight, bias, weight_scale)
     if weight_scale is None:
@@ -799,7 +809,9 @@ _layer_norm_once = torch.autograd.function.once_differentiable(_layer_norm_backw
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, var the biased variance.  x float32, float16
-    or bfloat16, the result of the same type (also inside an autocast region); arithmetic in float32."""
+    or bfloat16, the result of the same type (also inside an autocast region); arithmetic in float32.  Forward-mode
+    derivatives are refused."""
+    _refuse_tangents("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return Layer_Norm_Grad.apply(x, weight, bias, eps)

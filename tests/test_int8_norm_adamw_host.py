@@ -227,3 +227,29 @@ def test_a_reloaded_capturable_optimiser_has_one_step_count(monkeypatch):
     for which in ((1,), (1,), (0, 1, 2)):
         step(late, which)
     assert seen == [1, 2, 3, 4, 5, 6, 7]
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor need not require a gradient: its tangent must not be dropped without a word, whichever argument it
+    is and whether or not another one requires a gradient.  Tensors without a tangent go on to the kernel (refused here
+    for want of a device)."""
+    import torch.autograd.forward_ad as fw
+    import sc_functional as F
+    import sc_layers
+    x, v, w = torch.randn(3, 8), torch.randn(8), torch.randn(4, 8)
+    q, s = torch.zeros(4, 8, dtype=torch.int8), torch.ones(4)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))
+        frozen = sc_layers.Linear_Int8(8, 4)
+        frozen.weight_q, frozen.weight_scale, frozen.weight = torch.zeros(4, 128, dtype=torch.int8), s, None
+        for leaf in (False, True):
+            g = v.clone().requires_grad_(leaf)
+            for call in (lambda: F.layer_norm(dual(x), g), lambda: F.layer_norm(x, g, dual(v)), lambda: F.layer_norm(x, dual(v), g),
+                         lambda: F.linear_int8(dual(x), w), lambda: F.linear_int8(x, dual(w)), lambda: F.linear_int8(x, w, dual(s)),
+                         lambda: F.linear_int8(dual(x), q, weight_scale=s), lambda: F.linear_int8(x, q, weight_scale=dual(s)),
+                         lambda: sc_layers.LayerNorm(8)(dual(x)), lambda: frozen(dual(x))):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        for call in (lambda: F.layer_norm(x), lambda: F.linear_int8(x, q, weight_scale=s)):
+            with pytest.raises(RuntimeError, match="HIP device"):
+                call()
