@@ -28,6 +28,14 @@ Use_Approx = False    # config.py
 
 
 # ---- small helpers (utils_functional.py:52-91) ----------------------------------------------
+def _refuse_tangents(what, *tensors):
+    """Forward mode: a dual tensor need not require a gradient, and a kernel's result would lose its tangent silently."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("%s has no forward-mode derivative" % what)
+
+
 def setattr_default(obj, kwargs, att_string, default_value):
     if att_string in kwargs:
         setattr(obj, att_string, kwargs.pop(att_string))
@@ -454,6 +462,7 @@ def conv2d_generic(activation, weight, padding, stride, **kwargs):
                                       (prec_default, load_unit, load_wait_w), bin_config, gen_config, want_split=False,
                                       xnor=_ops.honour_xnor(XNOR), want_value=True)[3]
 
+        _refuse_tangents("conv2d_generic", activation, weight)
         if not (torch.is_grad_enabled() and (activation.requires_grad or weight.requires_grad)):
             return as_dtype(sc_forward())  # inference: the surrogate only ever supplies gradients
         # The integer kernels (VALU-bound) and the surrogate's float convolution (matrix cores) are
@@ -596,6 +605,7 @@ def linear_generic_sc(activation, weight, **kwargs):
               and activation.dtype == torch.float32 and weight.dtype == torch.float32
               and not torch.is_autocast_enabled() and weight.size(0) % 4 == 0)
     if merged:
+        _refuse_tangents("linear_generic_sc", activation, weight)
         with torch.no_grad():
             pos, neg = sc_extension_cuda.linear_generic_general_acc(
                 activation.data, weight.data, (prec_default, load_unit, load_wait_w), bit_length, LFSR_Length,
@@ -700,14 +710,6 @@ def linear_generic(activation, weight, **kwargs):
 
 
 # ---- 8-bit linear layer, layer norm --------------------------------------------------------------
-def _refuse_tangents(what, *tensors):
-    """Forward mode: a dual tensor need not require a gradient, and a kernel's result would lose its tangent silently."""
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError("%s has no forward-mode derivative" % what)
-
-
 def quantize_rows(x):
     """Rows of x [..., K] in 8 bits with a scale each: q = nearest(127 x / max|row|), ties to even and decided exactly,
     scale = max|row| / 127 -> (q int8 of x's shape, scale float32 of x.shape[:-1]).  A row of zeros has scale 0; a row

@@ -334,3 +334,20 @@ def test_pair_backward_on_float16_tensors_equals_widen_compute_round(or_n, cl):
     want = _ops.orn_pair_backward(go, s2f, outer2, inner2, c2, or_n)
     assert got.dtype == torch.float16 and want.dtype == torch.float32
     assert torch.equal(got, want.half()) and float(want.abs().max()) > 0
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Without a gradient asked for, the integer kernels alone run: a dual tensor's tangent must not be dropped there."""
+    import torch.autograd.forward_ad as fw
+    import sc_functional as uf
+    x, w = torch.rand(2, 4, 8, 8, device="cuda"), torch.randn(8, 4, 3, 3, device="cuda").clamp(-1, 0.99)
+    a, b = torch.rand(3, 16, device="cuda"), torch.randn(8, 16, device="cuda").clamp(-1, 0.99)
+    conv = lambda x, w: uf.conv2d_generic(x, w, (1, 1), (1, 1), bit_length=32, generator="lfsr", forward="or_2", sync=1, order=5)
+    linear = lambda a, b: uf.linear_generic_sc(a, b, bit_length=32, forward="or_2", generator="lfsr", sync=1)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))
+        for f, s, t in ((conv, x, w), (linear, a, b)):
+            assert f(s, t).isfinite().all()
+            for args in ((dual(s), t), (s, dual(t))):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    f(*args)
