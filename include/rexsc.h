@@ -335,7 +335,7 @@ int rexsc_int8_linear(const rexsc_int8_desc *d, const void *x, const int8_t *b, 
  * utils_functional.py:117-123): dx[m][k] = sum_n g[m][n] b_scale[n] b[n][k] in d->dtype,
  * dw[n][k] = sum_m g[m][n] a_scale[m] a[m][k] in d->weight_dtype, db[n] = sum_m g[m][n] in d->bias_dtype; any of the
  * three may be NULL (a and a_scale are read for dw only, b and b_scale for dx only).  g: dense [M][N] of d->dtype,
- * dx: dense [M][K], dw: dense [N][K].  A row of dx or dw whose sum takes in a NaN or an infinity is NaN. */
+ * dx: dense [M][K], dw: dense [N][K].  Infinities and NaN in g or a scale go where the products take them. */
 int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, const int8_t *a, const float *a_scale, const int8_t *b,
                         const float *b_scale, void *dx, void *dw, void *db, void *workspace, size_t workspace_bytes,
                         rexsc_stream_t stream);

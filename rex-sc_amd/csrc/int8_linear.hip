@@ -188,7 +188,7 @@ struct OperandArgs {
     f16_t *g_cols, *a_t;
     float *g_cols_scale;
     int ldm;
-    // statistics of g's columns over each of `shares` runs of `share_rows` rows: sum of g and largest |g * a_scale|
+    // statistics of g's columns over each of `shares` runs of `share_rows` rows: sum of g and largest finite |g * a_scale|
     float *sums;
     unsigned *tops;
     int shares, share_rows;
@@ -198,21 +198,23 @@ struct OperandArgs {
     unsigned row_blocks, b_blocks, a_blocks, stat_blocks;
 };
 
+// Magnitude as mag_bits has it, 0 for an infinity or a NaN: a row's power of two comes from its finite values.
+__device__ __forceinline__ unsigned finite_bits(float x)
+{
+    const unsigned b = mag_bits(x);
+    return b < 0x7f800000u ? b : 0u;
+}
 // Exponent e with top * 2^-e in [2^14, 2^15), or below where 2^e would not be a normal number; 0 for an empty row.
 __device__ __forceinline__ int piece_exponent(unsigned top)
 {
     return top == 0 ? 0 : max(ilogbf(__uint_as_float(top)) - 14, -126);
 }
-// What the row's sums are multiplied by: 2^e, or NaN where the row holds an infinity or a NaN.
-__device__ __forceinline__ float piece_scale(unsigned top, int e)
+// An infinity or a NaN is its own first piece, so the products are what they are in float32: infinities, or NaN.
+__device__ __forceinline__ void split(float v, int e, f16_t &high, f16_t &low)
 {
-    return top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : ldexpf(1.f, e);
-}
-__device__ __forceinline__ void split(float v, unsigned top, int e, f16_t &high, f16_t &low)
-{
-    const float t = top >= 0x7f800000u ? 0.f : ldexpf(v, -e);
+    const float t = ldexpf(v, -e);
     high = (f16_t)t;
-    low = (f16_t)(t - (float)high);
+    low = mag_bits(t) < 0x7f800000u ? (f16_t)(t - (float)high) : (f16_t)0.f;
 }
 
 // The first n of V = 16 / sizeof(T) elements of a row from its element c on, zeros behind them.  RAGGED: they lie
@@ -251,7 +253,7 @@ __device__ void split_row(const OperandArgs &p, size_t row, unsigned (&lds)[16])
         float v[V];
         load_scaled<RAGGED>(v, g, p.b_scale, c, p.N - c);
 #pragma unroll
-        for (int j = 0; j < V; j++) t = max(t, mag_bits(v[j]));
+        for (int j = 0; j < V; j++) t = max(t, finite_bits(v[j]));
     }
     t = row_top<256>(t, lds);
     const int e = piece_exponent(t);
@@ -262,11 +264,11 @@ __device__ void split_row(const OperandArgs &p, size_t row, unsigned (&lds)[16])
         typename VecOf<f16_t, V>::type h, l;
         f16_t *hp = (f16_t *)&h, *lp = (f16_t *)&l;
 #pragma unroll
-        for (int j = 0; j < V; j++) split(v[j], t, e, hp[j], lp[j]);
+        for (int j = 0; j < V; j++) split(v[j], e, hp[j], lp[j]);
         *(typename VecOf<f16_t, V>::type *)(high + c) = h;
         *(typename VecOf<f16_t, V>::type *)(low + c) = l;
     }
-    if (threadIdx.x == 0) p.g_rows_scale[row] = piece_scale(t, e);
+    if (threadIdx.x == 0) p.g_rows_scale[row] = ldexpf(1.f, e);
 }
 
 // q [rows][cols] int8 -> out [cols][ld] binary16, positions from rows to ld zero; a 64 x 64 tile.  q's rows are 16-byte
@@ -297,7 +299,7 @@ __device__ void transpose_tile(const int8_t *q, size_t stride, int rows, int col
     }
 }
 
-// Sum of g and largest |g * a_scale| of 64 columns over one share of the rows: 64 / V threads across, the rest down.
+// Sum of g and largest finite |g * a_scale| of 64 columns over one share of the rows: 64 / V threads across, the rest down.
 template <typename T, bool RAGGED>
 __device__ void column_stats(const OperandArgs &p, unsigned block, float (&ls)[32][64], unsigned (&lt)[32][64])
 {
@@ -315,7 +317,7 @@ __device__ void column_stats(const OperandArgs &p, unsigned block, float (&ls)[3
 #pragma unroll
             for (int j = 0; j < V; j++) {
                 s[j] += g[j];
-                t[j] = max(t[j], mag_bits(g[j] * scale));
+                t[j] = max(t[j], finite_bits(g[j] * scale));
             }
         }
 #pragma unroll
@@ -394,14 +396,12 @@ __global__ __launch_bounds__(256) void transposed_pieces_kernel(OperandArgs p)
     auto top_of = [&](int x) { return max(max(tops[0][x], tops[1][x]), max(tops[2][x], tops[3][x])); };
     if (m0 == 0 && threadIdx.x < 64 && n0 + threadIdx.x < p.N) {
         const int x = threadIdx.x;
-        const unsigned t = top_of(x);
-        p.g_cols_scale[n0 + x] = piece_scale(t, piece_exponent(t));
+        p.g_cols_scale[n0 + x] = ldexpf(1.f, piece_exponent(top_of(x)));
         if (p.db) store_any(p.db, p.db_dtype, n0 + x, ((sums[0][x] + sums[1][x]) + sums[2][x]) + sums[3][x]);
     }
     const int on = threadIdx.x / 4, om = threadIdx.x % 4 * 16;
     if (n0 + on >= p.N) return;
-    const unsigned t = top_of(on);
-    const int e = piece_exponent(t);
+    const int e = piece_exponent(top_of(on));
     f16_t *high = p.g_cols + (size_t)(n0 + on) * p.ldm + m0 + om, *low = high + (size_t)p.N * p.ldm;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(256) void transposed_pieces_kernel(OperandArgs p)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             f16_t a, b;
-            split(tile[om + 8 * h + i][on], t, e, a, b);
+            split(tile[om + 8 * h + i][on], e, a, b);
             hv[i] = a;
             lv[i] = b;
         }

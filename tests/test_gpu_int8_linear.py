@@ -667,3 +667,29 @@ def test_gradient_with_scales_of_any_layout(n):
 
     for scale in (table[:, 1], table[:, :1], table[:1, 0].expand(n), table[0, 2].expand(n), table[:, 0].flip(0)):
         assert all(torch.equal(a, b) for a, b in zip(both(scale), both(scale.contiguous())))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(6, 8, 40), (70, 33, 129), (300, 10, 2048)])
+def test_infinite_and_nan_gradients_go_where_the_product_takes_them(dt, m, n, k):
+    """inf times a nonzero value is an infinity of its sign, times 0 a NaN; the finite results are as without them."""
+    import sc_functional as F
+    g = torch.Generator().manual_seed(m + n)
+    x, w = torch.randint(-3, 4, (m, k), generator=g).to(dt), torch.randint(-3, 4, (n, k), generator=g).float()
+    x[:, 0], w[:, 0] = 3, -3
+    go = torch.randint(-8, 9, (m, n), generator=g).to(dt)
+    inf = float("inf")
+    go[1, 2], go[2, 0], go[3, 1], go[3, 4], go[4, 5], go[4, 6] = inf, float("nan"), -inf, inf, inf, inf
+    xt, wt = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    dx, dw = torch.autograd.grad(F.linear_int8(xt, wt), [xt, wt], go.cuda())
+    (qx, sx), (qw, sw) = quantised(x), quantised(w)
+    for got, a, b, s in ((dx, go.double() * sw.double(), qw, "dx"), (dw, (go.double() * sx.double()[:, None]).t(), qx, "dw")):
+        want = (a[:, :, None] * b[None]).sum(1) if a.shape[0] * b.numel() < 1 << 25 else torch.stack([(r[:, None] * b).sum(0) for r in a])
+        got = got.cpu().double()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf()), s
+        assert torch.equal(got[got.isinf()], want[want.isinf()])
+        ok = want.isfinite()
+        size = (a.abs().nan_to_num(0, 0, 0) @ b.abs())
+        tol = size * ((2 * a.shape[1] + 4) * 2.0 ** -23 + 2.0 ** -11) + _half(dt) * want.abs() * (1 + 2.0 ** -8) + _floor(dt)
+        assert ((got - want).abs() <= tol)[ok].all()
+    assert dx[1].isinf().any() and dx[4].isinf().any() and dw[2].isinf().any()
