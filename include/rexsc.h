@@ -312,7 +312,8 @@ typedef struct rexsc_int8_desc {
     int32_t reserved;        /* 0 */
     int64_t x_stride;        /* distance of x's rows in elements (rexsc_int8_linear only) */
     int64_t a_stride;        /* distance of the tokens' int8 rows in bytes: a multiple of 16, at least K */
-    int64_t b_stride;        /* distance of the channels' int8 rows in bytes: likewise */
+    int64_t b_stride;        /* distance of the channels' int8 rows in bytes: likewise.  Distances from 8 MiB on are
+                              * refused where the tiles take the product: with more than 48 tokens for certain */
 } rexsc_int8_desc;
 
 /* What a workspace is for. */

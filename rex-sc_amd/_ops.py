@@ -703,6 +703,7 @@ def _addr(t):
 
 ROW_PAD = 128  # int8 rows are laid out at a multiple of this many bytes: the product's step along the reduction
 MAX_K = 131071
+MAX_ROW_STRIDE = 8 << 20  # the tiled product reaches rows at distances below this
 
 
 def _dtype_code(t, what):
@@ -760,8 +761,8 @@ def quantize_rows(x):
 
 
 def _operand8(t, what):
-    """(int8 matrix as the product reads it, distance of its rows): rows 16-byte aligned and readable to the next
-    multiple of 16 bytes."""
+    """(int8 matrix as the product reads it, distance of its rows): rows 16-byte aligned, readable to the next multiple
+    of 16 bytes and less than MAX_ROW_STRIDE apart."""
     if t.dtype != torch.int8 or t.dim() != 2 or not 1 <= t.shape[1] <= MAX_K:
         raise RuntimeError("%s: expected an int8 matrix with 1 to %d columns (got %s %s)"
                            % (what, MAX_K, t.dtype, tuple(t.shape)))
@@ -769,7 +770,7 @@ def _operand8(t, what):
     step, inner = t.stride()
     if R <= 1:
         step = -(-K // 16) * 16
-    if (inner == 1 or K == 1) and step % 16 == 0 and step >= K and t.data_ptr() % 16 == 0:
+    if (inner == 1 or K == 1) and step % 16 == 0 and K <= step < MAX_ROW_STRIDE and t.data_ptr() % 16 == 0:
         if K % 16 == 0 or R == 0 or t.storage_offset() + (R - 1) * step + -(-K // 16) * 16 <= t.untyped_storage().nbytes():
             return t, step
     pad = -(-K // ROW_PAD) * ROW_PAD

@@ -693,3 +693,16 @@ def test_infinite_and_nan_gradients_go_where_the_product_takes_them(dt, m, n, k)
         tol = size * ((2 * a.shape[1] + 4) * 2.0 ** -23 + 2.0 ** -11) + _half(dt) * want.abs() * (1 + 2.0 ** -8) + _floor(dt)
         assert ((got - want).abs() <= tol)[ok].all()
     assert dx[1].isinf().any() and dx[4].isinf().any() and dw[2].isinf().any()
+
+
+@pytest.mark.parametrize("m", [3, 60])
+def test_weights_whose_rows_are_far_apart(m):
+    import sc_functional as F
+    store = torch.randint(-127, 128, ((16 << 20) + 64,), device="cuda", dtype=torch.int8)
+    x, s = torch.randn(m, 48, device="cuda"), torch.rand(3, device="cuda")
+    far = store.as_strided((3, 48), (8 << 20, 1))
+    xg = x.clone().requires_grad_(True)
+    y = F.linear_int8(xg, far, None, weight_scale=s)
+    want = F.linear_int8(xg, far.contiguous(), None, weight_scale=s)
+    assert torch.equal(y, want)
+    assert torch.equal(*(torch.autograd.grad(t.sum(), [xg])[0] for t in (y, want)))

@@ -253,3 +253,13 @@ def test_forward_mode_derivatives_are_refused():
         for call in (lambda: F.layer_norm(x), lambda: F.linear_int8(x, q, weight_scale=s)):
             with pytest.raises(RuntimeError, match="HIP device"):
                 call()
+
+
+def test_rows_far_apart_are_copied():
+    """The tiled product reaches rows less than 8 MiB apart: whether a layout works must not depend on the tokens' number."""
+    import _ops
+    far = torch.arange((8 << 20) + 64, dtype=torch.int64).to(torch.int8).as_strided((2, 48), (8 << 20, 1))
+    got, stride = _ops._operand8(far, "x")
+    assert torch.equal(got, far) and stride == 128 and got.data_ptr() != far.data_ptr()
+    near = torch.zeros((8 << 20) + 64, dtype=torch.int8).as_strided((2, 48), ((8 << 20) - 16, 1))
+    assert _ops._operand8(near, "x")[0].data_ptr() == near.data_ptr()
