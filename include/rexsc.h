@@ -320,6 +320,9 @@ typedef struct rexsc_int8_desc {
 enum { REXSC_INT8_PRODUCT = 0, REXSC_INT8_LINEAR = 1, REXSC_INT8_BACKWARD = 2 };
 /* Bytes of workspace a call needs (0: none).  (size_t)-1 and rexsc_last_error() if the descriptor is invalid. */
 size_t rexsc_int8_workspace_bytes(const rexsc_int8_desc *d, int what);
+/* The same for rexsc_int8_backward with some of the gradients only (REXSC_INT8_BACKWARD above: all of them). */
+enum { REXSC_INT8_DX = 1, REXSC_INT8_DW = 2, REXSC_INT8_DB = 4 };
+size_t rexsc_int8_backward_workspace_bytes(const rexsc_int8_desc *d, int wanted);
 
 /* y[m][n] = (sum_k a[m][k] b[n][k]) * a_scale[m] * b_scale[n] + bias[n].  a, b: int8, 16-byte aligned, every value of
  * -128..127 allowed; each row is readable up to the next multiple of 16 bytes, and what lies there does not matter.
@@ -336,7 +339,8 @@ int rexsc_int8_linear(const rexsc_int8_desc *d, const void *x, const int8_t *b, 
  * utils_functional.py:117-123): dx[m][k] = sum_n g[m][n] b_scale[n] b[n][k] in d->dtype,
  * dw[n][k] = sum_m g[m][n] a_scale[m] a[m][k] in d->weight_dtype, db[n] = sum_m g[m][n] in d->bias_dtype; any of the
  * three may be NULL (a and a_scale are read for dw only, b and b_scale for dx only).  g: dense [M][N] of d->dtype,
- * dx: dense [M][K], dw: dense [N][K].  Infinities and NaN in g or a scale go where the products take them. */
+ * dx: dense [M][K], dw: dense [N][K].  Infinities and NaN in g or a scale go where the products take them.  Sums over
+ * more than 4194240 channels (dx) or tokens (dw) are refused. */
 int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, const int8_t *a, const float *a_scale, const int8_t *b,
                         const float *b_scale, void *dx, void *dw, void *db, void *workspace, size_t workspace_bytes,
                         rexsc_stream_t stream);

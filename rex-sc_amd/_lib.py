@@ -81,6 +81,7 @@ ADAMW_TENSOR_FIELDS = 7
 ADAMW_COEF_BYTES = 256            # REXSC_ADAMW_COEF_BYTES
 F32, F16, BF16 = 0, 1, 2          # REXSC_F32, ...
 INT8_PRODUCT, INT8_LINEAR, INT8_BACKWARD = 0, 1, 2  # REXSC_INT8_*
+INT8_DX, INT8_DW, INT8_DB = 1, 2, 4
 
 
 class ProfileRecord(ctypes.Structure):
@@ -132,6 +133,7 @@ SIGNATURES = {
     "rexsc_fixed_conv2d": (_int, [ctypes.POINTER(FixedDesc), _vp, _vp, _vp, _vp, _sz, _vp]),
     "rexsc_quantize_rows": (_int, [_vp, _int, _sz, _sz, _sz, _vp, _sz, _vp, _vp]),
     "rexsc_int8_workspace_bytes": (_sz, [_i8d, _int]),
+    "rexsc_int8_backward_workspace_bytes": (_sz, [_i8d, _int]),
     "rexsc_int8_product": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "rexsc_int8_linear": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "rexsc_int8_backward": (_int, [_i8d, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

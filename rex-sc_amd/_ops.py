@@ -797,9 +797,9 @@ def _bias_vector(bias, n, what):
 _NO_BYTES = ctypes.c_size_t(-1).value
 
 
-def _int8_space(L, d, what, device):
-    """(workspace of a call or None, its bytes)"""
-    nbytes = L.rexsc_int8_workspace_bytes(d, what)
+def _int8_space(L, d, what, device, wanted=None):
+    """(workspace of a call or None, its bytes); wanted: the gradients of a backward pass"""
+    nbytes = L.rexsc_int8_workspace_bytes(d, what) if wanted is None else L.rexsc_int8_backward_workspace_bytes(d, wanted)
     if nbytes == 0:
         return None, 0
     if nbytes == _NO_BYTES:
@@ -921,7 +921,8 @@ def _int8_gradients(g, N, K, a, a_stride, a_scale, b, b_stride, b_scale, need_x,
         db = torch.empty(N, dtype=bias_dtype, device=device) if bias_dtype is not None else None
         d = _lib.Int8Desc.packed(gm.shape[0], N, K, code, 0 if db is None else _dtype_code(db, "linear_int8"),
                                  0 if dw is None else _dtype_code(dw, "linear_int8"), 0, 0, a_stride, b_stride)
-        ws, nbytes = _int8_space(L, d, _lib.INT8_BACKWARD, device)
+        wanted = ((0 if dx is None else _lib.INT8_DX) | (0 if dw is None else _lib.INT8_DW) | (0 if db is None else _lib.INT8_DB))
+        ws, nbytes = _int8_space(L, d, _lib.INT8_BACKWARD, device, wanted)
         rc = L.rexsc_int8_backward(d, gm.data_ptr(), a, a_scale, b, b_scale, _addr(dx), _addr(dw), _addr(db), _addr(ws), nbytes,
                                    _raw_stream(dev))
         if rc:

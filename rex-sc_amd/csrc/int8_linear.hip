@@ -449,7 +449,25 @@ constexpr int MAX_SHARES = 32, SHARE_ROWS = 512; // runs of g's rows whose colum
 int share_rows(int M) { return max(SHARE_ROWS, (M + MAX_SHARES - 1) / MAX_SHARES); }
 int shares(int M) { return (M + share_rows(M) - 1) / share_rows(M); }
 
-Space space(const rexsc_int8_desc *d, int what)
+constexpr int ALL = REXSC_INT8_DX | REXSC_INT8_DW | REXSC_INT8_DB;
+
+// Whether the launches of the wanted gradients hold d's sizes.
+int check_backward(const rexsc_int8_desc *d, int wanted)
+{
+    if (d->M == 0 || d->N == 0) return REXSC_OK;
+    const bool dx = wanted & REXSC_INT8_DX, dw = wanted & REXSC_INT8_DW, stats = wanted & (REXSC_INT8_DW | REXSC_INT8_DB);
+    const uint64_t tiles_k = (uint64_t)((d->K + 63) / 64), tiles_n = (uint64_t)pad64(d->N) / 64, tiles_m = (uint64_t)pad64(d->M) / 64;
+    // a launch has fewer than 2^32 threads
+    REXSC_CHECK_ARG((dx ? d->M + tiles_n * tiles_k : 0) + (dw ? tiles_m * tiles_k : 0) + (stats ? tiles_n * MAX_SHARES : 0) < (1ull << 24) &&
+                        (!dw || tiles_m * tiles_n < (1ull << 24)),
+                    "int8 linear: gradients of %d x %d x %d are more than a launch holds", d->M, d->N, d->K);
+    REXSC_CHECK_ARG((!dx || tiles_n * 128 < MAX_ROW_BYTES) && (!dw || tiles_m * 128 < MAX_ROW_BYTES),
+                    "int8 linear: sums over at most %zu tokens (weight's gradient) or channels (input's gradient)", MAX_ROW_BYTES / 2 - 64);
+    return REXSC_OK;
+}
+
+// wanted: the gradients that a workspace for them is to hold.
+Space space(const rexsc_int8_desc *d, int what, int wanted = ALL)
 {
     Space s{};
     size_t at = 0;
@@ -464,15 +482,23 @@ Space space(const rexsc_int8_desc *d, int what)
     } else if (M > 0 && N > 0) {
         // dx and dw follow each other on the stream, so their partial results share a place
         const size_t ldn = pad64(N), ldm = pad64(M);
-        s.product = take(max(tile_product_workspace(d->M, d->K, (int)ldn * 2, PIECES), tile_product_workspace(d->N, d->K, (int)ldm * 2, PIECES)));
-        s.g_rows = take(M * ldn * PIECES * 2);
-        s.g_rows_scale = take(M * 4);
-        s.b_t = take(K * ldn * 2);
-        s.g_cols = take(N * ldm * PIECES * 2);
-        s.g_cols_scale = take(N * 4);
-        s.a_t = take(K * ldm * 2);
-        s.sums = take((size_t)shares(d->M) * N * 4);
-        s.tops = take((size_t)shares(d->M) * N * 4);
+        const bool dx = wanted & REXSC_INT8_DX, dw = wanted & REXSC_INT8_DW;
+        s.product = take(max(dx ? tile_product_workspace(d->M, d->K, (int)ldn * 2, PIECES) : 0,
+                             dw ? tile_product_workspace(d->N, d->K, (int)ldm * 2, PIECES) : 0));
+        if (dx) {
+            s.g_rows = take(M * ldn * PIECES * 2);
+            s.g_rows_scale = take(M * 4);
+            s.b_t = take(K * ldn * 2);
+        }
+        if (dw) {
+            s.g_cols = take(N * ldm * PIECES * 2);
+            s.g_cols_scale = take(N * 4);
+            s.a_t = take(K * ldm * 2);
+        }
+        if (wanted & (REXSC_INT8_DW | REXSC_INT8_DB)) {
+            s.sums = take((size_t)shares(d->M) * N * 4);
+            s.tops = take((size_t)shares(d->M) * N * 4);
+        }
     }
     s.total = at;
     return s;
@@ -533,7 +559,17 @@ extern "C" size_t rexsc_int8_workspace_bytes(const rexsc_int8_desc *d, int what)
         set_error("int8 linear: no call has the number %d", what);
         return (size_t)-1;
     }
-    return space(d, what).total;
+    return what == REXSC_INT8_BACKWARD ? rexsc_int8_backward_workspace_bytes(d, ALL) : space(d, what).total;
+}
+
+extern "C" size_t rexsc_int8_backward_workspace_bytes(const rexsc_int8_desc *d, int wanted)
+{
+    if (check_int8(d)) return (size_t)-1;
+    if (wanted & ~ALL) {
+        set_error("int8 linear: no gradients have the flags %d", wanted);
+        return (size_t)-1;
+    }
+    return check_backward(d, wanted) ? (size_t)-1 : space(d, REXSC_INT8_BACKWARD, wanted).total;
 }
 
 extern "C" int rexsc_int8_product(const rexsc_int8_desc *d, const int8_t *a, const float *a_scale, const int8_t *b,
@@ -599,7 +635,9 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
         if (int rc = check_rows8("channels", b, d->b_stride, d->K)) return rc;
     if (dw)
         if (int rc = check_rows8("tokens", a, d->a_stride, d->K)) return rc;
-    const Space s = space(d, REXSC_INT8_BACKWARD);
+    const int wanted = (dx ? REXSC_INT8_DX : 0) | (dw ? REXSC_INT8_DW : 0) | (db ? REXSC_INT8_DB : 0);
+    if (int rc = check_backward(d, wanted)) return rc;
+    const Space s = space(d, REXSC_INT8_BACKWARD, wanted);
     if (int rc = check_space(s, workspace, workspace_bytes)) return rc;
     auto at = [&](size_t o) { return (char *)workspace + o; };
 
@@ -617,11 +655,6 @@ extern "C" int rexsc_int8_backward(const rexsc_int8_desc *d, const void *g, cons
     p.shares = shares(d->M); p.share_rows = share_rows(d->M);
     p.db = db; p.db_dtype = d->bias_dtype;
     const uint64_t tiles_k = (uint64_t)((d->K + 63) / 64), tiles_n = (uint64_t)p.ldn / 64, tiles_m = (uint64_t)p.ldm / 64;
-    // a launch has fewer than 2^32 threads
-    REXSC_CHECK_ARG((uint64_t)d->M + (tiles_n + tiles_m) * tiles_k + tiles_n * MAX_SHARES < (1ull << 24) && tiles_m * tiles_n < (1ull << 24),
-                    "int8 linear: gradients of %d x %d x %d are more than a launch holds", d->M, d->N, d->K);
-    REXSC_CHECK_ARG((size_t)p.ldn * 2 < MAX_ROW_BYTES && (size_t)p.ldm * 2 < MAX_ROW_BYTES,
-                    "int8 linear: gradients of at most %zu tokens or channels", MAX_ROW_BYTES / 2 - 64);
     p.row_blocks = dx ? (unsigned)d->M : 0;
     p.b_blocks = dx ? (unsigned)(tiles_n * tiles_k) : 0;
     p.a_blocks = dw ? (unsigned)(tiles_m * tiles_k) : 0;

@@ -706,3 +706,21 @@ def test_weights_whose_rows_are_far_apart(m):
     want = F.linear_int8(xg, far.contiguous(), None, weight_scale=s)
     assert torch.equal(y, want)
     assert torch.equal(*(torch.autograd.grad(t.sum(), [xg])[0] for t in (y, want)))
+
+
+def test_gradient_of_the_input_for_more_tokens_than_the_weights_sums_over():
+    """A frozen weight has no gradient to sum over the tokens: their number is not held to that sum's limit."""
+    import sc_functional as F
+    m, n, k = (1 << 22) + 5, 10, 24
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    wq = torch.randint(-127, 128, (n, k), device="cuda", generator=gen).to(torch.int8)
+    x = torch.zeros(m, k, device="cuda", dtype=torch.float16).requires_grad_(True)
+    go = torch.randint(-8, 9, (m, n), device="cuda", generator=gen).half()
+    b = torch.zeros(n, device="cuda", requires_grad=True)
+    y = F.linear_int8(x, wq, b, weight_scale=torch.ones(n, device="cuda"))
+    dx, db = torch.autograd.grad(y, [x, b], go)
+    assert torch.equal(dx, (go.float() @ wq.float()).half())  # integers below 2^24: exact, then rounded once
+    assert torch.equal(db.double(), go.double().sum(0))
+    w = wq.float().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="at most"):
+        torch.autograd.grad(F.linear_int8(x.detach(), w), [w], go)

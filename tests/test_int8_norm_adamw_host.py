@@ -263,3 +263,25 @@ def test_rows_far_apart_are_copied():
     assert torch.equal(got, far) and stride == 128 and got.data_ptr() != far.data_ptr()
     near = torch.zeros((8 << 20) + 64, dtype=torch.int8).as_strided((2, 48), ((8 << 20) - 16, 1))
     assert _ops._operand8(near, "x")[0].data_ptr() == near.data_ptr()
+
+
+def test_backward_workspace_holds_what_is_wanted():
+    import _lib
+    L = _lib.lib()
+    none = ctypes.c_size_t(-1).value
+    ws = lambda d, wanted: L.rexsc_int8_backward_workspace_bytes(ctypes.byref(d), wanted)
+    DX, DW, DB = _lib.INT8_DX, _lib.INT8_DW, _lib.INT8_DB
+    d = _int8(M=8192, N=4096, K=4096, a=4096, b=4096)
+    # both pieces of g for a gradient, and its other operand transposed, in binary16, and little beside them
+    dx, dw = 2 * (2 * 8192 * 4096 + 4096 * 4096), 2 * (2 * 4096 * 8192 + 4096 * 8192)
+    assert dx <= ws(d, DX) <= dx + (1 << 17) and dw <= ws(d, DW) <= dw + (1 << 20) and ws(d, DB) <= 1 << 20
+    assert ws(d, DX | DW | DB) == L.rexsc_int8_workspace_bytes(ctypes.byref(d), _lib.INT8_BACKWARD) >= dx + dw
+    assert ws(d, 0) == ws(_int8(M=0), DX) == ws(_int8(N=0), DW | DB) == 0 and ws(d, 8) == none and "flags 8" in _error(L)
+    # a workspace of that size is enough for such a call, and one byte less is not
+    back = lambda d, n, dx, dw, db: L.rexsc_int8_backward(ctypes.byref(d), FAKE, FAKE, FAKE, FAKE, FAKE, dx, dw, db, FAKE, n, None)
+    for wanted in range(1, 8):
+        assert back(d, ws(d, wanted) - 1, *(FAKE if wanted & f else None for f in (DX, DW, DB))) == -2, wanted
+    # more tokens than the weight's gradient sums over, and more channels than the input's: refused for that one alone
+    for d, no, yes in ((_int8(M=5000000, N=10), DW, DX | DB), (_int8(M=10, N=5000000), DX, DW | DB)):
+        assert ws(d, no) == none and "at most" in _error(L)
+        assert 0 < ws(d, yes) < none
