@@ -305,7 +305,8 @@ int rexsc_quantize_rows(const void *x, int dtype, size_t rows, size_t cols, size
 
 typedef struct rexsc_int8_desc {
     int32_t struct_size;     /* sizeof(rexsc_int8_desc) */
-    int32_t M, N, K;         /* tokens, output channels, reduction; 1 <= K <= 131071 (the int32 sum cannot overflow) */
+    int32_t M, N, K;         /* tokens, output channels, reduction; 0 <= M, N <= 2^31 - 256, 1 <= K <= 131071 (the int32
+                              * sum cannot overflow) */
     int32_t dtype;           /* type of y (and of x, of the incoming gradient and of dx where a call has them) */
     int32_t bias_dtype;      /* type of bias and of its gradient */
     int32_t weight_dtype;    /* type of the weight's gradient */

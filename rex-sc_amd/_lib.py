@@ -4,7 +4,6 @@ The library is the only compute path: if it is missing, or an entry point fails,
 gets a RuntimeError -- there is no Python/CPU fallback.
 """
 import ctypes
-import functools
 import os
 import struct
 
@@ -33,7 +32,13 @@ def _packer(cls):
     codes = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_double: "d"}
     s = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_))
     assert s.size == ctypes.sizeof(cls)
-    return functools.partial(s.pack, s.size)
+
+    def pack(*args):
+        try:
+            return s.pack(s.size, *args)
+        except struct.error as e:
+            raise RuntimeError("%s: a value does not fit its field (%s)" % (cls.__name__, e)) from None
+    return pack
 
 
 class ConvDesc(_Desc):

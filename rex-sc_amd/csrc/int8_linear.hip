@@ -21,6 +21,7 @@ namespace rexsc {
 namespace {
 
 constexpr int MAX_K = 131071; // 128 * 128 * K < 2^31
+constexpr int MAX_ROWS = 2147483647 - 255; // tokens or channels: a tile's rows behind the last one still have numbers
 
 // ---- rows to 8 bits ------------------------------------------------------------------------------
 // Bound by memory: x is read once, in vectors of 16 bytes wherever they lie (RAGGED: rows that begin anywhere and end
@@ -305,7 +306,8 @@ __device__ void column_stats(const OperandArgs &p, unsigned block, float (&ls)[3
 {
     constexpr int V = 16 / sizeof(T), ACROSS = 64 / V, DOWN = 256 / ACROSS; // 16 or 32 rows at once
     const int share = (int)(block % p.shares), x = threadIdx.x % ACROSS * V, c = (int)(block / p.shares) * 64 + x;
-    const int y = threadIdx.x / ACROSS, begin = share * p.share_rows, end = min(p.M, begin + p.share_rows);
+    const int y = threadIdx.x / ACROSS, begin = share * p.share_rows;
+    const int end = begin + min(p.share_rows, p.M - begin);
     float s[V] = {};
     unsigned t[V] = {};
     if (c < p.N)
@@ -422,7 +424,7 @@ __global__ __launch_bounds__(256) void transposed_pieces_kernel(OperandArgs p)
 int check_int8(const rexsc_int8_desc *d)
 {
     REXSC_CHECK_DESC(d, rexsc_int8_desc);
-    REXSC_CHECK_ARG(d->M >= 0 && d->N >= 0, "int8 linear: M %d, N %d", d->M, d->N);
+    REXSC_CHECK_ARG(d->M >= 0 && d->N >= 0 && d->M <= MAX_ROWS && d->N <= MAX_ROWS, "int8 linear: M %d, N %d", d->M, d->N);
     REXSC_CHECK_ARG(d->K >= 1 && d->K <= MAX_K, "int8 linear: K must be 1..%d, so that the int32 sum cannot overflow (got %d)",
                     MAX_K, d->K);
     REXSC_CHECK_ARG(dtype_ok(d->dtype) && dtype_ok(d->bias_dtype) && dtype_ok(d->weight_dtype),
@@ -447,7 +449,7 @@ struct Space { size_t tokens, scales, g_rows, g_rows_scale, b_t, g_cols, g_cols_
 
 constexpr int MAX_SHARES = 32, SHARE_ROWS = 512; // runs of g's rows whose column statistics are taken apart
 int share_rows(int M) { return max(SHARE_ROWS, (M + MAX_SHARES - 1) / MAX_SHARES); }
-int shares(int M) { return (M + share_rows(M) - 1) / share_rows(M); }
+int shares(int M) { return (M - 1) / share_rows(M) + 1; }
 
 constexpr int ALL = REXSC_INT8_DX | REXSC_INT8_DW | REXSC_INT8_DB;
 

@@ -285,3 +285,15 @@ def test_backward_workspace_holds_what_is_wanted():
     for d, no, yes in ((_int8(M=5000000, N=10), DW, DX | DB), (_int8(M=10, N=5000000), DX, DW | DB)):
         assert ws(d, no) == none and "at most" in _error(L)
         assert 0 < ws(d, yes) < none
+
+
+def test_sizes_at_the_end_of_32_bits():
+    import _lib
+    L = _lib.lib()
+    none = ctypes.c_size_t(-1).value
+    for kw in ({"M": 2 ** 31 - 1}, {"N": 2 ** 31 - 1}, {"M": 2 ** 31 - 255}):
+        for what in range(3):
+            assert L.rexsc_int8_workspace_bytes(ctypes.byref(_int8(**kw)), what) == none and "int8 linear: M " in _error(L)
+    assert L.rexsc_int8_workspace_bytes(ctypes.byref(_int8(M=2 ** 31 - 256)), _lib.INT8_LINEAR) >= (2 ** 31 - 256) * 132
+    with pytest.raises(RuntimeError, match="does not fit"):
+        _lib.Int8Desc.packed(2 ** 31, 4, 32, 0, 0, 0, 0, 32, 32, 32)
