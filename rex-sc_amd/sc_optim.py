@@ -25,6 +25,18 @@ def _dense(t):
     return True
 
 
+def _memory_order(shape, stride):
+    """What tells two orders of a dense tensor's elements in memory apart: its dimensions with their strides, or None for
+    row by row, however the shape is cut."""
+    kept = [(n, s) for n, s in zip(shape, stride) if n > 1]
+    at = 1
+    for n, s in reversed(kept):
+        if s != at:
+            return kept
+        at *= n
+    return None
+
+
 _T = torch.Tensor
 _PTR, _NUMEL, _DENSE, _DEV = _T.data_ptr, _T.numel, _T.is_contiguous, _T.get_device
 _DTYPE = operator.attrgetter("dtype")
@@ -150,7 +162,23 @@ class AdamW(torch.optim.Optimizer):
             return {"exp_avg": zeros(), "exp_avg_sq": zeros()}
         zeros = lambda: torch.zeros(p.numel(), dtype=torch.uint8, device=p.device).view(E4M3)
         scale = lambda: torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32, device=p.device)
-        return {"exp_avg": zeros(), "exp_avg_sq": zeros(), "exp_avg_scale": scale(), "exp_avg_sq_scale": scale()}
+        return {"exp_avg": zeros(), "exp_avg_sq": zeros(), "exp_avg_scale": scale(), "exp_avg_sq_scale": scale(),
+                "layout": (tuple(p.shape), p.stride())}
+
+    def _follow(self, p, state):
+        """Brings the states of a parameter that lies otherwise in memory than when they were made, or than the one whose
+        states were loaded, into its order."""
+        if "exp_avg_scale" in state:
+            now = (tuple(p.shape), p.stride())
+            if "layout" in state and _memory_order(*state["layout"]) != _memory_order(*now):
+                raise RuntimeError("AdamW: 8-bit states lie in blocks along the memory of a parameter of layout %s, this one's is "
+                                   "%s (shape, strides)" % (state["layout"], now))
+            state["layout"] = now
+        elif state["exp_avg"].shape == p.shape and _dense(p):  # (else adamw_step refuses them)
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: a parameter whose layout has changed needs an eager step before a captured one")
+            for k in ("exp_avg", "exp_avg_sq"):
+                state[k] = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(state[k])
 
     def load_state_dict(self, state_dict):
         # torch casts a state to its parameter's type on loading: 8-bit states and their scales keep their own
@@ -203,6 +231,8 @@ class AdamW(torch.optim.Optimizer):
                     state.update(self._new_state(p, group))
                     if not group["capturable"]:
                         state["step"] = 0
+                elif p.stride() != (state["layout"][1] if "layout" in state else state["exp_avg"].stride()):
+                    self._follow(p, state)
                 if group["capturable"]:
                     key = (p.dtype, p.device)
                 else:

@@ -297,3 +297,50 @@ def test_sizes_at_the_end_of_32_bits():
     assert L.rexsc_int8_workspace_bytes(ctypes.byref(_int8(M=2 ** 31 - 256)), _lib.INT8_LINEAR) >= (2 ** 31 - 256) * 132
     with pytest.raises(RuntimeError, match="does not fit"):
         _lib.Int8Desc.packed(2 ** 31, 4, 32, 0, 0, 0, 0, 32, 32, 32)
+
+
+def test_states_of_another_layout(monkeypatch):
+    """A parameter whose memory order changes after its states were made, or that loads those of another order: 32-bit
+    states follow it, 8-bit ones, whose blocks run along the memory, cannot and are refused."""
+    import sc_optim
+    seen = []
+    monkeypatch.setattr(sc_optim, "adamw_step", lambda params, grads, m, v, *rest, **kw: seen.append((params, m, v)))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    shape = (6, 5, 3, 3)
+    last = lambda t: t.contiguous(memory_format=torch.channels_last)
+
+    def optimiser(bits, make):
+        p = torch.nn.Parameter(make(torch.randn(shape)))
+        p.grad = torch.randn_like(p)
+        return p, sc_optim.AdamW([p], state_bits=bits)
+
+    for bits in (32, 8):
+        for a, b in ((last, torch.Tensor.contiguous), (torch.Tensor.contiguous, last)):
+            p, first = optimiser(bits, a)
+            first.step()
+            q, again = optimiser(bits, b)
+            if bits == 32:
+                first.state[p]["exp_avg"].copy_(torch.randn(shape))
+                again.load_state_dict(first.state_dict())
+                again.step()
+                state = again.state[q]["exp_avg"]
+                assert state.stride() == q.stride() and torch.equal(state, first.state[p]["exp_avg"])
+                p.data = b(p.data)  # and without a reload
+                before = first.state[p]["exp_avg"].clone()
+                first.step()
+                assert first.state[p]["exp_avg"].stride() == p.stride() and torch.equal(first.state[p]["exp_avg"], before)
+            else:
+                again.load_state_dict(first.state_dict())
+                for opt, t in ((again, q), (first, p)):
+                    t.data = b(t.data)
+                    with pytest.raises(RuntimeError, match="layout"):
+                        opt.step()
+                q.data = a(q.data)
+                again.step()
+    # dimensions of one element have no layout
+    p = torch.nn.Parameter(last(torch.randn(8, 4, 1, 1)))
+    p.grad = torch.randn_like(p)
+    opt = sc_optim.AdamW([p], state_bits=8)
+    opt.step()
+    p.data = p.data.contiguous()
+    opt.step()
