@@ -311,6 +311,9 @@ __global__ __launch_bounds__(256) void norm_backward_small_kernel(NormParams p, 
 }
 
 // ---- rows of any length --------------------------------------------------------------------------
+// By single elements, three reads of x forward and two of x and g backward, with another two for the weight's gradients:
+// 4096 x 28672 bfloat16 forward 448 us (1.05 TB/s of x and y once each), backward 959 us (0.73 of x, g and dx); float32
+// 554 us (1.7) and 1185 us (1.2).
 template <typename T>
 __global__ __launch_bounds__(STREAM_THREADS) void norm_forward_stream_kernel(NormParams p)
 {
