@@ -176,6 +176,8 @@ class AdamW(torch.optim.Optimizer):
             state["layout"] = now
         elif state["exp_avg"].shape == p.shape and _dense(p):  # (else adamw_step refuses them)
             if torch.cuda.is_current_stream_capturing():
+                if p.is_contiguous() and state["exp_avg"].is_contiguous():  # dimensions of one element apart
+                    return
                 raise RuntimeError("AdamW: a parameter whose layout has changed needs an eager step before a captured one")
             for k in ("exp_avg", "exp_avg_sq"):
                 state[k] = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(state[k])
@@ -202,7 +204,7 @@ class AdamW(torch.optim.Optimizer):
         if held and isinstance(held[0], torch.Tensor) and all(t is held[0] for t in held):
             step = held[0]
         else:  # the first step, a loaded state, or a group that was not capturable before
-            if held and torch.cuda.is_current_stream_capturing():
+            if held and key[1].type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: a group that becomes capturable needs an eager step before a captured one")
             step = torch.full((1,), max(map(int, held), default=0), dtype=torch.int64, device=key[1])
         for s in states:

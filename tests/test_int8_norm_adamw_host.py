@@ -344,3 +344,30 @@ def test_states_of_another_layout(monkeypatch):
     opt.step()
     p.data = p.data.contiguous()
     opt.step()
+
+
+def test_a_capturable_state_loads_without_a_device():
+    import sc_optim
+    make = lambda: sc_optim.AdamW([torch.nn.Parameter(torch.ones(n)) for n in (3, 4)], capturable=True)
+    opt = make()
+    step = torch.tensor([7])
+    for p in opt.param_groups[0]["params"]:
+        opt.state[p] = {**opt._new_state(p, opt.param_groups[0]), "step": step}
+    again = make()
+    again.load_state_dict(opt.state_dict())
+    a, b = (again.state[p]["step"] for p in again.param_groups[0]["params"])
+    assert a is b and a is not step and a.item() == 7 and a.dtype == torch.int64
+
+
+def test_a_captured_step_after_loading_states_that_differ_in_dimensions_of_one_element(monkeypatch):
+    import sc_optim
+    seen = []
+    monkeypatch.setattr(sc_optim, "adamw_step", lambda params, *rest, **kw: seen.append(params))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    p = torch.nn.Parameter(torch.randn(8, 4, 1, 1))
+    p.grad = torch.randn_like(p)
+    opt = sc_optim.AdamW([p], capturable=True)
+    last = lambda: torch.zeros(8, 4, 1, 1).as_strided((8, 4, 1, 1), (4, 1, 4, 4))
+    opt.state[p] = {"exp_avg": last(), "exp_avg_sq": last(), "step": torch.tensor([1])}
+    opt.step()
+    assert len(seen) == 1
