@@ -451,3 +451,25 @@ def test_a_reloaded_capturable_optimiser_goes_on_as_the_first_one(bits):
             b = fresh
         for p, q in zip(a.param_groups[0]["params"], b.param_groups[0]["params"]):
             assert torch.equal(p, q) and a.state[p]["step"].item() == b.state[q]["step"].item(), which
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_stored_8_bit_states_of_odd_lengths_and_a_scaled_gradient(dt):
+    """The same behind the last whole chunk, where elements go one by one, and with a gradient scaler's factor, a power of
+    two that the gradient takes exactly."""
+    import sc_optim
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    n = 300 * 4096 + 1001
+    pad = lambda t: torch.nn.functional.pad(t, (0, -n % 256))
+    g = torch.randn(n, generator=gen, device="cuda") * 0.1
+    p, g = torch.zeros(n + 1, device="cuda", dtype=dt)[1:], torch.cat([g[:1], g]).to(dt)[1:]
+    u8 = lambda: torch.zeros(n + 1, dtype=torch.uint8, device="cuda")[1:].view(E4M3)
+    (M, V), (MS, VS) = (u8(), u8()), (torch.zeros(-(-n // 256), device="cuda") for _ in range(2))
+    step, scale = torch.tensor([6], dtype=torch.int64, device="cuda"), torch.tensor(64.0, device="cuda")
+    sc_optim.adamw_step([p], [g * 64], [M], [V], [MS], [VS], step=step, grad_scale=scale, **H)
+    f = lambda v: torch.tensor(v, dtype=torch.float32, device="cuda")
+    gf = pad(g.float())
+    m, ms = stored8(gf * f(1 - H["beta1"]), False)
+    v, vs = stored8((gf * gf * f(1 - H["beta2"])).double().sqrt().float(), True)
+    assert torch.equal(M.float(), m[:n].float()) and torch.equal(V.float(), v[:n].float())
+    assert torch.equal(MS, ms) and torch.equal(VS, vs) and step.item() == 7
